@@ -67,14 +67,20 @@ def pair_indices():
     return [int(m) for m in re.findall(r"^GG_PAIR\((\d+),", text, flags=re.M)]
 
 
+OPERATORS = ("route_kernels",)
+
+
 def build_hip(force=False, jobs=None):
-    headers = [os.path.join(CSRC, f) for f in ("gmm_kernel.hpp", "gmm_generic.hpp", "gmm_variants.hpp",
-                                               "gmm_variants.def", "row_kernels.hpp")]
+    gemm_headers = [os.path.join(CSRC, f) for f in ("gmm_kernel.hpp", "gmm_generic.hpp", "gmm_variants.hpp",
+                                                    "gmm_variants.def", "row_kernels.hpp")]
+    # (the operators' headers, and the C ABI's, reach their own units and the API's only)
+    headers = gemm_headers + [os.path.join(CSRC, f) for f in ("operators.hpp", "wave_ops.hpp")]
     headers.append(os.path.join(ROOT, "include", "grouped_gemm_hip.h"))
+    outer = ("gmm_api", "row_kernels") + OPERATORS
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     obj_dir, hip_lib, extra = OBJ_DIR, HIP_LIB, []
     os.makedirs(obj_dir, exist_ok=True)
-    units = [(os.path.join(CSRC, f + ".hip"), os.path.join(obj_dir, f + ".o"), extra) for f in ("gmm_api", "row_kernels")]
+    units = [(os.path.join(CSRC, f + ".hip"), os.path.join(obj_dir, f + ".o"), extra) for f in outer]
     for i in pair_indices():   # (the largest units first)
         units.append((os.path.join(CSRC, "gmm_pair.hip"), os.path.join(obj_dir, f"gmm_pair_{i}.o"), extra + [f"-DGG_PAIR_INDEX={i}"]))
     for i in variant_indices():
@@ -83,7 +89,7 @@ def build_hip(force=False, jobs=None):
     for dt in range(4):   # gmm_generic.hpp, one translation unit per element type
         units.append((os.path.join(CSRC, "gmm_generic_variant.hip"), os.path.join(obj_dir, f"gmm_generic_{dt}.o"),
                       extra + [f"-DGG_GENERIC_DT={dt}"]))
-    todo = [u for u in units if force or not _newer(u[1], [u[0]] + headers)]
+    todo = [u for n, u in enumerate(units) if force or not _newer(u[1], [u[0]] + (headers if n < len(outer) else gemm_headers))]
     jobs = jobs or min(len(todo) or 1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 1)))
     if todo:
         print(f"compiling {len(todo)} translation units with {hipcc}, {jobs} at a time", flush=True)
@@ -97,27 +103,34 @@ def build_hip(force=False, jobs=None):
 
 def build_binding(force=False):
     import torch
-    src = os.path.join(CSRC, "torch_binding.cpp")
-    if not force and _newer(EXT_LIB, [src, HIP_LIB, os.path.join(ROOT, "include", "grouped_gemm_hip.h")]):
-        return EXT_LIB
     tdir = os.path.dirname(torch.__file__)
     tlib = os.path.join(tdir, "lib")
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    cmd = [
-        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+    cxx = os.environ.get("CXX", "g++")
+    compile_flags = [
+        "-O2", "-std=c++17", "-fPIC",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=grouped_gemm_backend",
         "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
         "-I" + os.path.join(tdir, "include"),
         "-I" + os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
         "-I" + os.path.join(rocm, "include"),
         "-I" + sysconfig.get_paths()["include"],
-        src, "-o", EXT_LIB,
+    ]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    header = os.path.join(ROOT, "include", "grouped_gemm_hip.h")
+    units = [(os.path.join(CSRC, f + ".cpp"), os.path.join(OBJ_DIR, f + ".o")) for f in ("torch_binding", "operators_binding")]
+    todo = [u for u in units if force or not _newer(u[1], [u[0], header])]
+    with ThreadPoolExecutor(max_workers=2) as pool:
+        list(pool.map(lambda u: _run([cxx] + compile_flags + ["-c", u[0], "-o", u[1]]), todo))
+    if not todo and _newer(EXT_LIB, [u[1] for u in units] + [HIP_LIB]):
+        return EXT_LIB
+    _run([cxx, "-shared"] + [u[1] for u in units] + [
+        "-o", EXT_LIB,
         "-L" + HERE, "-lgrouped_gemm_hip",
         "-L" + tlib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ltorch_hip",
         "-L" + os.path.join(rocm, "lib"), "-lamdhip64",
         "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + tlib, "-Wl,-rpath," + os.path.join(rocm, "lib"),
-    ]
-    _run(cmd)
+    ])
     return EXT_LIB
 
 

@@ -15,6 +15,7 @@
 
 #include "gmm_generic.hpp"
 #include "gmm_variants.hpp"
+#include "operators.hpp"
 #include "row_kernels.hpp"
 
 namespace gg {
@@ -1110,6 +1111,58 @@ int gg_debug_schedule(const int64_t* batch_sizes, int batch_sizes_on_device, int
     }
   }
   return dispatch_dump(short_shape, layout, p, hs, stream);
+}
+
+static int check_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score) {
+  if (dtype != GG_DTYPE_BF16 && dtype != GG_DTYPE_F16 && dtype != GG_DTYPE_F32)
+    return fail(GG_EINVAL, "dtype must be GG_DTYPE_BF16, GG_DTYPE_F16 or GG_DTYPE_F32");
+  if (tokens < 0 || experts < 1 || top_k < 1) return fail(GG_EINVAL, "tokens must not be negative, experts and top_k at least 1");
+  if (top_k > experts) return fail(GG_EINVAL, "top_k must not be more than experts");
+  if (experts > GG_ROUTE_MAX_EXPERTS || top_k > GG_ROUTE_MAX_TOP_K)
+    return fail(GG_ELIMIT, "at most %d experts, top_k at most %d", GG_ROUTE_MAX_EXPERTS, GG_ROUTE_MAX_TOP_K);
+  if (tokens >= (int64_t(1) << 31) / top_k) return fail(GG_ELIMIT, "tokens * top_k must be below 2^31");
+  if (score != GG_SCORE_SOFTMAX && score != GG_SCORE_SIGMOID) return fail(GG_EINVAL, "score must be one of GG_SCORE_*");
+  if (tokens > 0 && logits == nullptr) return fail(GG_EINVAL, "logits is null");
+  return GG_OK;
+}
+
+uint64_t gg_route_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k) {
+  if (tokens < 0 || experts < 1 || top_k < 1 || experts > GG_ROUTE_MAX_EXPERTS || top_k > GG_ROUTE_MAX_TOP_K ||
+      tokens >= (int64_t(1) << 31) / top_k)
+    return 0;
+  return gg::route_scratch_bytes(tokens, experts, top_k);
+}
+
+int gg_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, int normalize,
+             float* weights, int32_t* chosen, int64_t* batch_sizes, int32_t* row_index, int32_t* order, float* mass,
+             void* scratch, void* stream) {
+  const int rc = check_route(logits, dtype, tokens, experts, top_k, score);
+  if (rc != GG_OK) return rc;
+  if (batch_sizes == nullptr || (tokens > 0 && (weights == nullptr || chosen == nullptr || row_index == nullptr || order == nullptr)))
+    return fail(GG_EINVAL, "weights, chosen, batch_sizes, row_index or order is null");
+  if (scratch == nullptr && gg::route_scratch_bytes(tokens, experts, top_k) > 0) return fail(GG_EINVAL, "scratch is null");
+  DeviceInfo info;
+  const int init = device_info(&info);
+  if (init != GG_OK) return init;
+  const gg::RouteArgs a = {logits, dtype, tokens, (int32_t)experts, (int32_t)top_k, score == GG_SCORE_SIGMOID, normalize != 0,
+                           weights, chosen, batch_sizes, row_index, order, mass, scratch};
+  GG_HIP(gg::route(a, static_cast<hipStream_t>(stream)));
+  return GG_OK;
+}
+
+int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, int normalize,
+                      const int32_t* chosen, const float* weights_grad, const float* mass_grad, void* logits_grad, void* stream) {
+  const int rc = check_route(logits, dtype, tokens, experts, top_k, score);
+  if (rc != GG_OK) return rc;
+  if (tokens == 0) return GG_OK;
+  if (chosen == nullptr || logits_grad == nullptr) return fail(GG_EINVAL, "chosen or logits_grad is null");
+  DeviceInfo info;
+  const int init = device_info(&info);
+  if (init != GG_OK) return init;
+  const gg::RouteBackwardArgs a = {logits, dtype, tokens, (int32_t)experts, (int32_t)top_k, score == GG_SCORE_SIGMOID,
+                                   normalize != 0, chosen, weights_grad, mass_grad, logits_grad};
+  GG_HIP(gg::route_backward(a, static_cast<hipStream_t>(stream)));
+  return GG_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,124 @@
+// PyTorch-ROCm binding of the operators around the grouped GEMM: checks of the tensors, outputs and scratch from
+// torch's allocator, one call into the C ABI on torch's current stream.
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/extension.h>
+
+#include <tuple>
+
+#include "../../include/grouped_gemm_hip.h"
+
+namespace grouped_gemm {
+
+namespace {
+
+void* CurrentStream(const torch::Device& device) {
+  return static_cast<void*>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream());
+}
+
+torch::Tensor Scratch(uint64_t bytes, const torch::Tensor& like) {
+  if (bytes == 0) return torch::Tensor();
+  return torch::empty({(int64_t)bytes}, like.options().dtype(torch::kUInt8).requires_grad(false));
+}
+
+void* Pointer(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// ------------------------------------------------------------------ router
+
+int LogitsType(torch::ScalarType t) {
+  return t == torch::kFloat32 ? GG_DTYPE_F32 : (t == torch::kFloat16 ? GG_DTYPE_F16 : GG_DTYPE_BF16);
+}
+
+int Score(const std::string& score) {
+  TORCH_CHECK(score == "softmax" || score == "sigmoid", "grouped_gemm: score must be 'softmax' or 'sigmoid'");
+  return score == "softmax" ? GG_SCORE_SOFTMAX : GG_SCORE_SIGMOID;
+}
+
+void CheckLogits(const torch::Tensor& logits, int64_t top_k) {
+  TORCH_CHECK(logits.dim() == 2, "grouped_gemm: logits must be 2-d (tokens, experts)");
+  TORCH_CHECK(logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16 ||
+                  logits.scalar_type() == torch::kFloat16,
+              "grouped_gemm: logits must be float32, bfloat16 or float16");
+  TORCH_CHECK(logits.is_contiguous(), "grouped_gemm: logits must be contiguous");
+  TORCH_CHECK(top_k >= 1 && top_k <= logits.size(1), "grouped_gemm: top_k must be between 1 and the number of experts");
+  TORCH_CHECK(logits.size(1) <= GG_ROUTE_MAX_EXPERTS && top_k <= GG_ROUTE_MAX_TOP_K, "grouped_gemm: at most ",
+              GG_ROUTE_MAX_EXPERTS, " experts and a top_k of at most ", GG_ROUTE_MAX_TOP_K);
+  TORCH_CHECK(logits.is_cuda(), "grouped_gemm: logits must be a GPU tensor");
+}
+
+// weights, chosen, batch_sizes, row_index, order, mass (undefined where it is not wanted)
+torch::autograd::variable_list RunRoute(const torch::Tensor& logits, int64_t top_k, int score, bool normalize, bool with_mass) {
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  const auto f32 = logits.options().dtype(torch::kFloat32).requires_grad(false);
+  const auto i32 = f32.dtype(torch::kInt32);
+  torch::Tensor weights = torch::empty({tokens, top_k}, f32), chosen = torch::empty({tokens, top_k}, i32);
+  torch::Tensor batch_sizes = torch::empty({experts}, f32.dtype(torch::kInt64));
+  torch::Tensor row_index = torch::empty({tokens * top_k}, i32), order = torch::empty({tokens * top_k}, i32);
+  torch::Tensor mass = with_mass ? torch::empty({experts}, f32) : torch::Tensor();
+  const torch::Tensor scratch = Scratch(gg_route_scratch_bytes(tokens, experts, top_k), weights);
+  const int rc = gg_route(logits.data_ptr(), LogitsType(logits.scalar_type()), tokens, experts, top_k, score, normalize,
+                          weights.data_ptr<float>(), chosen.data_ptr<int32_t>(), batch_sizes.data_ptr<int64_t>(),
+                          row_index.data_ptr<int32_t>(), order.data_ptr<int32_t>(), static_cast<float*>(Pointer(mass)),
+                          Pointer(scratch), CurrentStream(logits.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return {weights, chosen, batch_sizes, row_index, order, mass};
+}
+
+class RouteNode : public torch::autograd::Function<RouteNode> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& logits, int64_t top_k,
+                                                int64_t score, bool normalize, bool with_mass) {
+    auto out = RunRoute(logits, top_k, (int)score, normalize, with_mass);
+    ctx->save_for_backward({logits, out[1]});
+    ctx->saved_data["score"] = score;
+    ctx->saved_data["normalize"] = normalize;
+    ctx->mark_non_differentiable({out[1], out[2], out[3], out[4]});
+    ctx->set_materialize_grads(false);
+    if (!with_mass) out.pop_back();
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const torch::Tensor &logits = saved[0], &chosen = saved[1];
+    torch::Tensor weights_grad = grads[0], mass_grad = grads.size() > 5 ? grads[5] : torch::Tensor();
+    torch::Tensor none;
+    if (!weights_grad.defined() && !mass_grad.defined()) return {none, none, none, none, none};
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+    if (weights_grad.defined()) weights_grad = weights_grad.contiguous();
+    if (mass_grad.defined()) mass_grad = mass_grad.contiguous();
+    torch::Tensor out = torch::empty(logits.sizes(), logits.options().requires_grad(false));
+    const int rc = gg_route_backward(logits.data_ptr(), LogitsType(logits.scalar_type()), logits.size(0), logits.size(1),
+                                     chosen.size(1), (int)ctx->saved_data["score"].toInt(), ctx->saved_data["normalize"].toBool(),
+                                     chosen.data_ptr<int32_t>(), static_cast<const float*>(Pointer(weights_grad)),
+                                     static_cast<const float*>(Pointer(mass_grad)), out.data_ptr(), CurrentStream(logits.device()));
+    TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+    return {out, none, none, none, none};
+  }
+};
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> Route(
+    const torch::Tensor& logits, int64_t top_k, const std::string& score, bool normalize, bool with_mass) {
+  const int which = Score(score);
+  CheckLogits(logits, top_k);
+  torch::autograd::variable_list out;
+  if (torch::GradMode::is_enabled() && logits.requires_grad()) {
+    out = RouteNode::apply(logits, top_k, (int64_t)which, normalize, with_mass);
+  } else {
+    out = RunRoute(logits, top_k, which, normalize, with_mass);
+  }
+  c10::optional<torch::Tensor> mass;
+  if (with_mass) mass = out[5];
+  return {out[0], out[1], out[2], out[3], out[4], mass};
+}
+
+}  // namespace
+
+void RegisterOperators(pybind11::module_& m) {
+  m.def("route", &Route, "weights, chosen experts, batch_sizes, row_index, order and mass of router logits.");
+  m.attr("route_max_experts") = GG_ROUTE_MAX_EXPERTS;
+  m.attr("route_max_top_k") = GG_ROUTE_MAX_TOP_K;
+}
+
+}  // namespace grouped_gemm

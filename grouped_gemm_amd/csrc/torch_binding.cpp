@@ -20,6 +20,8 @@
 
 namespace grouped_gemm {
 
+void RegisterOperators(pybind11::module_& m);   // operators_binding.cpp
+
 namespace {
 
 bool IsFloat8(torch::ScalarType t) { return t == torch::kFloat8_e4m3fn || t == torch::kFloat8_e5m2; }
@@ -673,6 +675,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("debug_schedule", &DebugSchedule, "Per-group table derived by the on-device scheduler.");
   m.attr("max_groups_per_launch") = GG_MAX_GROUPS_PER_LAUNCH;
   m.attr("sched_cols") = GG_SCHED_COLS;
+  RegisterOperators(m);
 }
 
 }  // namespace grouped_gemm

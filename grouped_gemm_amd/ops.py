@@ -5,7 +5,7 @@ backward is two more: the input gradient with the opposite layout of `b`, and th
 weight gradient with `trans_a` (per expert a_e^T @ grad_e, zeros for an expert
 without tokens).
 """
-from typing import Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -161,6 +161,34 @@ def gmm_swiglu(a, w, batch_sizes, trans_b=False, keep_products=True):
     held."""
     keep = keep_products and torch.is_grad_enabled() and (a.requires_grad or w.requires_grad)
     return GroupedGemmSwiGLU.apply(a, w, batch_sizes, trans_b, keep)
+
+
+# ------------------------------------------------------------------ router
+
+class Routing(NamedTuple):
+    """What route returns: where each token goes, in the form that gmm and its row indices take."""
+    weights: torch.Tensor          # float32 (tokens, top_k), differentiable
+    experts: torch.Tensor          # int32 (tokens, top_k), by descending logit
+    batch_sizes: torch.Tensor      # int64 (experts): rows of each expert
+    row_index: torch.Tensor        # int32 (tokens * top_k): the token of each row sorted by expert (gmm_gather)
+    order: torch.Tensor            # int32 (tokens * top_k): its place in `experts`, flattened (gmm_scatter)
+    mass: Optional[torch.Tensor]   # float32 (experts), differentiable: sum of the scores over the tokens
+
+
+def route(logits, top_k, score="softmax", normalize=True, with_mass=False):
+    """The router of an expert layer: the top_k largest of each token's logits (tokens, experts), their weights, and the
+    stable order that sorts the chosen rows by expert.
+
+    Scores are softmax(logits), or sigmoid(logits) with score="sigmoid"; a weight is the score of its expert, with
+    `normalize` divided by the sum over the token's chosen ones.  Of equal logits the lower expert is chosen first;
+    NaN counts as the largest.  An expert whose logit is -inf has a score of 0 and is chosen only where fewer than
+    top_k others are left, so that there always are tokens * top_k rows; a token all of whose logits are -inf has
+    weights of 0.  logits: float32, bfloat16 or float16; everything is computed in float32.
+
+    `mass`, with with_mass, is what balancing losses need beside batch_sizes.  Gradients flow from weights and mass
+    to the logits.  Nothing waits for the device: batch_sizes stays there, as gmm takes it.  Not part of the reference's surface, which
+    takes rows already sorted (grouped_gemm/ops.py:8)."""
+    return Routing(*backend.backend.route(logits, top_k, score, normalize, with_mass))
 
 
 # ------------------------------------------------------------------ traceable form

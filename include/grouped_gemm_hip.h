@@ -43,6 +43,7 @@ extern "C" {
 #define GG_DTYPE_F16 1
 #define GG_DTYPE_F8E4M3 2   /* OCP e4m3 (torch.float8_e4m3fn) in a and b, bf16 in c */
 #define GG_DTYPE_F8E5M2 3   /* OCP e5m2 (torch.float8_e5m2) in a and b, bf16 in c */
+#define GG_DTYPE_F32 4      /* router logits only (gg_route) */
 
 /* bits a launch ORs into *gg_gmm_args.size_status */
 #define GG_STATUS_NEGATIVE_SIZE 1   /* a device-resident batch size was negative (taken as 0) */
@@ -342,6 +343,40 @@ int gg_pad_rows(const void* src, void* dst, int64_t batches, int64_t src_rows, i
                 int64_t dst_rows, int64_t dst_cols, int elem_bytes, void* stream);
 int gg_unpad_rows(const void* src, void* dst, int64_t batches, int64_t src_rows, int64_t src_cols,
                   int64_t dst_rows, int64_t dst_cols, void* stream);
+
+/*
+ * The router: which experts each token goes to, with what weight, and the order that sorts the chosen rows by expert,
+ * as the grouped products and their row indices take it.  No counterpart in the reference, which takes rows already
+ * sorted (grouped_gemm/ops.py:8).
+ *
+ * With s = softmax(logits) (GG_SCORE_SOFTMAX) or 1 / (1 + exp(-logits)) (GG_SCORE_SIGMOID), per row of logits (tokens,
+ * experts), contiguous, of element type dtype (GG_DTYPE_BF16, GG_DTYPE_F16 or GG_DTYPE_F32):
+ *   chosen       (tokens, top_k) the experts of the top_k largest logits, in descending order; of equal ones the lower
+ *                number first (-0 equals +0, NaN is larger than any number)
+ *   weights      (tokens, top_k) s of the chosen; with normalize divided by their sum
+ *   batch_sizes  (experts) rows of each expert
+ *   order        (tokens * top_k) sorted by expert, those of one expert in their own order: the number of each row in
+ *                chosen, what gg_gmm takes as c_row_index to put rows back
+ *   row_index    (tokens * top_k) order / top_k: the token of each sorted row, what gg_gmm takes as a_row_index
+ *   mass         (experts) or NULL: sum of s over the tokens, for balancing losses
+ * A logit of -inf has a score of 0; it is chosen only where fewer than top_k others are left, with a weight of 0, so that
+ * there always are tokens * top_k rows.  A row of -inf alone has scores and weights of 0.  Scores are computed in fp32.
+ * The same bits on every call.  `scratch`: gg_route_scratch_bytes of device memory, 4-byte aligned, of any contents
+ * (NULL where that is 0).  At most GG_ROUTE_MAX_EXPERTS experts, top_k at most GG_ROUTE_MAX_TOP_K, tokens * top_k below 2^31.
+ *
+ * gg_route_backward: the gradient of the logits, of their element type, from those of weights and mass (fp32, either may be
+ * NULL) and the `chosen` that gg_route wrote.
+ */
+#define GG_SCORE_SOFTMAX 0
+#define GG_SCORE_SIGMOID 1
+#define GG_ROUTE_MAX_EXPERTS 1024
+#define GG_ROUTE_MAX_TOP_K 32
+uint64_t gg_route_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k);
+int gg_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, int normalize,
+             float* weights, int32_t* chosen, int64_t* batch_sizes, int32_t* row_index, int32_t* order, float* mass,
+             void* scratch, void* stream);
+int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, int normalize,
+                      const int32_t* chosen, const float* weights_grad, const float* mass_grad, void* logits_grad, void* stream);
 
 /*
  * Runs only the on-device scheduler of gg_gmm_bf16 (same device code, same

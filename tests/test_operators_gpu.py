@@ -1,0 +1,243 @@
+"""The operators around the grouped GEMM against their definitions in 64 bits, on the CPU: the router.
+
+Tolerances follow from how results are computed.  The router works in fp32: exp(x - top) is off by up to 2^-24 |x - top|
+from the rounding of its argument and two units in the last place of its own, a sum over at most 1024 positive terms
+and a quotient by less than 16 units; with |x - top| <= 64 that is below 1e-5 of a weight.  Gradients of the
+logits are differences of such products: off by 1e-5 of the largest term they are made of.  A result in bfloat16 or
+float16 is rounded once more, by 2^-8 or 2^-11 of itself (2^-25 absolute below float16's normal range).
+Whole numbers are equal."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+ROUNDING = {torch.float32: (0.0, 0.0), torch.bfloat16: (2.0 ** -8, 0.0), torch.float16: (2.0 ** -11, 2.0 ** -25)}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    from grouped_gemm import ops as _ops
+    return _ops
+
+
+def _announce(*what):
+    print("[case]", *what, flush=True)
+
+
+def _close(got, want, rtol, atol, what):
+    """Every element within atol + rtol |want|; what is not finite in `want` alike in `got`.  atol may be a tensor."""
+    got, want = got.double().cpu(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    if got.numel() == 0:
+        return
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in other places"
+    odd = ~torch.isfinite(want)
+    both_inf = torch.isinf(want)
+    assert torch.equal(got[both_inf], want[both_inf]), f"{what}: infinities differ"
+    off = ((got - want).abs() - (atol + rtol * want.abs())).masked_fill(odd, 0.0)
+    assert float(off.max()) <= 0.0, f"{what}: off by {float(off.max())} more than allowed"
+
+
+# ------------------------------------------------------------------ router
+
+def _route_reference(logits, k, score, normalize, weights_grad=None, mass_grad=None):
+    """The router by its definition in 64 bits: a sort, its formulas and their derivatives."""
+    x = logits.double()
+    t, e = x.shape
+    chosen = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :k]
+    closed = (x == -INF).all(1, keepdim=True)
+    safe = x.masked_fill(closed, 0.0)
+    if score == "softmax":
+        s = torch.softmax(safe, 1).masked_fill(closed, 0.0)
+        slope = torch.ones_like(s)
+    else:
+        s = torch.sigmoid(x)
+        slope = torch.sigmoid(-x)
+    picked = s.gather(1, chosen)
+    total = picked.sum(1, keepdim=True)
+    share = torch.where(total == 0, torch.zeros_like(picked), picked / total)
+    flat = chosen.reshape(-1)
+    order = torch.sort(flat, stable=True).indices
+    out = dict(weights=share if normalize else picked, experts=chosen, batch_sizes=torch.bincount(flat, minlength=e),
+               order=order, row_index=order // k, mass=s.sum(0))
+    if weights_grad is not None or mass_grad is not None:
+        g = weights_grad.double() if weights_grad is not None else torch.zeros(t, k, dtype=torch.float64)
+        u = mass_grad.double().expand(t, e) if mass_grad is not None else torch.zeros_like(x)
+        if not normalize:
+            u = u.scatter_add(1, chosen, g)
+        grad = s * (u - (u * s).sum(1, keepdim=True)) if score == "softmax" else s * slope * u
+        if normalize:
+            at = share * (g - (g * share).sum(1, keepdim=True)) * slope.gather(1, chosen)
+            grad = grad.scatter_add(1, chosen, at)
+        out["grad"] = grad
+        out["grad_scale"] = u.abs().amax(1, keepdim=True) + g.abs().amax(1, keepdim=True)
+    return out
+
+
+def _check_route(ops, logits, k, score="softmax", normalize=True, with_mass=True, what=""):
+    got = ops.route(logits.cuda(), k, score=score, normalize=normalize, with_mass=with_mass)
+    want = _route_reference(logits, k, score, normalize)
+    for name in ("experts", "batch_sizes", "order", "row_index"):
+        assert torch.equal(getattr(got, name).cpu().long(), want[name]), (what, name)
+    assert got.experts.dtype == got.order.dtype == got.row_index.dtype == torch.int32 and got.batch_sizes.dtype == torch.int64
+    assert got.weights.dtype == torch.float32
+    _close(got.weights, want["weights"], 1e-5, 1e-30, f"{what} weights")
+    if with_mass:
+        _close(got.mass, want["mass"], 1e-5, 1e-30, f"{what} mass")
+    else:
+        assert got.mass is None
+    return got, want
+
+
+# one token and none, sizes around a lane's, a group's and a workgroup's share, most experts and largest top_k
+ROUTE_SHAPES = [(0, 8, 2), (1, 1, 1), (1, 64, 6), (3, 5, 5), (7, 37, 3), (33, 64, 8), (64, 65, 32), (65, 128, 17), (100, 129, 1),
+                (513, 256, 8), (130, 257, 20), (77, 512, 10), (200, 1000, 32), (64, 1024, 32), (3000, 17, 4), (20001, 8, 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", ROUTE_SHAPES)
+def test_route_matches_its_definition(ops, shape, dtype):
+    t, e, k = shape
+    g = torch.Generator().manual_seed(t * 7 + e)
+    logits = (torch.randn(t, e, generator=g) * 2).to(dtype)   # (two-byte logits: many equal ones)
+    for score in ("softmax", "sigmoid"):
+        for normalize in (True, False):
+            _announce("route", shape, dtype, score, normalize)
+            _check_route(ops, logits, k, score, normalize, what=f"{shape} {score} {normalize}")
+    _check_route(ops, logits, k, with_mass=False, what=f"{shape}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("experts", [12, 200, 700])
+def test_route_odd_values(ops, tokens, experts, dtype):
+    """Closed experts, tokens that none is open to, equal logits, -0 and +0, infinities, NaN, the type's lowest value."""
+    g = torch.Generator().manual_seed(experts)
+    logits = torch.randn(tokens, experts, generator=g).to(dtype)
+    logits[torch.rand(tokens, experts, generator=g) < 0.3] = -INF
+    logits[0] = -INF
+    logits[1] = -INF
+    logits[1, 5] = 3.0                       # one open expert, fewer than are chosen
+    logits[2] = 1.25                         # all equal
+    logits[3] = 0.0
+    logits[3, ::2] = -0.0                    # equal as well
+    logits[4] = torch.finfo(dtype).min       # a mask of the lowest value instead of -inf
+    logits[4, 7] = 2.0
+    logits[5, 3] = float("nan")
+    logits[6, 9] = INF
+    logits[7] = torch.finfo(dtype).min
+    for score in ("softmax", "sigmoid"):
+        for normalize in (True, False):
+            _announce("route odd values", tokens, experts, dtype, score, normalize)
+            got = ops.route(logits.cuda(), 4, score=score, normalize=normalize, with_mass=True)
+            want = _route_reference(logits, 4, score, normalize)
+            for name in ("experts", "batch_sizes", "order", "row_index"):
+                assert torch.equal(getattr(got, name).cpu().long(), want[name]), name
+            # (row 7 under a normalized sigmoid: scores too small for 64 bits too, all alike)
+            if score == "sigmoid" and normalize:
+                want["weights"][7] = 0.25
+            _close(got.weights, want["weights"], 1e-5, 1e-30, "weights")
+            assert (got.weights[0] == 0).all()
+            finite = torch.cat([logits[:5], logits[7:]])
+            _check_route(ops, finite[:5], 4, score, normalize, what="finite rows")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 8, 2), (5, 64, 6), (70, 37, 3), (257, 256, 8), (90, 500, 32), (33, 1024, 5), (4099, 16, 4)])
+def test_route_gradient_matches_its_formula(ops, shape, dtype):
+    t, e, k = shape
+    g = torch.Generator().manual_seed(e)
+    logits = (torch.randn(t, e, generator=g) * 1.5).to(dtype)
+    logits[0, : e // 2] = -INF
+    if t > 2:
+        logits[2] = -INF
+    weights_grad, mass_grad = torch.randn(t, k, generator=g), torch.randn(e, generator=g)
+    for score in ("softmax", "sigmoid"):
+        for normalize in (True, False):
+            for with_weights, with_mass in ((True, True), (True, False), (False, True)):
+                _announce("route gradient", shape, dtype, score, normalize, with_weights, with_mass)
+                x = logits.cuda().requires_grad_(True)
+                r = ops.route(x, k, score=score, normalize=normalize, with_mass=with_mass)
+                loss = 0.0
+                if with_weights:
+                    loss = loss + (r.weights * weights_grad.cuda()).sum()
+                if with_mass:
+                    loss = loss + (r.mass * mass_grad.cuda()).sum()
+                loss.backward()
+                want = _route_reference(logits, k, score, normalize, weights_grad if with_weights else None,
+                                        mass_grad if with_mass else None)
+                assert x.grad.dtype == dtype
+                rtol, least = ROUNDING[dtype]
+                _close(x.grad, want["grad"], 1e-5 + rtol, 1e-5 * want["grad_scale"] + least, f"{score} {normalize}")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_gradient_matches_differences(ops, score, normalize):
+    """Central differences of the outputs, step h = 2^-6: the quotient is off by h^2 / 6 of a third derivative (at most 2 for
+    these functions of one logit, times the gradients' sizes, 5e-5 each) and by two fp32 errors of the loss over 2 h."""
+    g = torch.Generator().manual_seed(11)
+    t, e, k, h = 4, 10, 3, 2.0 ** -6
+    # well apart, so that no step changes which experts are chosen
+    logits = torch.stack([torch.randperm(e, generator=g).float() * 0.25 for _ in range(t)])
+    weights_grad, mass_grad = torch.randn(t, k, generator=g), torch.randn(e, generator=g)
+    x = logits.cuda().requires_grad_(True)
+    r = ops.route(x, k, score=score, normalize=normalize, with_mass=True)
+    got, = torch.autograd.grad((r.weights, r.mass), x, (weights_grad.cuda(), mass_grad.cuda()))
+
+    def loss(z):
+        q = ops.route(z.cuda(), k, score=score, normalize=normalize, with_mass=True)
+        return float((q.weights.cpu().double() * weights_grad).sum() + (q.mass.cpu().double() * mass_grad).sum())
+
+    scale = float(weights_grad.abs().sum() + mass_grad.abs().sum())
+    for i in range(t):
+        for j in range(e):
+            up, down = logits.clone(), logits.clone()
+            up[i, j] += h
+            down[i, j] -= h
+            want = (loss(up) - loss(down)) / (2 * h)
+            assert abs(float(got[i, j]) - want) <= scale * (h * h / 3 + 4 * 2.0 ** -22 / h), (i, j)
+
+
+def test_route_on_other_streams_and_in_a_graph(ops):
+    """The same bits on another stream, on every call and in every replay of a captured one, with eager work in between."""
+    logits = torch.randn(5000, 96, device="cuda").bfloat16()
+    small = torch.randn(9, 96, device="cuda")
+    want = [ops.route(logits, 6, with_mass=True), ops.route(small, 6, with_mass=True)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [ops.route(logits, 6, with_mass=True), ops.route(small, 6, with_mass=True)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [ops.route(logits, 6, with_mass=True), ops.route(small, 6, with_mass=True)]
+    for _ in range(3):
+        for r in captured:
+            for part in r:
+                part.zero_()
+        graph.replay()
+        eager = [ops.route(logits, 6, with_mass=True), ops.route(small, 6, with_mass=True)]
+        torch.cuda.synchronize()
+        for one in (again, captured, eager):
+            for r, w in zip(one, want):
+                for a, b in zip(r, w):
+                    assert torch.equal(a, b)
+
+
+def test_route_refuses(ops):
+    x = torch.zeros(4, 8, device="cuda")
+    bad = [
+        (lambda: ops.route(x.cpu(), 2), "GPU"), (lambda: ops.route(x[0], 2), "2-d"), (lambda: ops.route(x.double(), 2), "float32"),
+        (lambda: ops.route(x, 0), "top_k"), (lambda: ops.route(x, 9), "top_k"), (lambda: ops.route(x.t(), 2), "contiguous"),
+        (lambda: ops.route(x, 2, score="tanh"), "score"), (lambda: ops.route(torch.zeros(2, 1025, device="cuda"), 2), "at most"),
+        (lambda: ops.route(torch.zeros(2, 64, device="cuda"), 33), "at most"),
+    ]
+    for call, message in bad:
+        with pytest.raises(RuntimeError, match=message):
+            call()
