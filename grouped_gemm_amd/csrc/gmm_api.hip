@@ -1165,4 +1165,39 @@ int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t exp
   return GG_OK;
 }
 
+static int check_few_tokens(int dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, int trans_b) {
+  if (dtype != GG_DTYPE_BF16 && dtype != GG_DTYPE_F16) return fail(GG_EINVAL, "dtype must be GG_DTYPE_BF16 or GG_DTYPE_F16");
+  if (tokens < 0 || experts < 1 || top_k < 1 || hidden < 1 || ffn < 1)
+    return fail(GG_EINVAL, "tokens must not be negative, experts, top_k and hidden sizes at least 1");
+  if (tokens > GG_FEW_TOKENS_MAX || experts > GG_ROUTE_MAX_EXPERTS || top_k > GG_ROUTE_MAX_TOP_K)
+    return fail(GG_ELIMIT, "at most %d tokens, %d experts, top_k at most %d", GG_FEW_TOKENS_MAX, GG_ROUTE_MAX_EXPERTS, GG_ROUTE_MAX_TOP_K);
+  if (hidden >= (1 << 22) || ffn >= (1 << 22)) return fail(GG_ELIMIT, "hidden sizes must be below 2^22");
+  if (!gg::few_tokens_fits(tokens, experts, top_k, hidden, ffn, trans_b != 0))
+    return fail(GG_ELIMIT, "experts times hidden sizes are too large for one launch");
+  return GG_OK;
+}
+
+uint64_t gg_moe_few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, int trans_b) {
+  if (check_few_tokens(GG_DTYPE_BF16, tokens, experts, top_k, hidden, ffn, trans_b) != GG_OK) return 0;
+  return gg::few_tokens_scratch_bytes(tokens, experts, top_k, hidden, ffn, trans_b != 0);
+}
+
+int gg_moe_few_tokens(const void* x, const void* w13, const void* w2, const int32_t* chosen, const float* weights, void* out,
+                      int dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, int trans_b,
+                      void* scratch, void* stream) {
+  const int rc = check_few_tokens(dtype, tokens, experts, top_k, hidden, ffn, trans_b);
+  if (rc != GG_OK) return rc;
+  if (tokens == 0) return GG_OK;
+  if (x == nullptr || w13 == nullptr || w2 == nullptr || chosen == nullptr || weights == nullptr || out == nullptr || scratch == nullptr)
+    return fail(GG_EINVAL, "x, w13, w2, chosen, weights, out or scratch is null");
+  if (reinterpret_cast<uintptr_t>(scratch) & 255) return fail(GG_ELIMIT, "scratch must be on a 256-byte boundary");
+  DeviceInfo info;
+  const int init = device_info(&info);
+  if (init != GG_OK) return init;
+  const gg::FewTokensArgs a = {x, w13, w2, chosen, weights, out, scratch, dtype, trans_b != 0, (int32_t)tokens, (int32_t)experts,
+                               (int32_t)top_k, (int32_t)hidden, (int32_t)ffn};
+  GG_HIP(gg::few_tokens(a, static_cast<hipStream_t>(stream)));
+  return GG_OK;
+}
+
 }  // extern "C"

@@ -43,4 +43,25 @@ struct RouteBackwardArgs {
 };
 hipError_t route_backward(const RouteBackwardArgs& args, hipStream_t stream);
 
+constexpr int64_t kFewMaxTokens = 64;
+constexpr int64_t kFewMaxExperts = 1024;
+constexpr int64_t kFewMaxSlots = kFewMaxTokens * kRouteMaxTopK;
+
+struct FewTokensArgs {
+  const void* x;           // (tokens, hidden), element type dt (kBF16, kF16)
+  const void* w13;         // (experts, hidden, 2 * ffn), or (experts, 2 * ffn, hidden) with trans_b
+  const void* w2;          // (experts, ffn, hidden), or (experts, hidden, ffn) with trans_b
+  const int32_t* chosen;   // (tokens, top_k)
+  const float* weights;    // (tokens, top_k)
+  void* out;               // (tokens, hidden)
+  void* scratch;           // few_tokens_scratch_bytes, 256-byte aligned, any contents
+  int dt;
+  bool trans_b;
+  int32_t tokens, experts, top_k, hidden, ffn;
+};
+// Whether 32 bits hold the offsets and thread counts of such a call.
+bool few_tokens_fits(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b);
+uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b);
+hipError_t few_tokens(const FewTokensArgs& args, hipStream_t stream);
+
 }  // namespace gg

@@ -113,10 +113,58 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
   return {out[0], out[1], out[2], out[3], out[4], mass};
 }
 
+// ------------------------------------------------------------------ gated expert layer for a few tokens
+
+bool IsTwoByte(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16; }
+
+// Operators for serving have no gradient: a graph that asks for one is an error, not a silent zero.
+void RefuseGradients(std::initializer_list<const torch::Tensor*> tensors, const char* name, const char* instead) {
+  if (!torch::GradMode::is_enabled()) return;
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), "grouped_gemm: ", name, " has no gradient (", instead, ")");
+}
+
+torch::Tensor MoeFewTokens(const torch::Tensor& x, const torch::Tensor& w13, const torch::Tensor& w2, const torch::Tensor& experts,
+                           const torch::Tensor& weights, bool trans_b) {
+  TORCH_CHECK(x.dim() == 2, "grouped_gemm: x must be 2-d (tokens, hidden)");
+  TORCH_CHECK(IsTwoByte(x), "grouped_gemm: x must be bfloat16 or float16");
+  TORCH_CHECK(w13.dim() == 3 && w2.dim() == 3, "grouped_gemm: w13 and w2 must be 3-d");
+  TORCH_CHECK(w13.scalar_type() == x.scalar_type() && w2.scalar_type() == x.scalar_type(),
+              "grouped_gemm: w13 and w2 must have the element type of x");
+  const int64_t tokens = x.size(0), hidden = x.size(1), num = w13.size(0), both = w13.size(trans_b ? 1 : 2);
+  TORCH_CHECK(w13.size(trans_b ? 2 : 1) == hidden, "grouped_gemm: contraction dimensions of x and w13 differ");
+  TORCH_CHECK(both % 2 == 0, "grouped_gemm: w13 must hold gate | up, an even number of columns");
+  TORCH_CHECK(w2.size(0) == num && w2.size(trans_b ? 2 : 1) == both / 2 && w2.size(trans_b ? 1 : 2) == hidden,
+              "grouped_gemm: w2 must take gate's columns back to the columns of x, for as many experts as w13");
+  TORCH_CHECK(experts.dim() == 2 && experts.size(0) == tokens && experts.scalar_type() == torch::kInt32,
+              "grouped_gemm: experts must be int32 (tokens, top_k)");
+  TORCH_CHECK(weights.sizes() == experts.sizes() && weights.scalar_type() == torch::kFloat32,
+              "grouped_gemm: weights must be float32, of the shape of experts");
+  TORCH_CHECK(tokens <= GG_FEW_TOKENS_MAX, "grouped_gemm: at most ", GG_FEW_TOKENS_MAX,
+              " tokens (more belong in gmm_swiglu and gmm_scatter with the indices of route)");
+  for (const torch::Tensor* t : {&x, &w13, &w2, &experts, &weights})
+    TORCH_CHECK(t->is_contiguous(), "grouped_gemm: x, w13, w2, experts and weights must be contiguous");
+  for (const torch::Tensor* t : {&x, &w13, &w2, &experts, &weights})
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device(), "grouped_gemm: x, w13, w2, experts and weights must be on the same GPU");
+  RefuseGradients({&x, &w13, &w2, &weights}, "moe_few_tokens", "train through gmm_swiglu and gmm_scatter");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  torch::Tensor out = torch::empty({tokens, hidden}, x.options().requires_grad(false));
+  if (tokens == 0) return out;
+  const torch::Tensor scratch =
+      Scratch(gg_moe_few_tokens_scratch_bytes(tokens, num, experts.size(1), hidden, both / 2, trans_b), out);
+  const int rc = gg_moe_few_tokens(x.data_ptr(), w13.data_ptr(), w2.data_ptr(), experts.data_ptr<int32_t>(),
+                                   weights.data_ptr<float>(), out.data_ptr(), x.scalar_type() == torch::kFloat16 ? GG_DTYPE_F16 : GG_DTYPE_BF16,
+                                   tokens, num, experts.size(1), hidden, both / 2, trans_b, Pointer(scratch), CurrentStream(x.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return out;
+}
+
 }  // namespace
 
 void RegisterOperators(pybind11::module_& m) {
   m.def("route", &Route, "weights, chosen experts, batch_sizes, row_index, order and mass of router logits.");
+  m.def("moe_few_tokens", &MoeFewTokens, "A gated expert layer for a few tokens.");
+  m.attr("moe_few_tokens_max") = GG_FEW_TOKENS_MAX;
   m.attr("route_max_experts") = GG_ROUTE_MAX_EXPERTS;
   m.attr("route_max_top_k") = GG_ROUTE_MAX_TOP_K;
 }

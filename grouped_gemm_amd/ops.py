@@ -191,6 +191,24 @@ def route(logits, top_k, score="softmax", normalize=True, with_mass=False):
     return Routing(*backend.backend.route(logits, top_k, score, normalize, with_mass))
 
 
+# ------------------------------------------------------------------ expert layer of a decode step
+
+def moe_few_tokens(x, w13, w2, experts, weights, trans_b=False):
+    """A whole gated expert layer for the few tokens of a decode step, in two launches:
+
+        out[t] = sum over j of weights[t, j] * gated(x[t], e) @ w2[e],  e = experts[t, j],
+        gated(x, e) = silu(x @ gate_e) * (x @ up_e),  w13[e] = [gate_e | up_e]
+
+    x: bfloat16 or float16 (tokens, hidden), at most 64 tokens; w13 (num_experts, hidden, 2 * ffn) and w2 (num_experts, ffn,
+    hidden), or with trans_b (num_experts, 2 * ffn, hidden) and (num_experts, hidden, ffn), as for gmm_swiglu and gmm;
+    experts int32 and weights float32 (tokens, top_k), as route returns them.  A number that names no expert
+    contributes nothing.  Rounded once; the activation in between keeps twice the bits of the type.
+
+    For more tokens, and for training: gmm_swiglu and gmm_scatter with the indices of route.  This form has no
+    gradient, and refuses operands that ask for one.  Not part of the reference's surface (csrc/grouped_gemm.h:5-9)."""
+    return backend.backend.moe_few_tokens(x, w13, w2, experts, weights, trans_b)
+
+
 # ------------------------------------------------------------------ traceable form
 #
 # The same operator registered with torch.library, so that torch.compile sees one opaque node

@@ -379,6 +379,27 @@ int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t exp
                       const int32_t* chosen, const float* weights_grad, const float* mass_grad, void* logits_grad, void* stream);
 
 /*
+ * A gated expert layer for the few tokens of a decode step, in two launches: out[t] = sum over j of
+ * weights[t, j] * (silu(x[t] @ gate_e) * (x[t] @ up_e)) @ down_e with e = chosen[t, j] and silu(x) = x / (1 + exp(-x)).
+ *   x (tokens, hidden), out (tokens, hidden), element type dtype (GG_DTYPE_BF16 or GG_DTYPE_F16)
+ *   w13 (experts, hidden, 2 * ffn), or (experts, 2 * ffn, hidden) with trans_b: gate | up, gate first, as for GG_EPILOGUE_SWIGLU
+ *   w2 (experts, ffn, hidden), or (experts, hidden, ffn) with trans_b
+ *   chosen int32 (tokens, top_k), weights fp32 (tokens, top_k), as gg_route writes them
+ * all contiguous, aligned to their elements.  A number in `chosen` that names no expert contributes nothing; an expert named twice by a token
+ * counts twice.  Products and sums are in fp32; between the two the activations are handed on with twice the bits of the
+ * type, and the result is rounded once.  The same bits on every call.
+ * At most GG_FEW_TOKENS_MAX tokens (more belong in gg_gmm with row indices), GG_ROUTE_MAX_EXPERTS experts, top_k at
+ * most GG_ROUTE_MAX_TOP_K, hidden and ffn below 2^22.  `scratch`: gg_moe_few_tokens_scratch_bytes of device memory (0 for sizes that the
+ * call refuses), 256-byte aligned, of any contents; calls that share it must not overlap in time.
+ * No counterpart in the reference, whose operator is one product (csrc/grouped_gemm.h:5-9).
+ */
+#define GG_FEW_TOKENS_MAX 64
+uint64_t gg_moe_few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, int trans_b);
+int gg_moe_few_tokens(const void* x, const void* w13, const void* w2, const int32_t* chosen, const float* weights, void* out,
+                      int dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, int trans_b,
+                      void* scratch, void* stream);
+
+/*
  * Runs only the on-device scheduler of gg_gmm_bf16 (same device code, same
  * arguments) and writes what it derived to `table_out`, a device buffer of
  * num_groups * GG_SCHED_COLS int64: per group the problem (m, n, k), leading

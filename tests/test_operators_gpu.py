@@ -1,10 +1,18 @@
-"""The operators around the grouped GEMM against their definitions in 64 bits, on the CPU: the router.
+"""The operators around the grouped GEMM against their definitions in 64 bits, on the CPU: the router, the gated expert
+layer for a few tokens.
 
 Tolerances follow from how results are computed.  The router works in fp32: exp(x - top) is off by up to 2^-24 |x - top|
 from the rounding of its argument and two units in the last place of its own, a sum over at most 1024 positive terms
 and a quotient by less than 16 units; with |x - top| <= 64 that is below 1e-5 of a weight.  Gradients of the
 logits are differences of such products: off by 1e-5 of the largest term they are made of.  A result in bfloat16 or
 float16 is rounded once more, by 2^-8 or 2^-11 of itself (2^-25 absolute below float16's normal range).
+
+The layers' products are sums in fp32 of n products of two-byte numbers, which are exact: off by at most n 2^-24 times the sum of the
+terms' absolute values whatever the order (in matrix instructions too, which may round twice per step: 2 n 2^-24).  That
+sum of absolute values is computed beside the reference.  What is handed from one product to the next is rounded to
+twice the bits of the type (2^-16 of itself in bfloat16, 2^-21 in float16, there not below 2^-25), the gated activation's exponential and
+quotient are off by 2^-20, and the result is rounded once.
+
 Whole numbers are equal."""
 import ctypes
 import os
@@ -241,3 +249,187 @@ def test_route_refuses(ops):
     for call, message in bad:
         with pytest.raises(RuntimeError, match=message):
             call()
+
+
+# ------------------------------------------------------------------ gated expert layer for a few tokens
+
+HANDED_ON = {torch.bfloat16: (2.0 ** -16, 0.0), torch.float16: (2.0 ** -21, 2.0 ** -24)}
+
+
+def _moe_reference(x, w13, w2, experts, weights, trans_b):
+    """The layer in 64 bits, and by how much each element may be off before it is rounded."""
+    t, hidden = x.shape
+    num, ffn = w13.shape[0], w2.shape[2 if trans_b else 1]
+    unit, least = HANDED_ON[x.dtype]
+    out, off = torch.zeros(t, hidden, dtype=torch.float64), torch.zeros(t, hidden, dtype=torch.float64)
+    for i in range(t):
+        for j in range(experts.shape[1]):
+            e, w = int(experts[i, j]), float(weights[i, j])
+            if not 0 <= e < num:
+                continue
+            first, second = w13[e].double(), w2[e].double()
+            if trans_b:
+                first, second = first.t(), second.t()
+            both = x[i].double() @ first
+            err = (x[i].double().abs() @ first.abs()) * (2 * hidden * 2.0 ** -24)
+            gate, up = both[:ffn], both[ffn:]
+            s = torch.sigmoid(gate)
+            h = gate * s * up
+            # (the derivative of silu is at most 1.1)
+            h_off = 1.1 * err[:ffn] * (up.abs() + err[ffn:]) + (gate * s).abs() * err[ffn:] + h.abs() * (unit + 2.0 ** -20) + least
+            out[i] += w * (h @ second)
+            off[i] += abs(w) * ((h_off @ second.abs()) + (h.abs() @ second.abs()) * ((2 * ffn + 64) * 2.0 ** -24))
+    return out, off
+
+
+def _moe_case(t, num, k, hidden, ffn, dtype, trans_b, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, hidden, generator=g).to(dtype)
+    w13 = (torch.randn(num, hidden, 2 * ffn, generator=g) * hidden ** -0.5 * scale).to(dtype)
+    w2 = (torch.randn(num, ffn, hidden, generator=g) * ffn ** -0.5).to(dtype)
+    if trans_b:
+        w13, w2 = w13.transpose(1, 2).contiguous(), w2.transpose(1, 2).contiguous()
+    experts = torch.stack([torch.randperm(num, generator=g)[:k] for _ in range(t)]).to(torch.int32) if t else torch.zeros(0, k, dtype=torch.int32)
+    weights = torch.rand(t, k, generator=g)
+    return x, w13, w2, experts, weights
+
+
+def _check_moe(ops, case, trans_b, what):
+    x, w13, w2, experts, weights = case
+    got = ops.moe_few_tokens(*(v.cuda() for v in case), trans_b=trans_b)
+    assert got.dtype == x.dtype
+    want, off = _moe_reference(x, w13, w2, experts, weights, trans_b)
+    rtol, least = ROUNDING[x.dtype]
+    _close(got, want, rtol, off * (1 + rtol) + least, what)
+    return got
+
+
+# tokens, experts, top_k, hidden, ffn: widths below a lane's, a tile's and a strip's share, depths that end inside a step and before one
+MOE_SHAPES = [(1, 1, 1, 1, 1), (1, 4, 2, 8, 8), (1, 8, 2, 256, 512), (2, 3, 3, 5, 7), (3, 5, 2, 33, 9), (5, 8, 2, 100, 129),
+              (1, 8, 8, 64, 1000), (7, 4, 1, 1021, 67), (16, 6, 3, 72, 200), (17, 2, 2, 130, 96), (33, 3, 2, 257, 65), (64, 4, 3, 95, 71),
+              (64, 130, 8, 40, 33), (64, 1000, 1, 16, 24), (1, 2, 2, 2000, 2049), (4, 8, 2, 129, 1500), (0, 4, 2, 64, 64)]
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", MOE_SHAPES)
+def test_moe_few_tokens_matches_its_definition(ops, shape, dtype, trans_b):
+    _announce("moe few tokens", shape, dtype, trans_b)
+    _check_moe(ops, _moe_case(*shape, dtype, trans_b, seed=sum(shape)), trans_b, f"{shape}")
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_moe_few_tokens_odd_routing(ops, trans_b):
+    """All tokens at one expert, an expert named twice by a token, numbers that name no expert, tokens without any."""
+    for t in (3, 20, 64):
+        case = list(_moe_case(t, 6, 4, 96, 136, torch.bfloat16, trans_b, seed=t))
+        for name, experts in [
+            ("one expert", torch.full((t, 4), 2)),
+            ("none", torch.full((t, 4), -1)),
+            ("past the end", torch.full((t, 4), 6)),
+            ("largest", torch.full((t, 4), 2 ** 31 - 1)),
+            ("some", torch.randint(-2, 8, (t, 4), generator=torch.Generator().manual_seed(t))),
+        ]:
+            _announce("moe odd routing", t, name, trans_b)
+            case[3] = experts.to(torch.int32)
+            got = _check_moe(ops, case, trans_b, name)
+            if name in ("none", "past the end", "largest"):
+                assert (got == 0).all()
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_moe_few_tokens_reads_named_experts_only(ops, trans_b):
+    """NaN in every expert that is not named, and behind every tensor, reaches no output."""
+    x, w13, w2, experts, weights = _moe_case(5, 7, 2, 51, 43, torch.float16, trans_b, seed=3)
+    named = set(experts.flatten().tolist())
+    for e in range(7):
+        if e not in named:
+            w13[e], w2[e] = float("nan"), float("nan")
+
+    def framed(t):   # between NaN, off the 16-byte boundary
+        flat = torch.full((t.numel() + 67,), float("nan"), dtype=t.dtype, device="cuda")
+        flat[33:33 + t.numel()] = t.flatten().cuda()
+        return flat[33:33 + t.numel()].view(t.shape)
+
+    got = ops.moe_few_tokens(framed(x), framed(w13), framed(w2), experts.cuda(), framed(weights), trans_b=trans_b)
+    want, off = _moe_reference(x, w13, w2, experts, weights, trans_b)
+    rtol, least = ROUNDING[x.dtype]
+    _close(got, want, rtol, off * (1 + rtol) + least, "framed")
+
+
+def test_moe_few_tokens_large_values(ops):
+    """Gates far out on both sides: silu underflows to 0 on one and is the gate itself on the other; products past the
+    type's range become infinities, not NaN."""
+    x = torch.tensor([[1.0], [-1.0]], dtype=torch.bfloat16)
+    w13 = torch.tensor([[[200.0, 3.0]], [[2.0 ** 100, 2.0 ** 60]]], dtype=torch.bfloat16)
+    w2 = torch.ones(2, 1, 1, dtype=torch.bfloat16)
+    experts, weights = torch.tensor([[0], [0]], dtype=torch.int32), torch.ones(2, 1)
+    got = ops.moe_few_tokens(*(v.cuda() for v in (x, w13, w2, experts, weights))).cpu()
+    assert float(got[0]) == 600.0 and float(got[1]) == 0.0
+    got = ops.moe_few_tokens(x[:1].cuda(), w13.cuda(), w2.cuda(), experts[:1].cuda() + 1, weights[:1].cuda()).cpu()
+    assert float(got) == INF
+
+
+def test_moe_few_tokens_full_size_on_the_device(ops):
+    """A large layer against 32-bit products on the device, every element (both sum in fp32: 4096 products of either sign,
+    far within a rounding of the type)."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for trans_b, t in ((False, 1), (True, 1), (False, 40), (True, 40)):
+        x = torch.randn(t, 4096, device="cuda", generator=g).bfloat16()
+        w13 = (torch.randn(8, 4096, 2 * 7168, device="cuda", generator=g) * 0.0156).bfloat16()
+        w2 = (torch.randn(8, 7168, 4096, device="cuda", generator=g) * 0.0118).bfloat16()
+        r = ops.route(torch.randn(t, 8, device="cuda", generator=g), 2)
+        both = torch.matmul(x.float(), w13.float())   # (experts, tokens, 2 ffn)
+        gate, up = both.chunk(2, dim=2)
+        y = torch.matmul(torch.nn.functional.silu(gate) * up, w2.float())
+        want = (y[r.experts.long(), torch.arange(t, device="cuda")[:, None]] * r.weights[..., None]).sum(1)
+        if trans_b:
+            w13, w2 = w13.transpose(1, 2).contiguous(), w2.transpose(1, 2).contiguous()
+        _announce("moe full size", trans_b, t)
+        got = ops.moe_few_tokens(x, w13, w2, r.experts, r.weights, trans_b=trans_b)
+        off = (got.float() - want).abs() - (2.0 ** -8 * want.abs() + 1e-4 * want.abs().max())
+        assert float(off.max()) <= 0.0
+
+
+def test_moe_few_tokens_same_bits_on_streams_and_in_graphs(ops):
+    cases = [[v.cuda() for v in _moe_case(t, 8, 2, 512, 4096, torch.bfloat16, True, seed=t)] for t in (1, 24)]
+    want = [ops.moe_few_tokens(*c, trans_b=True) for c in cases]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [ops.moe_few_tokens(*c, trans_b=True) for c in cases]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [ops.moe_few_tokens(*c, trans_b=True) for c in cases]
+    for _ in range(4):
+        for out in captured:
+            out.zero_()
+        graph.replay()
+        eager = [ops.moe_few_tokens(*c, trans_b=True) for c in cases]
+        torch.cuda.synchronize()
+        for one in (again, captured, eager):
+            for a, b in zip(one, want):
+                assert torch.equal(a, b)
+
+
+def test_moe_few_tokens_refuses(ops):
+    x, w13, w2, experts, weights = (v.cuda() for v in _moe_case(2, 4, 2, 32, 48, torch.bfloat16, False, seed=1))
+
+    def call(**kw):
+        a = dict(x=x, w13=w13, w2=w2, experts=experts, weights=weights)
+        a.update(kw)
+        return ops.moe_few_tokens(**a)
+
+    bad = [(dict(x=x.cpu()), "same GPU"), (dict(x=x[0]), "2-d"), (dict(x=x.float()), "bfloat16"), (dict(w13=w13[0]), "3-d"),
+           (dict(w13=w13.half()), "element type"), (dict(w2=w2[:3]), "w2"), (dict(w2=w2[:, :47].contiguous()), "w2"),
+           (dict(w13=w13[:, :, :95].contiguous()), "even"), (dict(w13=w13[:, :31].contiguous()), "contraction"),
+           (dict(experts=experts.long()), "int32"), (dict(experts=experts[:1]), "int32"), (dict(weights=weights.half()), "float32"),
+           (dict(weights=weights[:, :1]), "float32"), (dict(w13=w13.transpose(0, 1).contiguous().transpose(0, 1)), "contiguous"),
+           (dict(x=x.repeat(40, 1), experts=experts.repeat(40, 1), weights=weights.repeat(40, 1)), "at most 64"),
+           (dict(x=x.clone().requires_grad_(True)), "no gradient"), (dict(w2=w2.clone().requires_grad_(True)), "no gradient")]
+    for kw, message in bad:
+        with pytest.raises(RuntimeError, match=message):
+            call(**kw)
+    with torch.no_grad():   # (a model's parameters, in serving)
+        call(w2=w2.clone().requires_grad_(True))
