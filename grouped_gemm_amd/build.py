@@ -67,14 +67,14 @@ def pair_indices():
     return [int(m) for m in re.findall(r"^GG_PAIR\((\d+),", text, flags=re.M)]
 
 
-OPERATORS = ("route_kernels", "few_tokens_kernels")
+OPERATORS = ("route_kernels", "few_tokens_kernels", "adapter_kernels")
 
 
 def build_hip(force=False, jobs=None):
     gemm_headers = [os.path.join(CSRC, f) for f in ("gmm_kernel.hpp", "gmm_generic.hpp", "gmm_variants.hpp",
                                                     "gmm_variants.def", "row_kernels.hpp")]
     # (the operators' headers, and the C ABI's, reach their own units and the API's only)
-    headers = gemm_headers + [os.path.join(CSRC, f) for f in ("operators.hpp", "wave_ops.hpp")]
+    headers = gemm_headers + [os.path.join(CSRC, f) for f in ("operators.hpp", "wave_ops.hpp", "few_rows.hpp")]
     headers.append(os.path.join(ROOT, "include", "grouped_gemm_hip.h"))
     outer = ("gmm_api", "row_kernels") + OPERATORS
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

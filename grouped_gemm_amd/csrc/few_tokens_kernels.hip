@@ -20,48 +20,15 @@
 
 #include <math.h>
 
+#include "few_rows.hpp"
 #include "gmm_kernel.hpp"
 #include "wave_ops.hpp"
 
 namespace gg {
 namespace {
 
-constexpr int kFewWaves = 8;
-constexpr int kFewThreads = kFewWaves * 64;
 constexpr int kFewWords = (int)(kFewMaxExperts / 32);
 static_assert(kFewWords <= 64, "");
-
-// 8 elements on any boundary.
-struct __attribute__((packed, aligned(2))) Packed8 {
-  u32x4 v;
-};
-__device__ __forceinline__ u32x4 load8(const uint16_t* p) { return reinterpret_cast<const Packed8*>(p)->v; }
-
-// Elements k .. k + 7 of a row of `depth`, zeros past its end; reads nothing outside the row.
-__device__ __forceinline__ u32x4 load8_within(const uint16_t* row, int k, int depth) {
-  if (k + 8 <= depth) return load8(row + k);
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (k >= depth) return v;
-  if (depth >= 8) {   // the row's last 8, those before k shifted out
-    const unsigned __int128 last = __builtin_bit_cast(unsigned __int128, load8(row + depth - 8));
-    return __builtin_bit_cast(u32x4, last >> (16 * (k + 8 - depth)));
-  }
-  uint16_t e[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = k + i < depth ? row[k + i] : uint16_t(0);
-  return __builtin_bit_cast(u32x4, e);
-}
-
-template <int DT>
-__device__ __forceinline__ uint16_t round_bits(float v) {
-  if constexpr (DT == kBF16) return __builtin_bit_cast(uint16_t, (__bf16)v);
-  else return __builtin_bit_cast(uint16_t, (_Float16)v);
-}
-template <int DT>
-__device__ __forceinline__ float widen_bits(uint16_t v) {
-  if constexpr (DT == kBF16) return __builtin_bit_cast(float, (uint32_t)v << 16);
-  else return (float)__builtin_bit_cast(_Float16, v);
-}
 
 struct FewParams {
   FewTokensArgs a;
@@ -116,177 +83,9 @@ __device__ __forceinline__ void gather_slots(const FewParams& p, FewSchedule& s,
   __syncthreads();
 }
 
-// One wave's stream: its share of the depth of a strip of weights against up to 16 * MT rows.
-//   NT   four tiles of 16 weight rows, two from `first` and two from `second` on; 64 deep at a time
-//   NN   128 columns, in each lane 8 neighbouring ones; 32 deep at a time
-// PARTS: the rows come as the sum of this many (high, or high and low).
-template <int DT, bool NT, int MT, int PARTS>
-struct Stream {
-  static constexpr int DEPTH = NT ? 64 : 32;      // of a step
-  static constexpr int TILES = NT ? 4 : 8;        // of 16 weight columns
-  static constexpr int XS = NT ? 2 : 1;           // loads of a row per step
-
-  struct Step {
-    u32x4 w[8];
-    u32x4 x[MT][PARTS][XS];
-  };
-
-  const uint16_t *first, *second;   // the same in all lanes: where the strip's columns begin, at depth 0
-  uint32_t at[NT ? 4 : 1];          // this lane's offset from there, in bytes
-  uint32_t pitch;                   // NN: bytes from one row of the depth to the next
-  int width;                        // NN: columns this lane may read, 8 or (of a matrix narrower than 8) fewer
-  const uint16_t* x[PARTS];         // the rows, the same in all lanes,
-  uint32_t row[MT];                 // ... and this lane's of them, as offsets in bytes
-  int depth;
-  f32x4 acc[TILES][MT];
-
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < TILES; ++i)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  __device__ __forceinline__ const uint16_t* lane_row(int p, int k, uint32_t offset) const {
-    return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(x[p] + k) + offset);
-  }
-
-  __device__ __forceinline__ void load(Step& s, int k) const {
-    const int q = (threadIdx.x & 63) >> 4;
-    if constexpr (NT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const char* base = reinterpret_cast<const char*>((i < 2 ? first : second) + k);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8(reinterpret_cast<const uint16_t*>(base + at[i]) + 8 * h);
-      }
-    } else {
-      const char* base = reinterpret_cast<const char*>(first) + (uint64_t)k * pitch;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s.w[i] = load8(reinterpret_cast<const uint16_t*>(base + (uint64_t)i * pitch + at[0]));
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int h = 0; h < XS; ++h) s.x[m][p][h] = load8(lane_row(p, k, row[m] + q * 16 * XS) + 8 * h);
-  }
-
-  // ... where the depth ends inside, or the matrix is narrower than a lane's columns
-  __device__ __forceinline__ void load_within(Step& s, int k) const {
-    const int q = (threadIdx.x & 63) >> 4;
-    if constexpr (NT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint16_t* base = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(i < 2 ? first : second) + at[i]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8_within(base - q * 16, k + q * 16 + 8 * h, depth);
-      }
-    } else {
-      const char* base = reinterpret_cast<const char*>(first) + (uint64_t)k * pitch;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s.w[i] = u32x4{0u, 0u, 0u, 0u};
-        if (k + q * 8 + i < depth) s.w[i] = load8_within(reinterpret_cast<const uint16_t*>(base + (uint64_t)i * pitch + at[0]), 0, width);
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int h = 0; h < XS; ++h) s.x[m][p][h] = load8_within(lane_row(p, 0, row[m]), k + q * 8 * XS + 8 * h, depth);
-  }
-
-  __device__ __forceinline__ void multiply(const Step& s) {
-    if constexpr (NT) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-              acc[i][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, s.w[2 * i + h]), __builtin_bit_cast(bf16x8, s.x[m][p][h]), acc[i][m]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = __builtin_amdgcn_perm(s.w[2 * i + 1][j / 2], s.w[2 * i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p)
-            acc[j][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, s.x[m][p][0]), acc[j][m]);
-      }
-    }
-  }
-
-  // Steps begin .. end - 1 of the depth, every kFewWaves-th of them; two in flight.
-  __device__ __forceinline__ void run(int begin, int end) {
-    const bool narrow = !NT && width < 8;
-    const int whole = narrow ? begin : min(end, depth / DEPTH);   // steps that end inside the depth
-    int step = begin + uniform((int)(threadIdx.x >> 6));
-    Step s0, s1;
-    if (step < whole) load(s0, step * DEPTH);
-    if (step + kFewWaves < whole) load(s1, (step + kFewWaves) * DEPTH);
-    while (step < whole) {
-      multiply(s0);
-      if (step + 2 * kFewWaves < whole) load(s0, (step + 2 * kFewWaves) * DEPTH);
-      step += kFewWaves;
-      if (step >= whole) break;
-      multiply(s1);
-      if (step + 2 * kFewWaves < whole) load(s1, (step + 2 * kFewWaves) * DEPTH);
-      step += kFewWaves;
-    }
-    for (; step < end; step += kFewWaves) {
-      load_within(s0, step * DEPTH);
-      multiply(s0);
-    }
-  }
-};
-
-// The waves' sums through LDS, 4 KiB of each wave at a time: NT its four tiles, NN the first or second 64 of its columns.
-template <bool NT>
-struct Exchange {
-  static constexpr int ROUNDS = NT ? 1 : 2;
-  f32x4* lds;   // [kFewWaves][256]
-
-  template <typename S>
-  __device__ __forceinline__ void put(const S& s, int m, int round) const {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if constexpr (NT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lds[wave * 256 + i * 64 + lane] = s.acc[i][m];
-    } else {
-      if ((lane >> 5) == round)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) lds[wave * 256 + j * 32 + (lane & 31)] = s.acc[j][m];
-    }
-  }
-  // Sum over the waves of weight column `column` (NT: of 64; NN: of 16 blocks of 8 lanes' columns, block i and column j of it) and row `token`
-  __device__ __forceinline__ float get(int item, int r) const {
-    const float* from = reinterpret_cast<const float*>(lds) + item * 4 + r;
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) sum += from[w * 1024];
-    return sum;
-  }
-  __device__ __forceinline__ float column_of_tiles(int column, int token) const {   // NT
-    return get((column >> 4) * 64 + ((column >> 2) & 3) * 16 + token, column & 3);
-  }
-  __device__ __forceinline__ float column_of_block(int block, int j, int token) const {   // NN, block of this round's 8
-    return get(j * 32 + (block >> 2) * 16 + token, block & 3);
-  }
-};
-
 template <int DT, bool NT, int MT>
 __global__ __launch_bounds__(kFewThreads, MT == 1 ? 4 : 2) void few_gate_up_kernel(FewParams p) {
-  using S = Stream<DT, NT, MT, 1>;
+  using S = Stream<DT, NT, 4, MT, 1>;
   constexpr int COLUMNS = NT ? 32 : 64;   // of h
   __shared__ FewSchedule schedule;
   __shared__ f32x4 lds[kFewWaves * 256];
@@ -365,7 +164,7 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 4 : 2) void few_gate_up_kern
 
 template <int DT, bool NT, int MT>
 __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewParams p) {
-  using S = Stream<DT, NT, MT, 2>;
+  using S = Stream<DT, NT, 4, MT, 2>;
   constexpr int COLUMNS = NT ? 64 : 128;
   __shared__ FewSchedule schedule;
   __shared__ f32x4 lds[kFewWaves * 256];

@@ -1200,4 +1200,37 @@ int gg_moe_few_tokens(const void* x, const void* w13, const void* w2, const int3
   return GG_OK;
 }
 
+static int check_lora(int dtype, int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
+  if (dtype != GG_DTYPE_BF16 && dtype != GG_DTYPE_F16) return fail(GG_EINVAL, "dtype must be GG_DTYPE_BF16 or GG_DTYPE_F16");
+  if (rows < 0 || num < 1 || rank < 1 || hidden_in < 1 || hidden_out < 1)
+    return fail(GG_EINVAL, "rows must not be negative, adapters, rank and hidden sizes at least 1");
+  if (rank > GG_LORA_MAX_RANK) return fail(GG_ELIMIT, "rank must be at most %d", GG_LORA_MAX_RANK);
+  if (rows >= (int64_t(1) << 31) || num >= (int64_t(1) << 31)) return fail(GG_ELIMIT, "rows and adapters must be below 2^31");
+  if (hidden_in >= (1 << 22) || hidden_out >= (1 << 22)) return fail(GG_ELIMIT, "hidden sizes must be below 2^22");
+  if (rows > 0 && !gg::adapters_fit(rows, num, rank, hidden_in, hidden_out)) return fail(GG_ELIMIT, "rows times hidden sizes are too large for one launch");
+  return GG_OK;
+}
+
+uint64_t gg_lora_scratch_bytes(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
+  if (check_lora(GG_DTYPE_BF16, rows, num, rank, hidden_in, hidden_out) != GG_OK || rows == 0) return 0;
+  return gg::adapters_scratch_bytes(rows, num, rank, hidden_in, hidden_out);
+}
+
+int gg_lora(const void* x, const void* a, const void* b, const int32_t* adapters, const float* scales, const void* base, void* out,
+            int dtype, int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out, void* scratch, void* stream) {
+  const int rc = check_lora(dtype, rows, num, rank, hidden_in, hidden_out);
+  if (rc != GG_OK) return rc;
+  if (rows == 0) return GG_OK;
+  if (x == nullptr || a == nullptr || b == nullptr || adapters == nullptr || out == nullptr || scratch == nullptr)
+    return fail(GG_EINVAL, "x, a, b, adapters, out or scratch is null");
+  if (reinterpret_cast<uintptr_t>(scratch) & 15) return fail(GG_ELIMIT, "scratch must be on a 16-byte boundary");
+  DeviceInfo info;
+  const int init = device_info(&info);
+  if (init != GG_OK) return init;
+  const gg::AdapterArgs args = {x, a, b, adapters, scales, base, out, scratch, dtype, rows, (int32_t)num, (int32_t)rank,
+                                (int32_t)hidden_in, (int32_t)hidden_out};
+  GG_HIP(gg::adapters(args, static_cast<hipStream_t>(stream)));
+  return GG_OK;
+}
+
 }  // extern "C"

@@ -64,4 +64,24 @@ bool few_tokens_fits(int64_t tokens, int64_t experts, int64_t top_k, int64_t hid
 uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b);
 hipError_t few_tokens(const FewTokensArgs& args, hipStream_t stream);
 
+constexpr int64_t kAdapterMaxRank = 256;
+
+struct AdapterArgs {
+  const void* x;             // (rows, hidden_in), element type dt (kBF16, kF16)
+  const void* a;             // (num, rank, hidden_in)
+  const void* b;             // (num, hidden_out, rank)
+  const int32_t* adapters;   // (rows)
+  const float* scales;       // (num) or null: 1
+  const void* base;          // (rows, hidden_out) or null: 0
+  void* out;                 // (rows, hidden_out), may be base
+  void* scratch;             // adapters_scratch_bytes, 16-byte aligned, any contents
+  int dt;
+  int64_t rows;
+  int32_t num, rank, hidden_in, hidden_out;
+};
+// Whether 32 bits hold the thread counts of such a call.
+bool adapters_fit(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out);
+uint64_t adapters_scratch_bytes(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out);
+hipError_t adapters(const AdapterArgs& args, hipStream_t stream);
+
 }  // namespace gg

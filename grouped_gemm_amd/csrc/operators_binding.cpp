@@ -159,12 +159,65 @@ torch::Tensor MoeFewTokens(const torch::Tensor& x, const torch::Tensor& w13, con
   return out;
 }
 
+// ------------------------------------------------------------------ low-rank adapters
+
+bool Overlap(const torch::Tensor& t, const torch::Tensor& u) {
+  const auto begin = [](const torch::Tensor& v) { return reinterpret_cast<uintptr_t>(v.data_ptr()); };
+  return begin(t) < begin(u) + u.nbytes() && begin(u) < begin(t) + t.nbytes();
+}
+
+torch::Tensor Lora(const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& adapters,
+                   const c10::optional<torch::Tensor>& base, const c10::optional<torch::Tensor>& scales,
+                   const c10::optional<torch::Tensor>& c) {
+  TORCH_CHECK(x.dim() == 2, "grouped_gemm: x must be 2-d (rows, hidden_in)");
+  TORCH_CHECK(IsTwoByte(x), "grouped_gemm: x must be bfloat16 or float16");
+  TORCH_CHECK(a.dim() == 3 && b.dim() == 3, "grouped_gemm: a and b must be 3-d");
+  TORCH_CHECK(a.scalar_type() == x.scalar_type() && b.scalar_type() == x.scalar_type(),
+              "grouped_gemm: a and b must have the element type of x");
+  const int64_t rows = x.size(0), num = a.size(0), rank = a.size(1), hidden_in = x.size(1), hidden_out = b.size(1);
+  TORCH_CHECK(a.size(2) == hidden_in, "grouped_gemm: a must be (adapters, rank, hidden_in)");
+  TORCH_CHECK(b.size(0) == num && b.size(2) == rank, "grouped_gemm: b must be (adapters, hidden_out, rank)");
+  TORCH_CHECK(rank <= GG_LORA_MAX_RANK, "grouped_gemm: a rank of at most ", GG_LORA_MAX_RANK);
+  TORCH_CHECK(adapters.dim() == 1 && adapters.size(0) == rows && adapters.scalar_type() == torch::kInt32,
+              "grouped_gemm: adapters must be int32, one number per row of x");
+  if (scales.has_value())
+    TORCH_CHECK(scales->dim() == 1 && scales->size(0) == num && scales->scalar_type() == torch::kFloat32,
+                "grouped_gemm: scales must be float32, one per adapter");
+  torch::Tensor none;
+  const torch::Tensor &from = base.has_value() ? *base : none, &scale = scales.has_value() ? *scales : none, &to = c.has_value() ? *c : none;
+  for (const torch::Tensor* t : {&from, &to})
+    TORCH_CHECK(!t->defined() || (t->dim() == 2 && t->size(0) == rows && t->size(1) == hidden_out && t->scalar_type() == x.scalar_type()),
+                "grouped_gemm: base and c must be (rows, hidden_out), of the element type of x");
+  for (const torch::Tensor* t : {&x, &a, &b, &adapters, &from, &scale, &to})
+    TORCH_CHECK(!t->defined() || t->is_contiguous(), "grouped_gemm: x, a, b, adapters, base, scales and c must be contiguous");
+  for (const torch::Tensor* t : {&x, &a, &b, &adapters, &from, &scale, &to})
+    TORCH_CHECK(!t->defined() || (t->is_cuda() && t->device() == x.device()),
+                "grouped_gemm: x, a, b, adapters, base, scales and c must be on the same GPU");
+  RefuseGradients({&x, &a, &b, &from, &scale, &to}, "lora", "train adapters through gmm, on rows sorted by adapter");
+  if (to.defined()) {
+    for (const torch::Tensor* t : {&x, &a, &b, &adapters, &scale})
+      TORCH_CHECK(!t->defined() || !Overlap(*t, to), "grouped_gemm: c must not overlap x, a, b, adapters or scales");
+    TORCH_CHECK(!from.defined() || from.data_ptr() == to.data_ptr() || !Overlap(from, to), "grouped_gemm: c must be base or not overlap it");
+  }
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  torch::Tensor out = to.defined() ? to : torch::empty({rows, hidden_out}, x.options().requires_grad(false));
+  if (rows == 0) return out;
+  const torch::Tensor scratch = Scratch(gg_lora_scratch_bytes(rows, num, rank, hidden_in, hidden_out), out);
+  const int rc = gg_lora(x.data_ptr(), a.data_ptr(), b.data_ptr(), adapters.data_ptr<int32_t>(), static_cast<const float*>(Pointer(scale)),
+                         Pointer(from), out.data_ptr(), x.scalar_type() == torch::kFloat16 ? GG_DTYPE_F16 : GG_DTYPE_BF16, rows, num, rank,
+                         hidden_in, hidden_out, Pointer(scratch), CurrentStream(x.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return out;
+}
+
 }  // namespace
 
 void RegisterOperators(pybind11::module_& m) {
   m.def("route", &Route, "weights, chosen experts, batch_sizes, row_index, order and mass of router logits.");
   m.def("moe_few_tokens", &MoeFewTokens, "A gated expert layer for a few tokens.");
   m.attr("moe_few_tokens_max") = GG_FEW_TOKENS_MAX;
+  m.def("lora", &Lora, "base + scale * (x @ a^T) @ b^T, with the adapter of each row.");
+  m.attr("lora_max_rank") = GG_LORA_MAX_RANK;
   m.attr("route_max_experts") = GG_ROUTE_MAX_EXPERTS;
   m.attr("route_max_top_k") = GG_ROUTE_MAX_TOP_K;
 }

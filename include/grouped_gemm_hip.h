@@ -400,6 +400,25 @@ int gg_moe_few_tokens(const void* x, const void* w13, const void* w2, const int3
                       void* scratch, void* stream);
 
 /*
+ * Low-rank adapters of many requests beside a shared projection: with l = adapters[t],
+ * out[t] = base[t] + scales[l] * (x[t] @ a[l]^T) @ b[l]^T.
+ *   x (rows, hidden_in), base and out (rows, hidden_out), element type dtype (GG_DTYPE_BF16 or GG_DTYPE_F16)
+ *   a (num, rank, hidden_in), b (num, hidden_out, rank): each adapter's two matrices stored (out, in)
+ *   adapters int32 (rows); a number that names no adapter leaves the row as it is in base
+ *   scales fp32 (num) or NULL (1); base NULL: 0
+ * all contiguous, aligned to their elements; out may be base (in place) and overlaps nothing else.  Rows may come in any order; rows of one
+ * request are best neighbours (rows are taken in windows of 64).  Sums are in fp32, x @ a^T is handed on with twice the bits of the type, the result
+ * is rounded once.  The same bits on every call.
+ * rank at most GG_LORA_MAX_RANK (smaller ranks beside larger ones: zeros), hidden sizes below 2^22.  `scratch`: gg_lora_scratch_bytes of device
+ * memory, 16-byte aligned, of any contents; calls that share it must not overlap in time.
+ * No counterpart in the reference, whose groups are consecutive rows of one matrix each (csrc/grouped_gemm.h:5-9).
+ */
+#define GG_LORA_MAX_RANK 256
+uint64_t gg_lora_scratch_bytes(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out);
+int gg_lora(const void* x, const void* a, const void* b, const int32_t* adapters, const float* scales, const void* base, void* out,
+            int dtype, int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out, void* scratch, void* stream);
+
+/*
  * Runs only the on-device scheduler of gg_gmm_bf16 (same device code, same
  * arguments) and writes what it derived to `table_out`, a device buffer of
  * num_groups * GG_SCHED_COLS int64: per group the problem (m, n, k), leading

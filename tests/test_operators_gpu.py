@@ -1,5 +1,5 @@
 """The operators around the grouped GEMM against their definitions in 64 bits, on the CPU: the router, the gated expert
-layer for a few tokens.
+layer for a few tokens, low-rank adapters.
 
 Tolerances follow from how results are computed.  The router works in fp32: exp(x - top) is off by up to 2^-24 |x - top|
 from the rounding of its argument and two units in the last place of its own, a sum over at most 1024 positive terms
@@ -433,3 +433,183 @@ def test_moe_few_tokens_refuses(ops):
             call(**kw)
     with torch.no_grad():   # (a model's parameters, in serving)
         call(w2=w2.clone().requires_grad_(True))
+
+
+# ------------------------------------------------------------------ low-rank adapters
+
+def _lora_reference(x, a, b, adapters, base, scales):
+    """The adapters in 64 bits, and by how much each element may be off before it is rounded."""
+    rows, hin = x.shape
+    num, r, hout = a.shape[0], a.shape[1], b.shape[1]
+    unit, least = HANDED_ON[x.dtype]
+    out = base.double().clone() if base is not None else torch.zeros(rows, hout, dtype=torch.float64)
+    off = torch.zeros(rows, hout, dtype=torch.float64)
+    for n in range(num):
+        at = torch.nonzero(adapters == n).squeeze(1)
+        if at.numel() == 0:
+            continue
+        xs, an, bn = x[at].double(), a[n].double(), b[n].double()
+        s = float(scales[n]) if scales is not None else 1.0
+        v = xs @ an.t()
+        # (float16's v is scaled to below 1, so that its lower half stays in range: relative to the row's largest)
+        v_off = (xs.abs() @ an.abs().t()) * (2 * hin * 2.0 ** -24) + v.abs() * unit + v.abs().amax(1, keepdim=True) * least
+        out[at] += s * (v @ bn.t())
+        off[at] += abs(s) * (v_off @ bn.abs().t() + (v.abs() @ bn.abs().t()) * ((4 * r + 8) * 2.0 ** -24))
+        off[at] += out[at].abs() * 2.0 ** -23
+    return out, off
+
+
+def _lora_case(rows, num, r, hin, hout, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, hin, generator=g).to(dtype)
+    a = (torch.randn(num, r, hin, generator=g) * hin ** -0.5).to(dtype)
+    b = (torch.randn(num, hout, r, generator=g) * r ** -0.5).to(dtype)
+    base = torch.randn(rows, hout, generator=g).to(dtype)
+    scales = torch.rand(num, generator=g) * 2 - 1
+    adapters = torch.randint(-1, num, (rows,), generator=g).to(torch.int32)
+    return x, a, b, adapters, base, scales
+
+
+def _check_lora(ops, case, what):
+    x, a, b, adapters, base, scales = case
+    cuda = [v.cuda() if v is not None else None for v in case]
+    got = ops.lora(cuda[0], cuda[1], cuda[2], cuda[3], base=cuda[4], scales=cuda[5])
+    assert got.dtype == x.dtype
+    want, off = _lora_reference(*case)
+    rtol, least = ROUNDING[x.dtype]
+    _close(got, want, rtol, off * (1 + rtol) + least, what)
+    untouched = ~((adapters >= 0) & (adapters < a.shape[0]))
+    if base is not None:
+        assert torch.equal(got.cpu()[untouched], base[untouched]), what
+    else:
+        assert (got.cpu()[untouched] == 0).all(), what
+    return got
+
+
+# rows, adapters, rank, hidden_in, hidden_out: parts of a window, of a tile, of a strip, of a step; several of each
+LORA_SHAPES = [(0, 2, 8, 16, 16), (1, 1, 1, 1, 1), (1, 3, 16, 64, 256), (2, 2, 3, 5, 7), (5, 40, 8, 130, 300), (17, 2, 11, 257, 67),
+               (64, 64, 16, 512, 200), (65, 1, 33, 100, 1030), (100, 5, 64, 1021, 129), (130, 3, 100, 72, 511), (200, 7, 256, 65, 90),
+               (70, 300, 4, 640, 64), (1, 2, 65, 4096, 515), (400, 2, 16, 3000, 48), (1025, 9, 17, 63, 33)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", LORA_SHAPES)
+def test_lora_matches_its_definition(ops, shape, dtype):
+    _announce("lora", shape, dtype)
+    _check_lora(ops, _lora_case(*shape, dtype, seed=sum(shape)), f"{shape}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lora_rows_in_any_order(ops, dtype):
+    """Prompts (runs of one adapter), one adapter for all, none for any, every row another, numbers that name none."""
+    rows, num = 150, 150
+    x, a, b, _, base, scales = _lora_case(rows, num, 20, 88, 140, dtype, seed=9)
+    g = torch.Generator().manual_seed(1)
+    for name, adapters in [
+        ("runs", torch.arange(rows) // 37), ("one", torch.full((rows,), 149)), ("none", torch.full((rows,), -1)),
+        ("all different", torch.randperm(num, generator=g)), ("past the end", torch.full((rows,), num)),
+        ("far out", torch.where(torch.arange(rows) % 3 == 0, 2 ** 31 - 1, -2 ** 31)), ("two in turn", torch.arange(rows) % 2),
+    ]:
+        for with_base, with_scales in ((True, True), (False, True), (True, False)):
+            _announce("lora order", dtype, name, with_base, with_scales)
+            _check_lora(ops, (x, a, b, adapters.to(torch.int32), base if with_base else None, scales if with_scales else None), name)
+
+
+def test_lora_in_place_and_into_a_given_tensor(ops):
+    case = [v.cuda() for v in _lora_case(90, 4, 12, 65, 333, torch.bfloat16, seed=4)]
+    x, a, b, adapters, base, scales = case
+    want = ops.lora(x, a, b, adapters, base=base, scales=scales)
+    c = torch.full_like(base, float("nan"))
+    assert ops.lora(x, a, b, adapters, base=base, scales=scales, c=c) is c and torch.equal(c, want)
+    again = base.clone()
+    ops.lora(x, a, b, adapters, base=again, scales=scales, c=again)
+    assert torch.equal(again, want)
+
+
+def test_lora_reads_named_adapters_only(ops):
+    """NaN in adapters that no row names, and around every tensor (off the 16-byte boundary), reaches no output."""
+    x, a, b, adapters, base, scales = _lora_case(40, 6, 13, 51, 77, torch.float16, seed=2)
+    adapters = torch.where(adapters == 3, -1, adapters)
+    a[3], b[3], scales[3] = float("nan"), float("nan"), float("nan")
+
+    def framed(t):
+        flat = torch.full((t.numel() + 67,), float("nan"), dtype=t.dtype, device="cuda")
+        flat[33:33 + t.numel()] = t.flatten().cuda()
+        return flat[33:33 + t.numel()].view(t.shape)
+
+    c = framed(torch.zeros_like(base))
+    got = ops.lora(framed(x), framed(a), framed(b), adapters.cuda(), base=framed(base), scales=framed(scales), c=c)
+    rtol, least = ROUNDING[x.dtype]
+    a[3], b[3], scales[3] = 0, 0, 0
+    want, off = _lora_reference(x, a, b, adapters, base, scales)
+    _close(got, want, rtol, off * (1 + rtol) + least, "framed")
+    assert torch.isnan(c._base[:33]).all() and torch.isnan(c._base[33 + c.numel():]).all()
+
+
+def test_lora_large_and_small_values(ops):
+    """What lies between the two products may be larger than float16 holds, or far smaller; an infinite row stays one."""
+    x = torch.full((3, 64), 1000.0, dtype=torch.float16)
+    x[1] = 2.0 ** -20
+    a = torch.full((1, 8, 64), 1000.0, dtype=torch.float16)           # v = 6.4e7, far past 65504
+    b = torch.full((1, 40, 8), 2.0 ** -20, dtype=torch.float16)
+    adapters, base = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 40, dtype=torch.float16)
+    scales = torch.ones(1)
+    _check_lora(ops, (x, a, b, adapters, base, scales), "large v")
+    x[2, 5] = INF
+    got = ops.lora(x.cuda(), a.cuda(), b.cuda(), adapters.cuda(), base=base.cuda()).cpu()
+    assert torch.isinf(got[2]).all() and torch.isfinite(got[:2]).all()
+    small = torch.full((1, 8, 64), 2.0 ** -24, dtype=torch.float16)
+    _check_lora(ops, (x[:2], small, torch.full((1, 40, 8), 1000.0, dtype=torch.float16), adapters[:2], base[:2], scales), "small v")
+
+
+def test_lora_same_bits_on_streams_and_in_graphs(ops):
+    cases = [[v.cuda() for v in _lora_case(t, 12, 16, 1024, 777, torch.bfloat16, seed=t)] for t in (1, 64, 300)]
+
+    def run():
+        return [ops.lora(x, a, b, adapters, base=base, scales=scales) for x, a, b, adapters, base, scales in cases]
+
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for _ in range(4):
+        for out in captured:
+            out.zero_()
+        graph.replay()
+        eager = run()
+        torch.cuda.synchronize()
+        for one in (again, captured, eager):
+            for got, w in zip(one, want):
+                assert torch.equal(got, w)
+
+
+def test_lora_refuses(ops):
+    x, a, b, adapters, base, scales = (v.cuda() for v in _lora_case(6, 3, 8, 32, 48, torch.bfloat16, seed=1))
+
+    def call(**kw):
+        args = dict(x=x, a=a, b=b, adapters=adapters, base=base, scales=scales)
+        args.update(kw)
+        return ops.lora(**args)
+
+    bad = [(dict(x=x.cpu()), "same GPU"), (dict(x=x[0]), "2-d"), (dict(x=x.float()), "bfloat16"), (dict(a=a[0]), "3-d"),
+           (dict(a=a.half()), "element type"), (dict(a=a[:, :, :31].contiguous()), "hidden_in"), (dict(b=b[:2]), "hidden_out"),
+           (dict(b=b[:, :, :7].contiguous()), "rank"), (dict(adapters=adapters.long()), "int32"), (dict(adapters=adapters[:5]), "int32"),
+           (dict(scales=scales[:2]), "float32"), (dict(scales=scales.half()), "float32"), (dict(base=base[:, :47]), "hidden_out"),
+           (dict(base=base.half()), "element type"), (dict(x=torch.zeros(32, 6, device="cuda", dtype=x.dtype).t()), "contiguous"),
+           (dict(c=base[:5]), "hidden_out"), (dict(a=torch.zeros(1, 257, 32, device="cuda", dtype=x.dtype),
+                                                   b=torch.zeros(1, 48, 257, device="cuda", dtype=x.dtype), scales=None), "at most 256"),
+           (dict(a=a.clone().requires_grad_(True)), "no gradient"), (dict(base=base.clone().requires_grad_(True)), "no gradient")]
+    for kw, message in bad:
+        with pytest.raises(RuntimeError, match=message):
+            call(**kw)
+    both = torch.zeros(7 * 48, device="cuda", dtype=x.dtype)
+    with pytest.raises(RuntimeError, match="overlap"):
+        call(base=both[:288].view(6, 48), c=both[48:].view(6, 48))
+    square = [v.cuda() for v in _lora_case(6, 3, 8, 48, 48, torch.bfloat16, seed=1)]
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.lora(square[0], square[1], square[2], square[3], c=square[0])
