@@ -66,7 +66,7 @@ struct Window {
 // v of one piece of the depth.  TILES: of 16 rows of a_l; more than 64 of them are taken 64 at a time.
 template <int DT, int TILES, int MT>
 __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterParams p) {
-  using S = Stream<DT, true, TILES, MT, 1>;
+  using S = Stream<DT, true, TILES, MT>;
   __shared__ f32x4 lds[kFewWaves * 256];
   const AdapterArgs& a = p.a;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
   S s;
   s.depth = a.hidden_in;
   s.width = 8;
-  s.x[0] = static_cast<const uint16_t*>(a.x) + (uint64_t)first * a.hidden_in;
+  s.x = static_cast<const uint16_t*>(a.x) + (uint64_t)first * a.hidden_in;
   const Exchange<true> exchange{lds};
   for (int turn = 0; w.left != 0; turn = turn + 1 == p.splits ? 0 : turn + 1) {
     int which;
@@ -95,9 +95,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
       for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          s.row[m] = (uint32_t)__shfl(list, min(row0 + 16 * m + c, rows - 1)) * (uint32_t)a.hidden_in * 2;
-        s.clear();
-        s.run(begin, end);
+          s.set_row(m, (uint32_t)__shfl(list, min(row0 + 16 * m + c, rows - 1)) * (uint32_t)a.hidden_in * 2);
+        s.prepare(begin, end);
+        s.run(end);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           if (row0 + 16 * m >= rows) break;
@@ -105,8 +105,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
           exchange.put(s, m, 0);
           __syncthreads();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int item = half * kFewThreads + threadIdx.x, token = item / (16 * TILES), n = item % (16 * TILES);
+          for (int turn_of = 0; turn_of < 1024 / kFewThreads; ++turn_of) {
+            const int item = turn_of * kFewThreads + threadIdx.x, token = item / (16 * TILES), n = item % (16 * TILES);
             const int row = row0 + 16 * m + token, from = __shfl(list, row & 63);
             if (token < 16 && row < rows && r0 + n < a.rank)
               v[(uint64_t)(first + from) * p.v_pitch + r0 + n] = exchange.column_of_tiles(n, token);

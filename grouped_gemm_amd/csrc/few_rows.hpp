@@ -9,7 +9,7 @@
 namespace gg {
 
 // Waves of a workgroup, which take the depth in turns.
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 4;
 constexpr int kFewThreads = kFewWaves * 64;
 
 // 8 elements on any boundary.
@@ -18,6 +18,15 @@ struct __attribute__((packed, aligned(2))) Packed8 {
 };
 __device__ __forceinline__ u32x4 load8(const uint16_t* p) { return reinterpret_cast<const Packed8*>(p)->v; }
 
+// ... at a base that all lanes share, and an offset of each in bytes.  The empty asm hides where the two come from: without it the compiler
+// keeps one 64-bit address per load in vector registers from step to step.
+__device__ __forceinline__ u32x4 load8_at(const void* base, uint32_t offset, int further = 0) {
+  using Bytes = const __attribute__((address_space(1))) char*;
+  using Eight = const __attribute__((address_space(1))) Packed8*;
+  uint64_t at = (uint64_t)uniform_ptr(static_cast<const char*>(base));
+  asm("" : "+s"(at), "+v"(offset));
+  return ((Eight)((Bytes)at + offset + further))->v;
+}
 __device__ __forceinline__ void store8(uint16_t* p, u32x4 v) { reinterpret_cast<Packed8*>(p)->v = v; }
 
 // Elements k .. k + 7 of a row of `depth`, zeros past its end; reads nothing outside the row.
@@ -49,8 +58,7 @@ __device__ __forceinline__ float widen_bits(uint16_t v) {
 // One wave's stream: its share of the depth of a strip of weights against up to 16 * MT rows.
 //   NT   tiles of 16 weight rows, the first half of them from `first` and the others from `second` on; 64 deep at a time
 //   NN   128 columns, in each lane 8 neighbouring ones; 32 deep at a time
-// PARTS: the rows come as the sum of this many (high, or high and low).
-template <int DT, bool NT, int NT_TILES, int MT, int PARTS>
+template <int DT, bool NT, int NT_TILES, int MT>
 struct Stream {
   static constexpr int DEPTH = NT ? 64 : 32;      // of a step
   static constexpr int TILES = NT ? NT_TILES : 8;        // of 16 weight columns
@@ -58,15 +66,15 @@ struct Stream {
 
   struct Step {
     u32x4 w[NT ? 2 * TILES : 8];
-    u32x4 x[MT][PARTS][XS];
+    u32x4 x[MT][XS];
   };
 
   const uint16_t *first, *second;   // the same in all lanes: where the strip's columns begin, at depth 0
   uint32_t at[NT ? TILES : 1];          // this lane's offset from there, in bytes
   uint32_t pitch;                   // NN: bytes from one row of the depth to the next
   int width;                        // NN: columns this lane may read, 8 or (of a matrix narrower than 8) fewer
-  const uint16_t* x[PARTS];         // the rows, the same in all lanes,
-  uint32_t row[MT];                 // ... and this lane's of them, as offsets in bytes
+  const uint16_t* x;                // the rows, the same in all lanes,
+  uint32_t row[MT];                 // ... and where in them this lane's step 0 begins, in bytes (set_row)
   int depth;
   f32x4 acc[TILES][MT];
 
@@ -77,30 +85,26 @@ struct Stream {
       for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  __device__ __forceinline__ const uint16_t* lane_row(int p, int k, uint32_t offset) const {
-    return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(x[p] + k) + offset);
-  }
+  // the lane's row of tile m begins `offset` bytes into x
+  __device__ __forceinline__ void set_row(int m, uint32_t offset) { row[m] = offset + ((threadIdx.x & 63) >> 4) * 16 * XS; }
 
-  __device__ __forceinline__ void load(Step& s, int k) const {
-    const int q = (threadIdx.x & 63) >> 4;
+  __device__ __forceinline__ void load_weights(Step& s, int k) const {
     if constexpr (NT) {
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) {
-        const char* base = reinterpret_cast<const char*>((2 * i < TILES ? first : second) + k);
+      for (int i = 0; i < TILES; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8(reinterpret_cast<const uint16_t*>(base + at[i]) + 8 * h);
-      }
+        for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8_at((2 * i < TILES ? first : second) + k, at[i], 16 * h);
     } else {
       const char* base = reinterpret_cast<const char*>(first) + (uint64_t)k * pitch;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s.w[i] = load8(reinterpret_cast<const uint16_t*>(base + (uint64_t)i * pitch + at[0]));
+      for (int i = 0; i < 8; ++i) s.w[i] = load8_at(base + (uint64_t)i * pitch, at[0]);
     }
+  }
+  __device__ __forceinline__ void load_rows(Step& s, int k) const {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int h = 0; h < XS; ++h) s.x[m][p][h] = load8(lane_row(p, k, row[m] + q * 16 * XS) + 8 * h);
+      for (int h = 0; h < XS; ++h) s.x[m][h] = load8_at(x + k, row[m], 16 * h);
   }
 
   // ... where the depth ends inside, or the matrix is narrower than a lane's columns
@@ -124,9 +128,7 @@ struct Stream {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int h = 0; h < XS; ++h) s.x[m][p][h] = load8_within(lane_row(p, 0, row[m]), k + q * 8 * XS + 8 * h, depth);
+      for (int h = 0; h < XS; ++h) s.x[m][h] = load8_within(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(x) + row[m]) - q * 8 * XS, k + q * 8 * XS + 8 * h, depth);
   }
 
   __device__ __forceinline__ void multiply(const Step& s) {
@@ -137,9 +139,7 @@ struct Stream {
         for (int i = 0; i < TILES; ++i)
 #pragma unroll
           for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-              acc[i][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, s.w[2 * i + h]), __builtin_bit_cast(bf16x8, s.x[m][p][h]), acc[i][m]);
+            acc[i][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, s.w[2 * i + h]), __builtin_bit_cast(bf16x8, s.x[m][h]), acc[i][m]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -149,29 +149,62 @@ struct Stream {
           w[i] = __builtin_amdgcn_perm(s.w[2 * i + 1][j / 2], s.w[2 * i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p)
-            acc[j][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, s.x[m][p][0]), acc[j][m]);
+          acc[j][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, s.x[m][0]), acc[j][m]);
       }
     }
   }
 
-  // Steps begin .. end - 1 of the depth, every kFewWaves-th of them; two in flight.
-  __device__ __forceinline__ void run(int begin, int end) {
+  // Steps begin .. end - 1 of the depth, every kFewWaves-th of them, two in flight.  The first two steps' weights are asked for by
+  // prepare(), which needs neither `row` nor `x`: whose rows they meet may still have to be found out.
+  Step s0, s1;
+  int step, whole;   // the wave's next step, and the end of those that lie inside the depth
+
+  __device__ __forceinline__ void prepare(int begin, int end) {
     const bool narrow = !NT && width < 8;
-    const int whole = narrow ? begin : min(end, depth / DEPTH);   // steps that end inside the depth
-    int step = begin + uniform((int)(threadIdx.x >> 6));
-    Step s0, s1;
-    if (step < whole) load(s0, step * DEPTH);
-    if (step + kFewWaves < whole) load(s1, (step + kFewWaves) * DEPTH);
-    while (step < whole) {
+    whole = narrow ? begin : min(end, depth / DEPTH);
+    step = begin + uniform((int)(threadIdx.x >> 6));
+    if (step < whole) load_weights(s0, step * DEPTH);
+    if (step + kFewWaves < whole) load_weights(s1, (step + kFewWaves) * DEPTH);
+  }
+  // multiply, then ask for what comes two of the wave's steps later
+  __device__ __forceinline__ void advance(Step& s) {
+    multiply(s);
+    __builtin_amdgcn_sched_barrier(0);   // (steps do not mix: their registers would not suffice)
+    load_weights(s, (step + 2 * kFewWaves) * DEPTH);
+    load_rows(s, (step + 2 * kFewWaves) * DEPTH);
+    step += kFewWaves;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ void run(int end) {
+    clear();
+    if (step < whole) load_rows(s0, step * DEPTH);
+    if (step + kFewWaves < whole) load_rows(s1, (step + kFewWaves) * DEPTH);
+    // (the loop's loads are under no condition of their own, and its first turn, whose loads came in another order, is
+    // outside it: the compiler then waits for a step's own loads only, not for all)
+    if (step + 3 * kFewWaves < whole) {
+      advance(s0);
+      advance(s1);
+      while (step + 3 * kFewWaves < whole) {
+        advance(s0);
+        advance(s1);
+      }
+    }
+    if (step < whole) {   // one to three steps are left, two of them loaded
+      const bool third = step + 2 * kFewWaves < whole;
       multiply(s0);
-      if (step + 2 * kFewWaves < whole) load(s0, (step + 2 * kFewWaves) * DEPTH);
+      if (third) {
+        load_weights(s0, (step + 2 * kFewWaves) * DEPTH);
+        load_rows(s0, (step + 2 * kFewWaves) * DEPTH);
+      }
       step += kFewWaves;
-      if (step >= whole) break;
-      multiply(s1);
-      if (step + 2 * kFewWaves < whole) load(s1, (step + 2 * kFewWaves) * DEPTH);
-      step += kFewWaves;
+      if (step < whole) {
+        multiply(s1);
+        step += kFewWaves;
+      }
+      if (third) {
+        multiply(s0);
+        step += kFewWaves;
+      }
     }
     for (; step < end; step += kFewWaves) {
       load_within(s0, step * DEPTH);

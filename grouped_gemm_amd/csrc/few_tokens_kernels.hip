@@ -36,71 +36,98 @@ struct FewParams {
   int32_t tiles;         // strips of this kernel
   int32_t pieces;        // of the depth of down
   int32_t counters;      // arrivals to clear for the second kernel
-  int32_t ffn_pitch;     // elements from one row of high (and low) to the next
+  int32_t ffn_pitch;     // elements from one row of h to the next
   int32_t* arrivals;     // [strips of down]
-  uint16_t* high;        // [slots][ffn_pitch] h rounded to the element type,
-  uint16_t* low;         // ... and what the rounding left: h is handed on with twice the bits of the type
+  uint16_t* h;           // [slots][2][ffn_pitch] h rounded to the element type, and what the rounding left: two rows for
+                         // the second product, which is then exact to twice the bits of the type
   float* parts;          // [pieces][slots][hidden]
 };
 
-// Which experts are named, and the slots of one of them.
-struct FewSchedule {
+// Which experts are named, and the slots of one of them (in any order: a token's results do not depend on its place).  Up to 64
+// slots every wave finds the expert by itself, from one load and a ballot for each; more go through LDS.
+struct FewLds {
   uint32_t named[kFewWords];
   int32_t rows;
-  int32_t expert;
   int32_t slot[kFewMaxSlots];
 };
 
-// All threads; the number of experts that are named.  Experts out of range are not.
-__device__ __forceinline__ int find_named(const FewParams& p, FewSchedule& s) {
-  if (threadIdx.x < kFewWords) s.named[threadIdx.x] = 0;
-  if (threadIdx.x == 0) s.rows = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.slots; i += kFewThreads) {
-    const uint32_t e = (uint32_t)p.a.chosen[i];
-    if (e < (uint32_t)p.a.experts) atomicOr(&s.named[e / 32], 1u << (e % 32));
-  }
-  __syncthreads();
+__device__ __forceinline__ int first_lane(uint64_t mask) { return __ffsll((unsigned long long)mask) - 1; }
+__device__ __forceinline__ bool few_slots(const FewParams& p) { return p.slots <= 64; }
+
+// All threads.  Returns the number of experts that are named; `mine` is for find_expert and gather_slots.
+__device__ __forceinline__ int find_named(const FewParams& p, FewLds& lds, int& mine) {
   const int lane = threadIdx.x & 63;
-  return __shfl(wave_prefix(lane < kFewWords ? __popc(s.named[lane]) : 0), 63);
+  int named = 0;
+  mine = -1;
+  if (few_slots(p)) {
+    if (lane < p.slots) mine = p.a.chosen[lane];
+    if ((uint32_t)mine >= (uint32_t)p.a.experts) mine = -1;
+    for (uint64_t left = __ballot(mine >= 0); left != 0; ++named) left &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, first_lane(left)));
+  } else {
+    if (threadIdx.x < kFewWords) lds.named[threadIdx.x] = 0;
+    if (threadIdx.x == 0) lds.rows = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.slots; i += kFewThreads) {
+      const uint32_t e = (uint32_t)p.a.chosen[i];
+      if (e < (uint32_t)p.a.experts) atomicOr(&lds.named[e / 32], 1u << (e % 32));
+    }
+    __syncthreads();
+    named = uniform(__shfl(wave_prefix(lane < kFewWords ? __popc(lds.named[lane]) : 0), 63));
+  }
+  return named;
 }
 
-// The which-th of the experts that are named, and its slots (in any order: a token's results do not depend on its place).
-__device__ __forceinline__ void gather_slots(const FewParams& p, FewSchedule& s, int which) {
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    uint32_t word = lane < kFewWords ? s.named[lane] : 0u;
-    const int upto = wave_prefix(__popc(word)), before = upto - __popc(word);
-    if (which >= before && which < upto) {
-      for (int i = before; i < which; ++i) word &= word - 1;
-      s.expert = lane * 32 + __ffs(word) - 1;
+// The which-th of them.
+__device__ __forceinline__ int find_expert(const FewParams& p, const FewLds& lds, int mine, int which) {
+  const int lane = threadIdx.x & 63;
+  if (few_slots(p)) {
+    uint64_t left = __ballot(mine >= 0);
+    for (int i = 0; i < which; ++i) left &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, first_lane(left)));
+    return __builtin_amdgcn_readlane(mine, first_lane(left));
+  }
+  uint32_t word = lane < kFewWords ? lds.named[lane] : 0u;
+  const int upto = wave_prefix(__popc(word)), before = upto - __popc(word);
+  const uint64_t here = __ballot(which >= before && which < upto);
+  for (int i = before; i < which && word != 0; ++i) word &= word - 1;
+  return __builtin_amdgcn_readlane(lane * 32 + __ffs(word) - 1, first_lane(here));
+}
+
+// All threads.  Writes the expert's slots to LDS and returns their number.
+__device__ __forceinline__ int gather_slots(const FewParams& p, FewLds& lds, int mine, int expert) {
+  const int lane = threadIdx.x & 63;
+  if (few_slots(p)) {
+    if (threadIdx.x < 64) {
+      const uint64_t same = __ballot(mine == expert);
+      if (mine == expert) lds.slot[__popcll(same & ((uint64_t(1) << lane) - 1))] = lane;
+      if (lane == 0) lds.rows = __popcll(same);
     }
+  } else {
+    for (int i = threadIdx.x; i < p.slots; i += kFewThreads)
+      if (p.a.chosen[i] == expert) lds.slot[atomicAdd(&lds.rows, 1)] = i;
   }
   __syncthreads();
-  const int expert = s.expert;
-  for (int i = threadIdx.x; i < p.slots; i += kFewThreads)
-    if (p.a.chosen[i] == expert) s.slot[atomicAdd(&s.rows, 1)] = i;
-  __syncthreads();
+  return uniform(lds.rows);
 }
 
 template <int DT, bool NT, int MT>
-__global__ __launch_bounds__(kFewThreads, MT == 1 ? 4 : 2) void few_gate_up_kernel(FewParams p) {
-  using S = Stream<DT, NT, 4, MT, 1>;
+__global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_gate_up_kernel(FewParams p) {
+  using S = Stream<DT, NT, 4, MT>;
   constexpr int COLUMNS = NT ? 32 : 64;   // of h
-  __shared__ FewSchedule schedule;
+  __shared__ FewLds few_lds;
   __shared__ f32x4 lds[kFewWaves * 256];
   const FewTokensArgs& a = p.a;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   if (blockIdx.x == 0)   // the second kernel's counters
     for (int i = threadIdx.x; i < p.counters; i += kFewThreads) p.arrivals[i] = 0;
-  const int named = find_named(p, schedule);
+  int mine;
+  const int named = find_named(p, few_lds, mine);
   const int which = blockIdx.x / p.tiles, column0 = (blockIdx.x - which * p.tiles) * COLUMNS;
   if (which >= named) return;
-  gather_slots(p, schedule, which);
-  const int rows = uniform(schedule.rows), ffn = a.ffn, hidden = a.hidden;
-  const uint16_t* w = static_cast<const uint16_t*>(a.w13) + (uint64_t)uniform(schedule.expert) * 2 * ffn * hidden;
+  const int expert = find_expert(p, few_lds, mine, which);
+  const int ffn = a.ffn, hidden = a.hidden;
+  const uint16_t* w = static_cast<const uint16_t*>(a.w13) + (uint64_t)expert * 2 * ffn * hidden;
   S s;
-  s.x[0] = static_cast<const uint16_t*>(a.x);
+  s.x = static_cast<const uint16_t*>(a.x);
   s.depth = hidden;
   s.width = 8;
   if constexpr (NT) {
@@ -118,12 +145,15 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 4 : 2) void few_gate_up_kern
     s.at[0] = q * 8 * s.pitch + (uint32_t)(column + (c & 1) * ffn) * 2;
   }
   const Exchange<NT> exchange{lds};
+  const int end = (hidden + S::DEPTH - 1) / S::DEPTH;
+  s.prepare(0, end);
+  const int rows = gather_slots(p, few_lds, mine, expert);
   for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
+    if (row0 > 0) s.prepare(0, end);
 #pragma unroll
     for (int m = 0; m < MT; ++m)   // (places past the last row: the last one's, not stored)
-      s.row[m] = (uint32_t)(schedule.slot[min(row0 + 16 * m + c, rows - 1)] / a.top_k) * (uint32_t)hidden * 2;
-    s.clear();
-    s.run(0, (hidden + S::DEPTH - 1) / S::DEPTH);
+      s.set_row(m, (uint32_t)(few_lds.slot[min(row0 + 16 * m + c, rows - 1)] / a.top_k) * (uint32_t)hidden * 2);
+    s.run(end);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (row0 + 16 * m >= rows) break;
@@ -132,30 +162,32 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 4 : 2) void few_gate_up_kern
         __syncthreads();
         exchange.put(s, m, round);
         __syncthreads();
-        const int token = threadIdx.x >> 5, n = threadIdx.x & 31;   // of 16 rows, of 32 columns
+        for (int item = threadIdx.x; item < 512; item += kFewThreads) {
+        const int token = item >> 5, n = item & 31;   // of 16 rows, of 32 columns
         float gate, up;
         int column;
-        bool mine;
+        bool own;
         if constexpr (NT) {
           gate = exchange.column_of_tiles(n, token);
           up = exchange.column_of_tiles(32 + n, token);
           column = column0 + n;
-          mine = column < ffn;
+          own = column < ffn;
         } else {
           const int block = n >> 3, start = column0 + round * 32 + block * 8;
           gate = exchange.column_of_block(2 * block, n & 7, token);
           up = exchange.column_of_block(2 * block + 1, n & 7, token);
           column = (ffn < 8 ? 0 : min(start, ffn - 8)) + (n & 7);
-          mine = column >= start && column < ffn;   // (a block that moved back: its own columns only)
+          own = column >= start && column < ffn;   // (a block that moved back: its own columns only)
         }
-        const int row = row0 + 16 * m + token;
-        if (mine && row < rows) {
+        const int row = row0 + 16 * m + token, slot = few_lds.slot[min(row, rows - 1)];
+        if (own && row < rows) {
           const float h = gate / (1.0f + expf(-gate)) * up;
           const uint16_t high = round_bits<DT>(h);
           const float rest = h - widen_bits<DT>(high);
-          const uint64_t to = (uint64_t)schedule.slot[row] * p.ffn_pitch + column;
-          p.high[to] = high;
-          p.low[to] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : uint16_t(0);   // (an infinite h has no rest)
+          uint16_t* to = p.h + (uint64_t)slot * 2 * p.ffn_pitch + column;
+          to[0] = high;
+          to[p.ffn_pitch] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : uint16_t(0);   // (an infinite h has no rest)
+        }
         }
       }
     }
@@ -163,15 +195,16 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 4 : 2) void few_gate_up_kern
 }
 
 template <int DT, bool NT, int MT>
-__global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewParams p) {
-  using S = Stream<DT, NT, 4, MT, 2>;
+__global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(FewParams p) {
+  using S = Stream<DT, NT, 4, MT>;
   constexpr int COLUMNS = NT ? 64 : 128;
-  __shared__ FewSchedule schedule;
+  __shared__ FewLds few_lds;
   __shared__ f32x4 lds[kFewWaves * 256];
   __shared__ int32_t arrived;
   const FewTokensArgs& a = p.a;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int named = find_named(p, schedule), hidden = a.hidden, ffn = a.ffn;
+  int mine;
+  const int named = find_named(p, few_lds, mine), hidden = a.hidden, ffn = a.ffn;
   const int arrivals = named * p.pieces;
   int tile, left = 0;
   if (named > 0) {
@@ -184,11 +217,10 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewParams p) {
   const int column0 = tile * COLUMNS;
   if (named > 0) {
     const int which = left / p.pieces, piece = left - which * p.pieces;
-    gather_slots(p, schedule, which);
-    const int rows = uniform(schedule.rows);
-    const uint16_t* w = static_cast<const uint16_t*>(a.w2) + (uint64_t)uniform(schedule.expert) * ffn * hidden;
+    const int expert = find_expert(p, few_lds, mine, which);
+    const uint16_t* w = static_cast<const uint16_t*>(a.w2) + (uint64_t)expert * ffn * hidden;
     S s;
-    s.x[0] = p.high, s.x[1] = p.low;
+    s.x = p.h;
     s.depth = ffn;
     s.width = 8;
     if constexpr (NT) {
@@ -206,11 +238,16 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewParams p) {
     const int end = (int)((int64_t)steps * (piece + 1) / p.pieces);
     const Exchange<NT> exchange{lds};
     float* parts = p.parts + (uint64_t)piece * p.slots * hidden;
+    s.prepare(begin, end);
+    const int rows = 2 * gather_slots(p, few_lds, mine, expert);   // of h, two for each slot
     for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
+      if (row0 > 0) s.prepare(begin, end);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) s.row[m] = (uint32_t)schedule.slot[min(row0 + 16 * m + c, rows - 1)] * (uint32_t)p.ffn_pitch * 2;
-      s.clear();
-      s.run(begin, end);
+      for (int m = 0; m < MT; ++m) {
+        const int row = min(row0 + 16 * m + c, rows - 1);
+        s.set_row(m, ((uint32_t)few_lds.slot[row / 2] * 2 + (row & 1)) * (uint32_t)p.ffn_pitch * 2);
+      }
+      s.run(end);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if (row0 + 16 * m >= rows) break;
@@ -219,28 +256,26 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewParams p) {
           __syncthreads();
           exchange.put(s, m, round);
           __syncthreads();
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int token = half * 8 + (threadIdx.x >> 6), n = threadIdx.x & 63;   // of 16 rows, of 64 columns
-            float y;
-            int column;
-            bool mine;
-            if constexpr (NT) {
-              y = exchange.column_of_tiles(n, token);
-              column = column0 + n;
-              mine = column < hidden;
-            } else {
-              const int start = column0 + round * 64 + (n >> 3) * 8;
-              y = exchange.column_of_block(n >> 3, n & 7, token);
-              column = (hidden < 8 ? 0 : min(start, hidden - 8)) + (n & 7);
-              mine = column >= start && column < hidden;
-            }
-            const int row = row0 + 16 * m + token;
-            if (mine && row < rows) {
-              const int slot = schedule.slot[row];
-              // (device scope: written to and read from where all XCDs see it, without a fence that empties whole L2s)
-              __hip_atomic_store(&parts[(uint64_t)slot * hidden + column], y * a.weights[slot], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+          for (int item = threadIdx.x; item < 512; item += kFewThreads) {
+          const int pair = item >> 6, n = item & 63;   // of 8 slots, of 64 columns
+          float y;
+          int column;
+          bool own;
+          if constexpr (NT) {
+            y = exchange.column_of_tiles(n, 2 * pair) + exchange.column_of_tiles(n, 2 * pair + 1);
+            column = column0 + n;
+            own = column < hidden;
+          } else {
+            const int start = column0 + round * 64 + (n >> 3) * 8;
+            y = exchange.column_of_block(n >> 3, n & 7, 2 * pair) + exchange.column_of_block(n >> 3, n & 7, 2 * pair + 1);
+            column = (hidden < 8 ? 0 : min(start, hidden - 8)) + (n & 7);
+            own = column >= start && column < hidden;
+          }
+          const int row = row0 + 16 * m + 2 * pair, slot = few_lds.slot[min(row, rows - 1) / 2];
+          if (own && row < rows) {
+            // (device scope: written to and read from where all XCDs see it, without a fence that empties whole L2s)
+            __hip_atomic_store(&parts[(uint64_t)slot * hidden + column], y * a.weights[slot], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
           }
         }
       }
@@ -259,15 +294,26 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewParams p) {
   // The strip's sums, in the order of a token's experts and of the pieces.
   uint16_t* out = static_cast<uint16_t*>(a.out);
   const int columns = min(COLUMNS, hidden - column0);
+  constexpr int IN_FLIGHT = 8;
   for (int i = threadIdx.x; i < a.tokens * COLUMNS; i += kFewThreads) {
     const int token = i / COLUMNS, n = i % COLUMNS;
     if (n >= columns) continue;
+    const float* from = p.parts + (uint64_t)token * a.top_k * hidden + column0 + n;
+    const int32_t* chosen = a.chosen + token * a.top_k;
+    const int terms = a.top_k * p.pieces;
     float sum = 0.0f;
-    for (int j = 0; j < a.top_k; ++j) {
-      const int slot = token * a.top_k + j;
-      if ((uint32_t)a.chosen[slot] >= (uint32_t)a.experts) continue;
-      for (int piece = 0; piece < p.pieces; ++piece)
-        sum += __hip_atomic_load(&p.parts[((uint64_t)piece * p.slots + slot) * hidden + column0 + n], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int j = 0, piece = 0;
+    for (int at = 0; at < terms; at += IN_FLIGHT) {   // (one by one each would wait for memory)
+      float term[IN_FLIGHT];
+#pragma unroll
+      for (int f = 0; f < IN_FLIGHT; ++f) {
+        term[f] = 0.0f;
+        if (at + f < terms && (uint32_t)chosen[j] < (uint32_t)a.experts)
+          term[f] = __hip_atomic_load(from + ((uint64_t)piece * p.slots + j) * hidden, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (++piece == p.pieces) piece = 0, j = min(j + 1, a.top_k - 1);
+      }
+#pragma unroll
+      for (int f = 0; f < IN_FLIGHT; ++f) sum += term[f];
     }
     out[(uint64_t)token * hidden + column0 + n] = round_bits<DT>(sum);
   }
@@ -293,7 +339,7 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   f.pieces = 1;
   while (f.pieces < 16 && f.named * f.down_tiles * f.pieces < kFewWorkgroups && steps >= 2 * f.pieces * 2 * kFewWaves) f.pieces *= 2;
   f.arrivals_bytes = (uint64_t)(f.down_tiles * 4 + 255) / 256 * 256;
-  f.h_bytes = ((uint64_t)f.slots * f.ffn_pitch * 2 + 255) / 256 * 256;
+  f.h_bytes = ((uint64_t)f.slots * f.ffn_pitch * 4 + 255) / 256 * 256;
   f.parts_bytes = (uint64_t)f.pieces * f.slots * hidden * 4;
   return f;
 }
@@ -306,9 +352,8 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   p.ffn_pitch = (int32_t)f.ffn_pitch;
   char* at = static_cast<char*>(a.scratch);
   p.arrivals = reinterpret_cast<int32_t*>(at);
-  p.high = reinterpret_cast<uint16_t*>(at + f.arrivals_bytes);
-  p.low = reinterpret_cast<uint16_t*>(at + f.arrivals_bytes + f.h_bytes);
-  p.parts = reinterpret_cast<float*>(at + f.arrivals_bytes + 2 * f.h_bytes);
+  p.h = reinterpret_cast<uint16_t*>(at + f.arrivals_bytes);
+  p.parts = reinterpret_cast<float*>(at + f.arrivals_bytes + f.h_bytes);
   p.tiles = (int32_t)f.up_tiles;
   p.pieces = (int32_t)f.pieces;
   p.counters = (int32_t)f.down_tiles;
@@ -325,17 +370,17 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
 bool few_tokens_fits(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
   const FewPlan f = few_plan(tokens, experts, top_k, hidden, ffn, trans_b);
   const int64_t most = (int64_t(1) << 32) / kFewThreads;   // (threads of a launch are counted in 32 bits)
-  return f.named * f.up_tiles < most && f.named * f.down_tiles * f.pieces < most && f.slots * f.ffn_pitch * 2 < (int64_t(1) << 32);
+  return f.named * f.up_tiles < most && f.named * f.down_tiles * f.pieces < most && f.slots * f.ffn_pitch * 4 < (int64_t(1) << 32);
 }
 
 uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
   const FewPlan f = few_plan(tokens, experts, top_k, hidden, ffn, trans_b);
-  return f.arrivals_bytes + 2 * f.h_bytes + f.parts_bytes;
+  return f.arrivals_bytes + f.h_bytes + f.parts_bytes;
 }
 
 hipError_t few_tokens(const FewTokensArgs& a, hipStream_t stream) {
   const FewPlan f = few_plan(a.tokens, a.experts, a.top_k, a.hidden, a.ffn, a.trans_b);
-  const bool one = a.tokens <= 16;   // rows of an expert fit one matrix tile (unless a token names an expert twice)
+  const bool one = a.tokens <= 16 || f.slots <= 8 * a.experts;   // rows of an expert fit one matrix tile (unless a token names an expert twice)
 #define GG_LAUNCH(DT)                                                                                            \
   (a.trans_b ? (one ? launch_few<DT, true, 1>(a, f, stream) : launch_few<DT, true, 2>(a, f, stream))             \
              : (one ? launch_few<DT, false, 1>(a, f, stream) : launch_few<DT, false, 2>(a, f, stream)))
