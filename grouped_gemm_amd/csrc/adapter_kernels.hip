@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
 #pragma unroll
         for (int m = 0; m < MT; ++m)
           s.set_row(m, (uint32_t)__shfl(list, min(row0 + 16 * m + c, rows - 1)) * (uint32_t)a.hidden_in * 2);
-        s.prepare(begin, end);
+        s.prepare(uniform((int)(threadIdx.x >> 6)), begin, end);
         s.run(end);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {

@@ -20,6 +20,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 #include "few_rows.hpp"
 #include "gmm_kernel.hpp"
 #include "wave_ops.hpp"
@@ -40,7 +42,9 @@ struct FewParams {
   int32_t* arrivals;     // [strips of down]
   uint16_t* h;           // [slots][2][ffn_pitch] h rounded to the element type, and what the rounding left: two rows for
                          // the second product, which is then exact to twice the bits of the type
-  float* parts;          // [pieces][slots][hidden]
+  int32_t hidden_pitch;  // elements from one row of parts to the next
+  uint32_t parts_bytes;
+  float* parts;          // [pieces][slots][hidden_pitch]
 };
 
 // Which experts are named, and the slots of one of them (in any order: a token's results do not depend on its place).  Up to 64
@@ -67,7 +71,7 @@ __device__ __forceinline__ int find_named(const FewParams& p, FewLds& lds, int& 
     if (threadIdx.x < kFewWords) lds.named[threadIdx.x] = 0;
     if (threadIdx.x == 0) lds.rows = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < p.slots; i += kFewThreads) {
+    for (int i = threadIdx.x; i < p.slots; i += (int)blockDim.x) {
       const uint32_t e = (uint32_t)p.a.chosen[i];
       if (e < (uint32_t)p.a.experts) atomicOr(&lds.named[e / 32], 1u << (e % 32));
     }
@@ -102,27 +106,32 @@ __device__ __forceinline__ int gather_slots(const FewParams& p, FewLds& lds, int
       if (lane == 0) lds.rows = __popcll(same);
     }
   } else {
-    for (int i = threadIdx.x; i < p.slots; i += kFewThreads)
+    for (int i = threadIdx.x; i < p.slots; i += (int)blockDim.x)
       if (p.a.chosen[i] == expert) lds.slot[atomicAdd(&lds.rows, 1)] = i;
   }
   __syncthreads();
   return uniform(lds.rows);
 }
 
+// Where the width is contiguous, gate and up have waves of their own, so that an instruction reads 256 neighbouring bytes of
+// a row (128 of each of the two: 5.3 TB/s instead of GATE_UP_RATE).
+constexpr int gate_up_threads(bool nt) { return nt ? kFewThreads : 2 * kFewThreads; }
+
 template <int DT, bool NT, int MT>
-__global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_gate_up_kernel(FewParams p) {
+__global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate_up_kernel(FewParams p) {
   using S = Stream<DT, NT, 4, MT>;
-  constexpr int COLUMNS = NT ? 32 : 64;   // of h
+  constexpr int COLUMNS = NT ? 32 : 128, OF_ROUND = NT ? 32 : 64;   // of h
+  constexpr int THREADS = gate_up_threads(NT);
   __shared__ FewLds few_lds;
-  __shared__ f32x4 lds[kFewWaves * 256];
+  __shared__ f32x4 lds[THREADS * 4];
   const FewTokensArgs& a = p.a;
-  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, wave = uniform((int)(threadIdx.x >> 6));
   if (blockIdx.x == 0)   // the second kernel's counters
-    for (int i = threadIdx.x; i < p.counters; i += kFewThreads) p.arrivals[i] = 0;
+    for (int i = threadIdx.x; i < p.counters; i += THREADS) p.arrivals[i] = 0;
   int mine;
   const int named = find_named(p, few_lds, mine);
-  const int which = blockIdx.x / p.tiles, column0 = (blockIdx.x - which * p.tiles) * COLUMNS;
-  if (which >= named) return;
+  if (blockIdx.x >= named * p.tiles) return;
+  const int task = (int)task_of_block(blockIdx.x, named * p.tiles), which = task / p.tiles, column0 = (task - which * p.tiles) * COLUMNS;
   const int expert = find_expert(p, few_lds, mine, which);
   const int ffn = a.ffn, hidden = a.hidden;
   const uint16_t* w = static_cast<const uint16_t*>(a.w13) + (uint64_t)expert * 2 * ffn * hidden;
@@ -137,19 +146,19 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_gate_up_kern
     for (int i = 0; i < 4; ++i)   // (rows past the last: the last one's, not stored)
       s.at[i] = (uint32_t)(min(16 * (i & 1) + c, ffn - 1 - column0)) * (uint32_t)hidden * 2 + q * 32;
   } else {
-    // lanes of even number have columns of gate, of odd number the same of up; blocks past the last column move back to it
-    const int column = ffn < 8 ? 0 : min(column0 + c / 2 * 8, ffn - 8);
+    // (a lane's 8 columns past the last column move back to it)
+    const int column = ffn < 8 ? 0 : min(column0 + c * 8, ffn - 8);
     s.width = min(ffn, 8);
-    s.first = w;
+    s.first = w + wave / kFewWaves * ffn;
     s.pitch = (uint32_t)ffn * 4;
-    s.at[0] = q * 8 * s.pitch + (uint32_t)(column + (c & 1) * ffn) * 2;
+    s.at[0] = q * 8 * s.pitch + (uint32_t)column * 2;
   }
   const Exchange<NT> exchange{lds};
   const int end = (hidden + S::DEPTH - 1) / S::DEPTH;
-  s.prepare(0, end);
+  s.prepare(wave % kFewWaves, 0, end);
   const int rows = gather_slots(p, few_lds, mine, expert);
   for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
-    if (row0 > 0) s.prepare(0, end);
+    if (row0 > 0) s.prepare(wave % kFewWaves, 0, end);
 #pragma unroll
     for (int m = 0; m < MT; ++m)   // (places past the last row: the last one's, not stored)
       s.set_row(m, (uint32_t)(few_lds.slot[min(row0 + 16 * m + c, rows - 1)] / a.top_k) * (uint32_t)hidden * 2);
@@ -162,32 +171,32 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_gate_up_kern
         __syncthreads();
         exchange.put(s, m, round);
         __syncthreads();
-        for (int item = threadIdx.x; item < 512; item += kFewThreads) {
-        const int token = item >> 5, n = item & 31;   // of 16 rows, of 32 columns
-        float gate, up;
-        int column;
-        bool own;
-        if constexpr (NT) {
-          gate = exchange.column_of_tiles(n, token);
-          up = exchange.column_of_tiles(32 + n, token);
-          column = column0 + n;
-          own = column < ffn;
-        } else {
-          const int block = n >> 3, start = column0 + round * 32 + block * 8;
-          gate = exchange.column_of_block(2 * block, n & 7, token);
-          up = exchange.column_of_block(2 * block + 1, n & 7, token);
-          column = (ffn < 8 ? 0 : min(start, ffn - 8)) + (n & 7);
-          own = column >= start && column < ffn;   // (a block that moved back: its own columns only)
-        }
-        const int row = row0 + 16 * m + token, slot = few_lds.slot[min(row, rows - 1)];
-        if (own && row < rows) {
+        for (int item = threadIdx.x; item < 16 * OF_ROUND; item += THREADS) {
+          const int token = item / OF_ROUND, n = item % OF_ROUND;
+          const int row = row0 + 16 * m + token;
+          if (row >= rows) break;
+          float gate, up;
+          int column;
+          bool own;
+          if constexpr (NT) {
+            gate = exchange.column_of_tiles(n, token);
+            up = exchange.column_of_tiles(32 + n, token);
+            column = column0 + n;
+            own = column < ffn;
+          } else {
+            const int start = column0 + round * 64 + (n >> 3) * 8;
+            gate = exchange.column_of_block(0, n >> 3, n & 7, token);
+            up = exchange.column_of_block(kFewWaves, n >> 3, n & 7, token);
+            column = (ffn < 8 ? 0 : min(start, ffn - 8)) + (n & 7);
+            own = column >= start && column < ffn;   // (of 8 columns that moved back: their own only)
+          }
+          if (!own) continue;
           const float h = gate / (1.0f + expf(-gate)) * up;
           const uint16_t high = round_bits<DT>(h);
           const float rest = h - widen_bits<DT>(high);
-          uint16_t* to = p.h + (uint64_t)slot * 2 * p.ffn_pitch + column;
+          uint16_t* to = p.h + (uint64_t)few_lds.slot[row] * 2 * p.ffn_pitch + column;
           to[0] = high;
           to[p.ffn_pitch] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : uint16_t(0);   // (an infinite h has no rest)
-        }
         }
       }
     }
@@ -205,16 +214,11 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   int mine;
   const int named = find_named(p, few_lds, mine), hidden = a.hidden, ffn = a.ffn;
-  const int arrivals = named * p.pieces;
-  int tile, left = 0;
-  if (named > 0) {
-    tile = blockIdx.x / arrivals;
-    left = blockIdx.x - tile * arrivals;
-  } else {
-    tile = blockIdx.x;
-  }
-  if (tile >= p.tiles) return;
-  const int column0 = tile * COLUMNS;
+  // strips one after the other, so that their sums are joined on the way (without any expert: zeros are stored)
+  const int arrivals = named * p.pieces, tasks = max(arrivals, 1) * p.tiles;
+  if (blockIdx.x >= tasks) return;
+  const int task = (int)task_of_block(blockIdx.x, tasks);
+  const int tile = task / max(arrivals, 1), left = task - tile * arrivals, column0 = tile * COLUMNS;
   if (named > 0) {
     const int which = left / p.pieces, piece = left - which * p.pieces;
     const int expert = find_expert(p, few_lds, mine, which);
@@ -237,11 +241,11 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
     const int steps = (ffn + S::DEPTH - 1) / S::DEPTH, begin = (int)((int64_t)steps * piece / p.pieces);
     const int end = (int)((int64_t)steps * (piece + 1) / p.pieces);
     const Exchange<NT> exchange{lds};
-    float* parts = p.parts + (uint64_t)piece * p.slots * hidden;
-    s.prepare(begin, end);
+    float* parts = p.parts + (uint64_t)piece * p.slots * p.hidden_pitch;
+    s.prepare(uniform((int)(threadIdx.x >> 6)), begin, end);
     const int rows = 2 * gather_slots(p, few_lds, mine, expert);   // of h, two for each slot
     for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
-      if (row0 > 0) s.prepare(begin, end);
+      if (row0 > 0) s.prepare(uniform((int)(threadIdx.x >> 6)), begin, end);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int row = min(row0 + 16 * m + c, rows - 1);
@@ -257,25 +261,26 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
           exchange.put(s, m, round);
           __syncthreads();
           for (int item = threadIdx.x; item < 512; item += kFewThreads) {
-          const int pair = item >> 6, n = item & 63;   // of 8 slots, of 64 columns
-          float y;
-          int column;
-          bool own;
-          if constexpr (NT) {
-            y = exchange.column_of_tiles(n, 2 * pair) + exchange.column_of_tiles(n, 2 * pair + 1);
-            column = column0 + n;
-            own = column < hidden;
-          } else {
-            const int start = column0 + round * 64 + (n >> 3) * 8;
-            y = exchange.column_of_block(n >> 3, n & 7, 2 * pair) + exchange.column_of_block(n >> 3, n & 7, 2 * pair + 1);
-            column = (hidden < 8 ? 0 : min(start, hidden - 8)) + (n & 7);
-            own = column >= start && column < hidden;
-          }
-          const int row = row0 + 16 * m + 2 * pair, slot = few_lds.slot[min(row, rows - 1) / 2];
-          if (own && row < rows) {
+            const int pair = item >> 6, n = item & 63;   // of 8 slots, of 64 columns
+            const int row = row0 + 16 * m + 2 * pair;
+            if (row >= rows) break;
+            float y;
+            int column;
+            bool own;
+            if constexpr (NT) {
+              y = exchange.column_of_tiles(n, 2 * pair) + exchange.column_of_tiles(n, 2 * pair + 1);
+              column = column0 + n;
+              own = column < hidden;
+            } else {
+              const int start = column0 + round * 64 + (n >> 3) * 8;
+              y = exchange.column_of_block(0, n >> 3, n & 7, 2 * pair) + exchange.column_of_block(0, n >> 3, n & 7, 2 * pair + 1);
+              column = (hidden < 8 ? 0 : min(start, hidden - 8)) + (n & 7);
+              own = column >= start && column < hidden;
+            }
+            if (!own) continue;
+            const int slot = few_lds.slot[row / 2];
             // (device scope: written to and read from where all XCDs see it, without a fence that empties whole L2s)
-            __hip_atomic_store(&parts[(uint64_t)slot * hidden + column], y * a.weights[slot], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          }
+            __hip_atomic_store(&parts[(uint64_t)slot * p.hidden_pitch + column], y * a.weights[slot], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           }
         }
       }
@@ -291,56 +296,60 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
       __syncthreads();
     }
   }
-  // The strip's sums, in the order of a token's experts and of the pieces.
-  uint16_t* out = static_cast<uint16_t*>(a.out);
-  const int columns = min(COLUMNS, hidden - column0);
+  // The strip's sums, in the order of a token's experts and of the pieces, four columns to a thread and IN_FLIGHT terms at a
+  // time (one by one each would wait for memory).
   constexpr int IN_FLIGHT = 8;
-  for (int i = threadIdx.x; i < a.tokens * COLUMNS; i += kFewThreads) {
-    const int token = i / COLUMNS, n = i % COLUMNS;
-    if (n >= columns) continue;
-    const float* from = p.parts + (uint64_t)token * a.top_k * hidden + column0 + n;
+  uint16_t* out = static_cast<uint16_t*>(a.out);
+  const __amdgpu_buffer_rsrc_t parts = make_rsrc(p.parts, p.parts_bytes);
+  for (int i = threadIdx.x; i < a.tokens * (COLUMNS / 4); i += kFewThreads) {
+    const int token = i / (COLUMNS / 4), column = column0 + i % (COLUMNS / 4) * 4;
+    if (column >= hidden) continue;
     const int32_t* chosen = a.chosen + token * a.top_k;
     const int terms = a.top_k * p.pieces;
-    float sum = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     int j = 0, piece = 0;
-    for (int at = 0; at < terms; at += IN_FLIGHT) {   // (one by one each would wait for memory)
-      float term[IN_FLIGHT];
+    for (int at = 0; at < terms; at += IN_FLIGHT) {
+      f32x4 term[IN_FLIGHT];
 #pragma unroll
       for (int f = 0; f < IN_FLIGHT; ++f) {
-        term[f] = 0.0f;
+        term[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (at + f < terms && (uint32_t)chosen[j] < (uint32_t)a.experts)
-          term[f] = __hip_atomic_load(from + ((uint64_t)piece * p.slots + j) * hidden, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          term[f] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                  parts, (uint32_t)((piece * p.slots + token * a.top_k + j) * p.hidden_pitch + column) * 4, 0, kDeviceScope));
         if (++piece == p.pieces) piece = 0, j = min(j + 1, a.top_k - 1);
       }
 #pragma unroll
       for (int f = 0; f < IN_FLIGHT; ++f) sum += term[f];
     }
-    out[(uint64_t)token * hidden + column0 + n] = round_bits<DT>(sum);
+    uint16_t* to = out + (uint64_t)token * hidden + column;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (column + e < hidden) to[e] = round_bits<DT>(sum[e]);
   }
 }
 
 struct FewPlan {
-  int64_t slots, named, up_tiles, down_tiles, pieces, ffn_pitch;
+  int64_t slots, named, up_tiles, down_tiles, pieces, ffn_pitch, hidden_pitch;
   uint64_t arrivals_bytes, h_bytes, parts_bytes;
 };
 
-// Workgroups that keep the device busy: two rounds of two on each of 256 compute units.
-constexpr int64_t kFewWorkgroups = 1024;
+constexpr int64_t kFewUnits = 256;   // compute units
 
 FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool nt) {
   FewPlan f;
   f.slots = tokens * top_k;
   f.named = f.slots < experts ? f.slots : experts;   // at most
-  f.up_tiles = (ffn + (nt ? 31 : 63)) / (nt ? 32 : 64);
+  f.up_tiles = (ffn + (nt ? 31 : 127)) / (nt ? 32 : 128);
   f.down_tiles = (hidden + (nt ? 63 : 127)) / (nt ? 64 : 128);
   f.ffn_pitch = (ffn + 7) / 8 * 8;
-  // the depth of down in pieces where its strips alone are too few, each at least two steps of every wave
-  const int64_t steps = (ffn + (nt ? 63 : 31)) / (nt ? 64 : 32);
-  f.pieces = 1;
-  while (f.pieces < 16 && f.named * f.down_tiles * f.pieces < kFewWorkgroups && steps >= 2 * f.pieces * 2 * kFewWaves) f.pieces *= 2;
+  // the depth of down in pieces where its strips alone are fewer than compute units, each of at least eight steps to a wave.  One
+  // token, 4096 -> 14336, in 1, 2, 4, 8 pieces: 64 strips 58, 34, 25, 26 us, 128 strips 65, 43, 44, 53, 512 strips 160, 185, 188, 193
+  const int64_t steps = (ffn + (nt ? 63 : 31)) / (nt ? 64 : 32), fit = kFewUnits / (f.named * f.down_tiles), deep = steps / (8 * kFewWaves);
+  f.pieces = std::max<int64_t>(1, std::min({fit, deep, int64_t(16)}));
   f.arrivals_bytes = (uint64_t)(f.down_tiles * 4 + 255) / 256 * 256;
   f.h_bytes = ((uint64_t)f.slots * f.ffn_pitch * 4 + 255) / 256 * 256;
-  f.parts_bytes = (uint64_t)f.pieces * f.slots * hidden * 4;
+  f.hidden_pitch = (hidden + 3) / 4 * 4;
+  f.parts_bytes = (uint64_t)f.pieces * f.slots * f.hidden_pitch * 4;
   return f;
 }
 
@@ -350,6 +359,8 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   p.a = a;
   p.slots = (int32_t)f.slots;
   p.ffn_pitch = (int32_t)f.ffn_pitch;
+  p.hidden_pitch = (int32_t)f.hidden_pitch;
+  p.parts_bytes = (uint32_t)f.parts_bytes;
   char* at = static_cast<char*>(a.scratch);
   p.arrivals = reinterpret_cast<int32_t*>(at);
   p.h = reinterpret_cast<uint16_t*>(at + f.arrivals_bytes);
@@ -357,7 +368,7 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   p.tiles = (int32_t)f.up_tiles;
   p.pieces = (int32_t)f.pieces;
   p.counters = (int32_t)f.down_tiles;
-  hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, MT>), dim3((uint32_t)(f.named * f.up_tiles)), dim3(kFewThreads), 0, stream, p);
+  hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, MT>), dim3((uint32_t)(f.named * f.up_tiles)), dim3(gate_up_threads(NT)), 0, stream, p);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   p.tiles = (int32_t)f.down_tiles;
@@ -369,8 +380,8 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
 
 bool few_tokens_fits(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
   const FewPlan f = few_plan(tokens, experts, top_k, hidden, ffn, trans_b);
-  const int64_t most = (int64_t(1) << 32) / kFewThreads;   // (threads of a launch are counted in 32 bits)
-  return f.named * f.up_tiles < most && f.named * f.down_tiles * f.pieces < most && f.slots * f.ffn_pitch * 4 < (int64_t(1) << 32);
+  const int64_t most = (int64_t(1) << 32) / gate_up_threads(false);   // (threads of a launch are counted in 32 bits)
+  return f.named * f.up_tiles < most && f.named * f.down_tiles * f.pieces < most && f.slots * f.ffn_pitch * 4 < (int64_t(1) << 32) && f.parts_bytes < (uint64_t(1) << 32);
 }
 
 uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
