@@ -13,6 +13,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 #include "few_rows.hpp"
 #include "gmm_kernel.hpp"
 #include "wave_ops.hpp"
@@ -22,25 +24,34 @@ namespace {
 
 constexpr int kWindow = 64;
 
-struct AdapterParams {
-  AdapterArgs a;
-  float* v;          // [pieces][rows][v_pitch]
-  int32_t v_pitch;
-  int32_t pieces;    // of the depth hidden_in
-  int32_t splits;    // workgroups that share a window's adapters
-  int32_t strips;    // of hidden_out
+// The adapters of a window in the order of their first rows, with the rows of each as a mask.  The first kernel writes it for the second.
+struct WindowPlan {
+  int32_t count;
+  int32_t pieces;          // of the depth, into which v of these rows is cut
+  uint64_t none;           // rows without an adapter
+  uint64_t rows[kWindow];
+  int32_t adapter[kWindow];
 };
 
-// The window's adapters one by one, in the order of their first rows: the rows of each as a mask of lanes.
+struct AdapterParams {
+  AdapterArgs a;
+  float* v;            // [pieces][rows][v_pitch]
+  WindowPlan* plans;   // [windows]
+  int32_t v_pitch;
+  int32_t pieces;      // of the depth hidden_in, at most
+  int32_t shares;      // workgroups of a window (of one of its strips)
+  int32_t strips;      // of hidden_out
+  int32_t strip;       // columns of a strip
+};
+
+// The same from the rows' adapters, in the lanes of a wave.
 struct Window {
   int32_t adapter;    // of this lane's row, -1 without one
   uint64_t left;      // rows not yet taken
-  uint64_t none;      // rows without an adapter
-  int32_t rows;
+  uint64_t none;
 
   __device__ __forceinline__ Window(const AdapterArgs& a, int64_t first) {
-    const int lane = threadIdx.x & 63;
-    rows = (int)(a.rows - first < kWindow ? a.rows - first : kWindow);
+    const int lane = threadIdx.x & 63, rows = (int)(a.rows - first < kWindow ? a.rows - first : kWindow);
     adapter = lane < rows ? a.adapters[first + lane] : -1;
     if ((uint32_t)adapter >= (uint32_t)a.num) adapter = -1;
     left = __ballot(adapter >= 0);
@@ -53,15 +64,16 @@ struct Window {
     left &= ~mine;
     return mine;
   }
-  // Lane i gets the number of the i-th row of `mine` in the window (lanes past the last: any).
-  static __device__ __forceinline__ int list(uint64_t mine) {
-    const int lane = threadIdx.x & 63, count = __popcll(mine);
-    const int before = __popcll(mine & ((uint64_t(1) << lane) - 1));
-    const bool in = (mine >> lane) & 1;
-    // (rows of the mask go to the first lanes, the others behind them: every lane is written once)
-    return __builtin_amdgcn_ds_permute(4 * (in ? before : count + lane - before), lane);
-  }
 };
+
+// Lane i gets the number of the i-th row of `mine` in its window (lanes past the last: any).
+__device__ __forceinline__ int list_rows(uint64_t mine) {
+  const int lane = threadIdx.x & 63, count = __popcll(mine);
+  const int before = __popcll(mine & ((uint64_t(1) << lane) - 1));
+  const bool in = (mine >> lane) & 1;
+  // (the rows of the mask go to the first lanes, the others behind them: every lane is written once)
+  return __builtin_amdgcn_ds_permute(4 * (in ? before : count + lane - before), lane);
+}
 
 // v of one piece of the depth.  TILES: of 16 rows of a_l; more than 64 of them are taken 64 at a time.
 template <int DT, int TILES, int MT>
@@ -70,22 +82,37 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
   __shared__ f32x4 lds[kFewWaves * 256];
   const AdapterArgs& a = p.a;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int64_t window = blockIdx.x / p.splits, first = window * kWindow;
-  const int split = (int)(blockIdx.x - window * p.splits), piece = blockIdx.y;
-  const int steps = (a.hidden_in + S::DEPTH - 1) / S::DEPTH;
-  const int begin = (int)((int64_t)steps * piece / p.pieces), end = (int)((int64_t)steps * (piece + 1) / p.pieces);
-  float* v = p.v + (uint64_t)piece * a.rows * p.v_pitch;
+  const int64_t window = blockIdx.x / p.shares, first = window * kWindow;
+  const int share = (int)(blockIdx.x - window * p.shares);
   Window w(a, first);
+  // What is in the window: the workgroups that its adapters leave cut the depth.
+  int count = 0;
+  {
+    Window all = w;
+    WindowPlan& plan = p.plans[window];
+    for (; all.left != 0; ++count) {
+      int which;
+      const uint64_t mine = all.next(which);
+      if (share == 0 && threadIdx.x == 0) plan.adapter[count] = which, plan.rows[count] = mine;
+    }
+  }
+  const int pieces = min(max(p.shares / max(count, 1), 1), p.pieces), splits = p.shares / pieces;
+  if (share == 0 && threadIdx.x == 0) p.plans[window].count = count, p.plans[window].pieces = pieces, p.plans[window].none = w.none;
+  const int piece = share % pieces, split = share / pieces;
+  if (split >= splits) return;
+  const int steps = (a.hidden_in + S::DEPTH - 1) / S::DEPTH;
+  const int begin = (int)((int64_t)steps * piece / pieces), end = (int)((int64_t)steps * (piece + 1) / pieces);
+  float* v = p.v + (uint64_t)piece * a.rows * p.v_pitch;
   S s;
   s.depth = a.hidden_in;
   s.width = 8;
   s.x = static_cast<const uint16_t*>(a.x) + (uint64_t)first * a.hidden_in;
   const Exchange<true> exchange{lds};
-  for (int turn = 0; w.left != 0; turn = turn + 1 == p.splits ? 0 : turn + 1) {
+  for (int turn = 0; w.left != 0; turn = turn + 1 == splits ? 0 : turn + 1) {
     int which;
     const uint64_t mine = w.next(which);
     if (turn != split) continue;
-    const int list = Window::list(mine), rows = __popcll(mine);
+    const int list = list_rows(mine), rows = __popcll(mine);
     const uint16_t* weights = static_cast<const uint16_t*>(a.a) + (uint64_t)which * a.rank * a.hidden_in;
     for (int r0 = 0; r0 < a.rank; r0 += 16 * TILES) {
       s.first = s.second = weights + (uint64_t)r0 * a.hidden_in;
@@ -117,164 +144,194 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
   }
 }
 
-// out for a strip of columns: each wave has 64 of them, a lane 16 neighbouring ones of one row of the 16 of a tile.
+// out for a strip of columns: 64 at a time for each wave, of which a lane has twice 8 neighbouring ones of one row of the 16 of a tile.
+// KS: the rank in steps of 32, rounded up to a power of two; 0: at most 16, where one step has both halves of v, each against the
+// same of b_l.  v is split in LDS, as many rows of it at a time as take 20 KiB at most.
 constexpr int kExpandWaves = 4;
 constexpr int kExpandThreads = kExpandWaves * 64;
-constexpr int kStrip = kExpandWaves * 64;
-constexpr int kRankStep = 64;                  // ranks in LDS at a time
-constexpr int kLowPitch = kRankStep + 8;       // (so that the 16 rows of a fragment start in different banks)
+constexpr int kBlock = kExpandWaves * 64;   // columns that a workgroup takes at a time
 
-template <int DT>
-__global__ __launch_bounds__(kExpandThreads, 2) void adapter_expand_kernel(AdapterParams p) {
-  __shared__ __attribute__((aligned(16))) uint16_t split_v[2][kWindow][kLowPitch];   // high, low
-  __shared__ float unit[kWindow];
+template <int DT, int KS>
+__global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expand_kernel(AdapterParams p) {
+  constexpr int STEPS = KS == 0 ? 1 : KS, RANKS = KS == 0 ? 16 : 32 * KS;
+  constexpr int M = KS <= 2 ? 4 : 8 / KS, GROUP = 16 * M;                  // tiles of rows, rows
+  constexpr int PITCH = RANKS + 8;                                         // (so that the 16 rows of a fragment start in different banks)
+  constexpr int TPR = kExpandThreads / GROUP, EACH = RANKS / TPR / 4;      // threads of a row, and times four of its ranks for each
+  constexpr int IN_FLIGHT = 4;                                             // pieces of v
+  __shared__ __attribute__((aligned(16))) uint16_t split_v[2][GROUP][PITCH];   // high, low
+  __shared__ float unit[GROUP];
   const AdapterArgs& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4, wave = uniform(tid >> 6);
   uint32_t block = blockIdx.x;
   const int strip = (int)(block % p.strips);
   block /= p.strips;
-  const int split = (int)(block % p.splits);
-  const int64_t first = (int64_t)(block / p.splits) * kWindow;
-  const int column0 = strip * kStrip + wave * 64;   // of the wave
-  const int own = column0 + q * 16;                 // the lane's first column
+  const int share = (int)(block % p.shares);
+  const WindowPlan& plan = p.plans[block / p.shares];
+  const int64_t first = (int64_t)(block / p.shares) * kWindow;
+  const int strip_begin = strip * p.strip, strip_end = min(strip_begin + p.strip, a.hidden_out), columns = a.hidden_out;
   const uint16_t* base = static_cast<const uint16_t*>(a.base);
   uint16_t* out = static_cast<uint16_t*>(a.out);
-  const int columns = a.hidden_out;
-  Window w(a, first);
-  if (split == 0 && w.none != 0 && out != base) {   // rows without an adapter
-    for (int r = wave; r < w.rows; r += kExpandWaves) {
-      if (!((w.none >> r) & 1)) continue;
-      const uint64_t at = (uint64_t)(first + r) * columns;
-      for (int n = strip * kStrip + lane; n < min(columns, (strip + 1) * kStrip); n += 64) out[at + n] = base != nullptr ? base[at + n] : uint16_t(0);
+  if (share == 0 && plan.none != 0 && out != base) {   // rows without an adapter
+    int r = 0;
+    for (uint64_t none = plan.none; none != 0; none &= none - 1, ++r) {
+      if (r % kExpandWaves != wave) continue;
+      const uint64_t at = (uint64_t)(first + __ffsll((unsigned long long)none) - 1) * columns;
+      for (int n = strip_begin + lane * 8; n < strip_end; n += 512) {
+        if (n + 8 <= strip_end) {
+          store8(out + at + n, base != nullptr ? load8(base + at + n) : u32x4{0u, 0u, 0u, 0u});
+        } else {
+          for (int e = n; e < strip_end; ++e) out[at + e] = base != nullptr ? base[at + e] : uint16_t(0);
+        }
+      }
     }
   }
-  for (int turn = 0; w.left != 0; turn = turn + 1 == p.splits ? 0 : turn + 1) {
-    int which;
-    const uint64_t mine = w.next(which);
-    if (turn != split) continue;
-    const int list = Window::list(mine), rows = __popcll(mine);
+  const int count = plan.count, pieces = plan.pieces;
+  for (int turn = share; turn < count; turn += p.shares) {
+    const int which = plan.adapter[turn];
+    const uint64_t mine = plan.rows[turn];
+    const int list = list_rows(mine), rows = __popcll(mine);
     const uint16_t* weights = static_cast<const uint16_t*>(a.b) + (uint64_t)which * columns * a.rank;
     const float scale = a.scales != nullptr ? a.scales[which] : 1.0f;
-    // the row of b_l that is this lane's row of tile i, so that a lane ends up with neighbouring columns
-    uint32_t at[4];
+    for (int row0 = 0; row0 < rows; row0 += GROUP) {
+      {
+        const int row = tid / TPR, part = tid % TPR;
+        const float* v = p.v + (uint64_t)(first + __shfl(list, min(row0 + row, rows - 1))) * p.v_pitch;
+        f32x4 x[EACH];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) at[i] = (uint32_t)min(column0 + (c >> 2) * 16 + i * 4 + (c & 3), columns - 1);
-    f32x4 acc[4][4];
+        for (int j = 0; j < EACH; ++j) x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int piece = 0; piece < pieces; piece += IN_FLIGHT) {
+          f32x4 one[IN_FLIGHT][EACH];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+          for (int f = 0; f < IN_FLIGHT; ++f)
 #pragma unroll
-      for (int m = 0; m < 4; ++m) acc[i][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    // four threads have a row of v: 4 of every 16 ranks each
-    const int row = tid >> 2, part = tid & 3;
-    const float* v = p.v + (uint64_t)(first + __shfl(list, row)) * p.v_pitch;
-    auto four = [&](int r) {
-      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (row >= rows) return sum;
-      for (int piece = 0; piece < p.pieces; ++piece) {
-        const f32x4 one = *reinterpret_cast<const f32x4*>(v + (uint64_t)piece * a.rows * p.v_pitch + r);
-        sum += one;
-      }
+            for (int j = 0; j < EACH; ++j) {
+              const int r = (j * TPR + part) * 4;
+              one[f][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+              if (piece + f < pieces && r < a.rank && row0 + row < rows)
+                one[f][j] = *reinterpret_cast<const f32x4*>(v + (uint64_t)(piece + f) * a.rows * p.v_pitch + r);
+            }
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (r + e >= a.rank) sum[e] = 0.0f;
-      return sum;
-    };
-    float scaling = 1.0f;
-    if constexpr (DT == kF16) {
-      // v may be larger than the type holds: its row is scaled to below 1 by a power of two, exactly
-      float most = 0.0f;
-      for (int r = part * 4; r < a.rank; r += 16) {
-        const f32x4 x = four(r);
+          for (int f = 0; f < IN_FLIGHT; ++f)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[e]));
-      }
-      most = fmaxf(most, __shfl_xor(most, 1));
-      most = fmaxf(most, __shfl_xor(most, 2));
-      // (rows of zeros, and of infinities, which stay what they are)
-      const int up = most > 0.0f && most < INFINITY ? min(max(ilogbf(most) + 1, -100), 120) : 0;
-      scaling = ldexpf(1.0f, -up);
-      __syncthreads();
-      if (part == 0) unit[row] = ldexpf(1.0f, up);
-    }
-    for (int r0 = 0; r0 < a.rank; r0 += kRankStep) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kRankStep / 16; ++j) {
-        const int r = j * 16 + part * 4;
-        const f32x4 x = r0 + r < a.rank ? four(r0 + r) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        u32x2 high, low;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t h[2], l[2];
-#pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            const float s = x[2 * e + o] * scaling;
-            h[o] = round_bits<DT>(s);
-            const float rest = s - widen_bits<DT>((uint16_t)h[o]);
-            l[o] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : 0u;
-          }
-          high[e] = h[0] | h[1] << 16;
-          low[e] = l[0] | l[1] << 16;
+            for (int j = 0; j < EACH; ++j) x[j] += one[f][j];
         }
-        *reinterpret_cast<u32x2*>(&split_v[0][row][r]) = high;
-        *reinterpret_cast<u32x2*>(&split_v[1][row][r]) = low;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((j * TPR + part) * 4 + e >= a.rank) x[j][e] = 0.0f;   // (what lies behind a row of v is not written)
+        float scaling = 1.0f;
+        int up = 0;
+        if constexpr (DT == kF16) {
+          // v may be larger than the type holds: its row is scaled to below 1 by a power of two, exactly
+          float most = 0.0f;
+#pragma unroll
+          for (int j = 0; j < EACH; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[j][e]));
+#pragma unroll
+          for (int other = 1; other < TPR; other *= 2) most = fmaxf(most, __shfl_xor(most, other));
+          // (rows of zeros, and of infinities, stay what they are)
+          if (most > 0.0f && most < INFINITY) up = min(max(ilogbf(most) + 1, -100), 120);
+          scaling = ldexpf(1.0f, -up);
+        }
+        __syncthreads();
+        if (DT == kF16 && part == 0) unit[row] = ldexpf(1.0f, up);
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          u32x2 high, low;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t h[2], l[2];
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+              const float s = x[j][2 * e + o] * scaling;
+              h[o] = round_bits<DT>(s);
+              const float rest = s - widen_bits<DT>((uint16_t)h[o]);
+              l[o] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : 0u;
+            }
+            high[e] = h[0] | h[1] << 16;
+            low[e] = l[0] | l[1] << 16;
+          }
+          const int r = (j * TPR + part) * 4;
+          *reinterpret_cast<u32x2*>(&split_v[0][row][r]) = high;
+          *reinterpret_cast<u32x2*>(&split_v[1][row][r]) = low;
+        }
+        __syncthreads();
       }
-      __syncthreads();
-      const int depth = min(kRankStep, a.rank - r0);
-      for (int k = 0; k < depth; k += 32) {
-        u32x4 b[4];
+      for (int column0 = strip_begin + wave * 64; column0 < strip_end; column0 += kBlock) {
+        const bool whole = column0 + 64 <= columns;
+        // a lane's columns: own .. own + 7 and own + 32 .. own + 39
+        const int own = column0 + q * 8;
+        u32x4 have[M][2];
+        uint64_t to[M];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = load8_within(weights + (uint64_t)at[i] * a.rank, r0 + k + q * 8, a.rank);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          if (16 * m >= rows) break;
-#pragma unroll
-          for (int part_of = 0; part_of < 2; ++part_of) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(&split_v[part_of][16 * m + c][k + q * 8]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              acc[i][m] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, x), acc[i][m]);
+        for (int m = 0; m < M; ++m) {
+          to[m] = (uint64_t)(first + __shfl(list, min(row0 + 16 * m + c, rows - 1))) * columns + own;
+          have[m][0] = have[m][1] = u32x4{0u, 0u, 0u, 0u};
+          if (base != nullptr && whole && row0 + 16 * m < rows) {
+            have[m][0] = load8(base + to[m]);
+            have[m][1] = load8(base + to[m] + 32);
           }
         }
-      }
-    }
+        // the row of b_l that is this lane's row of tile i
+        u32x4 b[STEPS][4];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      if (16 * m >= rows) break;
-      const int of = 16 * m + c, from = __shfl(list, of);
-      if (of >= rows || own >= columns) continue;
-      const float s = DT == kF16 ? scale * unit[of] : scale;
-      const uint64_t to = (uint64_t)(first + from) * columns + own;
-      float y[16];
+        for (int i = 0; i < 4; ++i) {
+          const uint16_t* from = weights + (uint64_t)min(column0 + i / 2 * 32 + (c >> 2) * 8 + i % 2 * 4 + (c & 3), columns - 1) * a.rank;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[4 * i + e] = s * acc[i][m][e];
-      if (own + 16 <= columns) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4 have = {0u, 0u, 0u, 0u};
-          if (base != nullptr) have = load8(base + to + 8 * h);
-          u32x4 bits;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float lo = widen_bits<DT>((uint16_t)have[e]) + y[8 * h + 2 * e];
-            const float hi = widen_bits<DT>((uint16_t)(have[e] >> 16)) + y[8 * h + 2 * e + 1];
-            bits[e] = round_bits<DT>(lo) | (uint32_t)round_bits<DT>(hi) << 16;
+          for (int k = 0; k < STEPS; ++k) {
+            const int r = KS == 0 ? (q & 1) * 8 : k * 32 + q * 8;
+            b[k][i] = a.rank == RANKS ? load8(from + r) : load8_within(from, r, a.rank);
           }
-          store8(out + to + 8 * h, bits);
         }
-      } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (own + e < columns) out[to + e] = round_bits<DT>((base != nullptr ? widen_bits<DT>(base[to + e]) : 0.0f) + y[e]);
+        for (int m = 0; m < M; ++m) {
+          if (row0 + 16 * m >= rows) break;
+          f32x4 acc[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int half = 0; half < (KS == 0 ? 1 : 2); ++half) {
+              const u32x4 x = *reinterpret_cast<const u32x4*>(KS == 0 ? &split_v[q >> 1][16 * m + c][(q & 1) * 8]
+                                                                       : &split_v[half][16 * m + c][k * 32 + q * 8]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[i] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, b[k][i]), __builtin_bit_cast(bf16x8, x), acc[i]);
+            }
+          if (row0 + 16 * m + c >= rows) continue;
+          const float s = DT == kF16 ? scale * unit[16 * m + c] : scale;
+          if (whole) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              u32x4 bits;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const f32x4& y = acc[2 * h + e / 2];
+                const float lo = widen_bits<DT>((uint16_t)have[m][h][e]) + s * y[e % 2 * 2];
+                const float hi = widen_bits<DT>((uint16_t)(have[m][h][e] >> 16)) + s * y[e % 2 * 2 + 1];
+                bits[e] = round_bits<DT>(lo) | (uint32_t)round_bits<DT>(hi) << 16;
+              }
+              store8(out + to[m] + 32 * h, bits);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int at = e / 8 * 32 + e % 8;
+              if (own + at < columns)
+                out[to[m] + at] = round_bits<DT>((base != nullptr ? widen_bits<DT>(base[to[m] + at]) : 0.0f) + s * acc[e / 4][e % 4]);
+            }
+          }
+        }
       }
     }
   }
 }
 
 struct AdapterPlan {
-  int64_t windows, v_pitch, pieces, shrink_splits, strips, expand_splits;
+  int64_t windows, v_pitch, pieces, v_shares, strip, strips, shares;
+  uint64_t plans_bytes;
 };
 
 // Workgroups that keep the device busy.
@@ -282,21 +339,27 @@ constexpr int64_t kBusy = 1024;
 
 AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
   AdapterPlan f;
-  const int64_t most = num < kWindow ? (num < rows ? num : rows) : (rows < kWindow ? rows : kWindow);   // adapters of a window
-  auto between = [](int64_t v, int64_t hi) { return v > hi ? (hi < 1 ? 1 : hi) : (v < 1 ? 1 : v); };
+  auto between = [](int64_t v, int64_t hi) { return std::max<int64_t>(1, std::min(v, hi)); };
+  const int64_t most = std::min({num, rows, int64_t(kWindow)});   // adapters of a window
   f.windows = (rows + kWindow - 1) / kWindow;
   f.v_pitch = (rank + 3) / 4 * 4;
-  f.shrink_splits = between(kBusy / f.windows, most);
-  // the depth in pieces of at least one step of every wave
-  f.pieces = between(between(hidden_in / (64 * kFewWaves), 8), kBusy / (f.windows * f.shrink_splits) < 1 ? 1 : kBusy / (f.windows * f.shrink_splits));
-  f.strips = (hidden_out + kStrip - 1) / kStrip;
-  f.expand_splits = between(kBusy / (f.windows * f.strips), most);
+  // pieces of the depth: at least one step of every wave
+  f.pieces = between(hidden_in / (64 * kFewWaves), 8);
+  f.v_shares = between(kBusy / f.windows, most * f.pieces);
+  f.pieces = std::min(f.pieces, f.v_shares);
+  // strips of several blocks where there are many, each of which would have to split v again
+  const int64_t blocks = (hidden_out + kBlock - 1) / kBlock;
+  f.strip = between(f.windows * blocks / kBusy, 8) * kBlock;
+  f.strips = (hidden_out + f.strip - 1) / f.strip;
+  f.shares = between(kBusy / (f.windows * f.strips), most);
+  f.plans_bytes = (uint64_t)f.windows * sizeof(WindowPlan);
+  static_assert(sizeof(WindowPlan) % 16 == 0, "");
   return f;
 }
 
 template <int DT, int TILES>
 void launch_shrink(const AdapterParams& p, const AdapterPlan& f, hipStream_t stream) {
-  const dim3 grid((uint32_t)(f.windows * f.shrink_splits), (uint32_t)f.pieces);
+  const dim3 grid((uint32_t)(f.windows * f.v_shares));
   if (p.a.rows <= kWindow) {
     hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, 1>), grid, dim3(kFewThreads), 0, stream, p);
   } else {
@@ -309,11 +372,13 @@ hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
   const AdapterPlan f = adapter_plan(a.rows, a.num, a.rank, a.hidden_in, a.hidden_out);
   AdapterParams p;
   p.a = a;
-  p.v = static_cast<float*>(a.scratch);
+  p.plans = static_cast<WindowPlan*>(a.scratch);
+  p.v = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + f.plans_bytes);
   p.v_pitch = (int32_t)f.v_pitch;
   p.pieces = (int32_t)f.pieces;
+  p.shares = (int32_t)f.v_shares;
   p.strips = (int32_t)f.strips;
-  p.splits = (int32_t)f.shrink_splits;
+  p.strip = (int32_t)f.strip;
   if (a.rank <= 16) {
     launch_shrink<DT, 1>(p, f, stream);
   } else if (a.rank <= 32) {
@@ -323,8 +388,19 @@ hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
   }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  p.splits = (int32_t)f.expand_splits;
-  hipLaunchKernelGGL((adapter_expand_kernel<DT>), dim3((uint32_t)(f.windows * f.expand_splits * f.strips)), dim3(kExpandThreads), 0, stream, p);
+  p.shares = (int32_t)f.shares;
+  const dim3 grid((uint32_t)(f.windows * f.shares * f.strips));
+  if (a.rank <= 16) {
+    hipLaunchKernelGGL((adapter_expand_kernel<DT, 0>), grid, dim3(kExpandThreads), 0, stream, p);
+  } else if (a.rank <= 32) {
+    hipLaunchKernelGGL((adapter_expand_kernel<DT, 1>), grid, dim3(kExpandThreads), 0, stream, p);
+  } else if (a.rank <= 64) {
+    hipLaunchKernelGGL((adapter_expand_kernel<DT, 2>), grid, dim3(kExpandThreads), 0, stream, p);
+  } else if (a.rank <= 128) {
+    hipLaunchKernelGGL((adapter_expand_kernel<DT, 4>), grid, dim3(kExpandThreads), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((adapter_expand_kernel<DT, 8>), grid, dim3(kExpandThreads), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
@@ -333,12 +409,12 @@ hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
 bool adapters_fit(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
   const AdapterPlan f = adapter_plan(rows, num, rank, hidden_in, hidden_out);
   const int64_t threads = int64_t(1) << 32;   // of a launch, which are counted in 32 bits
-  return f.windows * f.shrink_splits * kFewThreads < threads && f.windows * f.expand_splits * f.strips * kExpandThreads < threads;
+  return f.windows * f.v_shares * kFewThreads < threads && f.windows * f.shares * f.strips * kExpandThreads < threads;
 }
 
 uint64_t adapters_scratch_bytes(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
   const AdapterPlan f = adapter_plan(rows, num, rank, hidden_in, hidden_out);
-  return (uint64_t)(f.pieces * rows * f.v_pitch) * sizeof(float);
+  return f.plans_bytes + (uint64_t)(f.pieces * rows * f.v_pitch) * sizeof(float);
 }
 
 hipError_t adapters(const AdapterArgs& a, hipStream_t stream) {

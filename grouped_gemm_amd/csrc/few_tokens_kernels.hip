@@ -330,6 +330,7 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
 
 struct FewPlan {
   int64_t slots, named, up_tiles, down_tiles, pieces, ffn_pitch, hidden_pitch;
+  int up_rows, down_rows;   // of 16, that a workgroup takes at a time
   uint64_t arrivals_bytes, h_bytes, parts_bytes;
 };
 
@@ -346,6 +347,11 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   // token, 4096 -> 14336, in 1, 2, 4, 8 pieces: 64 strips 58, 34, 25, 26 us, 128 strips 65, 43, 44, 53, 512 strips 160, 185, 188, 193
   const int64_t steps = (ffn + (nt ? 63 : 31)) / (nt ? 64 : 32), fit = kFewUnits / (f.named * f.down_tiles), deep = steps / (8 * kFewWaves);
   f.pieces = std::max<int64_t>(1, std::min({fit, deep, int64_t(16)}));
+  // Rows taken at a time, by how many an expert has on average (of down two for each slot; those that do not fit read the weights again): more of them
+  // leave fewer waves to a compute unit.  us with 1, 2 and 4 times 16, averages 3, 4, 8, 16: gate | up 77 78 81, 279 281 281,
+  // 340 348 368, 528 361 373; down 48 54 54, 180 153 161, 281 176 178, 469 316 212.
+  f.up_rows = f.slots <= 8 * experts ? 1 : 2;
+  f.down_rows = f.slots < 4 * experts ? 1 : (f.slots <= 12 * experts ? 2 : 4);
   f.arrivals_bytes = (uint64_t)(f.down_tiles * 4 + 255) / 256 * 256;
   f.h_bytes = ((uint64_t)f.slots * f.ffn_pitch * 4 + 255) / 256 * 256;
   f.hidden_pitch = (hidden + 3) / 4 * 4;
@@ -353,7 +359,7 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   return f;
 }
 
-template <int DT, bool NT, int MT>
+template <int DT, bool NT>
 hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stream) {
   FewParams p;
   p.a = a;
@@ -368,11 +374,20 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   p.tiles = (int32_t)f.up_tiles;
   p.pieces = (int32_t)f.pieces;
   p.counters = (int32_t)f.down_tiles;
-  hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, MT>), dim3((uint32_t)(f.named * f.up_tiles)), dim3(gate_up_threads(NT)), 0, stream, p);
+  const dim3 up((uint32_t)(f.named * f.up_tiles)), down((uint32_t)(f.named * f.down_tiles * f.pieces));
+  if (f.up_rows == 1) {
+    hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, 1>), up, dim3(gate_up_threads(NT)), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, 2>), up, dim3(gate_up_threads(NT)), 0, stream, p);
+  }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   p.tiles = (int32_t)f.down_tiles;
-  hipLaunchKernelGGL((few_down_kernel<DT, NT, MT>), dim3((uint32_t)(f.named * f.down_tiles * f.pieces)), dim3(kFewThreads), 0, stream, p);
+  switch (f.down_rows) {
+    case 1: hipLaunchKernelGGL((few_down_kernel<DT, NT, 1>), down, dim3(kFewThreads), 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((few_down_kernel<DT, NT, 2>), down, dim3(kFewThreads), 0, stream, p); break;
+    default: hipLaunchKernelGGL((few_down_kernel<DT, NT, 4>), down, dim3(kFewThreads), 0, stream, p); break;
+  }
   return hipGetLastError();
 }
 
@@ -391,10 +406,7 @@ uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k
 
 hipError_t few_tokens(const FewTokensArgs& a, hipStream_t stream) {
   const FewPlan f = few_plan(a.tokens, a.experts, a.top_k, a.hidden, a.ffn, a.trans_b);
-  const bool one = a.tokens <= 16 || f.slots <= 8 * a.experts;   // rows of an expert fit one matrix tile (unless a token names an expert twice)
-#define GG_LAUNCH(DT)                                                                                            \
-  (a.trans_b ? (one ? launch_few<DT, true, 1>(a, f, stream) : launch_few<DT, true, 2>(a, f, stream))             \
-             : (one ? launch_few<DT, false, 1>(a, f, stream) : launch_few<DT, false, 2>(a, f, stream)))
+#define GG_LAUNCH(DT) (a.trans_b ? launch_few<DT, true>(a, f, stream) : launch_few<DT, false>(a, f, stream))
   return a.dt == kBF16 ? GG_LAUNCH(kBF16) : GG_LAUNCH(kF16);
 #undef GG_LAUNCH
 }
