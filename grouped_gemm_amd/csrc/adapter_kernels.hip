@@ -39,9 +39,7 @@ struct AdapterParams {
   WindowPlan* plans;   // [windows]
   int32_t v_pitch;
   int32_t pieces;      // of the depth hidden_in, at most
-  int32_t shares;      // workgroups of a window (of one of its strips)
-  int32_t strips;      // of hidden_out
-  int32_t strip;       // columns of a strip
+  int32_t shares;      // workgroups of a window
 };
 
 // The same from the rows' adapters, in the lanes of a wave.
@@ -162,31 +160,35 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
   __shared__ float unit[GROUP];
   const AdapterArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4, wave = uniform(tid >> 6);
-  uint32_t block = blockIdx.x;
-  const int strip = (int)(block % p.strips);
-  block /= p.strips;
-  const int share = (int)(block % p.shares);
-  const WindowPlan& plan = p.plans[block / p.shares];
-  const int64_t first = (int64_t)(block / p.shares) * kWindow;
-  const int strip_begin = strip * p.strip, strip_end = min(strip_begin + p.strip, a.hidden_out), columns = a.hidden_out;
+  const int64_t window = blockIdx.x / p.shares, first = window * kWindow;
+  const int share = (int)(blockIdx.x - window * p.shares), columns = a.hidden_out, blocks = (columns + kBlock - 1) / kBlock;
+  const WindowPlan& plan = p.plans[window];
   const uint16_t* base = static_cast<const uint16_t*>(a.base);
   uint16_t* out = static_cast<uint16_t*>(a.out);
-  if (share == 0 && plan.none != 0 && out != base) {   // rows without an adapter
+  if (plan.none != 0 && out != base) {   // rows without an adapter: every workgroup has a part of their columns
+    const int begin = (int)((int64_t)blocks * share / p.shares) * kBlock;
+    const int end = min((int)((int64_t)blocks * (share + 1) / p.shares) * kBlock, columns);
     int r = 0;
     for (uint64_t none = plan.none; none != 0; none &= none - 1, ++r) {
       if (r % kExpandWaves != wave) continue;
       const uint64_t at = (uint64_t)(first + __ffsll((unsigned long long)none) - 1) * columns;
-      for (int n = strip_begin + lane * 8; n < strip_end; n += 512) {
-        if (n + 8 <= strip_end) {
+      for (int n = begin + lane * 8; n < end; n += 512) {
+        if (n + 8 <= end) {
           store8(out + at + n, base != nullptr ? load8(base + at + n) : u32x4{0u, 0u, 0u, 0u});
         } else {
-          for (int e = n; e < strip_end; ++e) out[at + e] = base != nullptr ? base[at + e] : uint16_t(0);
+          for (int e = n; e < end; ++e) out[at + e] = base != nullptr ? base[at + e] : uint16_t(0);
         }
       }
     }
   }
   const int count = plan.count, pieces = plan.pieces;
-  for (int turn = share; turn < count; turn += p.shares) {
+  if (count == 0) return;
+  // the window's workgroups: one to a strip of columns of an adapter, or, of more adapters, all columns of every shares-th one
+  const int strips = min(max(p.shares / count, 1), blocks), strip = share / count;
+  if (count <= p.shares && strip >= strips) return;
+  const int strip_begin = count <= p.shares ? (int)((int64_t)blocks * strip / strips) * kBlock : 0;
+  const int strip_end = count <= p.shares ? min((int)((int64_t)blocks * (strip + 1) / strips) * kBlock, columns) : columns;
+  for (int turn = count <= p.shares ? share % count : share; turn < count; turn += p.shares) {
     const int which = plan.adapter[turn];
     const uint64_t mine = plan.rows[turn];
     const int list = list_rows(mine), rows = __popcll(mine);
@@ -263,17 +265,20 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
         const bool whole = column0 + 64 <= columns;
         // a lane's columns: own .. own + 7 and own + 32 .. own + 39
         const int own = column0 + q * 8;
-        u32x4 have[M][2];
-        uint64_t to[M];
+        constexpr int AHEAD = KS <= 1 ? M : (M < 2 ? M : 2);   // tiles of rows whose part of base is asked for early
+        u32x4 have[AHEAD][2];
+        uint64_t to[AHEAD];
+        auto ask = [&](int m) {
+          to[m % AHEAD] = (uint64_t)(first + __shfl(list, min(row0 + 16 * m + c, rows - 1))) * columns + own;
+          have[m % AHEAD][0] = have[m % AHEAD][1] = u32x4{0u, 0u, 0u, 0u};
+          if (base != nullptr && row0 + 16 * m < rows) {
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          to[m] = (uint64_t)(first + __shfl(list, min(row0 + 16 * m + c, rows - 1))) * columns + own;
-          have[m][0] = have[m][1] = u32x4{0u, 0u, 0u, 0u};
-          if (base != nullptr && whole && row0 + 16 * m < rows) {
-            have[m][0] = load8(base + to[m]);
-            have[m][1] = load8(base + to[m] + 32);
+            for (int h = 0; h < 2; ++h)
+              have[m % AHEAD][h] = whole ? load8(base + to[m % AHEAD] + 32 * h) : load8_within(base + to[m % AHEAD] - own, own + 32 * h, columns);
           }
-        }
+        };
+#pragma unroll
+        for (int m = 0; m < AHEAD; ++m) ask(m);
         // the row of b_l that is this lane's row of tile i
         u32x4 b[STEPS][4];
 #pragma unroll
@@ -300,29 +305,30 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
 #pragma unroll
               for (int i = 0; i < 4; ++i) acc[i] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, b[k][i]), __builtin_bit_cast(bf16x8, x), acc[i]);
             }
-          if (row0 + 16 * m + c >= rows) continue;
+          const bool mine_too = row0 + 16 * m + c < rows;
           const float s = DT == kF16 ? scale * unit[16 * m + c] : scale;
-          if (whole) {
+          if (mine_too) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               u32x4 bits;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const f32x4& y = acc[2 * h + e / 2];
-                const float lo = widen_bits<DT>((uint16_t)have[m][h][e]) + s * y[e % 2 * 2];
-                const float hi = widen_bits<DT>((uint16_t)(have[m][h][e] >> 16)) + s * y[e % 2 * 2 + 1];
+                const float lo = widen_bits<DT>((uint16_t)have[m % AHEAD][h][e]) + s * y[e % 2 * 2];
+                const float hi = widen_bits<DT>((uint16_t)(have[m % AHEAD][h][e] >> 16)) + s * y[e % 2 * 2 + 1];
                 bits[e] = round_bits<DT>(lo) | (uint32_t)round_bits<DT>(hi) << 16;
               }
-              store8(out + to[m] + 32 * h, bits);
-            }
-          } else {
+              uint16_t* at = out + to[m % AHEAD] + 32 * h;
+              if (whole || own + 32 * h + 8 <= columns) {
+                store8(at, bits);
+              } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int at = e / 8 * 32 + e % 8;
-              if (own + at < columns)
-                out[to[m] + at] = round_bits<DT>((base != nullptr ? widen_bits<DT>(base[to[m] + at]) : 0.0f) + s * acc[e / 4][e % 4]);
+                for (int e = 0; e < 8; ++e)
+                  if (own + 32 * h + e < columns) at[e] = (uint16_t)(bits[e / 2] >> (16 * (e % 2)));
+              }
             }
           }
+          if (m + AHEAD < M) ask(m + AHEAD);
         }
       }
     }
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
 }
 
 struct AdapterPlan {
-  int64_t windows, v_pitch, pieces, v_shares, strip, strips, shares;
+  int64_t windows, v_pitch, pieces, v_shares, shares;
   uint64_t plans_bytes;
 };
 
@@ -343,15 +349,12 @@ AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden
   const int64_t most = std::min({num, rows, int64_t(kWindow)});   // adapters of a window
   f.windows = (rows + kWindow - 1) / kWindow;
   f.v_pitch = (rank + 3) / 4 * 4;
-  // pieces of the depth: at least one step of every wave
+  // pieces of the depth: at least one step of every wave.  v and out in 1, 2, 4, 8, 16 pieces, us: one row (4096 -> 4096) 7.0 + 5.0,
+  // 5.3 + 5.2, 4.3 + 5.1, 4.0 + 5.4, 3.6 + 6.1; 8192 rows of prompts (4096 -> 14336) 173 + 169, 93 + 169, 57 + 174, 40 + 178, 40 + 179
   f.pieces = between(hidden_in / (64 * kFewWaves), 8);
   f.v_shares = between(kBusy / f.windows, most * f.pieces);
   f.pieces = std::min(f.pieces, f.v_shares);
-  // strips of several blocks where there are many, each of which would have to split v again
-  const int64_t blocks = (hidden_out + kBlock - 1) / kBlock;
-  f.strip = between(f.windows * blocks / kBusy, 8) * kBlock;
-  f.strips = (hidden_out + f.strip - 1) / f.strip;
-  f.shares = between(kBusy / (f.windows * f.strips), most);
+  f.shares = between(kBusy / f.windows, most * ((hidden_out + kBlock - 1) / kBlock));
   f.plans_bytes = (uint64_t)f.windows * sizeof(WindowPlan);
   static_assert(sizeof(WindowPlan) % 16 == 0, "");
   return f;
@@ -363,7 +366,7 @@ void launch_shrink(const AdapterParams& p, const AdapterPlan& f, hipStream_t str
   if (p.a.rows <= kWindow) {
     hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, 1>), grid, dim3(kFewThreads), 0, stream, p);
   } else {
-    hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, 4>), grid, dim3(kFewThreads), 0, stream, p);
+    hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, 2>), grid, dim3(kFewThreads), 0, stream, p);
   }
 }
 
@@ -377,8 +380,6 @@ hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
   p.v_pitch = (int32_t)f.v_pitch;
   p.pieces = (int32_t)f.pieces;
   p.shares = (int32_t)f.v_shares;
-  p.strips = (int32_t)f.strips;
-  p.strip = (int32_t)f.strip;
   if (a.rank <= 16) {
     launch_shrink<DT, 1>(p, f, stream);
   } else if (a.rank <= 32) {
@@ -389,7 +390,7 @@ hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   p.shares = (int32_t)f.shares;
-  const dim3 grid((uint32_t)(f.windows * f.shares * f.strips));
+  const dim3 grid((uint32_t)(f.windows * f.shares));
   if (a.rank <= 16) {
     hipLaunchKernelGGL((adapter_expand_kernel<DT, 0>), grid, dim3(kExpandThreads), 0, stream, p);
   } else if (a.rank <= 32) {
@@ -409,7 +410,7 @@ hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
 bool adapters_fit(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
   const AdapterPlan f = adapter_plan(rows, num, rank, hidden_in, hidden_out);
   const int64_t threads = int64_t(1) << 32;   // of a launch, which are counted in 32 bits
-  return f.windows * f.v_shares * kFewThreads < threads && f.windows * f.shares * f.strips * kExpandThreads < threads;
+  return f.windows * f.v_shares * kFewThreads < threads && f.windows * f.shares * kExpandThreads < threads;
 }
 
 uint64_t adapters_scratch_bytes(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {

@@ -63,6 +63,23 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
 
+// ... and of the 16 bits of a two-byte type.
+template <int DT>
+__device__ __forceinline__ uint32_t short_key(float x) {
+  const uint32_t bits = Logit<DT>::narrow(x + 0.0f);   // (exact)
+  const uint32_t key = (bits ^ ((bits & 0x8000u) ? 0xffffu : 0x8000u)) & 0xffffu;
+  return x != x ? 0xffffu : key;
+}
+template <int DT>
+__device__ __forceinline__ float short_key_value(uint32_t key) {
+  if constexpr (DT == kF32) return 0.0f;
+  return Logit<DT>::widen((typename Logit<DT>::T)(key ^ ((key & 0x8000u) ? 0x8000u : 0xffffu)));
+}
+
+// The exponential by the hardware's power of two, off by 2^-24 |x| and a unit in the last place: for the scores of all experts, whose
+// sums and gradients that does not show in.  The chosen weights are computed with the full functions.
+__device__ __forceinline__ float quick_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+__device__ __forceinline__ float quick_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + quick_exp(-x)); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.0f) - log1pf(expf(-fabsf(x))); }
 
@@ -104,9 +121,14 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
   for (int64_t t = first + group; t < last; t += kRouteThreads / G) {
     float x[VPL];
     load_logits<DT, VPL>(a.logits, t, a.experts, column, x);
+    // Two-byte logits leave room for their column below, so that no two keys are equal.
+    constexpr bool UNIQUE = DT != kF32;
     uint32_t key[VPL];
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) key[v] = column + v < a.experts ? order_key(x[v]) : 0u;
+    for (int v = 0; v < VPL; ++v) {
+      key[v] = column + v < a.experts ? order_key(x[v]) : 0u;
+      if (UNIQUE && column + v < a.experts) key[v] = (short_key<DT>(x[v]) << 16) | (uint32_t)(0xffff - (column + v));
+    }
     float value[KR];
     int index[KR];
 #pragma unroll
@@ -118,12 +140,20 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
       for (int v = 1; v < VPL; ++v) best = best > key[v] ? best : key[v];
       best = group_max<G>(best);
       uint32_t at = ~0u;
+      float found;
+      if constexpr (UNIQUE) {
 #pragma unroll
-      for (int v = VPL - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(column + v) : at;
-      at = group_min<G>(at);
+        for (int v = 0; v < VPL; ++v) key[v] = key[v] == best ? 0u : key[v];
+        at = 0xffffu - (best & 0xffffu);
+        found = short_key_value<DT>(best >> 16);
+      } else {
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) key[v] = at == (uint32_t)(column + v) ? 0u : key[v];
-      const float found = key_value(best);
+        for (int v = VPL - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(column + v) : at;
+        at = group_min<G>(at);
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) key[v] = at == (uint32_t)(column + v) ? 0u : key[v];
+        found = key_value(best);
+      }
       if (j == 0) top = found;
 #pragma unroll
       for (int r = 0; r < KR; ++r)
@@ -135,7 +165,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
       float s[VPL], sum = 0.0f;
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
-        s[v] = a.sigmoid ? sigmoid(x[v]) : expf(x[v] - base);
+        s[v] = a.sigmoid ? quick_sigmoid(x[v]) : quick_exp(x[v] - base);
         sum += s[v];
       }
       sum = group_sum<G>(sum);
@@ -419,7 +449,7 @@ __global__ __launch_bounds__(kBackThreads) void route_backward_kernel(RouteBackw
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
         at[v] = m[v] + (a.normalize ? 0.0f : at[v]);
-        s[v] = a.sigmoid ? sigmoid(x[v]) : expf(x[v] - base);
+        s[v] = a.sigmoid ? quick_sigmoid(x[v]) : quick_exp(x[v] - base);
         sum += s[v];
         dot += s[v] * at[v];
       }
@@ -432,7 +462,7 @@ __global__ __launch_bounds__(kBackThreads) void route_backward_kernel(RouteBackw
         for (int v = 0; v < VPL; ++v) out[v] += s[v] * scale * (at[v] - dot);
       } else {
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) out[v] += s[v] * sigmoid(-x[v]) * at[v];
+        for (int v = 0; v < VPL; ++v) out[v] += s[v] * quick_sigmoid(-x[v]) * at[v];   // (1 - s would lose all of a small difference)
       }
     }
     T* to = static_cast<T*>(a.logits_grad) + t * a.experts + column;
