@@ -339,7 +339,7 @@ constexpr int64_t kFewUnits = 256;   // compute units
 FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool nt) {
   FewPlan f;
   f.slots = tokens * top_k;
-  f.named = f.slots < experts ? f.slots : experts;   // at most
+  f.named = std::max<int64_t>(1, std::min(f.slots, experts));   // at most
   f.up_tiles = (ffn + (nt ? 31 : 127)) / (nt ? 32 : 128);
   f.down_tiles = (hidden + (nt ? 63 : 127)) / (nt ? 64 : 128);
   f.ffn_pitch = (ffn + 7) / 8 * 8;

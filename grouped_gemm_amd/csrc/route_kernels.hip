@@ -63,17 +63,19 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
 
-// ... and of the 16 bits of a two-byte type.
+// ... and of the bits of a two-byte type, in the upper half, with the column below: no two keys of a token are equal.
 template <int DT>
-__device__ __forceinline__ uint32_t short_key(float x) {
-  const uint32_t bits = Logit<DT>::narrow(x + 0.0f);   // (exact)
-  const uint32_t key = (bits ^ ((bits & 0x8000u) ? 0xffffu : 0x8000u)) & 0xffffu;
-  return x != x ? 0xffffu : key;
+__device__ __forceinline__ uint32_t unique_key(uint16_t bits, int column) {
+  constexpr uint32_t INFINITE = DT == kBF16 ? 0x7f80u : 0x7c00u;
+  uint32_t key = (uint32_t)bits == 0x8000u ? 0u : (uint32_t)bits;
+  key = (key & 0x7fffu) > INFINITE ? 0x7fffu : key;
+  key ^= (uint32_t)((int32_t)(key << 16) >> 31) | 0x8000u;
+  return key << 16 | (uint32_t)(0xffff - column);   // (bits above the 16 leave here)
 }
 template <int DT>
-__device__ __forceinline__ float short_key_value(uint32_t key) {
+__device__ __forceinline__ float unique_key_value(uint32_t key) {
   if constexpr (DT == kF32) return 0.0f;
-  return Logit<DT>::widen((typename Logit<DT>::T)(key ^ ((key & 0x8000u) ? 0x8000u : 0xffffu)));
+  else return Logit<DT>::widen((typename Logit<DT>::T)((key >> 16) ^ ((key >> 31) ? 0x8000u : 0xffffu)));
 }
 
 // The exponential by the hardware's power of two, off by 2^-24 |x| and a unit in the last place: for the scores of all experts, whose
@@ -91,19 +93,19 @@ struct RouteParams {
   float* mass_parts;       // [experts][blocks]
 };
 
-// The VPL logits of one lane, columns l * VPL .. of its token; columns past the last read as -inf.
+// The VPL logits of one lane, from `column` of its token on; columns past the last read as -inf.
 template <int DT, int VPL>
-__device__ __forceinline__ void load_logits(const void* logits, int64_t token, int experts, int column, float* x) {
+__device__ __forceinline__ Row<typename Logit<DT>::T, VPL> load_logits(const void* logits, int64_t token, int experts, int column) {
   using T = typename Logit<DT>::T;
   const T* from = static_cast<const T*>(logits) + token * experts + column;
+  Row<T, VPL> r;
   if (column + VPL <= experts) {
-    const Row<T, VPL> r = *reinterpret_cast<const Row<T, VPL>*>(from);
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) x[v] = Logit<DT>::widen(r.v[v]);
+    r = *reinterpret_cast<const Row<T, VPL>*>(from);
   } else {
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) x[v] = column + v < experts ? Logit<DT>::widen(from[v]) : -INFINITY;
+    for (int v = 0; v < VPL; ++v) r.v[v] = column + v < experts ? from[v] : Logit<DT>::narrow(-INFINITY);
   }
+  return r;
 }
 
 // Chooses for tokens first + group, first + group + groups, ... below last: a group of G lanes has one token,
@@ -119,45 +121,48 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
   const int group = threadIdx.x / G, l = threadIdx.x % G, column = l * VPL, k = a.top_k;
   const bool all_scores = a.mass != nullptr || !(a.normalize || a.sigmoid);
   for (int64_t t = first + group; t < last; t += kRouteThreads / G) {
-    float x[VPL];
-    load_logits<DT, VPL>(a.logits, t, a.experts, column, x);
-    // Two-byte logits leave room for their column below, so that no two keys are equal.
+    const auto raw = load_logits<DT, VPL>(a.logits, t, a.experts, column);
     constexpr bool UNIQUE = DT != kF32;
-    uint32_t key[VPL];
+    float x[VPL];
+    uint32_t key[VPL];   // (columns past the last are -inf, and behind all of the same: top_k others go before them)
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      key[v] = column + v < a.experts ? order_key(x[v]) : 0u;
-      if (UNIQUE && column + v < a.experts) key[v] = (short_key<DT>(x[v]) << 16) | (uint32_t)(0xffff - (column + v));
+      x[v] = Logit<DT>::widen(raw.v[v]);
+      if constexpr (UNIQUE) key[v] = unique_key<DT>(raw.v[v], column + v);
+      else key[v] = order_key(x[v]);
     }
-    float value[KR];
+    uint32_t chosen_key[KR], top_key = 0u;
     int index[KR];
 #pragma unroll
-    for (int r = 0; r < KR; ++r) value[r] = 0.0f, index[r] = 0;
-    float top = 0.0f;
+    for (int r = 0; r < KR; ++r) chosen_key[r] = 0u, index[r] = 0;
     for (int j = 0; j < k; ++j) {
       uint32_t best = key[0];
 #pragma unroll
       for (int v = 1; v < VPL; ++v) best = best > key[v] ? best : key[v];
       best = group_max<G>(best);
       uint32_t at = ~0u;
-      float found;
       if constexpr (UNIQUE) {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) key[v] = key[v] == best ? 0u : key[v];
-        at = 0xffffu - (best & 0xffffu);
-        found = short_key_value<DT>(best >> 16);
       } else {
 #pragma unroll
         for (int v = VPL - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(column + v) : at;
         at = group_min<G>(at);
 #pragma unroll
         for (int v = 0; v < VPL; ++v) key[v] = at == (uint32_t)(column + v) ? 0u : key[v];
-        found = key_value(best);
       }
-      if (j == 0) top = found;
+      if (j == 0) top_key = best;
 #pragma unroll
       for (int r = 0; r < KR; ++r)
-        if (j == l + r * G) value[r] = found, index[r] = (int)at;
+        if (r * G <= j && j == l + r * G) chosen_key[r] = best, index[r] = (int)at;
+    }
+    auto decode = [](uint32_t key) { return UNIQUE ? unique_key_value<DT>(key) : key_value(key); };
+    const float top = decode(top_key);
+    float value[KR];
+#pragma unroll
+    for (int r = 0; r < KR; ++r) {
+      value[r] = decode(chosen_key[r]);
+      if (UNIQUE) index[r] = 0xffff - (int)(chosen_key[r] & 0xffffu);
     }
     const float base = top == -INFINITY ? 0.0f : top;
     float share[KR], scale = 0.0f;
@@ -179,6 +184,8 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
       float sum = 0.0f;
 #pragma unroll
       for (int r = 0; r < KR; ++r) {
+        share[r] = 0.0f;
+        if (r * G >= k) continue;   // (the same in all lanes)
         share[r] = expf(a.sigmoid ? log_sigmoid(value[r]) - log_top : value[r] - base);
         if (l + r * G >= k) share[r] = 0.0f;
         sum += share[r];
@@ -188,7 +195,10 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
       for (int r = 0; r < KR; ++r) share[r] = sum == 0.0f ? 0.0f : share[r] / sum;
     } else {
 #pragma unroll
-      for (int r = 0; r < KR; ++r) share[r] = a.sigmoid ? sigmoid(value[r]) : expf(value[r] - base) * scale;
+      for (int r = 0; r < KR; ++r) {
+        share[r] = 0.0f;
+        if (r * G < k) share[r] = a.sigmoid ? sigmoid(value[r]) : expf(value[r] - base) * scale;
+      }
     }
 #pragma unroll
     for (int r = 0; r < KR; ++r) {
@@ -378,24 +388,25 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(RouteParams 
 //   normalized weights q = w add q_j (g_j - <g, q>) at the chosen (times 1 - s_j with the sigmoid).
 // What falls on the chosen columns goes to their lanes through LDS, one row of it for each group.
 constexpr int kBackThreads = 256;
+constexpr int64_t kBackBlocks = 1024;   // (65536 tokens x 256: 35 us; 768, 1536, 2048, 4096: 39, 36, 40, 49)
 
 template <int DT, int G, int VPL>
-__global__ __launch_bounds__(kBackThreads) void route_backward_kernel(RouteBackwardArgs a) {
+__global__ __launch_bounds__(kBackThreads, 4) void route_backward_kernel(RouteBackwardArgs a) {
   using T = typename Logit<DT>::T;
-  constexpr int KR = G == 16 ? 2 : 1, GROUPS = kBackThreads / G, WIDTH = G * VPL;
-  __shared__ __attribute__((aligned(16))) float rows[GROUPS * WIDTH];
+  constexpr int KR = G == 16 ? 2 : 1, GROUPS = kBackThreads / G, PITCH = VPL + 4;   // (of a lane's columns in LDS: 16 lanes start in different banks)
+  __shared__ __attribute__((aligned(16))) float rows[GROUPS * G * PITCH];
   const int group = threadIdx.x / G, l = threadIdx.x % G, column = l * VPL, k = a.top_k;
-  float* row = rows + group * WIDTH;
+  float *row = rows + group * G * PITCH, *own = row + l * PITCH;
   float m[VPL];
 #pragma unroll
   for (int v = 0; v < VPL; ++v) m[v] = a.mass_grad != nullptr && column + v < a.experts ? a.mass_grad[column + v] : 0.0f;
   const bool dense = a.mass_grad != nullptr || !a.normalize;
   for (int64_t t = (int64_t)blockIdx.x * GROUPS + group; t < a.tokens; t += (int64_t)gridDim.x * GROUPS) {
-    float x[VPL];
-    load_logits<DT, VPL>(a.logits, t, a.experts, column, x);
+    const auto raw = load_logits<DT, VPL>(a.logits, t, a.experts, column);
+    auto x = [&](int v) { return Logit<DT>::widen(raw.v[v]); };
     float top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) top = fmaxf(top, x[v]);
+    for (int v = 0; v < VPL; ++v) top = fmaxf(top, x(v));
     top = group_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); });
     const float base = top == -INFINITY ? 0.0f : top;
     // what falls on the chosen columns
@@ -414,7 +425,9 @@ __global__ __launch_bounds__(kBackThreads) void route_backward_kernel(RouteBackw
       float q[KR], sum = 0.0f, dot = 0.0f;
 #pragma unroll
       for (int r = 0; r < KR; ++r) {
-        q[r] = index[r] >= 0 ? expf(a.sigmoid ? log_sigmoid(value[r]) - log_top : value[r] - base) : 0.0f;
+        q[r] = 0.0f;
+        if (r * G >= k) continue;   // (the same in all lanes)
+        if (index[r] >= 0) q[r] = expf(a.sigmoid ? log_sigmoid(value[r]) - log_top : value[r] - base);
         sum += q[r];
       }
       sum = group_sum<G>(sum);
@@ -425,56 +438,58 @@ __global__ __launch_bounds__(kBackThreads) void route_backward_kernel(RouteBackw
       }
       dot = group_sum<G>(dot);
 #pragma unroll
-      for (int r = 0; r < KR; ++r) grad[r] = q[r] * (grad[r] - dot) * (a.sigmoid ? sigmoid(-value[r]) : 1.0f);
+      for (int r = 0; r < KR; ++r)
+        if (r * G < k) grad[r] = q[r] * (grad[r] - dot) * (a.sigmoid ? sigmoid(-value[r]) : 1.0f);
     }
     // (a row belongs to one wave, whose LDS accesses stay in order)
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) row[column + v] = 0.0f;
+    for (int v = 0; v < VPL; ++v) own[v] = 0.0f;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int r = 0; r < KR; ++r)
-      if (index[r] >= 0) row[index[r]] = grad[r];
+      if (index[r] >= 0) row[index[r] / VPL * PITCH + index[r] % VPL] = grad[r];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    float at[VPL], out[VPL];
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) at[v] = row[column + v];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) out[v] = a.normalize ? at[v] : 0.0f;
-    if (dense) {
-      float s[VPL], sum = 0.0f, dot = 0.0f;
+    // (everything else per column where it is needed, scores twice: registers are what this kernel is short of)
+    auto gradient = [&](int v) { return a.normalize ? m[v] : m[v] + own[v]; };   // of the column's score
+    float scale = 0.0f, dot = 0.0f;
+    if (dense && !a.sigmoid) {
+      float sum = 0.0f;
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
-        at[v] = m[v] + (a.normalize ? 0.0f : at[v]);
-        s[v] = a.sigmoid ? quick_sigmoid(x[v]) : quick_exp(x[v] - base);
-        sum += s[v];
-        dot += s[v] * at[v];
+        const float s = quick_exp(x(v) - base);
+        sum += s;
+        dot += s * gradient(v);
       }
-      if (!a.sigmoid) {
-        sum = group_sum<G>(sum);
-        dot = group_sum<G>(dot);
-        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-        dot *= scale;
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) out[v] += s[v] * scale * (at[v] - dot);
-      } else {
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) out[v] += s[v] * quick_sigmoid(-x[v]) * at[v];   // (1 - s would lose all of a small difference)
-      }
+      sum = group_sum<G>(sum);
+      scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+      dot = group_sum<G>(dot) * scale;
     }
+    Row<T, VPL> out;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      float sum = a.normalize ? own[v] : 0.0f;
+      if (dense) {
+        if (a.sigmoid) {
+          // (1 - score would lose all of a small difference; an infinite e has a score of 0)
+          const float e = quick_exp(-x(v)), score = __builtin_amdgcn_rcpf(1.0f + e);
+          sum += score * (fminf(e, 1e37f) * score) * gradient(v);
+        } else {
+          sum += quick_exp(x(v) - base) * scale * (gradient(v) - dot);
+        }
+      }
+      out.v[v] = Logit<DT>::narrow(sum);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     T* to = static_cast<T*>(a.logits_grad) + t * a.experts + column;
     if (column + VPL <= a.experts) {
-      Row<T, VPL> r;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) r.v[v] = Logit<DT>::narrow(out[v]);
-      *reinterpret_cast<Row<T, VPL>*>(to) = r;
+      *reinterpret_cast<Row<T, VPL>*>(to) = out;
     } else {
 #pragma unroll
       for (int v = 0; v < VPL; ++v)
-        if (column + v < a.experts) to[v] = Logit<DT>::narrow(out[v]);
+        if (column + v < a.experts) to[v] = out.v[v];
     }
   }
 }
@@ -522,7 +537,7 @@ template <int DT, int G, int VPL>
 hipError_t launch_backward(const RouteBackwardArgs& a, hipStream_t stream) {
   constexpr int64_t GROUPS = kBackThreads / G;
   const int64_t blocks = (a.tokens + GROUPS - 1) / GROUPS;
-  hipLaunchKernelGGL((route_backward_kernel<DT, G, VPL>), dim3((uint32_t)(blocks < 2048 ? blocks : 2048)), dim3(kBackThreads), 0, stream, a);
+  hipLaunchKernelGGL((route_backward_kernel<DT, G, VPL>), dim3((uint32_t)(blocks < kBackBlocks ? blocks : kBackBlocks)), dim3(kBackThreads), 0, stream, a);
   return hipGetLastError();
 }
 

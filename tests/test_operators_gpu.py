@@ -613,3 +613,25 @@ def test_lora_refuses(ops):
     square = [v.cuda() for v in _lora_case(6, 3, 8, 48, 48, torch.bfloat16, seed=1)]
     with pytest.raises(RuntimeError, match="overlap"):
         ops.lora(square[0], square[1], square[2], square[3], c=square[0])
+
+
+# ------------------------------------------------------------------ together
+
+def test_example_runs_the_operators_together(ops):
+    """Training lowers the loss; the decode form gives what the training form gives (which rounds the activation and each
+    expert's row to bfloat16 in between, each by up to 2^-8 of itself); the adapted projection gives the sum of its parts."""
+    import importlib.util
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "expert_layer.py")
+    spec = importlib.util.spec_from_file_location("expert_layer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, one, other, y, projection, x, adapters = example.main(steps=12)
+    assert losses[-1][0] < losses[0][0]
+    scale = float(one.float().pow(2).mean().sqrt())
+    assert float((one.float() - other.float()).abs().max()) <= 6 * 2.0 ** -8 * scale + 2.0 ** -7 * float(one.float().abs().max())
+    want = x.double() @ projection.weight[0].detach().double().t()
+    for i, n in enumerate(adapters.tolist()):
+        if n >= 0:
+            want[i] += 0.5 * (projection.b[n].double() @ (projection.a[n].double() @ x[i].double()))
+    off = (y.double() - want).abs() - (2.0 ** -7 * want.abs() + 2.0 ** -8 * float(want.detach().abs().max()))   # (rounded twice: the shared part, the sum)
+    assert float(off.max()) <= 0.0
