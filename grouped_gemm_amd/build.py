@@ -67,7 +67,7 @@ def pair_indices():
     return [int(m) for m in re.findall(r"^GG_PAIR\((\d+),", text, flags=re.M)]
 
 
-OPERATORS = ("route_kernels", "few_tokens_kernels", "adapter_kernels")
+OPERATORS = ("operators_api", "route_kernels", "few_tokens_kernels", "adapter_kernels")
 
 
 def build_hip(force=False, jobs=None):
