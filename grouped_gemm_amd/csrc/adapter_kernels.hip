@@ -74,8 +74,11 @@ __device__ __forceinline__ int list_rows(uint64_t mine) {
 }
 
 // v of one piece of the depth.  TILES: of 16 rows of a_l; more than 64 of them are taken 64 at a time.
-template <int DT, int TILES, int MT>
+// MT: of 16 rows, taken at a time (1 and 2, us: 64 rows of one adapter, rank 64, 15.0, 12.4; decode, a row or two to an adapter, 8.3, 8.4; one row 3.9, 4.1;
+// 8192 rows of prompts 59, 41).
+template <int DT, int TILES>
 __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterParams p) {
+  constexpr int MT = 2;
   using S = Stream<DT, true, TILES, MT>;
   __shared__ f32x4 lds[kFewWaves * 256];
   const AdapterArgs& a = p.a;
@@ -261,74 +264,117 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
         }
         __syncthreads();
       }
-      for (int column0 = strip_begin + wave * 64; column0 < strip_end; column0 += kBlock) {
-        const bool whole = column0 + 64 <= columns;
-        // a lane's columns: own .. own + 7 and own + 32 .. own + 39
-        const int own = column0 + q * 8;
-        constexpr int AHEAD = KS <= 1 ? M : (M < 2 ? M : 2);   // tiles of rows whose part of base is asked for early
-        u32x4 have[AHEAD][2];
-        uint64_t to[AHEAD];
-        auto ask = [&](int m) {
-          to[m % AHEAD] = (uint64_t)(first + __shfl(list, min(row0 + 16 * m + c, rows - 1))) * columns + own;
-          have[m % AHEAD][0] = have[m % AHEAD][1] = u32x4{0u, 0u, 0u, 0u};
-          if (base != nullptr && row0 + 16 * m < rows) {
+      auto product = [&](const u32x4 (&b)[STEPS][4], int m, f32x4 (&acc)[4]) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              have[m % AHEAD][h] = whole ? load8(base + to[m % AHEAD] + 32 * h) : load8_within(base + to[m % AHEAD] - own, own + 32 * h, columns);
+        for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+          for (int half = 0; half < (KS == 0 ? 1 : 2); ++half) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(KS == 0 ? &split_v[q >> 1][16 * m + c][(q & 1) * 8]
+                                                                     : &split_v[half][16 * m + c][k * 32 + q * 8]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, b[k][i]), __builtin_bit_cast(bf16x8, x), acc[i]);
           }
+      };
+      auto joined = [&](u32x4 base, const f32x4& y0, const f32x4& y1, int m) {
+        const float s = DT == kF16 ? scale * unit[16 * m + c] : scale;
+        u32x4 bits;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4& y = e < 2 ? y0 : y1;
+          const float lo = widen_bits<DT>((uint16_t)base[e]) + s * y[e % 2 * 2];
+          const float hi = widen_bits<DT>((uint16_t)(base[e] >> 16)) + s * y[e % 2 * 2 + 1];
+          bits[e] = round_bits<DT>(lo) | (uint32_t)round_bits<DT>(hi) << 16;
+        }
+        return bits;
+      };
+      // the row of tile i of b_l that is this lane's, of the 64 of a block
+      auto row_of_b = [&](int i) { return i / 2 * 32 + (c >> 2) * 8 + i % 2 * 4 + (c & 3); };
+      int column0 = strip_begin + wave * 64;
+      const int whole_end = a.rank == RANKS ? min(strip_end, columns - 63) : 0;
+      if (column0 < whole_end) {
+        // Whole blocks: all that a block needs is asked for at once, under no condition of a lane's.
+        u32x4 have[M][2], b[STEPS][4];
+        uint32_t of_row[M];
+        const uint16_t* base_window = base + first * columns;
+        uint16_t* out_window = out + first * columns;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          of_row[m] = ((uint32_t)__shfl(list, min(row0 + 16 * m + c, rows - 1)) * (uint32_t)columns + q * 8) * 2;
+        const uint32_t of_b = (uint32_t)(row_of_b(0) * RANKS + (KS == 0 ? (q & 1) * 8 : q * 8)) * 2;
+        auto ask_base = [&](int m, int at) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) have[m][h] = load8_at(base_window + at, of_row[m], 64 * h);
+        };
+        auto ask_b = [&](int at) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) b[k][i] = load8_at(weights + (uint64_t)(at + i / 2 * 32) * RANKS, of_b, i % 2 * 8 * RANKS + 64 * k);
         };
 #pragma unroll
-        for (int m = 0; m < AHEAD; ++m) ask(m);
-        // the row of b_l that is this lane's row of tile i
+        for (int m = 0; m < M; ++m) have[m][0] = have[m][1] = u32x4{0u, 0u, 0u, 0u};
+        for (; column0 < whole_end; column0 += kBlock) {
+          ask_b(column0);
+          if (base != nullptr) {
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+              if (row0 + 16 * m < rows) ask_base(m, column0);   // (places past the last row: the last one's, not stored)
+          }
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            if (row0 + 16 * m >= rows) break;
+            f32x4 acc[4];
+            product(b, m, acc);
+            const u32x4 lo = joined(have[m][0], acc[0], acc[1], m), hi = joined(have[m][1], acc[2], acc[3], m);
+            if (row0 + 16 * m + c < rows) {
+              store8_at(out_window + column0, of_row[m], lo);
+              store8_at(out_window + column0, of_row[m], hi, 64);
+            }
+          }
+        }
+      }
+      for (; column0 < strip_end; column0 += kBlock) {
+        int rank = a.rank, columns = a.hidden_out;
+        asm("" : "+s"(rank), "+s"(columns));   // (nothing of this loop is worked out, and kept in registers, ahead of the one above)
         u32x4 b[STEPS][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint16_t* from = weights + (uint64_t)min(column0 + i / 2 * 32 + (c >> 2) * 8 + i % 2 * 4 + (c & 3), columns - 1) * a.rank;
+          const uint16_t* from = weights + (uint64_t)min(column0 + row_of_b(i), columns - 1) * rank;
 #pragma unroll
-          for (int k = 0; k < STEPS; ++k) {
-            const int r = KS == 0 ? (q & 1) * 8 : k * 32 + q * 8;
-            b[k][i] = a.rank == RANKS ? load8(from + r) : load8_within(from, r, a.rank);
+          for (int k = 0; k < STEPS; ++k) b[k][i] = load8_within(from, KS == 0 ? (q & 1) * 8 : k * 32 + q * 8, rank);
+        }
+        u32x4 have[M][2];
+        uint64_t to[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          to[m] = (uint64_t)(first + __shfl(list, min(row0 + 16 * m + c, rows - 1))) * columns;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            have[m][h] = u32x4{0u, 0u, 0u, 0u};
+            if (base != nullptr && row0 + 16 * m < rows) have[m][h] = load8_within(base + to[m], column0 + q * 8 + 32 * h, columns);
           }
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
           if (row0 + 16 * m >= rows) break;
           f32x4 acc[4];
+          product(b, m, acc);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int h = 0; h < 2; ++h) {
+            const u32x4 bits = joined(have[m][h], acc[2 * h], acc[2 * h + 1], m);
+            const int own = column0 + q * 8 + 32 * h;
+            uint16_t* at = out + to[m] + own;
+            if (row0 + 16 * m + c >= rows) continue;
+            if (own + 8 <= columns) {
+              store8(at, bits);
+            } else {
 #pragma unroll
-          for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-            for (int half = 0; half < (KS == 0 ? 1 : 2); ++half) {
-              const u32x4 x = *reinterpret_cast<const u32x4*>(KS == 0 ? &split_v[q >> 1][16 * m + c][(q & 1) * 8]
-                                                                       : &split_v[half][16 * m + c][k * 32 + q * 8]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[i] = mfma_16x16x32<DT>(__builtin_bit_cast(bf16x8, b[k][i]), __builtin_bit_cast(bf16x8, x), acc[i]);
-            }
-          const bool mine_too = row0 + 16 * m + c < rows;
-          const float s = DT == kF16 ? scale * unit[16 * m + c] : scale;
-          if (mine_too) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              u32x4 bits;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const f32x4& y = acc[2 * h + e / 2];
-                const float lo = widen_bits<DT>((uint16_t)have[m % AHEAD][h][e]) + s * y[e % 2 * 2];
-                const float hi = widen_bits<DT>((uint16_t)(have[m % AHEAD][h][e] >> 16)) + s * y[e % 2 * 2 + 1];
-                bits[e] = round_bits<DT>(lo) | (uint32_t)round_bits<DT>(hi) << 16;
-              }
-              uint16_t* at = out + to[m % AHEAD] + 32 * h;
-              if (whole || own + 32 * h + 8 <= columns) {
-                store8(at, bits);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (own + 32 * h + e < columns) at[e] = (uint16_t)(bits[e / 2] >> (16 * (e % 2)));
-              }
+              for (int e = 0; e < 8; ++e)
+                if (own + e < columns) at[e] = (uint16_t)(bits[e / 2] >> (16 * (e % 2)));
             }
           }
-          if (m + AHEAD < M) ask(m + AHEAD);
         }
       }
     }
@@ -340,8 +386,9 @@ struct AdapterPlan {
   uint64_t plans_bytes;
 };
 
-// Workgroups that keep the device busy.
-constexpr int64_t kBusy = 1024;
+// Workgroups that keep the device busy: of the first kernel, where more cut the depth finer than pays (256, 512, 1024, 2048 of them, us: 8192 rows of
+// prompts, rank 64, 50, 41, 39, 60; 8192 rows, rank 16, 26, 21, 20, 27; 2048 rows of 64 adapters in turns 45, 40, 50, 51), and of the second.
+constexpr int64_t kBusyShrink = 512, kBusy = 1024;
 
 AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
   AdapterPlan f;
@@ -352,7 +399,7 @@ AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden
   // pieces of the depth: at least one step of every wave.  v and out in 1, 2, 4, 8, 16 pieces, us: one row (4096 -> 4096) 7.0 + 5.0,
   // 5.3 + 5.2, 4.3 + 5.1, 4.0 + 5.4, 3.6 + 6.1; 8192 rows of prompts (4096 -> 14336) 173 + 169, 93 + 169, 57 + 174, 40 + 178, 40 + 179
   f.pieces = between(hidden_in / (64 * kFewWaves), 8);
-  f.v_shares = between(kBusy / f.windows, most * f.pieces);
+  f.v_shares = between(kBusyShrink / f.windows, most * f.pieces);
   f.pieces = std::min(f.pieces, f.v_shares);
   f.shares = between(kBusy / f.windows, most * ((hidden_out + kBlock - 1) / kBlock));
   f.plans_bytes = (uint64_t)f.windows * sizeof(WindowPlan);
@@ -363,11 +410,7 @@ AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden
 template <int DT, int TILES>
 void launch_shrink(const AdapterParams& p, const AdapterPlan& f, hipStream_t stream) {
   const dim3 grid((uint32_t)(f.windows * f.v_shares));
-  if (p.a.rows <= kWindow) {
-    hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, 1>), grid, dim3(kFewThreads), 0, stream, p);
-  } else {
-    hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, 2>), grid, dim3(kFewThreads), 0, stream, p);
-  }
+  hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES>), grid, dim3(kFewThreads), 0, stream, p);
 }
 
 template <int DT>

@@ -28,6 +28,13 @@ __device__ __forceinline__ u32x4 load8_at(const void* base, uint32_t offset, int
   return ((Eight)((Bytes)at + offset + further))->v;
 }
 __device__ __forceinline__ void store8(uint16_t* p, u32x4 v) { reinterpret_cast<Packed8*>(p)->v = v; }
+__device__ __forceinline__ void store8_at(void* base, uint32_t offset, u32x4 v, int further = 0) {
+  using Bytes = __attribute__((address_space(1))) char*;
+  using Eight = __attribute__((address_space(1))) Packed8*;
+  uint64_t at = (uint64_t)uniform_ptr(static_cast<const char*>(base));
+  asm("" : "+s"(at), "+v"(offset));
+  ((Eight)((Bytes)at + offset + further))->v = v;
+}
 
 // Elements k .. k + 7 of a row of `depth`, zeros past its end; reads nothing outside the row.
 __device__ __forceinline__ u32x4 load8_within(const uint16_t* row, int k, int depth) {
