@@ -63,15 +63,40 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
 
-// ... and of the bits of a two-byte type, in the upper half, with the column below: no two keys of a token are equal.
-template <int DT>
-__device__ __forceinline__ uint32_t unique_key(uint16_t bits, int column) {
-  constexpr uint32_t INFINITE = DT == kBF16 ? 0x7f80u : 0x7c00u;
-  uint32_t key = (uint32_t)bits == 0x8000u ? 0u : (uint32_t)bits;
-  key = (key & 0x7fffu) > INFINITE ? 0x7fffu : key;
-  key ^= (uint32_t)((int32_t)(key << 16) >> 31) | 0x8000u;
-  return key << 16 | (uint32_t)(0xffff - column);   // (bits above the 16 leave here)
+// ... and of the bits of a two-byte type, in the upper half, with the lane's columns below in falling order: with key_of_lane() added, no two
+// keys of a token are equal.  Two elements at a time; -0 and NaN, which few tokens have, are looked for first and made +0 and one NaN.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+
+template <int DT, int VPL>
+__device__ __forceinline__ void unique_keys(const uint16_t (&bits)[VPL], uint32_t (&key)[VPL]) {
+  constexpr uint16_t INFINITE = DT == kBF16 ? 0x7f80 : 0x7c00;
+  u16x2 pair[VPL / 2], most = {0, 0}, least = {0xffff, 0xffff};
+#pragma unroll
+  for (int i = 0; i < VPL / 2; ++i) {
+    pair[i] = u16x2{bits[2 * i], bits[2 * i + 1]};
+    most = __builtin_elementwise_max(most, pair[i] & (uint16_t)0x7fff);
+    least = __builtin_elementwise_min(least, pair[i] ^ (uint16_t)0x8000);
+  }
+  if (__any(most.x > INFINITE || most.y > INFINITE || least.x == 0 || least.y == 0)) {
+#pragma unroll
+    for (int i = 0; i < VPL / 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint16_t one = pair[i][e];
+        pair[i][e] = one == 0x8000 ? uint16_t(0) : ((one & 0x7fff) > INFINITE ? uint16_t(0x7fff) : one);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < VPL / 2; ++i) {
+    const u16x2 sign = __builtin_bit_cast(u16x2, __builtin_bit_cast(i16x2, pair[i]) >> (int16_t)15);
+    const uint32_t both = __builtin_bit_cast(uint32_t, pair[i] ^ (sign | (uint16_t)0x8000));
+    key[2 * i] = both << 16 | (uint32_t)(VPL - 1 - 2 * i);
+    key[2 * i + 1] = (both & 0xffff0000u) | (uint32_t)(VPL - 2 - 2 * i);
+  }
 }
+template <int VPL>
+__device__ __forceinline__ uint32_t key_of_lane(int column) { return (uint32_t)(0xffff - column - (VPL - 1)); }
 template <int DT>
 __device__ __forceinline__ float unique_key_value(uint32_t key) {
   if constexpr (DT == kF32) return 0.0f;
@@ -83,7 +108,10 @@ __device__ __forceinline__ float unique_key_value(uint32_t key) {
 __device__ __forceinline__ float quick_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 __device__ __forceinline__ float quick_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + quick_exp(-x)); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
-__device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.0f) - log1pf(expf(-fabsf(x))); }
+// sigmoid(x) / exp(min(top, 0)), for x up to top: of a token all of whose sigmoids are too small for a float, what is left of them to compare.
+__device__ __forceinline__ float scaled_sigmoid(float x, float top) {
+  return (x >= 0.0f ? 1.0f : expf(x - fminf(top, 0.0f))) / (1.0f + expf(-fabsf(x)));
+}
 
 struct RouteParams {
   RouteArgs a;
@@ -128,23 +156,28 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
       x[v] = Logit<DT>::widen(raw.v[v]);
-      if constexpr (UNIQUE) key[v] = unique_key<DT>(raw.v[v], column + v);
-      else key[v] = order_key(x[v]);
+      if constexpr (!UNIQUE) key[v] = order_key(x[v]);
     }
-    uint32_t chosen_key[KR], top_key = 0u;
+    if constexpr (UNIQUE) unique_keys<DT>(raw.v, key);
+    uint32_t chosen_key[KR], top_key = 0u, last = 0u;
     int index[KR];
 #pragma unroll
     for (int r = 0; r < KR; ++r) chosen_key[r] = 0u, index[r] = 0;
     for (int j = 0; j < k; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int v = 1; v < VPL; ++v) best = best > key[v] ? best : key[v];
-      best = group_max<G>(best);
-      uint32_t at = ~0u;
+      uint32_t best, at = ~0u;
       if constexpr (UNIQUE) {
+        // the largest below the last: modulo 2^32, the differences of those below are larger than all others, and in their order
+        const uint32_t from = last - key_of_lane<VPL>(column);
+        best = key[0] - from;
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) key[v] = key[v] == best ? 0u : key[v];
+        for (int v = 1; v < VPL; ++v) best = max(best, key[v] - from);
+        best = group_max<G>(best) + last;
+        last = best;
       } else {
+        best = key[0];
+#pragma unroll
+        for (int v = 1; v < VPL; ++v) best = max(best, key[v]);
+        best = group_max<G>(best);
 #pragma unroll
         for (int v = VPL - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(column + v) : at;
         at = group_min<G>(at);
@@ -166,27 +199,30 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t first, int64_
     }
     const float base = top == -INFINITY ? 0.0f : top;
     float share[KR], scale = 0.0f;
-    if (all_scores) {   // (the sigmoid's own sum is not used)
-      float s[VPL], sum = 0.0f;
+    if (all_scores) {
+      if (a.sigmoid) {
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        s[v] = a.sigmoid ? quick_sigmoid(x[v]) : quick_exp(x[v] - base);
-        sum += s[v];
+        for (int v = 0; v < VPL; ++v) mass[v] += quick_sigmoid(x[v]);
+      } else {
+        float s[VPL], sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+          s[v] = quick_exp(x[v] - base);
+          sum += s[v];
+        }
+        sum = group_sum<G>(sum);
+        scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) mass[v] += s[v] * scale;
       }
-      sum = group_sum<G>(sum);
-      scale = a.sigmoid ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) mass[v] += s[v] * scale;
     }
     if (a.normalize) {
-      // (of sigmoids by their logarithms: their sum may be too small for a float)
-      const float log_top = a.sigmoid ? log_sigmoid(base) : 0.0f;
       float sum = 0.0f;
 #pragma unroll
       for (int r = 0; r < KR; ++r) {
         share[r] = 0.0f;
         if (r * G >= k) continue;   // (the same in all lanes)
-        share[r] = expf(a.sigmoid ? log_sigmoid(value[r]) - log_top : value[r] - base);
+        share[r] = a.sigmoid ? scaled_sigmoid(value[r], base) : expf(value[r] - base);
         if (l + r * G >= k) share[r] = 0.0f;
         sum += share[r];
       }
@@ -421,13 +457,12 @@ __global__ __launch_bounds__(kBackThreads, 4) void route_backward_kernel(RouteBa
       value[r] = index[r] >= 0 ? Logit<DT>::widen(static_cast<const T*>(a.logits)[t * a.experts + index[r]]) : -INFINITY;
     }
     if (a.normalize) {
-      const float log_top = a.sigmoid ? log_sigmoid(base) : 0.0f;
       float q[KR], sum = 0.0f, dot = 0.0f;
 #pragma unroll
       for (int r = 0; r < KR; ++r) {
         q[r] = 0.0f;
         if (r * G >= k) continue;   // (the same in all lanes)
-        if (index[r] >= 0) q[r] = expf(a.sigmoid ? log_sigmoid(value[r]) - log_top : value[r] - base);
+        if (index[r] >= 0) q[r] = a.sigmoid ? scaled_sigmoid(value[r], base) : expf(value[r] - base);
         sum += q[r];
       }
       sum = group_sum<G>(sum);

@@ -8,10 +8,11 @@ namespace gg {
 
 // The value of another lane of the same 16: exchanges by DPP, which need neither LDS nor a wait.  The four steps below
 // pair lanes as a butterfly does, once the steps before them made the lanes of a half equal: every lane ends with the
-// same bits, also of a float sum.
+// same bits, also of a float sum.  (Every source lane is there; with the 0 for one that is not, the compiler makes the exchange part of the
+// instruction that uses it.)
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 enum : int { kDppXor1 = 0xb1, kDppXor2 = 0x4e, kDppHalfMirror = 0x141, kDppMirror = 0x140 };
 
