@@ -12,6 +12,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "gmm_kernel.hpp"
 #include "wave_ops.hpp"
 
@@ -436,26 +438,46 @@ __global__ __launch_bounds__(kBackThreads, 4) void route_backward_kernel(RouteBa
   float m[VPL];
 #pragma unroll
   for (int v = 0; v < VPL; ++v) m[v] = a.mass_grad != nullptr && column + v < a.experts ? a.mass_grad[column + v] : 0.0f;
-  const bool dense = a.mass_grad != nullptr || !a.normalize;
-  for (int64_t t = (int64_t)blockIdx.x * GROUPS + group; t < a.tokens; t += (int64_t)gridDim.x * GROUPS) {
-    const auto raw = load_logits<DT, VPL>(a.logits, t, a.experts, column);
-    auto x = [&](int v) { return Logit<DT>::widen(raw.v[v]); };
-    float top = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) top = fmaxf(top, x(v));
-    top = group_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); });
-    const float base = top == -INFINITY ? 0.0f : top;
-    // what falls on the chosen columns
-    float value[KR], grad[KR];
-    int index[KR];
+  // The next token's rows are asked for while one is under way.
+  Row<T, VPL> next_raw;
+  int next_index[KR];
+  float next_grad[KR];
+  auto ask = [&](int64_t t) {
+    if (t >= a.tokens) return;
+    next_raw = load_logits<DT, VPL>(a.logits, t, a.experts, column);
 #pragma unroll
     for (int r = 0; r < KR; ++r) {
       const int j = l + r * G;
-      index[r] = j < k ? a.chosen[t * k + j] : -1;
-      if ((uint32_t)index[r] >= (uint32_t)a.experts) index[r] = -1;   // (names no expert: no gradient)
-      grad[r] = index[r] >= 0 && a.weights_grad != nullptr ? a.weights_grad[t * k + j] : 0.0f;
+      next_index[r] = j < k ? a.chosen[t * k + j] : -1;
+      if ((uint32_t)next_index[r] >= (uint32_t)a.experts) next_index[r] = -1;   // (names no expert: no gradient)
+      next_grad[r] = j < k && a.weights_grad != nullptr ? a.weights_grad[t * k + j] : 0.0f;
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * GROUPS;
+  int64_t t = (int64_t)blockIdx.x * GROUPS + group;
+  ask(t);
+  for (; t < a.tokens; t += stride) {
+    const auto raw = next_raw;
+    float value[KR], grad[KR];   // what falls on the chosen columns
+    int index[KR];
+#pragma unroll
+    for (int r = 0; r < KR; ++r) {
+      index[r] = next_index[r];
+      grad[r] = index[r] >= 0 ? next_grad[r] : 0.0f;
       value[r] = index[r] >= 0 ? Logit<DT>::widen(static_cast<const T*>(a.logits)[t * a.experts + index[r]]) : -INFINITY;
     }
+    ask(t + stride);
+    auto x = [&](int v) { return Logit<DT>::widen(raw.v[v]); };
+    float top = -INFINITY;   // of all columns, or, for sigmoids, of the chosen
+    if (a.sigmoid) {
+#pragma unroll
+      for (int r = 0; r < KR; ++r) top = fmaxf(top, value[r]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) top = fmaxf(top, x(v));
+    }
+    top = group_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); });
+    const float base = top == -INFINITY ? 0.0f : top;
     if (a.normalize) {
       float q[KR], sum = 0.0f, dot = 0.0f;
 #pragma unroll
@@ -486,36 +508,38 @@ __global__ __launch_bounds__(kBackThreads, 4) void route_backward_kernel(RouteBa
       if (index[r] >= 0) row[index[r] / VPL * PITCH + index[r] % VPL] = grad[r];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    // (everything else per column where it is needed, scores twice: registers are what this kernel is short of)
-    auto gradient = [&](int v) { return a.normalize ? m[v] : m[v] + own[v]; };   // of the column's score
-    float scale = 0.0f, dot = 0.0f;
-    if (dense && !a.sigmoid) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const float s = quick_exp(x(v) - base);
-        sum += s;
-        dot += s * gradient(v);
-      }
-      sum = group_sum<G>(sum);
-      scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-      dot = group_sum<G>(dot) * scale;
-    }
+    // (scores are computed where they are needed, of the softmax twice: registers are what this kernel is short of)
     Row<T, VPL> out;
+    auto finish = [&](auto normalized) {
+      auto gradient = [&](int v) { return normalized ? m[v] : m[v] + own[v]; };   // of the column's score
+      auto rest = [&](int v) { return normalized ? own[v] : 0.0f; };
+      if (normalized && a.mass_grad == nullptr) {
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      float sum = a.normalize ? own[v] : 0.0f;
-      if (dense) {
-        if (a.sigmoid) {
-          // (1 - score would lose all of a small difference; an infinite e has a score of 0)
-          const float e = quick_exp(-x(v)), score = __builtin_amdgcn_rcpf(1.0f + e);
-          sum += score * (fminf(e, 1e37f) * score) * gradient(v);
-        } else {
-          sum += quick_exp(x(v) - base) * scale * (gradient(v) - dot);
+        for (int v = 0; v < VPL; ++v) out.v[v] = Logit<DT>::narrow(own[v]);
+      } else if (a.sigmoid) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+          // s (1 - s), the same for x and -x, without the difference, which would lose all of a small one
+          const float e = quick_exp(-fabsf(x(v))), score = __builtin_amdgcn_rcpf(1.0f + e);
+          out.v[v] = Logit<DT>::narrow(rest(v) + score * (e * score) * gradient(v));
         }
+      } else {
+        float sum = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+          const float s = quick_exp(x(v) - base);
+          sum += s;
+          dot += s * gradient(v);
+        }
+        sum = group_sum<G>(sum);
+        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+        dot = group_sum<G>(dot) * scale;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) out.v[v] = Logit<DT>::narrow(rest(v) + quick_exp(x(v) - base) * scale * (gradient(v) - dot));
       }
-      out.v[v] = Logit<DT>::narrow(sum);
-    }
+    };
+    if (a.normalize) finish(std::true_type());
+    else finish(std::false_type());
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     T* to = static_cast<T*>(a.logits_grad) + t * a.experts + column;
