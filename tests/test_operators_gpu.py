@@ -156,6 +156,31 @@ def test_route_odd_values(ops, tokens, experts, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts", [9, 100, 256, 600])
+def test_route_nan_of_either_sign(ops, experts, dtype):
+    """NaN of any sign and payload counts as one value above all others, ties by the lower index; other tokens do not notice."""
+    g = torch.Generator().manual_seed(experts)
+    logits = torch.randn(70, experts, generator=g).to(dtype)
+    whole, least = (torch.int32, 0x80000000 - 2 ** 32) if dtype == torch.float32 else (torch.int16, 0x8000 - 2 ** 16)
+    quiet = int(torch.tensor([float("nan")], dtype=dtype).view(whole)[0])
+    bits = logits.view(whole)
+    bits[3, 2] = quiet | least           # negative
+    bits[3, 7] = quiet                   # positive
+    bits[3, 8] = quiet | 1
+    bits[10, experts - 1] = quiet | least | 1
+    bits[11, :] = quiet | least
+    logits[12, 4] = INF
+    bits[12, 6] = quiet | least
+    _announce("route NaN", experts, dtype)
+    got = ops.route(logits.cuda(), 5, with_mass=False)
+    want = _route_reference(logits, 5, "softmax", True)
+    for name in ("experts", "batch_sizes", "order", "row_index"):
+        assert torch.equal(getattr(got, name).cpu().long(), want[name]), name
+    rest = torch.tensor([t for t in range(70) if t not in (3, 10, 11, 12)])
+    _close(got.weights.cpu()[rest], want["weights"][rest], 1e-5, 1e-30, "weights")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(1, 8, 2), (5, 64, 6), (70, 37, 3), (257, 256, 8), (90, 500, 32), (33, 1024, 5), (4099, 16, 4)])
 def test_route_gradient_matches_its_formula(ops, shape, dtype):
     t, e, k = shape
@@ -513,6 +538,22 @@ def test_lora_rows_in_any_order(ops, dtype):
         for with_base, with_scales in ((True, True), (False, True), (True, False)):
             _announce("lora order", dtype, name, with_base, with_scales)
             _check_lora(ops, (x, a, b, adapters.to(torch.int32), base if with_base else None, scales if with_scales else None), name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank", [16, 32, 64, 128, 256])
+def test_lora_whole_blocks_of_columns(ops, rank, dtype):
+    """Ranks that fill their steps, blocks of 64 columns with and without a rest, several to a wave; also in place and off 16 bytes."""
+    for rows, num, columns in ((3, 1, 64), (70, 2, 600), (21, 9, 1536), (150, 3, 2900)):
+        _announce("lora whole blocks", rank, dtype, rows, num, columns)
+        case = _lora_case(rows, num, rank, 96, columns, dtype, seed=rank + columns)
+        x, a, b, adapters, base, scales = case
+        got = _check_lora(ops, case, f"{rank} {columns}")
+        _check_lora(ops, (x, a, b, adapters, None, scales), f"{rank} {columns}, no base")
+        own = torch.empty(base.numel() + 3, dtype=dtype, device="cuda")[3:].view(base.shape)
+        own.copy_(base)
+        ops.lora(x.cuda(), a.cuda(), b.cuda(), adapters.cuda(), base=own, scales=scales.cuda(), c=own)
+        assert torch.equal(own, got)
 
 
 def test_lora_in_place_and_into_a_given_tensor(ops):
