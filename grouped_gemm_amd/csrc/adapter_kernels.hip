@@ -2,7 +2,10 @@
 //
 //   v[t] = a_l x[t]   (a_l: rank x hidden_in)        out[t] = base[t] + scale_l * b_l v[t]   (b_l: hidden_out x rank)
 //
-// Bound by base and out for many rows, by the adapters' weights for rows of many adapters, and by the launches for one.
+// Bound by base and out for many rows, by the adapters' weights for rows of many adapters, and by the latencies of two launches for few.
+// 8192 rows of prompts, bf16, 4096 -> 14336: rank 64 41 + 144 us (556 MB in all; the second kernel moves 470 MB of base and out at 3.3 TB/s, and
+// reads as much of b_l again from the L2s, 64 rows at a time: with one adapter 129 us), rank 16, 4096 wide 21 + 34 us (134 MB: 4.0 TB/s, as a
+// copy).  64 rows of 64 adapters, rank 16, 4096 wide 5.6 + 5.2 us, one row 4.1 + 4.6.
 // Rows are taken in windows of 64 in their own order, and the rows of a window that share an adapter together: the
 // rows of a prompt are neighbours, and the rows of a decode step are one window, so nothing has to be sorted.  A wave knows
 // its window's rows from one load and a ballot for each adapter.
@@ -294,7 +297,8 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
       int column0 = strip_begin + wave * 64;
       const int whole_end = a.rank == RANKS ? min(strip_end, columns - 63) : 0;
       if (column0 < whole_end) {
-        // Whole blocks: all that a block needs is asked for at once, under no condition of a lane's.
+        // Whole blocks: all that a block needs is asked for at once, under no condition of a lane's (as the loop below does it, rank 64: 174 us
+        // instead of 144; asked for while the block before is under way, between its stores: 162).
         u32x4 have[M][2], b[STEPS][4];
         uint32_t of_row[M];
         const uint16_t* base_window = base + first * columns;
@@ -387,7 +391,8 @@ struct AdapterPlan {
 };
 
 // Workgroups that keep the device busy: of the first kernel, where more cut the depth finer than pays (256, 512, 1024, 2048 of them, us: 8192 rows of
-// prompts, rank 64, 50, 41, 39, 60; 8192 rows, rank 16, 26, 21, 20, 27; 2048 rows of 64 adapters in turns 45, 40, 50, 51), and of the second.
+// prompts, rank 64, 50, 41, 39, 60; 8192 rows, rank 16, 26, 21, 20, 27; 2048 rows of 64 adapters in turns 45, 40, 50, 51), and of the second (512, 1024,
+// 2048, us: 8192 rows of prompts, one adapter, rank 64 149, 143, 153; rank 16 37, 34, 35; decode 10.8, 11.1, 15.4; 2048 rows in 30 prompts 40, 33, 31).
 constexpr int64_t kBusyShrink = 512, kBusy = 1024;
 
 AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out) {
@@ -396,8 +401,9 @@ AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden
   const int64_t most = std::min({num, rows, int64_t(kWindow)});   // adapters of a window
   f.windows = (rows + kWindow - 1) / kWindow;
   f.v_pitch = (rank + 3) / 4 * 4;
-  // pieces of the depth: at least one step of every wave.  v and out in 1, 2, 4, 8, 16 pieces, us: one row (4096 -> 4096) 7.0 + 5.0,
-  // 5.3 + 5.2, 4.3 + 5.1, 4.0 + 5.4, 3.6 + 6.1; 8192 rows of prompts (4096 -> 14336) 173 + 169, 93 + 169, 57 + 174, 40 + 178, 40 + 179
+  // pieces of the depth: at least one step of every wave.  v and out in at most 1, 2, 4, 8, 16 pieces, us: one row (4096 -> 4096) 8.2 + 3.9,
+  // 5.7 + 4.1, 4.7 + 4.4, 4.1 + 4.6, 3.7 + 5.3; 333 rows (2047 -> 1023) 38 + 13, 21 + 13, 13 + 13, 10.9 + 12.6, 10.8 + 12.9; 64 rows of one
+  // adapter, rank 64 47 + 8, 26 + 8, 17 + 9, 13 + 10, 9 + 13; 8192 rows of prompts (4096 -> 14336) 92 + 140, 52 + 141, 41 + 145, 41 + 144, 41 + 145
   f.pieces = between(hidden_in / (64 * kFewWaves), 8);
   f.v_shares = between(kBusyShrink / f.windows, most * f.pieces);
   f.pieces = std::min(f.pieces, f.v_shares);

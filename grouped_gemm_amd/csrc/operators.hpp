@@ -1,4 +1,4 @@
-// Launches of the operators around the grouped GEMM that the C ABI (gmm_api.hip) is built on: the router
+// Launches of the operators around the grouped GEMM that the C ABI (operators_api.hip) is built on: the router
 // (route_kernels.hip), the gated expert layer for a few tokens (few_tokens_kernels.hip), low-rank adapters
 // (adapter_kernels.hip).  Arguments are checked by the caller.
 #pragma once
