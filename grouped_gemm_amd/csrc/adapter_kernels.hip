@@ -5,7 +5,7 @@
 // Bound by base and out for many rows, by the adapters' weights for rows of many adapters, and by the latencies of two launches for few.
 // 8192 rows of prompts, bf16, 4096 -> 14336: rank 64 41 + 144 us (556 MB in all; the second kernel moves 470 MB of base and out at 3.3 TB/s, and
 // reads as much of b_l again from the L2s, 64 rows at a time: with one adapter 129 us), rank 16, 4096 wide 21 + 34 us (134 MB: 4.0 TB/s, as a
-// copy).  64 rows of 64 adapters, rank 16, 4096 wide 5.6 + 5.2 us, one row 4.1 + 4.6.
+// copy).  64 rows of 64 adapters, rank 16, 4096 wide 4.7 + 5.2 us, one row 3.8 + 4.6.
 // Rows are taken in windows of 64 in their own order, and the rows of a window that share an adapter together: the
 // rows of a prompt are neighbours, and the rows of a decode step are one window, so nothing has to be sorted.  A wave knows
 // its window's rows from one load and a ballot for each adapter.
@@ -89,19 +89,20 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
   const int64_t window = blockIdx.x / p.shares, first = window * kWindow;
   const int share = (int)(blockIdx.x - window * p.shares);
   Window w(a, first);
-  // What is in the window: the workgroups that its adapters leave cut the depth.
-  int count = 0;
-  {
-    Window all = w;
-    WindowPlan& plan = p.plans[window];
-    for (; all.left != 0; ++count) {
-      int which;
-      const uint64_t mine = all.next(which);
-      if (share == 0 && threadIdx.x == 0) plan.adapter[count] = which, plan.rows[count] = mine;
-    }
+  // What is in the window, the i-th adapter and its rows in lane i: the workgroups that its adapters leave cut the depth.
+  int count = 0, its_adapter = 0;
+  uint64_t its_rows = 0;
+  for (; w.left != 0; ++count) {
+    int which;
+    const uint64_t mine = w.next(which);
+    if (lane == count) its_adapter = which, its_rows = mine;
   }
   const int pieces = min(max(p.shares / max(count, 1), 1), p.pieces), splits = p.shares / pieces;
-  if (share == 0 && threadIdx.x == 0) p.plans[window].count = count, p.plans[window].pieces = pieces, p.plans[window].none = w.none;
+  if (share == 0 && threadIdx.x < kWindow) {
+    WindowPlan& plan = p.plans[window];
+    plan.adapter[lane] = its_adapter, plan.rows[lane] = its_rows;
+    if (lane == 0) plan.count = count, plan.pieces = pieces, plan.none = w.none;
+  }
   const int piece = share % pieces, split = share / pieces;
   if (split >= splits) return;
   const int steps = (a.hidden_in + S::DEPTH - 1) / S::DEPTH;
@@ -112,10 +113,10 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
   s.width = 8;
   s.x = static_cast<const uint16_t*>(a.x) + (uint64_t)first * a.hidden_in;
   const Exchange<true> exchange{lds};
-  for (int turn = 0; w.left != 0; turn = turn + 1 == splits ? 0 : turn + 1) {
-    int which;
-    const uint64_t mine = w.next(which);
-    if (turn != split) continue;
+  for (int turn = split; turn < count; turn += splits) {
+    const int which = __builtin_amdgcn_readlane(its_adapter, turn);
+    const uint64_t mine = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(its_rows >> 32), turn) << 32 |
+                          (uint32_t)__builtin_amdgcn_readlane((int)its_rows, turn);
     const int list = list_rows(mine), rows = __popcll(mine);
     const uint16_t* weights = static_cast<const uint16_t*>(a.a) + (uint64_t)which * a.rank * a.hidden_in;
     for (int r0 = 0; r0 < a.rank; r0 += 16 * TILES) {
