@@ -11,8 +11,8 @@
 //
 // Choosing and the gradient are bound by the vector units' issue, not by memory: every logit is read once, but takes an exponential (four
 // times the time of an addition), and a subtraction and half a maximum for each of the top_k.  65536 tokens of 256 experts, bf16, sigmoid,
-// top 8: choosing 26 us (33.6 MB: 1.3 TB/s), summing the counts 5, placing 524288 rows 13 (latency of scattered 4-byte stores), the gradient
-// 26 (67 MB and the chosen: 2.7 TB/s).  Few tokens are bound by the launches: one token 3.6 us in one, 8192 of 64 experts 5 + 4 + 4 and 4.
+// top 8: choosing 27 us (33.6 MB: 1.3 TB/s), summing the counts 5, placing 524288 rows 11 (latency of scattered 4-byte stores), the gradient
+// 26 (67 MB and the chosen: 2.7 TB/s).  Few tokens are bound by the launches: one token 3.7 us in one, 8192 of 64 experts 5 + 4 + 4 and 4.
 #include "operators.hpp"
 
 #include <math.h>
@@ -28,10 +28,10 @@ namespace {
 constexpr int kRouteThreads = 512;
 constexpr int kRouteWaves = kRouteThreads / 64;
 // Workgroups that choose and place, at most: two on each of 256 compute units; a column of their counts is 8 words for each lane of the wave
-// that sums it.  Choosing, summing, placing for 65536 tokens of 256 experts with 256, 512, 1024: 29 + 4.7 + 12, 27 + 4.8 + 13, 28 + 7 + 13 us.
+// that sums it.  Choosing, summing, placing for 65536 tokens of 256 experts with 256, 512, 1024: 29 + 4.7 + 12, 27 + 4.8 + 13, 28 + 7 + 13 us (placing now 11).
 constexpr int kRouteBlocks = 512;
 // Up to this many tokens and chosen rows one workgroup does everything in one launch.  That and three launches (their sum, without what lies
-// between them), us: 1 token of 64 experts 3.6, 8.6; 64 of 64 4.9, 9.6; 64 of 256 8.2, 13; 128 of 64 8.8, 10.0; 256 of 64 14.7, 11.1; 256 of 256
+// between them), us: 1 token of 64 experts 3.6, 8.6; 64 of 64 5.0, 9.6; 64 of 256 7.4, 12; 128 of 64 8.8, 10.0; 256 of 64 14.7, 11.1; 256 of 256
 // 30, 13.
 constexpr int kSmallTokens = 64, kSmallSlots = 2048;
 
@@ -326,20 +326,25 @@ __device__ __forceinline__ void place(int n, int experts, int top_k, int64_t fir
   }
 }
 
-// Exclusive prefix sums of the experts' counts, in LDS, by the first wave; ends with a barrier.
+// Exclusive prefix sums of the experts' counts, in LDS; all threads, ends with a barrier.
 template <typename Count>
 __device__ __forceinline__ void expert_starts(int experts, int32_t* starts, Count count) {
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    int before = 0;
-    for (int e0 = 0; e0 < experts; e0 += 64) {
-      const int mine = e0 + lane < experts ? count(e0 + lane) : 0;
-      const int upto = wave_prefix(mine);
-      if (e0 + lane < experts) starts[e0 + lane] = before + upto - mine;
-      before += __shfl(upto, 63);
+  __shared__ int32_t totals[kRouteWaves];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  int before = 0;
+  for (int e0 = 0; e0 < experts; e0 += kRouteThreads) {
+    const int e = e0 + (int)threadIdx.x, mine = e < experts ? count(e) : 0, upto = wave_prefix(mine);
+    if (lane == 63) totals[wave] = upto;
+    __syncthreads();
+    int at = before + upto - mine;
+#pragma unroll
+    for (int w = 0; w < kRouteWaves; ++w) {
+      at += w < wave ? totals[w] : 0;
+      before += totals[w];
     }
+    if (e < experts) starts[e] = at;
+    __syncthreads();
   }
-  __syncthreads();
 }
 
 // Everything in one workgroup, for the few tokens of a decode step, where a second launch would cost more than the rest.
@@ -420,11 +425,24 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(RouteParams 
   extern __shared__ int32_t lds[];
   const RouteArgs& a = p.a;
   int32_t *starts = lds, *next = lds + a.experts;
+  // (asked for before anything waits: where this workgroup's rows of the thread's experts begin)
+  constexpr int EACH = (int)kRouteMaxExperts / kRouteThreads;
+  int own[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = i * kRouteThreads + (int)threadIdx.x;
+    own[i] = e < a.experts ? p.counts[(int64_t)e * p.blocks + blockIdx.x] : 0;
+  }
   expert_starts(a.experts, starts, [&](int e) { return (int)a.batch_sizes[e]; });
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = i * kRouteThreads + (int)threadIdx.x;
+    if (e < a.experts) starts[e] += own[i];   // (its own thread's only, here and in place())
+  }
   const int64_t first = (int64_t)blockIdx.x * p.chunk, last = first + p.chunk < a.tokens ? first + p.chunk : a.tokens;
   const int32_t* chosen = a.chosen + first * a.top_k;
   place((int)(last - first) * a.top_k, a.experts, a.top_k, first * a.top_k, next, [&](int i) { return chosen[i]; },
-        [&](int e) { return starts[e] + p.counts[(int64_t)e * p.blocks + blockIdx.x]; }, a.row_index, a.order);
+        [&](int e) { return starts[e]; }, a.row_index, a.order);
 }
 
 // Gradient of the logits, one pass: with g the gradients of the chosen weights and m those of the mass,
