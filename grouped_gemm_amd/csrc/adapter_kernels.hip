@@ -5,7 +5,7 @@
 // Bound by base and out for many rows, by the adapters' weights for rows of many adapters, and by the latencies of two launches for few.
 // 8192 rows of prompts, bf16, 4096 -> 14336: rank 64 41 + 144 us (556 MB in all; the second kernel moves 470 MB of base and out at 3.3 TB/s, and
 // reads as much of b_l again from the L2s, 64 rows at a time: with one adapter 129 us), rank 16, 4096 wide 21 + 34 us (134 MB: 4.0 TB/s, as a
-// copy).  64 rows of 64 adapters, rank 16, 4096 wide 4.7 + 5.2 us, one row 3.8 + 4.6.
+// copy).  64 rows of 16 adapters, rank 16, 4096 wide 4.7 + 5.2 us, one row 3.8 + 4.6.
 // Rows are taken in windows of 64 in their own order, and the rows of a window that share an adapter together: the
 // rows of a prompt are neighbours, and the rows of a decode step are one window, so nothing has to be sorted.  A wave knows
 // its window's rows from one load and a ballot for each adapter.
@@ -392,7 +392,7 @@ struct AdapterPlan {
 };
 
 // Workgroups that keep the device busy: of the first kernel, where more cut the depth finer than pays (256, 512, 1024, 2048 of them, us: 8192 rows of
-// prompts, rank 64, 50, 41, 39, 60; 8192 rows, rank 16, 26, 21, 20, 27; 2048 rows of 64 adapters in turns 45, 40, 50, 51), and of the second (512, 1024,
+// prompts, rank 64, 50, 41, 39, 60; 8192 rows, rank 16, 26, 21, 20, 27; 2048 rows of 64 adapters at random 45, 40, 50, 51), and of the second (512, 1024,
 // 2048, us: 8192 rows of prompts, one adapter, rank 64 149, 143, 153; rank 16 37, 34, 35; decode 10.8, 11.1, 15.4; 2048 rows in 30 prompts 40, 33, 31).
 constexpr int64_t kBusyShrink = 512, kBusy = 1024;
 
