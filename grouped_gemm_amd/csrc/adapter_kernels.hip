@@ -79,10 +79,10 @@ __device__ __forceinline__ int list_rows(uint64_t mine) {
 // v of one piece of the depth.  TILES: of 16 rows of a_l; more than 64 of them are taken 64 at a time.
 // MT: of 16 rows, taken at a time (1 and 2, us: 64 rows of one adapter, rank 64, 15.0, 12.4; decode, a row or two to an adapter, 8.3, 8.4; one row 3.9, 4.1;
 // 8192 rows of prompts 59, 41).
-template <int DT, int TILES>
+template <int DT, int TILES, bool ODD>
 __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterParams p) {
   constexpr int MT = 2;
-  using S = Stream<DT, true, TILES, MT>;
+  using S = Stream<DT, true, TILES, MT, ODD>;
   __shared__ f32x4 lds[kFewWaves * 256];
   const AdapterArgs& a = p.a;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
@@ -124,6 +124,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void adapter_shrink_kernel(AdapterP
 #pragma unroll
       for (int i = 0; i < TILES; ++i)   // (rows past the last: the last one's, not stored)
         s.at[i] = (uint32_t)(min(16 * i + c, a.rank - 1 - r0)) * (uint32_t)a.hidden_in * 2 + q * 32;
+      s.set_weights();
       for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -417,7 +418,11 @@ AdapterPlan adapter_plan(int64_t rows, int64_t num, int64_t rank, int64_t hidden
 template <int DT, int TILES>
 void launch_shrink(const AdapterParams& p, const AdapterPlan& f, hipStream_t stream) {
   const dim3 grid((uint32_t)(f.windows * f.v_shares));
-  hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES>), grid, dim3(kFewThreads), 0, stream, p);
+  if (on_any_element(p.a.a, p.a.x, p.a.hidden_in)) {
+    hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, true>), grid, dim3(kFewThreads), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((adapter_shrink_kernel<DT, TILES, false>), grid, dim3(kFewThreads), 0, stream, p);
+  }
 }
 
 template <int DT>

@@ -27,6 +27,14 @@ __device__ __forceinline__ u32x4 load8_at(const void* base, uint32_t offset, int
   asm("" : "+s"(at), "+v"(offset));
   return ((Eight)((Bytes)at + offset + further))->v;
 }
+// ... one dword of them, on a boundary of 4 bytes
+__device__ __forceinline__ uint32_t load_dword_at(const void* base, uint32_t offset) {
+  using Bytes = const __attribute__((address_space(1))) char*;
+  using Dword = const __attribute__((address_space(1))) uint32_t*;
+  uint64_t at = (uint64_t)uniform_ptr(static_cast<const char*>(base));
+  asm("" : "+s"(at), "+v"(offset));
+  return *(Dword)((Bytes)at + offset);
+}
 __device__ __forceinline__ void store8(uint16_t* p, u32x4 v) { reinterpret_cast<Packed8*>(p)->v = v; }
 __device__ __forceinline__ void store8_at(void* base, uint32_t offset, u32x4 v, int further = 0) {
   using Bytes = __attribute__((address_space(1))) char*;
@@ -65,8 +73,13 @@ __device__ __forceinline__ float widen_bits(uint16_t v) {
 // One wave's stream: its share of the depth of a strip of weights against up to 16 * MT rows.
 //   NT   tiles of 16 weight rows, the first half of them from `first` and the others from `second` on; 64 deep at a time
 //   NN   128 columns, in each lane 8 neighbouring ones; 32 deep at a time
-template <int DT, bool NT, int NT_TILES, int MT>
+// ODD (NT): rows may begin on any element.  Loads of 16 bytes that are not on a boundary of 4 take three times as long, so a lane loads from the
+// boundary before its 16 elements on, one dword more, and shifts; each of those dwords holds an element of its own, so that nothing is read that
+// could not be.  Without and with it, us: 8192 rows of 4097 against adapters of rank 64 117, 52 (of 4098: 41); gate and up of two experts, 4097 ->
+// 14337, 202, 137 (of 4098: 101); one row 4.3, 4.4.  NN has whole rows of 256 bytes to an instruction, and loses an eighth.
+template <int DT, bool NT, int NT_TILES, int MT, bool ODD = false>
 struct Stream {
+  static_assert(NT || !ODD, "");
   static constexpr int DEPTH = NT ? 64 : 32;      // of a step
   static constexpr int TILES = NT ? NT_TILES : 8;        // of 16 weight columns
   static constexpr int XS = NT ? 2 : 1;           // loads of a row per step
@@ -74,6 +87,7 @@ struct Stream {
   struct Step {
     u32x4 w[NT ? 2 * TILES : 8];
     u32x4 x[MT][XS];
+    uint32_t w_end[ODD ? TILES : 1], x_end[ODD ? MT : 1];
   };
 
   const uint16_t *first, *second;   // the same in all lanes: where the strip's columns begin, at depth 0
@@ -82,6 +96,7 @@ struct Stream {
   int width;                        // NN: columns this lane may read, 8 or (of a matrix narrower than 8) fewer
   const uint16_t* x;                // the rows, the same in all lanes,
   uint32_t row[MT];                 // ... and where in them this lane's step 0 begins, in bytes (set_row)
+  uint32_t w_turn[ODD ? TILES : 1], x_turn[ODD ? MT : 1];   // ODD: bytes from the boundary to there, 0 or 2 (`at` and `row` are the boundary's)
   int depth;
   f32x4 acc[TILES][MT];
 
@@ -92,15 +107,38 @@ struct Stream {
       for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  static __device__ __forceinline__ const uint16_t* boundary(const uint16_t* p) {
+    return ODD ? reinterpret_cast<const uint16_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3)) : p;
+  }
+  static __device__ __forceinline__ void turn(const uint16_t* base, uint32_t& offset, uint32_t& bytes) {
+    offset += (uint32_t)(reinterpret_cast<uintptr_t>(base) & 2);
+    bytes = offset & 2;
+    offset -= bytes;
+  }
   // the lane's row of tile m begins `offset` bytes into x
-  __device__ __forceinline__ void set_row(int m, uint32_t offset) { row[m] = offset + ((threadIdx.x & 63) >> 4) * 16 * XS; }
+  __device__ __forceinline__ void set_row(int m, uint32_t offset) {
+    row[m] = offset + ((threadIdx.x & 63) >> 4) * 16 * XS;
+    if constexpr (ODD) turn(x, row[m], x_turn[m]);
+  }
+  __device__ __forceinline__ const uint16_t* matrix(int i) const { return 2 * i < TILES ? first : second; }
+  // once `at`, first and second are set
+  __device__ __forceinline__ void set_weights() {
+    if constexpr (ODD) {
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) turn(matrix(i), at[i], w_turn[i]);
+    }
+  }
 
   __device__ __forceinline__ void load_weights(Step& s, int k) const {
     if constexpr (NT) {
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8_at((2 * i < TILES ? first : second) + k, at[i], 16 * h);
+        for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8_at(boundary(matrix(i)) + k, at[i], 16 * h);
+      if constexpr (ODD) {   // (where nothing is to be shifted: the last dword again, not one past it)
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) s.w_end[i] = load_dword_at(boundary(matrix(i)) + k, at[i] + 28 + 2 * w_turn[i]);
+      }
     } else {
       const char* base = reinterpret_cast<const char*>(first) + (uint64_t)k * pitch;
 #pragma unroll
@@ -111,7 +149,11 @@ struct Stream {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int h = 0; h < XS; ++h) s.x[m][h] = load8_at(x + k, row[m], 16 * h);
+      for (int h = 0; h < XS; ++h) s.x[m][h] = load8_at(boundary(x) + k, row[m], 16 * h);
+    if constexpr (ODD) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s.x_end[m] = load_dword_at(boundary(x) + k, row[m] + 28 + 2 * x_turn[m]);
+    }
   }
 
   // ... where the depth ends inside, or the matrix is narrower than a lane's columns
@@ -120,7 +162,8 @@ struct Stream {
     if constexpr (NT) {
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
-        const uint16_t* base = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(2 * i < TILES ? first : second) + at[i]);
+        const uint16_t* base = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(boundary(matrix(i))) + at[i]);
+        if constexpr (ODD) base += w_turn[i] / 2;
 #pragma unroll
         for (int h = 0; h < 2; ++h) s.w[2 * i + h] = load8_within(base - q * 16, k + q * 16 + 8 * h, depth);
       }
@@ -133,9 +176,30 @@ struct Stream {
       }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(boundary(x)) + row[m]) - q * 8 * XS;
+      if constexpr (ODD) from += x_turn[m] / 2;
 #pragma unroll
-      for (int h = 0; h < XS; ++h) s.x[m][h] = load8_within(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(x) + row[m]) - q * 8 * XS, k + q * 8 * XS + 8 * h, depth);
+      for (int h = 0; h < XS; ++h) s.x[m][h] = load8_within(from, k + q * 8 * XS + 8 * h, depth);
+    }
+  }
+
+  // ODD, of what load_weights and load_rows brought: from the boundary on -> from the lane's first element on
+  static __device__ __forceinline__ void shift(u32x4& low, u32x4& high, uint32_t end, uint32_t bytes) {
+    const uint32_t d[9] = {low[0], low[1], low[2], low[3], high[0], high[1], high[2], high[3], end};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      low[j] = __builtin_amdgcn_alignbyte(d[j + 1], d[j], bytes);
+      high[j] = __builtin_amdgcn_alignbyte(d[j + 5], d[j + 4], bytes);
+    }
+  }
+  __device__ __forceinline__ void shift(Step& s) const {
+    if constexpr (ODD) {
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) shift(s.w[2 * i], s.w[2 * i + 1], s.w_end[i], w_turn[i]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) shift(s.x[m][0], s.x[m][1], s.x_end[m], x_turn[m]);
+    }
   }
 
   __device__ __forceinline__ void multiply(const Step& s) {
@@ -176,6 +240,7 @@ struct Stream {
   }
   // multiply, then ask for what comes two of the wave's steps later
   __device__ __forceinline__ void advance(Step& s) {
+    shift(s);
     multiply(s);
     __builtin_amdgcn_sched_barrier(0);   // (steps do not mix: their registers would not suffice)
     load_weights(s, (step + 2 * kFewWaves) * DEPTH);
@@ -199,6 +264,7 @@ struct Stream {
     }
     if (step < whole) {   // one to three steps are left, two of them loaded
       const bool third = step + 2 * kFewWaves < whole;
+      shift(s0);
       multiply(s0);
       if (third) {
         load_weights(s0, (step + 2 * kFewWaves) * DEPTH);
@@ -206,10 +272,12 @@ struct Stream {
       }
       step += kFewWaves;
       if (step < whole) {
+        shift(s1);
         multiply(s1);
         step += kFewWaves;
       }
       if (third) {
+        shift(s0);
         multiply(s0);
         step += kFewWaves;
       }
@@ -220,6 +288,11 @@ struct Stream {
     }
   }
 };
+
+// Whether rows of `depth` elements of these matrices begin elsewhere than on boundaries of 4 bytes: what ODD streams are for.
+inline bool on_any_element(const void* p, const void* q, int64_t depth) {
+  return ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 3) != 0 || depth % 2 != 0;
+}
 
 // The waves' sums through LDS, 4 KiB of each wave at a time: NT its tiles (up to four), NN the first or second 64 of its columns.
 template <bool NT>

@@ -122,9 +122,9 @@ __device__ __forceinline__ int gather_slots(const FewParams& p, FewLds& lds, int
 // 338 us = 5.6 TB/s, 344.
 constexpr int gate_up_threads(bool nt) { return nt ? kFewThreads : 2 * kFewThreads; }
 
-template <int DT, bool NT, int MT>
+template <int DT, bool NT, int MT, bool ODD>
 __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate_up_kernel(FewParams p) {
-  using S = Stream<DT, NT, 4, MT>;
+  using S = Stream<DT, NT, 4, MT, ODD>;
   constexpr int COLUMNS = NT ? 32 : 128, OF_ROUND = NT ? 32 : 64;   // of h
   constexpr int THREADS = gate_up_threads(NT);
   __shared__ FewLds few_lds;
@@ -158,6 +158,7 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
     s.pitch = (uint32_t)ffn * 4;
     s.at[0] = q * 8 * s.pitch + (uint32_t)column * 2;
   }
+  s.set_weights();
   const Exchange<NT> exchange{lds};
   const int end = (hidden + S::DEPTH - 1) / S::DEPTH;
   s.prepare(wave % kFewWaves, 0, end);
@@ -208,9 +209,9 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
   }
 }
 
-template <int DT, bool NT, int MT>
+template <int DT, bool NT, int MT, bool ODD>
 __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(FewParams p) {
-  using S = Stream<DT, NT, 4, MT>;
+  using S = Stream<DT, NT, 4, MT, ODD>;
   constexpr int COLUMNS = NT ? 64 : 128;
   __shared__ FewLds few_lds;
   __shared__ f32x4 lds[kFewWaves * 256];
@@ -243,6 +244,7 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
       s.pitch = (uint32_t)hidden * 2;
       s.at[0] = q * 8 * s.pitch + (uint32_t)column * 2;
     }
+    s.set_weights();
     const int steps = (ffn + S::DEPTH - 1) / S::DEPTH, begin = (int)((int64_t)steps * piece / p.pieces);
     const int end = (int)((int64_t)steps * (piece + 1) / p.pieces);
     const Exchange<NT> exchange{lds};
@@ -349,7 +351,8 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   f.down_tiles = (hidden + (nt ? 63 : 127)) / (nt ? 64 : 128);
   f.ffn_pitch = (ffn + 7) / 8 * 8;
   // the depth of down in pieces where its strips alone are fewer than compute units, each of at least eight steps to a wave.  One
-  // token, 4096 -> 14336, in 1, 2, 4, 8 pieces: 64 strips 58, 34, 25, 26 us, 128 strips 65, 43, 44, 53, 512 strips 160, 185, 188, 193
+  // token, 4096 -> 14336, in 1, 2, 4, 8 pieces: 64 strips 58, 34, 25, 26 us, 128 strips 65, 43, 44, 53, 512 strips 160, 185, 188, 193; 130 to 250
+  // strips of 4096 in 1 and 2: 130 20.7, 25.1, 150 21.0, 26.0, 200 24.5, 27.2, 250 29.1, 30.4
   const int64_t steps = (ffn + (nt ? 63 : 31)) / (nt ? 64 : 32), fit = kFewUnits / (f.named * f.down_tiles), deep = steps / (8 * kFewWaves);
   f.pieces = std::max<int64_t>(1, std::min({fit, deep, int64_t(16)}));
   // Rows taken at a time, by how many an expert has on average (of down two for each slot; those that do not fit read the weights again): more of them
@@ -362,6 +365,24 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   f.hidden_pitch = (hidden + 3) / 4 * 4;
   f.parts_bytes = (uint64_t)f.pieces * f.slots * f.hidden_pitch * 4;
   return f;
+}
+
+template <int DT, bool NT, bool ODD>
+void launch_gate_up(const FewParams& p, const FewPlan& f, dim3 grid, hipStream_t stream) {
+  if (f.up_rows == 1) {
+    hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, 1, ODD>), grid, dim3(gate_up_threads(NT)), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, 2, ODD>), grid, dim3(gate_up_threads(NT)), 0, stream, p);
+  }
+}
+
+template <int DT, bool NT, bool ODD>
+void launch_down(const FewParams& p, const FewPlan& f, dim3 grid, hipStream_t stream) {
+  switch (f.down_rows) {
+    case 1: hipLaunchKernelGGL((few_down_kernel<DT, NT, 1, ODD>), grid, dim3(kFewThreads), 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((few_down_kernel<DT, NT, 2, ODD>), grid, dim3(kFewThreads), 0, stream, p); break;
+    default: hipLaunchKernelGGL((few_down_kernel<DT, NT, 4, ODD>), grid, dim3(kFewThreads), 0, stream, p); break;
+  }
 }
 
 template <int DT, bool NT>
@@ -380,18 +401,18 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   p.pieces = (int32_t)f.pieces;
   p.counters = (int32_t)f.down_tiles;
   const dim3 up((uint32_t)(f.named * f.up_tiles)), down((uint32_t)(f.named * f.down_tiles * f.pieces));
-  if (f.up_rows == 1) {
-    hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, 1>), up, dim3(gate_up_threads(NT)), 0, stream, p);
+  if (NT && on_any_element(a.w13, a.x, a.hidden)) {
+    launch_gate_up<DT, NT, NT>(p, f, up, stream);
   } else {
-    hipLaunchKernelGGL((few_gate_up_kernel<DT, NT, 2>), up, dim3(gate_up_threads(NT)), 0, stream, p);
+    launch_gate_up<DT, NT, false>(p, f, up, stream);
   }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   p.tiles = (int32_t)f.down_tiles;
-  switch (f.down_rows) {
-    case 1: hipLaunchKernelGGL((few_down_kernel<DT, NT, 1>), down, dim3(kFewThreads), 0, stream, p); break;
-    case 2: hipLaunchKernelGGL((few_down_kernel<DT, NT, 2>), down, dim3(kFewThreads), 0, stream, p); break;
-    default: hipLaunchKernelGGL((few_down_kernel<DT, NT, 4>), down, dim3(kFewThreads), 0, stream, p); break;
+  if (NT && on_any_element(a.w2, nullptr, a.ffn)) {
+    launch_down<DT, NT, NT>(p, f, down, stream);
+  } else {
+    launch_down<DT, NT, false>(p, f, down, stream);
   }
   return hipGetLastError();
 }

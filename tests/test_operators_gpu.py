@@ -556,6 +556,33 @@ def test_lora_whole_blocks_of_columns(ops, rank, dtype):
         assert torch.equal(own, got)
 
 
+def _shifted(t, elements):
+    """The same values `elements` behind a boundary of 16 bytes."""
+    flat = torch.empty(t.numel() + 16, dtype=t.dtype, device="cuda")
+    out = flat[elements:elements + t.numel()].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_that_begin_on_any_element(ops, dtype):
+    """Even sizes behind odd addresses, odd sizes behind either: the same bits as from a boundary."""
+    for depth in (640, 641, 1000, 1027):
+        x, a, b, adapters, base, scales = [v.cuda() for v in _lora_case(70, 3, 40, depth, 96, dtype, seed=depth)]
+        w13 = torch.randn(4, 2 * 72, depth, device="cuda").mul_(depth ** -0.5).to(dtype)
+        w2 = torch.randn(4, depth, 72, device="cuda").mul_(0.1).to(dtype)
+        few, experts = x[:9].contiguous(), torch.randint(0, 4, (9, 2), dtype=torch.int32, device="cuda")
+        weights = torch.rand(9, 2, device="cuda")
+        want = ops.lora(x, a, b, adapters, base=base, scales=scales)
+        want_few = ops.moe_few_tokens(few, w13, w2, experts, weights, trans_b=True)
+        for at in ((1, 0), (0, 1), (1, 1), (2, 3)):
+            _announce("rows on any element", dtype, depth, at)
+            got = ops.lora(_shifted(x, at[0]), _shifted(a, at[1]), _shifted(b, at[0]), adapters, base=_shifted(base, at[1]), scales=scales)
+            assert torch.equal(got, want)
+            got = ops.moe_few_tokens(_shifted(few, at[0]), _shifted(w13, at[1]), _shifted(w2, at[0]), experts, weights, trans_b=True)
+            assert torch.equal(got, want_few)
+
+
 def test_lora_in_place_and_into_a_given_tensor(ops):
     case = [v.cuda() for v in _lora_case(90, 4, 12, 65, 333, torch.bfloat16, seed=4)]
     x, a, b, adapters, base, scales = case
