@@ -263,6 +263,29 @@ def test_route_on_other_streams_and_in_a_graph(ops):
                     assert torch.equal(a, b)
 
 
+def test_route_past_32_bits(ops):
+    """More than 2^32 bytes and 2^31 elements of logits: the last tokens as in a call of their own, the order as a stable sort gives it."""
+    tokens, experts, k = 8_500_000, 256, 4
+    logits = torch.empty(tokens, experts, dtype=torch.bfloat16, device="cuda").normal_()
+    assert logits.numel() > 2 ** 31
+    _announce("route past 32 bits")
+    got = ops.route(logits, k)
+    alone = ops.route(logits[-1000:].contiguous(), k)
+    assert torch.equal(got.weights[-1000:], alone.weights) and torch.equal(got.experts[-1000:], alone.experts)
+    flat = got.experts.view(-1)
+    order = torch.sort(flat, stable=True).indices.int()
+    assert torch.equal(got.order, order) and torch.equal(got.row_index, order // k)
+    assert torch.equal(got.batch_sizes, torch.bincount(flat, minlength=experts))
+    del got, order, flat
+    logits.requires_grad_(True)
+    r = ops.route(logits, k)
+    grad = torch.randn(tokens, k, device="cuda")
+    full, = torch.autograd.grad((r.weights,), (logits,), (grad,))
+    last = logits.detach()[-1000:].contiguous().requires_grad_(True)
+    one, = torch.autograd.grad((ops.route(last, k).weights,), (last,), (grad[-1000:].contiguous(),))
+    assert torch.equal(full[-1000:], one)
+
+
 def test_route_refuses(ops):
     x = torch.zeros(4, 8, device="cuda")
     bad = [
@@ -562,6 +585,23 @@ def _shifted(t, elements):
     out = flat[elements:elements + t.numel()].view(t.shape)
     out.copy_(t)
     return out
+
+
+def test_lora_past_32_bits(ops):
+    """More than 2^32 bytes of base and out: windows at the end, in the middle and at the beginning as in calls of their own."""
+    rows, num, rank, hin, hout = 600_001, 7, 16, 64, 4096
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, hin, device="cuda", generator=g).bfloat16()
+    a = torch.randn(num, rank, hin, device="cuda", generator=g).bfloat16()
+    b = torch.randn(num, hout, rank, device="cuda", generator=g).bfloat16()
+    base = torch.empty(rows, hout, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    adapters = torch.randint(-1, num, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    assert base.numel() > 2 ** 31
+    _announce("lora past 32 bits")
+    got = ops.lora(x, a, b, adapters, base=base)
+    for begin in (0, 64 * 4000, rows // 64 * 64 - 128):
+        at = slice(begin, min(begin + 192, rows))
+        assert torch.equal(got[at], ops.lora(x[at].contiguous(), a, b, adapters[at].contiguous(), base=base[at].contiguous()))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
