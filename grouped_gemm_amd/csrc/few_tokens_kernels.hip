@@ -41,6 +41,7 @@ struct FewParams {
   int32_t slots;         // tokens * top_k
   int32_t tiles;         // strips of this kernel
   int32_t pieces;        // of the depth of down
+  int32_t shares;        // of this kernel's: workgroups that an expert's rows are shared among
   int32_t counters;      // arrivals to clear for the second kernel
   int32_t ffn_pitch;     // elements from one row of h to the next
   int32_t* arrivals;     // [strips of down]
@@ -51,11 +52,13 @@ struct FewParams {
   float* parts;          // [pieces][slots][hidden_pitch]
 };
 
-// Which experts are named, and the slots of one of them (in any order: a token's results do not depend on its place).  Up to 64
-// slots every wave finds the expert by itself, from one load and a ballot for each; more go through LDS.
+// Which experts are named, and the slots of one of them: in any order (a token's results do not depend on its place), or, where workgroups
+// share them and have to agree, in their own.  Up to 64 slots every wave finds the expert by itself, from one load and a ballot for each;
+// more go through LDS.
 struct FewLds {
   uint32_t named[kFewWords];
   int32_t rows;
+  int32_t of_wave[2 * kFewWaves];
   int32_t slot[kFewMaxSlots];
 };
 
@@ -109,9 +112,29 @@ __device__ __forceinline__ int gather_slots(const FewParams& p, FewLds& lds, int
       if (mine == expert) lds.slot[__popcll(same & ((uint64_t(1) << lane) - 1))] = lane;
       if (lane == 0) lds.rows = __popcll(same);
     }
-  } else {
+  } else if (p.shares == 1) {
     for (int i = threadIdx.x; i < p.slots; i += (int)blockDim.x)
       if (p.a.chosen[i] == expert) lds.slot[atomicAdd(&lds.rows, 1)] = i;
+  } else {
+    // every wave its share of the slots: how many are the expert's, then where they go (3 % of the largest launches, whose rows nobody shares)
+    const int waves = (int)blockDim.x / 64, wave = threadIdx.x / 64, share = ((p.slots + waves - 1) / waves + 63) / 64 * 64;
+    const int begin = min(wave * share, p.slots), end = min(begin + share, p.slots);
+    int count = 0;
+    for (int i = begin + lane; i - lane < end; i += 64) count += __popcll(__ballot(i < end && p.a.chosen[i] == expert));
+    if (lane == 0) lds.of_wave[wave] = count;
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < waves; ++w) {
+      at += w < wave ? lds.of_wave[w] : 0;
+      all += lds.of_wave[w];
+    }
+    for (int i = begin + lane; i - lane < end; i += 64) {
+      const bool its = i < end && p.a.chosen[i] == expert;
+      const uint64_t same = __ballot(its);
+      if (its) lds.slot[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = i;
+      at += __popcll(same);
+    }
+    if (threadIdx.x == 0) lds.rows = all;
   }
   __syncthreads();
   return uniform(lds.rows);
@@ -135,8 +158,10 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
     for (int i = threadIdx.x; i < p.counters; i += THREADS) p.arrivals[i] = 0;
   int mine;
   const int named = find_named(p, few_lds, mine);
-  if (blockIdx.x >= named * p.tiles) return;
-  const int task = (int)task_of_block(blockIdx.x, named * p.tiles), which = task / p.tiles, column0 = (task - which * p.tiles) * COLUMNS;
+  const int of_expert = p.tiles * p.shares;
+  if (blockIdx.x >= named * of_expert) return;
+  const int task = (int)task_of_block(blockIdx.x, named * of_expert), which = task / of_expert, left = task - which * of_expert;
+  const int tile = left / p.shares, column0 = tile * COLUMNS, row_first = (left - tile * p.shares) * 16 * MT, row_step = p.shares * 16 * MT;
   const int expert = find_expert(p, few_lds, mine, which);
   const int ffn = a.ffn, hidden = a.hidden;
   const uint16_t* w = static_cast<const uint16_t*>(a.w13) + (uint64_t)expert * 2 * ffn * hidden;
@@ -163,8 +188,8 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
   const int end = (hidden + S::DEPTH - 1) / S::DEPTH;
   s.prepare(wave % kFewWaves, 0, end);
   const int rows = gather_slots(p, few_lds, mine, expert);
-  for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
-    if (row0 > 0) s.prepare(wave % kFewWaves, 0, end);
+  for (int row0 = row_first; row0 < rows; row0 += row_step) {
+    if (row0 > row_first) s.prepare(wave % kFewWaves, 0, end);
 #pragma unroll
     for (int m = 0; m < MT; ++m)   // (places past the last row: the last one's, not stored)
       s.set_row(m, (uint32_t)(few_lds.slot[min(row0 + 16 * m + c, rows - 1)] / a.top_k) * (uint32_t)hidden * 2);
@@ -221,12 +246,13 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
   int mine;
   const int named = find_named(p, few_lds, mine), hidden = a.hidden, ffn = a.ffn;
   // strips one after the other, so that their sums are joined on the way (without any expert: zeros are stored)
-  const int arrivals = named * p.pieces, tasks = max(arrivals, 1) * p.tiles;
+  const int arrivals = named * p.pieces * p.shares, tasks = max(arrivals, 1) * p.tiles;
   if (blockIdx.x >= tasks) return;
   const int task = (int)task_of_block(blockIdx.x, tasks);
   const int tile = task / max(arrivals, 1), left = task - tile * arrivals, column0 = tile * COLUMNS;
   if (named > 0) {
-    const int which = left / p.pieces, piece = left - which * p.pieces;
+    const int which = left / (p.pieces * p.shares), in_expert = left - which * p.pieces * p.shares, piece = in_expert / p.shares;
+    const int row_first = (in_expert - piece * p.shares) * 16 * MT, row_step = p.shares * 16 * MT;
     const int expert = find_expert(p, few_lds, mine, which);
     const uint16_t* w = static_cast<const uint16_t*>(a.w2) + (uint64_t)expert * ffn * hidden;
     S s;
@@ -251,8 +277,8 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
     float* parts = p.parts + (uint64_t)piece * p.slots * p.hidden_pitch;
     s.prepare(uniform((int)(threadIdx.x >> 6)), begin, end);
     const int rows = 2 * gather_slots(p, few_lds, mine, expert);   // of h, two for each slot
-    for (int row0 = 0; row0 < rows; row0 += 16 * MT) {
-      if (row0 > 0) s.prepare(uniform((int)(threadIdx.x >> 6)), begin, end);
+    for (int row0 = row_first; row0 < rows; row0 += row_step) {
+      if (row0 > row_first) s.prepare(uniform((int)(threadIdx.x >> 6)), begin, end);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int row = min(row0 + 16 * m + c, rows - 1);
@@ -338,6 +364,7 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
 struct FewPlan {
   int64_t slots, named, up_tiles, down_tiles, pieces, ffn_pitch, hidden_pitch;
   int up_rows, down_rows;   // of 16, that a workgroup takes at a time
+  int64_t up_shares, down_shares;   // workgroups that an expert's rows are shared among
   uint64_t arrivals_bytes, h_bytes, parts_bytes;
 };
 
@@ -360,6 +387,14 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   // 340 348 368, 528 361 373; down 48 54 54, 180 153 161, 281 176 178, 469 316 212.
   f.up_rows = f.slots <= 8 * experts ? 1 : 2;
   f.down_rows = f.slots < 4 * experts ? 1 : (f.slots <= 12 * experts ? 2 : 4);
+  // Where the strips leave compute units, an expert's rows are shared among as many workgroups as there are turns on average.  us without and
+  // with: 64 tokens, all of 4 experts, 1024 -> 2048 36 + 71, 21 + 47; all of 8, 512 -> 1024 28 + 71, 18 + 47; 4 of 5, 700 -> 300 14 + 27, 10 + 21.
+  auto shares = [&](int64_t rows, int64_t strips) {
+    const int64_t turns = (f.slots + experts * rows - 1) / (experts * rows);
+    return std::max<int64_t>(1, std::min(turns, kFewUnits / strips));
+  };
+  f.up_shares = shares(16 * f.up_rows, f.named * f.up_tiles);
+  f.down_shares = shares(8 * f.down_rows, f.named * f.down_tiles * f.pieces);
   f.arrivals_bytes = (uint64_t)(f.down_tiles * 4 + 255) / 256 * 256;
   f.h_bytes = ((uint64_t)f.slots * f.ffn_pitch * 4 + 255) / 256 * 256;
   f.hidden_pitch = (hidden + 3) / 4 * 4;
@@ -400,7 +435,8 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   p.tiles = (int32_t)f.up_tiles;
   p.pieces = (int32_t)f.pieces;
   p.counters = (int32_t)f.down_tiles;
-  const dim3 up((uint32_t)(f.named * f.up_tiles)), down((uint32_t)(f.named * f.down_tiles * f.pieces));
+  p.shares = (int32_t)f.up_shares;
+  const dim3 up((uint32_t)(f.named * f.up_tiles * f.up_shares)), down((uint32_t)(f.named * f.down_tiles * f.pieces * f.down_shares));
   if (NT && on_any_element(a.w13, a.x, a.hidden)) {
     launch_gate_up<DT, NT, NT>(p, f, up, stream);
   } else {
@@ -409,6 +445,7 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   p.tiles = (int32_t)f.down_tiles;
+  p.shares = (int32_t)f.down_shares;
   if (NT && on_any_element(a.w2, nullptr, a.ffn)) {
     launch_down<DT, NT, NT>(p, f, down, stream);
   } else {
@@ -422,7 +459,7 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
 bool few_tokens_fits(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
   const FewPlan f = few_plan(tokens, experts, top_k, hidden, ffn, trans_b);
   const int64_t most = (int64_t(1) << 32) / gate_up_threads(false);   // (threads of a launch are counted in 32 bits)
-  return f.named * f.up_tiles < most && f.named * f.down_tiles * f.pieces < most && f.slots * f.ffn_pitch * 4 < (int64_t(1) << 32) && f.parts_bytes < (uint64_t(1) << 32);
+  return f.named * f.up_tiles * f.up_shares < most && f.named * f.down_tiles * f.pieces * f.down_shares < most && f.slots * f.ffn_pitch * 4 < (int64_t(1) << 32) && f.parts_bytes < (uint64_t(1) << 32);
 }
 
 uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
