@@ -77,9 +77,13 @@ __device__ __forceinline__ float widen_bits(uint16_t v) {
 // boundary before its 16 elements on, one dword more, and shifts; each of those dwords holds an element of its own, so that nothing is read that
 // could not be.  Without and with it, us: 8192 rows of 4097 against adapters of rank 64 117, 52 (of 4098: 41); gate and up of two experts, 4097 ->
 // 14337, 202, 137 (of 4098: 101); one row 4.3, 4.4.  NN has whole rows of 256 bytes to an instruction, and loses an eighth.
-template <int DT, bool NT, int NT_TILES, int MT, bool ODD = false>
+// SCALED (float16): a row's elements are kept as multiples of a power of two of each block of them, and are brought to one that the whole row
+// shares on their way into the instructions.
+template <int DT, bool NT, int NT_TILES, int MT, bool ODD = false, bool SCALED = false>
 struct Stream {
   static_assert(NT || !ODD, "");
+  static_assert(DT == kF16 || !SCALED, "");
+  static constexpr int BLOCK = NT ? 32 : 64;      // SCALED: elements of a block
   static constexpr int DEPTH = NT ? 64 : 32;      // of a step
   static constexpr int TILES = NT ? NT_TILES : 8;        // of 16 weight columns
   static constexpr int XS = NT ? 2 : 1;           // loads of a row per step
@@ -88,6 +92,7 @@ struct Stream {
     u32x4 w[NT ? 2 * TILES : 8];
     u32x4 x[MT][XS];
     uint32_t w_end[ODD ? TILES : 1], x_end[ODD ? MT : 1];
+    int32_t unit[SCALED ? MT : 1];
   };
 
   const uint16_t *first, *second;   // the same in all lanes: where the strip's columns begin, at depth 0
@@ -97,6 +102,9 @@ struct Stream {
   const uint16_t* x;                // the rows, the same in all lanes,
   uint32_t row[MT];                 // ... and where in them this lane's step 0 begins, in bytes (set_row)
   uint32_t w_turn[ODD ? TILES : 1], x_turn[ODD ? MT : 1];   // ODD: bytes from the boundary to there, 0 or 2 (`at` and `row` are the boundary's)
+  const int32_t* units;             // SCALED: the exponents of the rows' blocks, the same in all lanes,
+  uint32_t unit_row[SCALED ? MT : 1];   // ... where in them those of this lane's row begin, in bytes,
+  int32_t row_unit[SCALED ? MT : 1];    // ... and the exponent that the row is brought to, none of its blocks' being larger
   int depth;
   f32x4 acc[TILES][MT];
 
@@ -154,6 +162,10 @@ struct Stream {
 #pragma unroll
       for (int m = 0; m < MT; ++m) s.x_end[m] = load_dword_at(boundary(x) + k, row[m] + 28 + 2 * x_turn[m]);
     }
+    if constexpr (SCALED) {   // (a lane's elements of a step lie in one block)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s.unit[m] = (int32_t)load_dword_at(units + (uint32_t)k / BLOCK, unit_row[m] + (NT ? (threadIdx.x & 32) / 8 : 0));
+    }
   }
 
   // ... where the depth ends inside, or the matrix is narrower than a lane's columns
@@ -181,6 +193,7 @@ struct Stream {
       if constexpr (ODD) from += x_turn[m] / 2;
 #pragma unroll
       for (int h = 0; h < XS; ++h) s.x[m][h] = load8_within(from, k + q * 8 * XS + 8 * h, depth);
+      if constexpr (SCALED) s.unit[m] = units[unit_row[m] / 4 + min(k + q * 8 * XS, depth - 1) / BLOCK];   // (of zeros past the end: the last one's)
     }
   }
 
@@ -202,7 +215,32 @@ struct Stream {
     }
   }
 
-  __device__ __forceinline__ void multiply(const Step& s) {
+  // SCALED: the rows' elements times 2^(their block's exponent - the row's), a power of two not above 1, in two factors: elements are below 2^15, and
+  // down to 2^-39 of that the product is a number of float16, where the power itself is not.  Blocks of one row seldom need the second.
+  __device__ __forceinline__ void scale(Step& s) const {
+    if constexpr (SCALED) {
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        auto times = [&](int power) {   // (below -24: to zero)
+          const _Float16 factor = (_Float16)ldexpf(1.0f, power);
+#pragma unroll
+          for (int h = 0; h < XS; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t pair = s.x[m][h][j];
+              s.x[m][h][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pair) * f16x2{factor, factor});
+            }
+        };
+        const int power = s.unit[m] - row_unit[m];
+        times(max(power, -14));
+        if (__any(power < -14)) times(max(min(power + 14, 0), -26));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void multiply(Step& s) {
+    scale(s);
     if constexpr (NT) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -248,10 +286,13 @@ struct Stream {
     step += kFewWaves;
     __builtin_amdgcn_sched_barrier(0);
   }
-  __device__ __forceinline__ void run(int end) {
+  // `meanwhile` is called once the first loads are under way (by all threads)
+  template <typename Meanwhile>
+  __device__ __forceinline__ void run(int end, Meanwhile meanwhile) {
     clear();
     if (step < whole) load_rows(s0, step * DEPTH);
     if (step + kFewWaves < whole) load_rows(s1, (step + kFewWaves) * DEPTH);
+    meanwhile();
     // (the loop's loads are under no condition of their own, and its first turn, whose loads came in another order, is
     // outside it: the compiler then waits for a step's own loads only, not for all)
     if (step + 3 * kFewWaves < whole) {
@@ -286,6 +327,9 @@ struct Stream {
       load_within(s0, step * DEPTH);
       multiply(s0);
     }
+  }
+  __device__ __forceinline__ void run(int end) {
+    run(end, [] {});
   }
 };
 

@@ -47,6 +47,8 @@ struct FewParams {
   int32_t* arrivals;     // [strips of down]
   uint16_t* h;           // [slots][2][ffn_pitch] h rounded to the element type, and what the rounding left: two rows for
                          // the second product, which is then exact to twice the bits of the type
+  int32_t* units;        // float16: [slots][blocks] h of each block of columns is kept as a multiple of 2^unit
+  int32_t blocks;
   int32_t hidden_pitch;  // elements from one row of parts to the next
   uint32_t parts_bytes;
   float* parts;          // [pieces][slots][hidden_pitch]
@@ -61,6 +63,17 @@ struct FewLds {
   int32_t of_wave[2 * kFewWaves];
   int32_t slot[kFewMaxSlots];
 };
+
+// h may be larger than float16 holds, or too small for its bits.  Every block of 32 or 64 columns (a strip's) is kept as multiples of a power of two
+// that brings its largest to 2^14 .. 2^15; the second kernel brings the blocks to the largest of a row's units, as it multiplies, and its sums
+// back.  So h is exact to 2^-22 of itself and to 2^-37 of its row's largest, whatever its size.  Without and with it, us: one token, two of 8 experts,
+// 4096 -> 14336 135, 136; 5 tokens, top 6 of 64, 2048 -> 1408 80, 80; 64, top 8 of 128, 4096 -> 2048 1180, 1182; where many rows meet few weights
+// the multiplications show, 64, top 8 of 8, 2048 -> 2048, 138, 161, along the depth 110, 128.
+constexpr int kNoUnit = -1024;   // of a block of zeros: below all others
+__device__ __forceinline__ int unit_of(float most) {
+  if (!(most > 0.0f)) return kNoUnit;
+  return (most < INFINITY ? ilogbf(most) + 1 : 129) - 15;   // (beside an infinity, whose place no finite sum can show in, all else may vanish)
+}
 
 __device__ __forceinline__ int first_lane(uint64_t mask) { return __ffsll((unsigned long long)mask) - 1; }
 __device__ __forceinline__ bool few_slots(const FewParams& p) { return p.slots <= 64; }
@@ -148,7 +161,7 @@ constexpr int gate_up_threads(bool nt) { return nt ? kFewThreads : 2 * kFewThrea
 template <int DT, bool NT, int MT, bool ODD>
 __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate_up_kernel(FewParams p) {
   using S = Stream<DT, NT, 4, MT, ODD>;
-  constexpr int COLUMNS = NT ? 32 : 128, OF_ROUND = NT ? 32 : 64;   // of h
+  constexpr int COLUMNS = NT ? 32 : 128, OF_ROUND = NT ? 32 : 64;   // of h; of a round: a block with a unit of its own
   constexpr int THREADS = gate_up_threads(NT);
   __shared__ FewLds few_lds;
   __shared__ f32x4 lds[THREADS * 4];
@@ -221,8 +234,14 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
             column = (ffn < 8 ? 0 : min(start, ffn - 8)) + (n & 7);
             own = column >= start && column < ffn;   // (of 8 columns that moved back: their own only)
           }
+          float h = own ? gate / (1.0f + expf(-gate)) * up : 0.0f;
+          if constexpr (DT == kF16) {   // (the lanes of a row's block are all here)
+            const int unit = unit_of(group_reduce<OF_ROUND>(fabsf(h), [](float p, float q) { return fmaxf(p, q); }));
+            const int block = column0 / OF_ROUND + round;
+            if (n == 0 && block < p.blocks) p.units[(uint64_t)few_lds.slot[row] * p.blocks + block] = unit;
+            h = ldexpf(h, -unit);
+          }
           if (!own) continue;
-          const float h = gate / (1.0f + expf(-gate)) * up;
           const uint16_t high = round_bits<DT>(h);
           const float rest = h - widen_bits<DT>(high);
           uint16_t* to = p.h + (uint64_t)few_lds.slot[row] * 2 * p.ffn_pitch + column;
@@ -236,8 +255,10 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
 
 template <int DT, bool NT, int MT, bool ODD>
 __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(FewParams p) {
-  using S = Stream<DT, NT, 4, MT, ODD>;
+  constexpr bool SCALED = DT == kF16;
+  using S = Stream<DT, NT, 4, MT, ODD, SCALED>;
   constexpr int COLUMNS = NT ? 64 : 128;
+  __shared__ int32_t row_units[SCALED ? 8 * MT : 1];   // of the slots whose rows are taken
   __shared__ FewLds few_lds;
   __shared__ f32x4 lds[kFewWaves * 256];
   __shared__ int32_t arrived;
@@ -283,8 +304,30 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
       for (int m = 0; m < MT; ++m) {
         const int row = min(row0 + 16 * m + c, rows - 1);
         s.set_row(m, ((uint32_t)few_lds.slot[row / 2] * 2 + (row & 1)) * (uint32_t)p.ffn_pitch * 2);
+        if constexpr (SCALED) s.unit_row[m] = (uint32_t)few_lds.slot[row / 2] * (uint32_t)p.blocks * 4;
       }
-      s.run(end);
+      if constexpr (SCALED) {
+        s.units = p.units;
+        s.run(end, [&] {   // the largest unit of each row's blocks that lie in this piece of the depth
+          constexpr int OF_SLOT = kFewThreads / (8 * MT), IN_FLIGHT = 4;   // threads
+          const int part = (int)threadIdx.x % OF_SLOT, pair = (int)threadIdx.x / OF_SLOT;
+          const int last = (min(end * S::DEPTH, ffn) - 1) / S::BLOCK;
+          const int32_t* units = p.units + (uint64_t)few_lds.slot[min(row0 / 2 + pair, rows / 2 - 1)] * p.blocks;
+          int most = kNoUnit;
+          for (int b = begin * S::DEPTH / S::BLOCK + part; b <= last; b += IN_FLIGHT * OF_SLOT)
+#pragma unroll
+            for (int f = 0; f < IN_FLIGHT; ++f) most = max(most, units[min(b + f * OF_SLOT, last)]);
+#pragma unroll
+          for (int other = 1; other < OF_SLOT; other *= 2) most = max(most, __shfl_xor(most, other));
+          __syncthreads();   // (what was there is read no more)
+          if (part == 0) row_units[pair] = most;
+          __syncthreads();
+#pragma unroll
+          for (int m = 0; m < MT; ++m) s.row_unit[m] = row_units[8 * m + c / 2];
+        });
+      } else {
+        s.run(end);
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if (row0 + 16 * m >= rows) break;
@@ -312,8 +355,10 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
             }
             if (!own) continue;
             const int slot = few_lds.slot[row / 2];
+            float part = y * a.weights[slot];
+            if constexpr (SCALED) part = ldexpf(part, row_units[8 * m + pair]);
             // (device scope: written to and read from where all XCDs see it, without a fence that empties whole L2s)
-            __hip_atomic_store(&parts[(uint64_t)slot * p.hidden_pitch + column], y * a.weights[slot], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&parts[(uint64_t)slot * p.hidden_pitch + column], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           }
         }
       }
@@ -362,10 +407,10 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
 }
 
 struct FewPlan {
-  int64_t slots, named, up_tiles, down_tiles, pieces, ffn_pitch, hidden_pitch;
+  int64_t slots, named, up_tiles, down_tiles, pieces, ffn_pitch, blocks, hidden_pitch;
   int up_rows, down_rows;   // of 16, that a workgroup takes at a time
   int64_t up_shares, down_shares;   // workgroups that an expert's rows are shared among
-  uint64_t arrivals_bytes, h_bytes, parts_bytes;
+  uint64_t arrivals_bytes, h_bytes, units_bytes, parts_bytes;
 };
 
 constexpr int64_t kFewUnits = 256;   // compute units
@@ -397,6 +442,8 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   f.down_shares = shares(8 * f.down_rows, f.named * f.down_tiles * f.pieces);
   f.arrivals_bytes = (uint64_t)(f.down_tiles * 4 + 255) / 256 * 256;
   f.h_bytes = ((uint64_t)f.slots * f.ffn_pitch * 4 + 255) / 256 * 256;
+  f.blocks = (ffn + (nt ? 31 : 63)) / (nt ? 32 : 64);
+  f.units_bytes = ((uint64_t)f.slots * f.blocks * 4 + 255) / 256 * 256;
   f.hidden_pitch = (hidden + 3) / 4 * 4;
   f.parts_bytes = (uint64_t)f.pieces * f.slots * f.hidden_pitch * 4;
   return f;
@@ -431,7 +478,9 @@ hipError_t launch_few(const FewTokensArgs& a, const FewPlan& f, hipStream_t stre
   char* at = static_cast<char*>(a.scratch);
   p.arrivals = reinterpret_cast<int32_t*>(at);
   p.h = reinterpret_cast<uint16_t*>(at + f.arrivals_bytes);
-  p.parts = reinterpret_cast<float*>(at + f.arrivals_bytes + f.h_bytes);
+  p.units = reinterpret_cast<int32_t*>(at + f.arrivals_bytes + f.h_bytes);
+  p.blocks = (int32_t)f.blocks;
+  p.parts = reinterpret_cast<float*>(at + f.arrivals_bytes + f.h_bytes + f.units_bytes);
   p.tiles = (int32_t)f.up_tiles;
   p.pieces = (int32_t)f.pieces;
   p.counters = (int32_t)f.down_tiles;
@@ -464,7 +513,7 @@ bool few_tokens_fits(int64_t tokens, int64_t experts, int64_t top_k, int64_t hid
 
 uint64_t few_tokens_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, bool trans_b) {
   const FewPlan f = few_plan(tokens, experts, top_k, hidden, ffn, trans_b);
-  return f.arrivals_bytes + f.h_bytes + f.parts_bytes;
+  return f.arrivals_bytes + f.h_bytes + f.units_bytes + f.parts_bytes;
 }
 
 hipError_t few_tokens(const FewTokensArgs& a, hipStream_t stream) {

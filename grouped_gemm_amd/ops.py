@@ -202,7 +202,7 @@ def moe_few_tokens(x, w13, w2, experts, weights, trans_b=False):
     x: bfloat16 or float16 (tokens, hidden), at most 64 tokens; w13 (num_experts, hidden, 2 * ffn) and w2 (num_experts, ffn,
     hidden), or with trans_b (num_experts, 2 * ffn, hidden) and (num_experts, hidden, ffn), as for gmm_swiglu and gmm;
     experts int32 and weights float32 (tokens, top_k), as route returns them.  A number that names no expert
-    contributes nothing.  Rounded once; the activation in between keeps twice the bits of the type.
+    contributes nothing.  Rounded once; the activation in between keeps twice the bits of the type, whatever its size.
 
     For more tokens, and for training: gmm_swiglu and gmm_scatter with the indices of route.  This form has no
     gradient, and refuses operands that ask for one.  Not part of the reference's surface (csrc/grouped_gemm.h:5-9)."""

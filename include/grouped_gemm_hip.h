@@ -387,7 +387,8 @@ int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t exp
  *   chosen int32 (tokens, top_k), weights fp32 (tokens, top_k), as gg_route writes them
  * all contiguous, aligned to their elements.  A number in `chosen` that names no expert contributes nothing; an expert named twice by a token
  * counts twice.  Products and sums are in fp32; between the two the activations are handed on with twice the bits of the
- * type, and the result is rounded once.  The same bits on every call.
+ * type, of any size (fp16: scaled by powers of two, exact to 2^-37 of a row's largest), and the result is rounded once.  The same
+ * bits on every call.
  * At most GG_FEW_TOKENS_MAX tokens (more belong in gg_gmm with row indices), GG_ROUTE_MAX_EXPERTS experts, top_k at
  * most GG_ROUTE_MAX_TOP_K, hidden and ffn below 2^22.  `scratch`: gg_moe_few_tokens_scratch_bytes of device memory (0 for sizes that the
  * call refuses), 256-byte aligned, of any contents; calls that share it must not overlap in time.

@@ -418,6 +418,79 @@ def test_moe_few_tokens_large_values(ops):
     assert float(got) == INF
 
 
+def _moe_reference_of_range(x, w13, w2, experts, weights, trans_b):
+    """The layer in 64 bits, and by how much each element may be off where what is handed on keeps its bits whatever its size: 2^-16 of itself
+    in bfloat16; in float16 2^-21 of itself and 2^-37 of the row's largest: its two halves are scaled by blocks, the largest to 2^14 at least (the
+    lower one is off by up to 2^-25 there), and then to the row's largest (each off by the same once more, at most half of it again where the
+    power of two is applied in two steps: 4 x 2^-25 of 2^14)."""
+    t, hidden = x.shape
+    ffn = w2.shape[2 if trans_b else 1]
+    unit, of_largest = (2.0 ** -16, 0.0) if x.dtype == torch.bfloat16 else (2.0 ** -21, 2.0 ** -37)
+    out, off = torch.zeros(t, hidden, dtype=torch.float64), torch.zeros(t, hidden, dtype=torch.float64)
+    for i in range(t):
+        for j in range(experts.shape[1]):
+            e, w = int(experts[i, j]), float(weights[i, j])
+            first, second = w13[e].double(), w2[e].double()
+            if trans_b:
+                first, second = first.t(), second.t()
+            both = x[i].double() @ first
+            err = (x[i].double().abs() @ first.abs()) * (2 * hidden * 2.0 ** -24)
+            gate, up = both[:ffn], both[ffn:]
+            s = torch.sigmoid(gate)
+            h = gate * s * up
+            h_off = 1.1 * err[:ffn] * (up.abs() + err[ffn:]) + (gate * s).abs() * err[ffn:] + h.abs() * (unit + 2.0 ** -20)
+            h_off += h.abs().max() * of_largest
+            out[i] += w * (h @ second)
+            off[i] += abs(w) * ((h_off @ second.abs()) + (h.abs() @ second.abs()) * ((2 * ffn + 64) * 2.0 ** -24))
+    return out, off
+
+
+# one block of columns, parts of blocks, pieces of the depth, odd sizes, more rows than are taken at a time, rows that workgroups share
+RANGE_SHAPES = [(1, 4, 2, 64, 24), (5, 8, 2, 100, 129), (2, 3, 2, 72, 2100), (33, 3, 2, 57, 65), (64, 4, 3, 95, 271), (64, 130, 8, 40, 33)]
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["large", "small", "mixed"])
+@pytest.mark.parametrize("shape", RANGE_SHAPES)
+def test_moe_few_tokens_activations_of_any_size(ops, shape, kind, dtype, trans_b):
+    """Activations far past float16's largest number, far below its least, and of sizes 2^24 apart in one row, each made up for by the second
+    weights: the result is an ordinary number, and has to be as exact as one."""
+    t, num, k, hidden, ffn = shape
+    x, w13, w2, experts, weights = _moe_case(t, num, k, hidden, ffn, torch.float32, False, seed=sum(shape))
+    if kind == "large":     # gates and ups of 2^10 or so
+        w13, w2 = w13 * 2.0 ** 10, w2 * 2.0 ** -14
+    elif kind == "small":   # ... of 2^-12
+        w13, w2 = w13 * 2.0 ** -12, w2 * 2.0 ** 12
+    else:
+        size = torch.randint(-6, 7, (ffn,), generator=torch.Generator().manual_seed(ffn)).double()
+        w13 = (w13 * torch.exp2(torch.cat([size, size]))).float()
+        w2 = (w2 * torch.exp2(-2 * size)[:, None]).float()
+    if trans_b:
+        w13, w2 = w13.transpose(1, 2), w2.transpose(1, 2)
+    case = [v.to(dtype).contiguous() for v in (x, w13, w2)] + [experts, weights]
+    _announce("moe activations of any size", shape, kind, dtype, trans_b)
+    got = ops.moe_few_tokens(*(v.cuda() for v in case), trans_b=trans_b)
+    want, off = _moe_reference_of_range(*case, trans_b)
+    rtol, least = ROUNDING[dtype]
+    assert float(want.abs().max()) < 3e4
+    _close(got, want, rtol, off * (1 + rtol) + least, f"{shape} {kind}")
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_moe_few_tokens_float16_past_its_largest_activation(ops, trans_b):
+    """gate = up = 300: 90000 between the two products.  Against a small weight, one of zero, and one of the other sign."""
+    x = torch.tensor([[1.0, 0.0], [0.0, 1.0]], dtype=torch.float16)
+    w13 = torch.tensor([[[300.0, 300.0, 300.0, 300.0], [300.0, 300.0, -300.0, 300.0]]], dtype=torch.float16)   # gates | ups
+    w2 = torch.tensor([[[2.0 ** -10, 0.0], [2.0 ** -11, 0.0]]], dtype=torch.float16)
+    if trans_b:
+        w13, w2 = w13.transpose(1, 2).contiguous(), w2.transpose(1, 2).contiguous()
+    experts, weights = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1)
+    got = ops.moe_few_tokens(*(v.cuda() for v in (x, w13, w2, experts, weights)), trans_b=trans_b).cpu().double()
+    want = torch.tensor([[90000 * (2.0 ** -10 + 2.0 ** -11), 0.0], [-90000 * 2.0 ** -10 + 90000 * 2.0 ** -11, 0.0]], dtype=torch.float64)
+    _close(got, want, 2.0 ** -11 + 2.0 ** -20, 2.0 ** -25, "past the largest")
+
+
 def test_moe_few_tokens_full_size_on_the_device(ops):
     """A large layer against 32-bit products on the device, every element (both sum in fp32: 4096 products of either sign,
     far within a rounding of the type)."""
