@@ -11,7 +11,8 @@
 // its window's rows from one load and a ballot for each adapter.
 //
 // v is kept in fp32, summed over pieces of the depth by its readers, and split there into two numbers of the
-// element type (high, and what its rounding left), each multiplied by b_l: nothing of v is lost that the result could show.
+// element type (high, and what its rounding left), each multiplied by b_l: v is exact to twice the bits of the type, in float16 to 2^-38 of its
+// row's largest.
 #include "operators.hpp"
 
 #include <math.h>
@@ -233,7 +234,8 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
         float scaling = 1.0f;
         int up = 0;
         if constexpr (DT == kF16) {
-          // v may be larger than the type holds: its row is scaled to below 1 by a power of two, exactly
+          // v may be larger than the type holds, or have elements too small for its bits: its row is scaled by a power of two, exactly, so that
+          // the largest comes to 2^14 .. 2^15
           float most = 0.0f;
 #pragma unroll
           for (int j = 0; j < EACH; ++j)
@@ -241,8 +243,8 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
             for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[j][e]));
 #pragma unroll
           for (int other = 1; other < TPR; other *= 2) most = fmaxf(most, __shfl_xor(most, other));
-          // (rows of zeros, and of infinities, stay what they are)
-          if (most > 0.0f && most < INFINITY) up = min(max(ilogbf(most) + 1, -100), 120);
+          // (rows of zeros stay what they are; beside an infinity, whose place no finite sum can show in, all else may vanish)
+          if (most > 0.0f) up = most < INFINITY ? max(ilogbf(most) - 14, -126) : 114;
           scaling = ldexpf(1.0f, -up);
         }
         __syncthreads();

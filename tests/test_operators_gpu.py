@@ -15,6 +15,7 @@ quotient are off by 2^-20, and the result is rounded once.
 
 Whole numbers are equal."""
 import ctypes
+import math
 import os
 
 import pytest
@@ -741,6 +742,31 @@ def test_lora_large_and_small_values(ops):
     assert torch.isinf(got[2]).all() and torch.isfinite(got[:2]).all()
     small = torch.full((1, 8, 64), 2.0 ** -24, dtype=torch.float16)
     _check_lora(ops, (x[:2], small, torch.full((1, 40, 8), 1000.0, dtype=torch.float16), adapters[:2], base[:2], scales), "small v")
+
+
+@pytest.mark.parametrize("rank", [2, 16, 30, 64, 128])
+def test_lora_float16_small_beside_large(ops, rank):
+    """float16's v is handed on in two halves, its row scaled to 2^14 at least: off by 2^-21 of itself and twice 2^-25 of that, 2^-38 of the row's largest.
+    Half of each row is 2^20 times smaller than the other, and meets b that is as much larger."""
+    x, a, b, adapters, base, _ = _lora_case(70, 3, rank, 96, 130, torch.float16, seed=rank)
+    a[:, ::2] = a[:, ::2] * 2.0 ** 10
+    a[:, 1::2] = a[:, 1::2] * 2.0 ** -10
+    b[:, :, ::2] = b[:, :, ::2] * 2.0 ** -10
+    b[:, :, 1::2] = b[:, :, 1::2] * 2.0 ** 10
+    base[:] = 0
+    want, off = torch.zeros(70, 130, dtype=torch.float64), torch.zeros(70, 130, dtype=torch.float64)
+    for t in range(70):
+        n = int(adapters[t])
+        if n < 0:
+            continue
+        an, bn = a[n].double(), b[n].double()
+        v = an @ x[t].double()
+        v_off = (an.abs() @ x[t].double().abs()) * (2 * 96 * 2.0 ** -24) + v.abs() * 2.0 ** -21 + v.abs().max() * 2.0 ** -38
+        want[t] = bn @ v
+        off[t] = bn.abs() @ v_off + (bn.abs() @ v.abs()) * ((4 * rank + 8) * 2.0 ** -24)
+    _announce("lora small beside large", rank)
+    got = ops.lora(x.cuda(), a.cuda(), b.cuda(), adapters.cuda(), base=base.cuda())
+    _close(got, want, 2.0 ** -11, off * (1 + 2.0 ** -11) + 2.0 ** -25, "small beside large")
 
 
 def test_lora_same_bits_on_streams_and_in_graphs(ops):
