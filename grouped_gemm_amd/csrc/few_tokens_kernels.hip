@@ -340,21 +340,22 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void few_down_kernel(
             const int pair = item >> 6, n = item & 63;   // of 8 slots, of 64 columns
             const int row = row0 + 16 * m + 2 * pair;
             if (row >= rows) break;
-            float y;
+            float y, lower;   // of the two halves of h
             int column;
             bool own;
             if constexpr (NT) {
-              y = exchange.column_of_tiles(n, 2 * pair) + exchange.column_of_tiles(n, 2 * pair + 1);
+              y = exchange.column_of_tiles(n, 2 * pair), lower = exchange.column_of_tiles(n, 2 * pair + 1);
               column = column0 + n;
               own = column < hidden;
             } else {
               const int start = column0 + round * 64 + (n >> 3) * 8;
-              y = exchange.column_of_block(0, n >> 3, n & 7, 2 * pair) + exchange.column_of_block(0, n >> 3, n & 7, 2 * pair + 1);
+              y = exchange.column_of_block(0, n >> 3, n & 7, 2 * pair), lower = exchange.column_of_block(0, n >> 3, n & 7, 2 * pair + 1);
               column = (hidden < 8 ? 0 : min(start, hidden - 8)) + (n & 7);
               own = column >= start && column < hidden;
             }
             if (!own) continue;
             const int slot = few_lds.slot[row / 2];
+            if (fabsf(y) < INFINITY) y += lower;   // (against an infinite weight the lower half, zero or of any sign, would make NaN)
             float part = y * a.weights[slot];
             if constexpr (SCALED) part = ldexpf(part, row_units[8 * m + pair]);
             // (device scope: written to and read from where all XCDs see it, without a fence that empties whole L2s)

@@ -492,6 +492,27 @@ def test_moe_few_tokens_float16_past_its_largest_activation(ops, trans_b):
     _close(got, want, 2.0 ** -11 + 2.0 ** -20, 2.0 ** -25, "past the largest")
 
 
+@pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_moe_few_tokens_infinite_weights(ops, dtype, trans_b):
+    """An infinite weight of the second product gives an infinity of its sign, as its formula does, whatever is left of the activation in its lower
+    half: nothing (600, 3), or something of either sign (silu(1) = 0.7310586, silu(2) = 1.7615942); other columns do not notice."""
+    for gate, up in ((200.0, 3.0), (1.0, 1.0), (2.0, 1.0), (2.0, -1.0)):
+        x = torch.ones(3, 1, dtype=dtype)
+        w13 = torch.tensor([[[gate, up]]], dtype=dtype)
+        w2 = torch.tensor([[[1.0, INF, -INF]]], dtype=dtype)
+        x, w13, w2 = torch.cat([x, x, x], 1), torch.cat([w13, 0 * w13, 0 * w13], 1), w2   # (hidden is 3)
+        if trans_b:
+            w13, w2 = w13.transpose(1, 2).contiguous(), w2.transpose(1, 2).contiguous()
+        experts, weights = torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, 1)
+        _announce("moe infinite weights", gate, up, dtype, trans_b)
+        got = ops.moe_few_tokens(*(v.cuda() for v in (x, w13, w2, experts, weights)), trans_b=trans_b).cpu().double()
+        h = gate / (1 + math.exp(-gate)) * up
+        want = torch.tensor([[h, math.copysign(INF, h), math.copysign(INF, -h)]] * 3, dtype=torch.float64)
+        rtol, least = ROUNDING[dtype]
+        _close(got, want, rtol + 2.0 ** -15, least, "infinite weights")
+
+
 def test_moe_few_tokens_full_size_on_the_device(ops):
     """A large layer against 32-bit products on the device, every element (both sum in fp32: 4096 products of either sign,
     far within a rounding of the type)."""
