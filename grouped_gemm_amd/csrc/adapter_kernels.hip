@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
   __shared__ __attribute__((aligned(16))) uint16_t split_v[2][GROUP][PITCH];   // high, low
   __shared__ float unit[GROUP];
   const AdapterArgs& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4, wave = uniform(tid >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int64_t window = blockIdx.x / p.shares, first = window * kWindow;
   const int share = (int)(blockIdx.x - window * p.shares), columns = a.hidden_out, blocks = (columns + kBlock - 1) / kBlock;
   const WindowPlan& plan = p.plans[window];
@@ -204,6 +204,9 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
     const uint16_t* weights = static_cast<const uint16_t*>(a.b) + (uint64_t)which * columns * a.rank;
     const float scale = a.scales != nullptr ? a.scales[which] : 1.0f;
     for (int row0 = 0; row0 < rows; row0 += GROUP) {
+      int thread = threadIdx.x;
+      asm("" : "+v"(thread));   // (what follows from it is worked out here, where it is used: kept from ahead of the loops, some would be spilled)
+      const int tid = thread, lane = tid & 63, c = lane & 15, q = lane >> 4;
       {
         const int row = tid / TPR, part = tid % TPR;
         const float* v = p.v + (uint64_t)(first + __shfl(list, min(row0 + row, rows - 1))) * p.v_pitch;
@@ -243,12 +246,12 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
             for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[j][e]));
 #pragma unroll
           for (int other = 1; other < TPR; other *= 2) most = fmaxf(most, __shfl_xor(most, other));
-          // (rows of zeros stay what they are; beside an infinity, whose place no finite sum can show in, all else may vanish)
-          if (most > 0.0f) up = most < INFINITY ? max(ilogbf(most) - 14, -126) : 114;
-          scaling = ldexpf(1.0f, -up);
+          // (beside an infinity, whose place no finite sum can show in, all else may vanish)
+          up = max((int)(__builtin_bit_cast(uint32_t, most) >> 23 & 0xff) - 127 - 14, -126);
+          scaling = __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);   // 2^-up
         }
         __syncthreads();
-        if (DT == kF16 && part == 0) unit[row] = ldexpf(1.0f, up);
+        if (DT == kF16 && part == 0) unit[row] = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
           u32x2 high, low;
