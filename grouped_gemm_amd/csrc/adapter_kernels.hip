@@ -259,12 +259,7 @@ __global__ __launch_bounds__(kExpandThreads, KS <= 2 ? 4 : 2) void adapter_expan
           for (int e = 0; e < 2; ++e) {
             uint32_t h[2], l[2];
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-              const float s = x[j][2 * e + o] * scaling;
-              h[o] = round_bits<DT>(s);
-              const float rest = s - widen_bits<DT>((uint16_t)h[o]);
-              l[o] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : 0u;
-            }
+            for (int o = 0; o < 2; ++o) split<DT>(x[j][2 * e + o] * scaling, h[o], l[o]);
             high[e] = h[0] | h[1] << 16;
             low[e] = l[0] | l[1] << 16;
           }

@@ -70,6 +70,15 @@ __device__ __forceinline__ float widen_bits(uint16_t v) {
   else return (float)__builtin_bit_cast(_Float16, v);
 }
 
+// v in two numbers of the type: rounded, but not past the largest, and what that left: finite both where v is (float16's callers keep it below
+// 2^15).  Of an infinity, and of NaN, the second is one.
+template <int DT>
+__device__ __forceinline__ void split(float v, uint32_t& high, uint32_t& low) {
+  constexpr float LARGEST = DT == kBF16 ? 0x1.fep127f : 65504.0f;
+  high = round_bits<DT>(__builtin_amdgcn_fmed3f(v, -LARGEST, LARGEST));
+  low = round_bits<DT>(v - widen_bits<DT>((uint16_t)high));
+}
+
 // One wave's stream: its share of the depth of a strip of weights against up to 16 * MT rows.
 //   NT   tiles of 16 weight rows, the first half of them from `first` and the others from `second` on; 64 deep at a time
 //   NN   128 columns, in each lane 8 neighbouring ones; 32 deep at a time

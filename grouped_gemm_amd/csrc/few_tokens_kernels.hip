@@ -242,11 +242,10 @@ __global__ __launch_bounds__(gate_up_threads(NT), MT == 1 ? 3 : 2) void few_gate
             h = ldexpf(h, -unit);
           }
           if (!own) continue;
-          const uint16_t high = round_bits<DT>(h);
-          const float rest = h - widen_bits<DT>(high);
           uint16_t* to = p.h + (uint64_t)few_lds.slot[row] * 2 * p.ffn_pitch + column;
-          to[0] = high;
-          to[p.ffn_pitch] = fabsf(rest) < INFINITY ? round_bits<DT>(rest) : uint16_t(0);   // (an infinite h has no rest)
+          uint32_t high, low;
+          split<DT>(h, high, low);
+          to[0] = (uint16_t)high, to[p.ffn_pitch] = (uint16_t)low;
         }
       }
     }

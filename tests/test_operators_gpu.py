@@ -513,6 +513,21 @@ def test_moe_few_tokens_infinite_weights(ops, dtype, trans_b):
         _close(got, want, rtol + 2.0 ** -15, least, "infinite weights")
 
 
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_moe_few_tokens_bfloat16_largest_activation(ops, trans_b):
+    """An activation between the largest bfloat16 and the largest float, which rounds up to an infinity: (2 - 2^-9) 2^127."""
+    x = torch.ones(1, 2, dtype=torch.bfloat16)
+    w13 = torch.tensor([[[(2 - 2.0 ** -7) * 2.0 ** 64, 2.0 ** 63], [0.75 * 2.0 ** 57, 0.0]]], dtype=torch.float64)
+    w2 = torch.tensor([[[2.0 ** -100, 0.0]]], dtype=torch.bfloat16)
+    w13 = w13.bfloat16()
+    if trans_b:
+        w13, w2 = w13.transpose(1, 2).contiguous(), w2.transpose(1, 2).contiguous()
+    got = ops.moe_few_tokens(x.cuda(), w13.cuda(), w2.cuda(), torch.zeros(1, 1, dtype=torch.int32).cuda(), torch.ones(1, 1).cuda(),
+                             trans_b=trans_b).cpu().double()
+    want = torch.tensor([[(2 - 2.0 ** -9) * 2.0 ** 27, 0.0]], dtype=torch.float64)
+    _close(got, want, 2.0 ** -8 + 2.0 ** -15, 0.0, "largest")
+
+
 def test_moe_few_tokens_full_size_on_the_device(ops):
     """A large layer against 32-bit products on the device, every element (both sum in fp32: 4096 products of either sign,
     far within a rounding of the type)."""
@@ -763,6 +778,16 @@ def test_lora_large_and_small_values(ops):
     assert torch.isinf(got[2]).all() and torch.isfinite(got[:2]).all()
     small = torch.full((1, 8, 64), 2.0 ** -24, dtype=torch.float16)
     _check_lora(ops, (x[:2], small, torch.full((1, 40, 8), 1000.0, dtype=torch.float16), adapters[:2], base[:2], scales), "small v")
+
+
+def test_lora_bfloat16_largest_value(ops):
+    """Between the two products, a number between the largest bfloat16 and the largest float, which rounds up to an infinity: (2 - 2^-9) 2^127."""
+    x = torch.ones(1, 2, dtype=torch.bfloat16)
+    a = torch.tensor([[[(2 - 2.0 ** -7) * 2.0 ** 127, 0.75 * 2.0 ** 120]]], dtype=torch.float64).bfloat16()
+    b = torch.tensor([[[2.0 ** -100], [0.0]]], dtype=torch.bfloat16)
+    got = ops.lora(x.cuda(), a.cuda(), b.cuda(), torch.zeros(1, dtype=torch.int32).cuda()).cpu().double()
+    want = torch.tensor([[(2 - 2.0 ** -9) * 2.0 ** 27, 0.0]], dtype=torch.float64)
+    _close(got, want, 2.0 ** -8 + 2.0 ** -15, 0.0, "largest")
 
 
 @pytest.mark.parametrize("rank", [2, 16, 30, 64, 128])
