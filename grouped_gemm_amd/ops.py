@@ -219,7 +219,7 @@ def lora(x, a, b, adapters, base=None, scales=None, c=None):
     x: bfloat16 or float16 (rows, hidden_in); a (num_adapters, rank, hidden_in) and b (num_adapters, hidden_out, rank), as linear
     layers store them (rank at most 256, smaller ones beside it padded with zeros); adapters int32 (rows), where a
     number that names no adapter, as -1, leaves the row as it is in base; base (rows, hidden_out) the shared projection's
-    result, None: zeros; scales float32 (num_adapters), None: 1.  c receives the result; it may be base itself.  Rows come in any order.
+    result, None: zeros; scales float32 (num_adapters), None: 1.  b is finite: an infinite element gives NaN.  c receives the result; it may be base itself.  Rows come in any order.
 
     No gradient: adapters are trained with gmm on rows sorted by adapter, and operands that ask for one are refused.  Not part of the reference's
     surface (csrc/grouped_gemm.h:5-9)."""

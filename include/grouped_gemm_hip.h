@@ -409,7 +409,8 @@ int gg_moe_few_tokens(const void* x, const void* w13, const void* w2, const int3
  *   scales fp32 (num) or NULL (1); base NULL: 0
  * all contiguous, aligned to their elements; out may be base (in place) and overlaps nothing else.  Rows may come in any order; rows of one
  * request are best neighbours (rows are taken in windows of 64).  Sums are in fp32, x @ a^T is handed on with twice the bits of the type (fp16:
- * scaled by powers of two, exact to 2^-38 of a row's largest), the result is rounded once.  The same bits on every call.
+ * scaled by powers of two, exact to 2^-38 of a row's largest), the result is rounded once.  An infinite element of b gives NaN in its column, not an
+ * infinity (v is multiplied in two parts, of which one may be zero).  The same bits on every call.
  * rank at most GG_LORA_MAX_RANK (smaller ranks beside larger ones: zeros), hidden sizes below 2^22.  `scratch`: gg_lora_scratch_bytes of device
  * memory, 16-byte aligned, of any contents; calls that share it must not overlap in time.
  * No counterpart in the reference, whose groups are consecutive rows of one matrix each (csrc/grouped_gemm.h:5-9).

@@ -528,6 +528,28 @@ def test_moe_few_tokens_bfloat16_largest_activation(ops, trans_b):
     _close(got, want, 2.0 ** -8 + 2.0 ** -15, 0.0, "largest")
 
 
+@pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_moe_few_tokens_infinite_activations(ops, dtype, trans_b):
+    """An infinite activation gives infinities, NaN against a weight of zero, as its formula does; other tokens do not notice."""
+    x, w13, w2, experts, weights = _moe_case(5, 3, 2, 40, 100, dtype, trans_b, seed=8)
+    x[3] = 0
+    x[3, 0] = INF
+    for e in range(3):
+        first, second = (w13[e].t(), w2[e].t()) if trans_b else (w13[e], w2[e])   # (views)
+        first[0] = first[0].abs() + 0.125           # every gate and every up of token 3 infinite
+        second[:, 5], second[:, 6], second[:, 7] = second[:, 5].abs() + 0.125, -second[:, 6].abs() - 0.125, 0.0
+    _announce("moe infinite activations", dtype, trans_b)
+    got = ops.moe_few_tokens(*(v.cuda() for v in (x, w13, w2, experts, weights)), trans_b=trans_b).cpu()
+    x[3, 0] = 0
+    want, off = _moe_reference(x, w13, w2, experts, weights, trans_b)
+    rtol, least = ROUNDING[dtype]
+    others = torch.tensor([0, 1, 2, 4])
+    _close(got[others], want[others], rtol, (off * (1 + rtol) + least)[others], "other tokens")
+    assert got[3, 5] == INF and got[3, 6] == -INF and torch.isnan(got[3, 7])
+    assert not torch.isfinite(got[3]).any()
+
+
 def test_moe_few_tokens_full_size_on_the_device(ops):
     """A large layer against 32-bit products on the device, every element (both sum in fp32: 4096 products of either sign,
     far within a rounding of the type)."""
