@@ -23,6 +23,12 @@ torch::Tensor Scratch(uint64_t bytes, const torch::Tensor& like) {
 
 void* Pointer(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Kernels see values only: a tangent that came in would be dropped without a word (in any mode of gradients, which forward mode does not heed).
+void RefuseTangents(std::initializer_list<const torch::Tensor*> tensors, const char* name) {
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "grouped_gemm: ", name, " has no forward-mode derivative");
+}
+
 // ------------------------------------------------------------------ router
 
 int LogitsType(torch::ScalarType t) {
@@ -85,6 +91,7 @@ class RouteNode : public torch::autograd::Function<RouteNode> {
     torch::Tensor weights_grad = grads[0], mass_grad = grads.size() > 5 ? grads[5] : torch::Tensor();
     torch::Tensor none;
     if (!weights_grad.defined() && !mass_grad.defined()) return {none, none, none, none, none};
+    RefuseTangents({&weights_grad, &mass_grad}, "the gradient of route");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
     if (weights_grad.defined()) weights_grad = weights_grad.contiguous();
     if (mass_grad.defined()) mass_grad = mass_grad.contiguous();
@@ -102,6 +109,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
     const torch::Tensor& logits, int64_t top_k, const std::string& score, bool normalize, bool with_mass) {
   const int which = Score(score);
   CheckLogits(logits, top_k);
+  RefuseTangents({&logits}, "route");
   torch::autograd::variable_list out;
   if (torch::GradMode::is_enabled() && logits.requires_grad()) {
     out = RouteNode::apply(logits, top_k, (int64_t)which, normalize, with_mass);
@@ -119,6 +127,7 @@ bool IsTwoByte(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloa
 
 // Operators for serving have no gradient: a graph that asks for one is an error, not a silent zero.
 void RefuseGradients(std::initializer_list<const torch::Tensor*> tensors, const char* name, const char* instead) {
+  RefuseTangents(tensors, name);
   if (!torch::GradMode::is_enabled()) return;
   for (const torch::Tensor* t : tensors)
     TORCH_CHECK(!t->defined() || !t->requires_grad(), "grouped_gemm: ", name, " has no gradient (", instead, ")");

@@ -238,6 +238,19 @@ def test_route_gradient_matches_differences(ops, score, normalize):
             assert abs(float(got[i, j]) - want) <= scale * (h * h / 3 + 4 * 2.0 ** -22 / h), (i, j)
 
 
+def test_route_refuses_forward_mode(ops):
+    """A tangent is an error, not a result without one, with and without gradient mode; gradients in reverse go on as before."""
+    x = torch.randn(6, 8, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        for leaf in (x, x.clone().requires_grad_(True)):
+            dual = torch.autograd.forward_ad.make_dual(leaf, torch.randn_like(x))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.route(dual, 2)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.route(dual, 2, with_mass=True)
+        ops.route(x, 2)
+
+
 def test_route_on_other_streams_and_in_a_graph(ops):
     """The same bits on another stream, on every call and in every replay of a captured one, with eager work in between."""
     logits = torch.randn(5000, 96, device="cuda").bfloat16()
@@ -615,6 +628,16 @@ def test_moe_few_tokens_refuses(ops):
         call(w2=w2.clone().requires_grad_(True))
 
 
+def test_moe_few_tokens_refuses_forward_mode(ops):
+    case = [v.cuda() for v in _moe_case(2, 4, 2, 32, 48, torch.bfloat16, False, seed=1)]
+    with torch.autograd.forward_ad.dual_level():
+        for i in (0, 1, 2, 4):
+            dual = list(case)
+            dual[i] = torch.autograd.forward_ad.make_dual(case[i], torch.ones_like(case[i]))
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.moe_few_tokens(*dual)
+
+
 # ------------------------------------------------------------------ low-rank adapters
 
 def _lora_reference(x, a, b, adapters, base, scales):
@@ -861,6 +884,17 @@ def test_lora_same_bits_on_streams_and_in_graphs(ops):
         for one in (again, captured, eager):
             for got, w in zip(one, want):
                 assert torch.equal(got, w)
+
+
+def test_lora_refuses_forward_mode(ops):
+    x, a, b, adapters, base, scales = (v.cuda() for v in _lora_case(6, 3, 8, 32, 48, torch.bfloat16, seed=1))
+    args = dict(x=x, a=a, b=b, adapters=adapters, base=base, scales=scales)
+    with torch.autograd.forward_ad.dual_level():
+        for name in ("x", "a", "b", "base", "scales"):
+            dual = dict(args)
+            dual[name] = torch.autograd.forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                ops.lora(**dual)
 
 
 def test_lora_refuses(ops):
