@@ -71,6 +71,33 @@ torch::autograd::variable_list RunRoute(const torch::Tensor& logits, int64_t top
   return {weights, chosen, batch_sizes, row_index, order, mass};
 }
 
+torch::Tensor RunRouteBackward(const torch::Tensor& logits, const torch::Tensor& chosen, torch::Tensor weights_grad, torch::Tensor mass_grad,
+                               int score, bool normalize) {
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  if (weights_grad.defined()) weights_grad = weights_grad.contiguous();
+  if (mass_grad.defined()) mass_grad = mass_grad.contiguous();
+  torch::Tensor out = torch::empty(logits.sizes(), logits.options().requires_grad(false));
+  const int rc = gg_route_backward(logits.data_ptr(), LogitsType(logits.scalar_type()), logits.size(0), logits.size(1), chosen.size(1), score,
+                                   normalize, chosen.data_ptr<int32_t>(), static_cast<const float*>(Pointer(weights_grad)),
+                                   static_cast<const float*>(Pointer(mass_grad)), out.data_ptr(), CurrentStream(logits.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return out;
+}
+
+// The gradient where a graph of it is wanted (create_graph): a second derivative through it is an error, not a silent zero.
+class RouteGradientNode : public torch::autograd::Function<RouteGradientNode> {
+ public:
+  static torch::Tensor forward(torch::autograd::AutogradContext*, const torch::Tensor& logits, const torch::Tensor& chosen,
+                               const c10::optional<torch::Tensor>& weights_grad, const c10::optional<torch::Tensor>& mass_grad, int64_t score,
+                               bool normalize) {
+    return RunRouteBackward(logits, chosen, weights_grad.value_or(torch::Tensor()), mass_grad.value_or(torch::Tensor()), (int)score, normalize);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "grouped_gemm: route has no second derivative");
+  }
+};
+
 class RouteNode : public torch::autograd::Function<RouteNode> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& logits, int64_t top_k,
@@ -88,19 +115,18 @@ class RouteNode : public torch::autograd::Function<RouteNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor &logits = saved[0], &chosen = saved[1];
-    torch::Tensor weights_grad = grads[0], mass_grad = grads.size() > 5 ? grads[5] : torch::Tensor();
-    torch::Tensor none;
+    const torch::Tensor weights_grad = grads[0], mass_grad = grads.size() > 5 ? grads[5] : torch::Tensor(), none;
     if (!weights_grad.defined() && !mass_grad.defined()) return {none, none, none, none, none};
     RefuseTangents({&weights_grad, &mass_grad}, "the gradient of route");
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
-    if (weights_grad.defined()) weights_grad = weights_grad.contiguous();
-    if (mass_grad.defined()) mass_grad = mass_grad.contiguous();
-    torch::Tensor out = torch::empty(logits.sizes(), logits.options().requires_grad(false));
-    const int rc = gg_route_backward(logits.data_ptr(), LogitsType(logits.scalar_type()), logits.size(0), logits.size(1),
-                                     chosen.size(1), (int)ctx->saved_data["score"].toInt(), ctx->saved_data["normalize"].toBool(),
-                                     chosen.data_ptr<int32_t>(), static_cast<const float*>(Pointer(weights_grad)),
-                                     static_cast<const float*>(Pointer(mass_grad)), out.data_ptr(), CurrentStream(logits.device()));
-    TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+    const int64_t score = ctx->saved_data["score"].toInt();
+    const bool normalize = ctx->saved_data["normalize"].toBool();
+    torch::Tensor out;
+    if (torch::GradMode::is_enabled()) {
+      const auto given = [](const torch::Tensor& t) { return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt; };
+      out = RouteGradientNode::apply(logits, chosen, given(weights_grad), given(mass_grad), score, normalize);
+    } else {
+      out = RunRouteBackward(logits, chosen, weights_grad, mass_grad, (int)score, normalize);
+    }
     return {out, none, none, none, none};
   }
 };

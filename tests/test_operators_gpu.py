@@ -251,6 +251,30 @@ def test_route_refuses_forward_mode(ops):
         ops.route(x, 2)
 
 
+@pytest.mark.parametrize("parts", ["weights", "mass", "both"])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_refuses_a_second_derivative(ops, normalize, parts):
+    """With create_graph the gradient is the same, other terms of a loss have their second derivative, and one through the router's is an error."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(6, 6, device="cuda", generator=g).requires_grad_(True)
+    x, at = torch.randn(5, 6, device="cuda", generator=g), torch.randn(5, 2, device="cuda", generator=g)
+
+    def loss():
+        r = ops.route(x @ w, 2, normalize=normalize, with_mass=True)
+        weights, mass = (r.weights * at).sum(), r.mass.square().sum()
+        return w.pow(3).sum() + {"weights": weights, "mass": mass, "both": weights + mass}[parts]
+
+    want, = torch.autograd.grad(loss(), w)
+    got, = torch.autograd.grad(loss(), w, create_graph=True)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(got.sum(), w)
+    both = loss()
+    cubes, = torch.autograd.grad(w.pow(3).sum() + 0 * both.detach(), w, create_graph=True)
+    second, = torch.autograd.grad(cubes.sum(), w)
+    assert torch.equal(second, 6 * w.detach())
+
+
 def test_route_on_other_streams_and_in_a_graph(ops):
     """The same bits on another stream, on every call and in every replay of a captured one, with eager work in between."""
     logits = torch.randn(5000, 96, device="cuda").bfloat16()
