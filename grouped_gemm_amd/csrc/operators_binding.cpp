@@ -242,6 +242,7 @@ torch::Tensor Lora(const torch::Tensor& x, const torch::Tensor& a, const torch::
                          Pointer(from), out.data_ptr(), x.scalar_type() == torch::kFloat16 ? GG_DTYPE_F16 : GG_DTYPE_BF16, rows, num, rank,
                          hidden_in, hidden_out, Pointer(scratch), CurrentStream(x.device()));
   TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  if (to.defined() && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();   // (a write that a graph which saved c has to notice)
   return out;
 }
 

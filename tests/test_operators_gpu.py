@@ -921,6 +921,24 @@ def test_lora_refuses_forward_mode(ops):
                 ops.lora(**dual)
 
 
+def test_lora_into_a_given_tensor_is_a_write(ops):
+    """What saved c for its gradient notices, as with torch's own writes; without a graph, and on tensors that keep no count of writes, it just writes."""
+    x, a, b, adapters, base, scales = (v.cuda() for v in _lora_case(6, 3, 8, 32, 48, torch.bfloat16, seed=1))
+    p = torch.ones_like(base).requires_grad_(True)
+    y = (p * base).sum()
+    ops.lora(x, a, b, adapters, base=base, scales=scales, c=base)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    fresh = base.clone()
+    y = (p * base).sum()
+    ops.lora(x, a, b, adapters, base=base, scales=scales, c=fresh)
+    y.backward()
+    assert torch.equal(p.grad, base)
+    with torch.inference_mode():
+        c = torch.empty_like(base)
+        assert torch.equal(ops.lora(x, a, b, adapters, base=base, scales=scales, c=c), fresh)
+
+
 def test_lora_refuses(ops):
     x, a, b, adapters, base, scales = (v.cuda() for v in _lora_case(6, 3, 8, 32, 48, torch.bfloat16, seed=1))
 
