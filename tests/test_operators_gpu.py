@@ -630,6 +630,40 @@ def test_moe_few_tokens_same_bits_on_streams_and_in_graphs(ops):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+# more than 64 slots (listed in any order), an expert's rows shared among workgroups in the second product, in the first one too (listed in their own)
+@pytest.mark.parametrize("shape", [(24, 8, 4, 512, 1000), (64, 130, 8, 96, 200), (64, 4, 4, 1024, 2048), (64, 4, 4, 256, 512), (64, 3, 3, 129, 333)])
+def test_moe_few_tokens_same_bits_of_many_slots(ops, shape, dtype, trans_b):
+    """On every call, on another stream and in every replay, whatever the scratch held before."""
+    case = [v.cuda() for v in _moe_case(*shape, dtype, trans_b, seed=sum(shape))]
+    _announce("moe same bits", shape, dtype, trans_b)
+
+    def poisoned():
+        junk = [torch.full((n,), float("nan"), device="cuda") for n in (1 << 12, 1 << 16, 1 << 20, 1 << 21)]
+        del junk
+
+    want = ops.moe_few_tokens(*case, trans_b=trans_b)
+    for _ in range(8):
+        poisoned()
+        assert torch.equal(ops.moe_few_tokens(*case, trans_b=trans_b), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ops.moe_few_tokens(*case, trans_b=trans_b)
+    torch.cuda.synchronize()
+    assert torch.equal(other, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops.moe_few_tokens(*case, trans_b=trans_b)
+    for _ in range(4):
+        captured.zero_()
+        graph.replay()
+        eager = ops.moe_few_tokens(*case, trans_b=trans_b)
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want) and torch.equal(eager, want)
+
+
 def test_moe_few_tokens_refuses(ops):
     x, w13, w2, experts, weights = (v.cuda() for v in _moe_case(2, 4, 2, 32, 48, torch.bfloat16, False, seed=1))
 
