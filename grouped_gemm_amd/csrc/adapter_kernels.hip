@@ -3,9 +3,11 @@
 //   v[t] = a_l x[t]   (a_l: rank x hidden_in)        out[t] = base[t] + scale_l * b_l v[t]   (b_l: hidden_out x rank)
 //
 // Bound by base and out for many rows, by the adapters' weights for rows of many adapters, and by the latencies of two launches for few.
-// 8192 rows of prompts, bf16, 4096 -> 14336: rank 64 41 + 144 us (556 MB in all; the second kernel moves 470 MB of base and out at 3.3 TB/s, and
-// reads as much of b_l again from the L2s, 64 rows at a time: with one adapter 129 us), rank 16, 4096 wide 21 + 34 us (134 MB: 4.0 TB/s, as a
-// copy).  64 rows of 16 adapters, rank 16, 4096 wide 4.7 + 5.2 us, one row 3.8 + 4.6.
+// 8192 rows of prompts, bf16, 4096 -> 14336: rank 64 42 + 143 us (556 MB in all; the second kernel moves 470 MB of base and out at 3.3 TB/s, and
+// reads as much of b_l again from the L2s, 64 rows at a time: with one adapter 127 us; vector instructions are in 16 % of its cycles, and a block's
+// loads stand behind the stores of the one before it), rank 16, 4096 wide 21 + 34 us (134 MB: 4.0 TB/s, as a
+// copy), rank 8 19 + 35.  64 rows of 16 adapters, rank 16, 4096 wide 4.9 + 5.1 us, one row 4.0 + 5.0.  The second kernel spills
+// 4 to 18 words of ranks 17 to 64 (four waves to a SIMD leave 128 registers): none of them is read in the loop over whole blocks.
 // Rows are taken in windows of 64 in their own order, and the rows of a window that share an adapter together: the
 // rows of a prompt are neighbours, and the rows of a decode step are one window, so nothing has to be sorted.  A wave knows
 // its window's rows from one load and a ballot for each adapter.

@@ -19,7 +19,9 @@
 //
 // Measured: 64 tokens, top 8 of 128 experts, 7168 -> 2048, weights contiguous along the depth (11.1 GB) 1184 us of gate and up (6.2 TB/s) and
 // 698 of down (5.3 TB/s); one token, two experts, 4096 -> 14336 (705 MB) 85 + 47 us (5.5, 5.0 TB/s), of which about 10 us each are the
-// start, the first loads and the joins.  12 waves to a compute unit in workgroups of 4; in workgroups of 8, 16 waves, gate and up run at 5.4 TB/s.
+// start, the first loads and the joins.  Where 16 rows are taken at a time, three waves to a SIMD have registers: 12 to a compute unit in workgroups of 4
+// (with 16, in workgroups of 8, gate and up along the depth run at 5.4 TB/s), 8 where gate and up of a contiguous width are one workgroup of 8.
+// Where 32 or 64 are, two have: 8.
 #include "operators.hpp"
 
 #include <math.h>
@@ -428,8 +430,9 @@ FewPlan few_plan(int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
   const int64_t steps = (ffn + (nt ? 63 : 31)) / (nt ? 64 : 32), fit = kFewUnits / (f.named * f.down_tiles), deep = steps / (8 * kFewWaves);
   f.pieces = std::max<int64_t>(1, std::min({fit, deep, int64_t(16)}));
   // Rows taken at a time, by how many an expert has on average (of down two for each slot; those that do not fit read the weights again): more of them
-  // leave fewer waves to a compute unit.  us with 1, 2 and 4 times 16, averages 3, 4, 8, 16: gate | up 77 78 81, 279 281 281,
-  // 340 348 368, 528 361 373; down 48 54 54, 180 153 161, 281 176 178, 469 316 212.
+  // leave fewer waves to a compute unit, and 4 spill registers: inside the loop bf16 with the width contiguous and fp16 on any element (36 and 28 words in
+  // two steps), others around it or none.  us with 1, 2 and 4 times 16, averages 3, 4, 8, 16 (bf16): gate | up 77 78 81, 279 281 281, 340 348 368, 528 361 373;
+  // down 48 54 54, 180 153 161, 281 176 178, 469 316 212.
   f.up_rows = f.slots <= 8 * experts ? 1 : 2;
   f.down_rows = f.slots < 4 * experts ? 1 : (f.slots <= 12 * experts ? 2 : 4);
   // Where the strips leave compute units, an expert's rows are shared among as many workgroups as there are turns on average.  us without and

@@ -9,10 +9,11 @@
 // Sorting is by counting, in a fixed order: a workgroup counts its tokens' experts, the counts are summed over
 // the workgroups before each, and the rows are placed by how many earlier rows of the same expert there are.
 //
-// Choosing and the gradient are bound by the vector units' issue, not by memory: every logit is read once, but takes an exponential (four
-// times the time of an addition), and a subtraction and half a maximum for each of the top_k.  65536 tokens of 256 experts, bf16, sigmoid,
-// top 8: choosing 27 us (33.6 MB: 1.3 TB/s), summing the counts 5, placing 524288 rows 11 (latency of scattered 4-byte stores), the gradient
-// 26 (67 MB and the chosen: 2.7 TB/s).  Few tokens are bound by the launches: one token 3.7 us in one, 8192 of 64 experts 5 + 4 + 4 and 4.
+// Choosing is bound by the vector units' issue: every logit is read once, but takes an exponential (four times the time of an addition), and a
+// subtraction and half a maximum for each of the top_k.  65536 tokens of 256 experts, bf16, sigmoid, top 8: choosing 26 us (33.6 MB: 1.3 TB/s;
+// vector instructions in 81 % of the cycles), summing the counts 5, placing 524288 rows 11 (latency of scattered 4-byte stores), the gradient 26 (67
+// MB and the chosen: 2.7 TB/s; vector instructions in half of the cycles, memory's latency in the others: a token's loads follow one another, see
+// there).  Few tokens are bound by the launches: one token 3.8 us in one, 8192 of 64 experts 5 + 4 + 4 and 4.
 #include "operators.hpp"
 
 #include <math.h>
@@ -463,7 +464,8 @@ __global__ __launch_bounds__(kBackThreads, 4) void route_backward_kernel(RouteBa
   float m[VPL];
 #pragma unroll
   for (int v = 0; v < VPL; ++v) m[v] = a.mass_grad != nullptr && column + v < a.experts ? a.mass_grad[column + v] : 0.0f;
-  // The next token's rows are asked for while one is under way.
+  // The next token's rows are read ahead, but what is made of them here waits for them here: `chosen` is compared, and two-byte rows are taken apart.
+  // With the chosen logits, which are gathered from memory, a token has three waits for memory, one after the other.
   Row<T, VPL> next_raw;
   int next_index[KR];
   float next_grad[KR];
