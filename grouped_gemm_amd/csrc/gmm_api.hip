@@ -15,6 +15,7 @@
 
 #include "gmm_generic.hpp"
 #include "gmm_variants.hpp"
+#include "operators.hpp"
 #include "row_kernels.hpp"
 
 namespace gg {
@@ -783,6 +784,88 @@ int run_pair(const gg_gmm_args* first, const Strides* strides1, const gg_gmm_arg
   return rc == GG_OK ? launch_call(*second, &plan.second) : rc;
 }
 
+// ---- products of 8-bit integers (gg_gmm_int8)
+
+constexpr int64_t kInt8MostDepth = 131071;   // 128 * 128 * depth below 2^31: no sum overflows
+constexpr int64_t kInt8FewRows = 32;         // average rows to a group up to which they go to the kernel for few rows
+
+int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_scales) {
+  if (args == nullptr) return fail(GG_EINVAL, "args is null");
+  if (args->struct_bytes != sizeof(gg_gmm_args))
+    return fail(GG_EINVAL, "gg_gmm_args.struct_bytes is not the %zu this library expects", sizeof(gg_gmm_args));
+  const gg_gmm_args& g = *args;
+  int rc = check_common(g.batch_sizes, g.num_groups, g.tokens, g.hidden_in, g.hidden_out, g.trans_a, g.trans_b);
+  if (rc != GG_OK) return rc;
+  if (g.dtype != GG_DTYPE_BF16 && g.dtype != GG_DTYPE_F16) return fail(GG_EINVAL, "dtype, of c, must be GG_DTYPE_BF16 or GG_DTYPE_F16");
+  if (g.trans_a || !g.trans_b) return fail(GG_EINVAL, "8-bit integers come with b stored transposed (trans_b, not trans_a)");
+  if (g.epilogue != GG_EPILOGUE_NONE || g.accumulate_f32 || g.a_row_index || g.b_row_index || g.c_row_index)
+    return fail(GG_EINVAL, "8-bit integers have neither an epilogue, an fp32 c nor row indices");
+  if (g.hidden_in > kInt8MostDepth) return fail(GG_ELIMIT, "hidden_in of 8-bit integers must be at most %lld", (long long)kInt8MostDepth);
+  if (g.num_groups == 0 || g.tokens == 0 || g.hidden_out == 0) return GG_OK;
+  if (g.c == nullptr || a_scales == nullptr || b_scales == nullptr) return fail(GG_EINVAL, "c, a_scales or b_scales is null");
+  if (g.hidden_in > 0 && (g.a == nullptr || g.b == nullptr)) return fail(GG_EINVAL, "a or b is null");
+  if ((reinterpret_cast<uintptr_t>(g.c) & 1) || ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3))
+    return fail(GG_ELIMIT, "c and the scales must be aligned to their element size");
+  if (!gg::int8_rows_fit(g.tokens, std::min<int64_t>(g.num_groups, GG_MAX_GROUPS_PER_LAUNCH), g.hidden_in, g.hidden_out))
+    return fail(GG_ELIMIT, "tokens times hidden_out are too large for one launch");
+  return GG_OK;
+}
+
+bool int8_streams(const gg_gmm_args& g) {
+  return g.tokens > kInt8FewRows * g.num_groups && g.hidden_in > 0 && g.hidden_in % 16 == 0 && g.hidden_out % 8 == 0 &&
+         ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | reinterpret_cast<uintptr_t>(g.c)) & 15) == 0;
+}
+
+// The same call on fp8 operands, whose tiles, schedule and workspace those of 8-bit integers are.
+gg_gmm_args int8_as_fp8(const gg_gmm_args& g) {
+  gg_gmm_args f = g;
+  f.dtype = GG_DTYPE_F8E4M3;
+  return f;
+}
+
+int int8_by_rows(const gg_gmm_args& g, const float* a_scales, const float* b_scales) {
+  DeviceInfo info;
+  int rc = device_info(&info);
+  if (rc != GG_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(g.workspace) & 255) return fail(GG_ELIMIT, "the workspace must be 256-byte aligned");
+  if (!g.batch_sizes_on_device) {
+    int64_t row = 0;
+    for (int64_t e = 0; e < g.num_groups; ++e) {
+      if (g.batch_sizes[e] < 0) return fail(GG_EINVAL, "batch_sizes[%lld] is negative", (long long)e);
+      if (g.batch_sizes[e] > g.tokens - row)
+        return fail(GG_EINVAL, "batch_sizes sum past the %lld rows of a", (long long)g.tokens);
+      row += g.batch_sizes[e];
+    }
+  }
+  int64_t row = 0;
+  for (int64_t first = 0; first < g.num_groups; first += GG_MAX_GROUPS_PER_LAUNCH) {
+    const int64_t count = std::min<int64_t>(g.num_groups - first, GG_MAX_GROUPS_PER_LAUNCH);
+    gg::HostSizes hs;
+    gg::Int8Args a = {static_cast<const int8_t*>(g.a), a_scales, static_cast<const int8_t*>(g.b), b_scales, g.c, g.dtype == GG_DTYPE_F16,
+                      g.batch_sizes_on_device ? g.batch_sizes : nullptr, g.batch_sizes_on_device ? g.size_status : nullptr, g.tokens, row,
+                      (int32_t)first, (int32_t)count, (int32_t)g.hidden_in, (int32_t)g.hidden_out, nullptr, nullptr};
+    if (!g.batch_sizes_on_device)
+      for (int64_t i = 0; i < count; ++i) {
+        hs.v[i] = (int32_t)g.batch_sizes[first + i];
+        row += g.batch_sizes[first + i];
+      }
+    GG_HIP(gg::int8_rows(a, hs, g.workspace, g.workspace_bytes, static_cast<hipStream_t>(g.stream)));
+  }
+  return GG_OK;
+}
+
+int int8_by_tiles(const gg_gmm_args& g, const float* a_scales, const float* b_scales) {
+  const gg_gmm_args f = int8_as_fp8(g);
+  Plan plan;
+  const int rc = plan_call(f, false, &plan);
+  if (rc != GG_OK || plan.empty) return rc;
+  plan.variant = find_variant(g.dtype == GG_DTYPE_F16 ? gg::kI8ToF16 : gg::kI8, plan.layout, plan.shape.id, gg::kEpiStore, 0);
+  if (plan.variant == nullptr) return fail(GG_EINVAL, "no kernel for this combination of arguments");
+  plan.p.a_scales = a_scales;
+  plan.p.b_scales = b_scales;
+  return launch_call(f, &plan);
+}
+
 }  // namespace
 
 // For the entry points beside the grouped GEMM (operators_api.hip): the calling thread's error message, and the checks and set-up of the
@@ -819,6 +902,25 @@ int gg_tile_shape(int64_t num_groups, int64_t tokens, int trans_a, int trans_b, 
   if (bn) *bn = s ? Short::BN : Wide::BN;
   if (bk) *bk = gg::BK;
   return GG_OK;
+}
+
+uint64_t gg_gmm_int8_workspace_bytes(const gg_gmm_args* args) {
+  if (args == nullptr || args->struct_bytes != sizeof(gg_gmm_args) || args->num_groups <= 0 || args->tokens <= 0 || args->hidden_in <= 0 ||
+      args->hidden_out <= 0)
+    return 0;
+  if (int8_streams(*args)) {
+    const gg_gmm_args f = int8_as_fp8(*args);
+    return gg_workspace_bytes_for(&f);
+  }
+  const int64_t groups = std::min<int64_t>(args->num_groups, GG_MAX_GROUPS_PER_LAUNCH);
+  return gg::int8_rows_in_pieces(args->tokens, groups, args->hidden_in, args->hidden_out) ? GG_WORKSPACE_BYTES : 0;
+}
+
+int gg_gmm_int8(const gg_gmm_args* args, const float* a_scales, const float* b_scales) {
+  const int rc = check_int8(args, a_scales, b_scales);
+  if (rc != GG_OK) return rc;
+  if (args->num_groups == 0 || args->tokens == 0 || args->hidden_out == 0) return GG_OK;
+  return int8_streams(*args) ? int8_by_tiles(*args, a_scales, b_scales) : int8_by_rows(*args, a_scales, b_scales);
 }
 
 int gg_debug_tile(const gg_gmm_args* args, int* bm, int* bn) {

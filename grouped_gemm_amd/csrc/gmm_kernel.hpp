@@ -31,9 +31,11 @@ constexpr int kSchedCols = 14;
 
 enum : int { kNN = 0, kNT = 1, kTN = 2 };
 // Element types of a and b.  Two-byte types give a c of the same type; the one-byte (OCP fp8)
-// types give a bf16 c.
-enum : int { kBF16 = 0, kF16 = 1, kF8E4M3 = 2, kF8E5M2 = 3 };
+// types give a bf16 c.  8-bit integers (NT layout), whose sums are scaled by row and by column, give a bf16 or an f16 c.
+// (4: GG_DTYPE_F32, of no operand here)
+enum : int { kBF16 = 0, kF16 = 1, kF8E4M3 = 2, kF8E5M2 = 3, kI8 = 5, kI8ToF16 = 6 };
 constexpr bool is_f8(int dt) { return dt == kF8E4M3 || dt == kF8E5M2; }
+constexpr bool is_i8(int dt) { return dt == kI8 || dt == kI8ToF16; }
 
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
@@ -45,6 +47,7 @@ using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using i32x4 = __attribute__((ext_vector_type(4))) int;
 using i32x8 = __attribute__((ext_vector_type(8))) int;
+using i32x16 = __attribute__((ext_vector_type(16))) int;
 
 #define GG_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
 
@@ -68,8 +71,14 @@ struct GmmParams {
   int32_t lda, ldb;    // elements from one row of a (of b) in memory to the next: more than a row has in copies
                        // that are padded to whole lines, with zeros where the rows run along the depth
   // the variants with row indices only:
-  const int32_t* a_rows;   // row r of the left operand is row a_rows[r] of a, or nullptr (rows in place)
-  const int32_t* c_rows;   // row r of the output goes to row c_rows[r] of c, or nullptr
+  union {
+    const int32_t* a_rows;   // row r of the left operand is row a_rows[r] of a, or nullptr (rows in place)
+    const float* a_scales;   // 8-bit integers, whose rows are in place: (tokens)
+  };
+  union {
+    const int32_t* c_rows;   // row r of the output goes to row c_rows[r] of c, or nullptr
+    const float* b_scales;   // 8-bit integers: (groups, hidden_out)
+  };
   uint32_t a_bytes;        // bytes of a and of c in memory, below kOutOfRangeIndexed
   uint32_t c_bytes;
   uint32_t a_index_rows;   // rows of a and of c in memory: an index that names no row of them is a
@@ -443,6 +452,12 @@ __device__ __forceinline__ f32x16 mfma_32x32x64_f8(bf16x8 x_lo, bf16x8 x_hi, bf1
                                           3, 4, 5, 6, 7);
   constexpr int FORMAT = DT == kF8E5M2 ? 1 : 0;   // e4m3 : e5m2, for both operands; no block scales
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc, FORMAT, FORMAT, 0, 0, 0, 0);
+}
+
+// The same depth of 8-bit integers, in two instructions: sums are exact, so that it does not matter which depth values meet in which.
+__device__ __forceinline__ i32x16 mfma_32x32x64_i8(bf16x8 x_lo, bf16x8 x_hi, bf16x8 y_lo, bf16x8 y_hi, i32x16 acc) {
+  acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, x_lo), __builtin_bit_cast(i32x4, y_lo), acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, x_hi), __builtin_bit_cast(i32x4, y_hi), acc, 0, 0, 0);
 }
 
 // Four fp32 values rounded (to nearest even) to the element type, as 8 bytes.
@@ -1676,8 +1691,10 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   constexpr bool ACC_F32 = EPI == kEpiAccF32 || EPI == kEpiAccF32Atomic, KEEP = EPI == kEpiSwiGLUKeep, GATE_UP = EPI == kEpiSwiGLU || KEEP;
   // One-byte elements (NT layout only: both operands depth-contiguous).  The tile movers see them
   // as two-byte elements, two to one: same bytes per row and slice, BK_ELEMS depth values a slice.
-  constexpr bool F8 = is_f8(DT);
-  constexpr int ES = F8 ? 1 : 2, BK_ELEMS = BK * 2 / ES, OUT_DT = DT == kF16 ? kF16 : kBF16;
+  // I8: 8-bit integers, which move as fp8 does; only what multiplies and sums them differs.
+  constexpr bool I8 = is_i8(DT), F8 = is_f8(DT) || I8;
+  constexpr int ES = F8 ? 1 : 2, BK_ELEMS = BK * 2 / ES, OUT_DT = DT == kF16 || DT == kI8ToF16 ? kF16 : kBF16;
+  static_assert(!I8 || (LAYOUT == kNT && EPI == kEpiStore && !INDEXED), "8-bit integers: NT layout, plain rows and epilogue");
   static_assert(!F8 || !GATE_UP || LAYOUT == kNT, "fp8 with gate | up rows streams in the NT layout only");
   static_assert(!ACC_F32 || LAYOUT == kTN, "the fp32 accumulator is the weight gradient's");
   static_assert(!(GATE_UP || INDEXED) || LAYOUT != kTN, "row indices and gate | up are for the NN and NT layouts");
@@ -1819,6 +1836,8 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
     {
       int32_t words[kTileInfoDwords];
       pack_tile(fti, words);
+      if constexpr (I8)   // (the group, for its columns' scales)
+        words[23] = p.first_group + (fti.valid ? ((p.flags & kFlagByTileRows) != 0 ? uniform((int)sched->order[fetch_cur.e]) : fetch_cur.e) : 0);
       int32_t* slot = tile_ring + (fetch_n % Cfg::TILE_RING_SLOTS) * kTileInfoDwords;
       if (lane == 0) {
 #pragma unroll
@@ -1996,6 +2015,32 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   auto partial_at = [&](int i, int j, int q) -> uint32_t { return (((i * NB + j) * 4 + q) * NT + threadIdx.x) * 16; };
   bool fix_pending = false;   // this workgroup's depth piece was the last of its tile to arrive
 
+  // 8-bit integers: the scales of a tile's BM rows, then of its BN columns, in LDS behind everything else.
+  float* const tile_scales = reinterpret_cast<float*>(smem + Cfg::LDS_BYTES);
+  // The waves load them in turns, 64 at a time, in the first slice of a tile once all waves have left the tile before; the wait for the next
+  // slice, whose loads come later, is one for them.
+  auto load_scales = [&](const TileInfo& tile) {
+    if constexpr (I8) {
+      const int group = uniform(tile_ring[(tile_n % Cfg::TILE_RING_SLOTS) * kTileInfoDwords + 23]);
+      const rsrc_words of_rows = make_rsrc_words(p.a_scales + tile.g.row0 + tile.m0, (uint32_t)tile.rows_valid * 4u);
+      const rsrc_words of_columns =
+          make_rsrc_words(p.b_scales + (int64_t)group * p.hidden_out + tile.n0, tile.valid ? (uint32_t)min(BN, tile.g.n - tile.n0) * 4u : 0u);
+#pragma unroll
+      for (int first = 0; first < (BM + BN) / 64; first += WAVES_M * WAVES_N) {
+        const int unit = first + wave;
+        if ((BM + BN) / 64 % (WAVES_M * WAVES_N) != 0 && unit >= (BM + BN) / 64) break;
+        const bool rows = unit < BM / 64;
+        rsrc_words rsrc;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) rsrc[w] = uniform(rows ? of_rows[w] : of_columns[w]);
+        settle<5>(rsrc);
+        const uint32_t offset = (uint32_t)(unit - (rows ? 0 : BM / 64)) * 256u + (uint32_t)lane * 4u;
+        const uint32_t to = uniform(lds_address(tile_scales) + (uint32_t)unit * 256u);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(to), "v"(offset), "s"(rsrc) : "memory", "m0");
+      }
+    }
+  };
+
   // Where a tile's rows of c are: a descriptor of them, or of all of c when rows go through an
   // index, the byte offset of row `row` of the tile in it and that of one of its columns (C_OOR: no
   // such row or column, nothing is stored).
@@ -2094,13 +2139,13 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
     constexpr int ML = decltype(ml_tag)::value;
     // MFMAs: blocks of 32 x 32 outputs for fp8, of 16 x 16 for two-byte elements
     constexpr int EDGE = F8 ? 1 : 2, MFMA_M = ML * EDGE, MFMA_N = NB * EDGE;
-    std::conditional_t<F8, f32x16, f32x4> acc[MFMA_M][MFMA_N];
+    std::conditional_t<I8, i32x16, std::conditional_t<F8, f32x16, f32x4>> acc[MFMA_M][MFMA_N];
 #pragma unroll
     for (int i = 0; i < MFMA_M; ++i)
 #pragma unroll
       for (int j = 0; j < MFMA_N; ++j)
 #pragma unroll
-        for (int r = 0; r < (F8 ? 16 : 4); ++r) acc[i][j][r] = 0.0f;
+        for (int r = 0; r < (F8 ? 16 : 4); ++r) acc[i][j][r] = 0;
     // Group q (see group_row) of the 32 x 32 block (i, j), moved out of the accumulation registers here and no earlier:
     // all of them at once would not fit beside the next tile's fragments.  (How that is said decides what the compiler
     // makes of it: read in assembly, the plain epilogues of full tiles get by without moves and spills; tied
@@ -2111,8 +2156,12 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       if constexpr (TIED) asm volatile("" : "+a"(from));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = from[F8 ? 4 * q + r : r];
-        if constexpr (F8 || (MB * NB > 4 && !TIED)) {
+        auto x = from[F8 ? 4 * q + r : r];
+        if constexpr (I8) {
+          int sum;
+          asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(sum) : "a"(x));
+          v[r] = (float)sum * tile_scales[(wm + i * WAVES_M) * 32 + group_row(q)] * tile_scales[BM + wn * Cfg::WTN + j * 32 + group_col(q) + r];
+        } else if constexpr (F8 || (MB * NB > 4 && !TIED)) {
           asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[r]) : "a"(x));
         } else {
           asm volatile("" : "+v"(x));
@@ -2139,7 +2188,9 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
         constexpr int hi = quarter / 2, hj = quarter == 1 || quarter == 2 ? 1 : 0;   // halves of A's and of B's block
         // operands swapped: the result block is held transposed, so a lane owns four
         // consecutive columns of one output row
-        if constexpr (F8) {   // (takes both halves of both fragments)
+        if constexpr (I8) {
+          acc[i][j] = mfma_32x32x64_i8(fb[set][j], fb[set + 1][j], fa[set][i], fa[set + 1][i], acc[i][j]);
+        } else if constexpr (F8) {   // (takes both halves of both fragments)
           acc[i][j] = mfma_32x32x64_f8<DT>(fb[set][j], fb[set + 1][j], fa[set][i], fa[set + 1][i], acc[i][j]);
         } else {
           f32x4& sum = acc[2 * i + hi][2 * j + hj];
@@ -2192,6 +2243,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       // every wave has all fragments of this slice in registers
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       block_barrier();
+      if (I8 && kt == 0) load_scales(ti);
       slots(IRelease{}, IReady{}, y);
       // the next slice has landed for every wave (only the loads just issued may be pending and, in the first
       // slice after a tile that was stored, its stores)
@@ -2201,7 +2253,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       // moves a slice.  Without a copy and without a move, the waits chosen among in assembly and every accumulator's zeros its
       // own, the loop is slower for the branches in each slice: 8 x 4096 rows, 4096 x 14336: 2632 / 2702 us; 256 x 256, 2048 x 7168:
       // 2561 / 2600)
-      if (LATE_LOADS || (LAYOUT == kTN && kt > 0) || __builtin_expect(uniform(stored) == 0, 1)) {
+      if (LATE_LOADS || I8 || (LAYOUT == kTN && kt > 0) || __builtin_expect(uniform(stored) == 0, 1)) {
         wait_vmcnt<PENDING>();
       } else {
         if (uniform(stored) == MB) {
@@ -2231,9 +2283,9 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
         for (int j = 0; j < NB; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            f32x4 v;
+            std::conditional_t<I8, i32x4, f32x4> v;
             if constexpr (F8) {
-              v = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+              v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
             } else {
               v = acc[2 * i + q / 2][2 * j + q % 2];
             }
@@ -2547,20 +2599,21 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
     const __amdgpu_buffer_rsrc_t rc = c_rsrc(ft);
     const int live = LAYOUT == kTN ? MB : (ft.blocks - wm + WAVES_M - 1) / WAVES_M;
     for (int i = 0; i < live; ++i) {
-      f32x4 sum[NB][4];
+      using Sum = std::conditional_t<I8, i32x4, f32x4>;
+      Sum sum[NB][4];
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum[j][q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int q = 0; q < 4; ++q) sum[j][q] = Sum{0, 0, 0, 0};
       for (int piece = 0; piece < ft.pieces; piece += 2) {
         const __amdgpu_buffer_rsrc_t from0 = partial_rsrc(ft, piece), from1 = partial_rsrc(ft, piece + 1);
-        f32x4 v0[NB][4], v1[NB][4];
+        Sum v0[NB][4], v1[NB][4];
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            v0[j][q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from0, partial_at(i, j, q), 0, kDeviceScope));
-            v1[j][q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from1, partial_at(i, j, q), 0, kDeviceScope));
+            v0[j][q] = __builtin_bit_cast(Sum, __builtin_amdgcn_raw_buffer_load_b128(from0, partial_at(i, j, q), 0, kDeviceScope));
+            v1[j][q] = __builtin_bit_cast(Sum, __builtin_amdgcn_raw_buffer_load_b128(from1, partial_at(i, j, q), 0, kDeviceScope));
           }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -2596,7 +2649,16 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
             const uint32_t row_off = rows_off[q / 2];
             const int col = ft.n0 + wn * Cfg::WTN + j * 32 + group_col(q);
             const uint32_t off = c_at(ft, row_off, col);
-            if (FIX_ANY_ROWS && ((p.flags & kFlagAnyRows) != 0 || uniform(ft.g.n & 3) != 0)) {
+            if constexpr (I8) {
+              // (a row or column that is not there has no scale to read, and is not stored)
+              const int row = (wm + i * WAVES_M) * 32 + group_row(q);
+              const float of_row = row < ft.rows_valid ? p.a_scales[ft.g.row0 + ft.m0 + row] : 0.0f;
+              const float* of_columns = p.b_scales + (int64_t)uniform(words[23]) * p.hidden_out + col;
+              float v[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) v[r] = (float)sum[j][q][r] * of_row * (col < ft.g.n ? of_columns[r] : 0.0f);
+              __builtin_amdgcn_raw_buffer_store_b64(round4<OUT_DT>(v[0], v[1], v[2], v[3]), rc, off, 0, kStoreMerging);
+            } else if (FIX_ANY_ROWS && ((p.flags & kFlagAnyRows) != 0 || uniform(ft.g.n & 3) != 0)) {
               const u32x2 v = round4<OUT_DT>(sum[j][q][0], sum[j][q][1], sum[j][q][2], sum[j][q][3]);
               store_any(ft, row_off, col, 4, u32x4{v[0], v[1], 0u, 0u});
             } else if constexpr (ACC_F32) {

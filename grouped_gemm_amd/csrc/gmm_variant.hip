@@ -26,6 +26,10 @@ using V = VariantDef<GG_VARIANT_INDEX>;
 using S = V::Shape;
 using Cfg = GmmConfig<V::LAYOUT, S::BM, S::BN, BK, STAGES, S::WAVES_M, S::WAVES_N>;
 
+// (8-bit integers: the scales of a tile's rows and columns behind the rest)
+constexpr int LDS_BYTES = Cfg::LDS_BYTES + (is_i8(V::DT) ? (S::BM + S::BN) * 4 : 0);
+static_assert(LDS_BYTES * Cfg::WORKGROUPS_PER_CU <= 160 * 1024, "");
+
 const void* kernel_address() {
   return reinterpret_cast<const void*>(
       &gmm_kernel<V::DT, V::LAYOUT, S::BM, S::BN, BK, STAGES, S::WAVES_M, S::WAVES_N, V::EPI, V::INDEXED,
@@ -33,7 +37,7 @@ const void* kernel_address() {
 }
 
 hipError_t prepare() {
-  return hipFuncSetAttribute(kernel_address(), hipFuncAttributeMaxDynamicSharedMemorySize, Cfg::LDS_BYTES);
+  return hipFuncSetAttribute(kernel_address(), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
 }
 
 hipError_t launch(const GmmParams& p, const HostSizes& hs, int grid, hipStream_t stream) {
@@ -41,10 +45,10 @@ hipError_t launch(const GmmParams& p, const HostSizes& hs, int grid, hipStream_t
   HostSizes sizes = hs;
   void* args[2] = {&params, &sizes};
   return hipLaunchKernel(kernel_address(), dim3(grid), dim3(S::WAVES_M * S::WAVES_N * 64), args,
-                         Cfg::LDS_BYTES, stream);
+                         LDS_BYTES, stream);
 }
 
-const VariantOps kOps = {V::DT, V::LAYOUT, S::kId, V::EPI, V::INDEXED ? 1 : 0, Cfg::LDS_BYTES, Cfg::WORKGROUPS_PER_CU, &prepare, &launch};
+const VariantOps kOps = {V::DT, V::LAYOUT, S::kId, V::EPI, V::INDEXED ? 1 : 0, LDS_BYTES, Cfg::WORKGROUPS_PER_CU, &prepare, &launch};
 
 }  // namespace
 

@@ -86,6 +86,53 @@ int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t exp
   return GG_OK;
 }
 
+static int check_balance(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, const int32_t* offsets,
+                         int64_t sequences) {
+  const int rc = check_route(logits, dtype, tokens, experts, top_k, score);
+  if (rc != GG_OK) return rc;
+  if (sequences < 0 || (offsets == nullptr && sequences != 1)) return fail(GG_EINVAL, "sequences must not be negative, and 1 without offsets");
+  if (sequences >= (int64_t(1) << 31) - 1) return fail(GG_ELIMIT, "sequences must be below 2^31 - 1");
+  return GG_OK;
+}
+
+uint64_t gg_balance_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t sequences) {
+  if (tokens < 0 || experts < 1 || top_k < 1 || experts > GG_ROUTE_MAX_EXPERTS || top_k > GG_ROUTE_MAX_TOP_K || sequences < 0 ||
+      tokens >= (int64_t(1) << 31) / top_k || sequences >= (int64_t(1) << 31) - 1)
+    return 0;
+  return gg::balance_scratch_bytes(tokens, experts, sequences);
+}
+
+int gg_balance(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, const int32_t* chosen,
+               const int32_t* offsets, int64_t sequences, const uint8_t* mask, float* balance, float* z, int32_t* counts, float* share,
+               float* inverse, void* scratch, void* stream) {
+  const int rc = check_balance(logits, dtype, tokens, experts, top_k, score, offsets, sequences);
+  if (rc != GG_OK) return rc;
+  if (tokens > 0 && chosen == nullptr) return fail(GG_EINVAL, "chosen is null");
+  if (balance == nullptr || z == nullptr || inverse == nullptr || scratch == nullptr || (sequences > 0 && (counts == nullptr || share == nullptr)))
+    return fail(GG_EINVAL, "balance, z, counts, share, inverse or scratch is null");
+  const int init = gg::prepare_device();
+  if (init != GG_OK) return init;
+  const gg::BalanceArgs a = {logits, dtype, score == GG_SCORE_SIGMOID, tokens, (int32_t)experts, (int32_t)top_k, (int32_t)sequences, chosen,
+                             offsets, mask, balance, z, counts, share, inverse, scratch};
+  GG_HIP(gg::balance(a, static_cast<hipStream_t>(stream)));
+  return GG_OK;
+}
+
+int gg_balance_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int score, const int32_t* offsets,
+                        int64_t sequences, const uint8_t* mask, const float* share, const float* inverse, const float* balance_grad,
+                        const float* z_grad, void* logits_grad, void* stream) {
+  const int rc = check_balance(logits, dtype, tokens, experts, 1, score, offsets, sequences);
+  if (rc != GG_OK) return rc;
+  if (tokens == 0) return GG_OK;
+  if (logits_grad == nullptr || inverse == nullptr || (sequences > 0 && share == nullptr)) return fail(GG_EINVAL, "logits_grad, share or inverse is null");
+  const int init = gg::prepare_device();
+  if (init != GG_OK) return init;
+  const gg::BalanceBackwardArgs a = {logits, dtype, score == GG_SCORE_SIGMOID, tokens, (int32_t)experts, (int32_t)sequences, offsets, mask,
+                                     share, inverse, balance_grad, z_grad, logits_grad};
+  GG_HIP(gg::balance_backward(a, static_cast<hipStream_t>(stream)));
+  return GG_OK;
+}
+
 static int check_few_tokens(int dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, int trans_b) {
   if (dtype != GG_DTYPE_BF16 && dtype != GG_DTYPE_F16) return fail(GG_EINVAL, "dtype must be GG_DTYPE_BF16 or GG_DTYPE_F16");
   if (tokens < 0 || experts < 1 || top_k < 1 || hidden < 1 || ffn < 1)
@@ -150,6 +197,43 @@ int gg_lora(const void* x, const void* a, const void* b, const int32_t* adapters
                                 (int32_t)hidden_in, (int32_t)hidden_out};
   GG_HIP(gg::adapters(args, static_cast<hipStream_t>(stream)));
   return GG_OK;
+}
+
+static int check_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, int64_t least, int8_t* q, float* scales) {
+  if (dtype != GG_DTYPE_BF16 && dtype != GG_DTYPE_F16 && dtype != GG_DTYPE_F32)
+    return fail(GG_EINVAL, "dtype must be GG_DTYPE_BF16, GG_DTYPE_F16 or GG_DTYPE_F32");
+  if (rows < 0 || cols < 1) return fail(GG_EINVAL, "rows must not be negative, cols at least 1");
+  if (cols >= (1 << 22)) return fail(GG_ELIMIT, "cols must be below 2^22");
+  if (rows >= (int64_t(1) << 40)) return fail(GG_ELIMIT, "rows must be below 2^40");
+  if (rows > 1 && stride < least) return fail(GG_EINVAL, "rows overlap: they are closer together than they are long");
+  if (stride >= (int64_t(1) << 40)) return fail(GG_ELIMIT, "rows are too far apart");
+  if (rows > 0 && (q == nullptr || scales == nullptr)) return fail(GG_EINVAL, "q or scales is null");
+  return GG_OK;
+}
+
+static int run_quantize(const gg::QuantizeArgs& a, void* stream) {
+  const int init = gg::prepare_device();
+  if (init != GG_OK) return init;
+  GG_HIP(gg::quantize(a, static_cast<hipStream_t>(stream)));
+  return GG_OK;
+}
+
+int gg_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, const int32_t* row_index, int64_t x_rows,
+                     int8_t* q, float* scales, void* stream) {
+  const int rc = check_quantize(x, dtype, rows, cols, x_stride, cols, q, scales);
+  if (rc != GG_OK) return rc;
+  if (x_rows < 0 || (row_index == nullptr && x_rows < rows)) return fail(GG_EINVAL, "x_rows must not be negative, nor without a row index below rows");
+  if (rows == 0) return GG_OK;
+  if (x == nullptr && x_rows > 0) return fail(GG_EINVAL, "x is null");
+  return run_quantize({x, dtype, false, rows, cols, x_stride, row_index, x_rows, q, scales}, stream);
+}
+
+int gg_swiglu_quantize(const void* gate_up, int dtype, int64_t rows, int64_t cols, int64_t stride, int8_t* q, float* scales, void* stream) {
+  const int rc = check_quantize(gate_up, dtype, rows, cols, stride, 2 * cols, q, scales);
+  if (rc != GG_OK) return rc;
+  if (rows == 0) return GG_OK;
+  if (gate_up == nullptr) return fail(GG_EINVAL, "gate_up is null");
+  return run_quantize({gate_up, dtype, true, rows, cols, stride, nullptr, rows, q, scales}, stream);
 }
 
 }  // extern "C"

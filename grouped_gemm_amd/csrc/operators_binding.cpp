@@ -10,6 +10,10 @@
 
 namespace grouped_gemm {
 
+// torch_binding.cpp
+torch::Tensor AttachCallWorkspace(gg_gmm_args* g, uint64_t bytes, const torch::Device& device, void* stream);
+int32_t* CallSizeStatusWord();
+
 namespace {
 
 void* CurrentStream(const torch::Device& device) {
@@ -147,6 +151,121 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
   return {out[0], out[1], out[2], out[3], out[4], mass};
 }
 
+// ------------------------------------------------------------------ balance loss
+
+struct BalanceInputs {
+  torch::Tensor logits, offsets, mask;   // the last two undefined: one sequence, every token counts
+  int score;
+  int64_t sequences() const { return offsets.defined() ? offsets.size(0) - 1 : 1; }
+  const int32_t* offsets_data() const { return static_cast<const int32_t*>(Pointer(offsets)); }
+  const uint8_t* mask_data() const { return static_cast<const uint8_t*>(Pointer(mask)); }
+};
+
+// balance, z, counts, and for the gradient share and inverse
+torch::autograd::variable_list RunBalance(const BalanceInputs& in, const torch::Tensor& chosen) {
+  const torch::Tensor& logits = in.logits;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  const auto f32 = logits.options().dtype(torch::kFloat32).requires_grad(false);
+  torch::Tensor balance = torch::empty({}, f32), z = torch::empty({}, f32), inverse = torch::empty({}, f32);
+  torch::Tensor counts = torch::empty({in.sequences(), experts}, f32.dtype(torch::kInt32)), share = torch::empty({in.sequences(), experts}, f32);
+  const torch::Tensor scratch = Scratch(gg_balance_scratch_bytes(tokens, experts, chosen.size(1), in.sequences()), balance);
+  const int rc = gg_balance(logits.data_ptr(), LogitsType(logits.scalar_type()), tokens, experts, chosen.size(1), in.score,
+                            chosen.data_ptr<int32_t>(), in.offsets_data(), in.sequences(), in.mask_data(), balance.data_ptr<float>(),
+                            z.data_ptr<float>(), counts.data_ptr<int32_t>(), share.data_ptr<float>(), inverse.data_ptr<float>(), Pointer(scratch),
+                            CurrentStream(logits.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return {balance, z, counts, share, inverse};
+}
+
+torch::Tensor RunBalanceBackward(const BalanceInputs& in, const torch::Tensor& share, const torch::Tensor& inverse, torch::Tensor balance_grad,
+                                 torch::Tensor z_grad) {
+  const torch::Tensor& logits = in.logits;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  torch::Tensor out = torch::empty(logits.sizes(), logits.options().requires_grad(false));
+  const int rc = gg_balance_backward(logits.data_ptr(), LogitsType(logits.scalar_type()), logits.size(0), logits.size(1), in.score, in.offsets_data(),
+                                     in.sequences(), in.mask_data(), share.data_ptr<float>(), inverse.data_ptr<float>(),
+                                     static_cast<const float*>(Pointer(balance_grad)), static_cast<const float*>(Pointer(z_grad)), out.data_ptr(),
+                                     CurrentStream(logits.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return out;
+}
+
+c10::optional<torch::Tensor> Given(const torch::Tensor& t) { return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt; }
+
+// (as RouteGradientNode)
+class BalanceGradientNode : public torch::autograd::Function<BalanceGradientNode> {
+ public:
+  static torch::Tensor forward(torch::autograd::AutogradContext*, const torch::Tensor& logits, const torch::Tensor& share, const torch::Tensor& inverse,
+                               const c10::optional<torch::Tensor>& offsets, const c10::optional<torch::Tensor>& mask,
+                               const c10::optional<torch::Tensor>& balance_grad, const c10::optional<torch::Tensor>& z_grad, int64_t score) {
+    const torch::Tensor none;
+    return RunBalanceBackward({logits, offsets.value_or(none), mask.value_or(none), (int)score}, share, inverse, balance_grad.value_or(none),
+                              z_grad.value_or(none));
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "grouped_gemm: balance_loss has no second derivative");
+  }
+};
+
+class BalanceNode : public torch::autograd::Function<BalanceNode> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& chosen,
+                                                const c10::optional<torch::Tensor>& offsets, const c10::optional<torch::Tensor>& mask, int64_t score) {
+    const BalanceInputs in = {logits, offsets.value_or(torch::Tensor()), mask.value_or(torch::Tensor()), (int)score};
+    auto out = RunBalance(in, chosen);
+    ctx->save_for_backward({logits, in.offsets, in.mask, out[3], out[4]});
+    ctx->saved_data["score"] = score;
+    ctx->mark_non_differentiable({out[2]});
+    ctx->set_materialize_grads(false);
+    out.resize(3);
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const torch::Tensor &balance_grad = grads[0], &z_grad = grads[1], none;
+    if (!balance_grad.defined() && !z_grad.defined()) return {none, none, none, none, none};
+    RefuseTangents({&balance_grad, &z_grad}, "the gradient of balance_loss");
+    const BalanceInputs in = {saved[0], saved[1], saved[2], (int)ctx->saved_data["score"].toInt()};
+    torch::Tensor out;
+    if (torch::GradMode::is_enabled()) {
+      out = BalanceGradientNode::apply(in.logits, saved[3], saved[4], Given(in.offsets), Given(in.mask), Given(balance_grad), Given(z_grad), (int64_t)in.score);
+    } else {
+      out = RunBalanceBackward(in, saved[3], saved[4], balance_grad, z_grad);
+    }
+    return {out, none, none, none, none};
+  }
+};
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> BalanceLoss(const torch::Tensor& logits, const torch::Tensor& experts,
+                                                                    const c10::optional<torch::Tensor>& offsets,
+                                                                    const c10::optional<torch::Tensor>& mask, const std::string& score) {
+  const int which = Score(score);
+  TORCH_CHECK(experts.dim() == 2 && experts.scalar_type() == torch::kInt32, "grouped_gemm: experts must be int32 (tokens, top_k)");
+  CheckLogits(logits, experts.size(1));
+  TORCH_CHECK(experts.size(0) == logits.size(0), "grouped_gemm: experts must be int32 (tokens, top_k)");
+  TORCH_CHECK(experts.is_contiguous(), "grouped_gemm: experts must be contiguous");
+  TORCH_CHECK(experts.device() == logits.device(), "grouped_gemm: logits and experts must be on the same GPU");
+  if (offsets.has_value())
+    TORCH_CHECK(offsets->dim() == 1 && offsets->size(0) >= 1 && offsets->scalar_type() == torch::kInt32 && offsets->is_contiguous() &&
+                    offsets->device() == logits.device(),
+                "grouped_gemm: offsets must be int32 (sequences + 1), contiguous and on the logits' GPU");
+  if (mask.has_value())
+    TORCH_CHECK(mask->dim() == 1 && mask->size(0) == logits.size(0) && mask->scalar_type() == torch::kBool && mask->is_contiguous() &&
+                    mask->device() == logits.device(),
+                "grouped_gemm: mask must be bool (tokens), contiguous and on the logits' GPU");
+  RefuseTangents({&logits}, "balance_loss");
+  torch::autograd::variable_list out;
+  if (torch::GradMode::is_enabled() && logits.requires_grad()) {
+    out = BalanceNode::apply(logits, experts, offsets, mask, (int64_t)which);
+  } else {
+    out = RunBalance({logits, offsets.value_or(torch::Tensor()), mask.value_or(torch::Tensor()), which}, experts);
+  }
+  return {out[0], out[1], out[2]};
+}
+
 // ------------------------------------------------------------------ gated expert layer for a few tokens
 
 bool IsTwoByte(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16; }
@@ -246,10 +365,118 @@ torch::Tensor Lora(const torch::Tensor& x, const torch::Tensor& a, const torch::
   return out;
 }
 
+// ------------------------------------------------------------------ 8-bit integers
+
+void CheckQuantized(const torch::Tensor& x, const char* what) {
+  TORCH_CHECK(x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kFloat16, "grouped_gemm: ", what,
+              " must be float32, bfloat16 or float16");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "grouped_gemm: ", what, " must have rows of at least one element");
+  // (rows may lie further apart than they are long)
+  TORCH_CHECK(x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) >= x.size(1))), "grouped_gemm: ", what,
+              " must be contiguous, or 2-d with contiguous rows that do not overlap");
+  TORCH_CHECK(x.is_cuda(), "grouped_gemm: ", what, " must be a GPU tensor");
+}
+
+int64_t RowStride(const torch::Tensor& x) { return !x.is_contiguous() ? x.stride(0) : x.size(-1); }
+
+std::tuple<torch::Tensor, torch::Tensor> QuantizeRows(const torch::Tensor& x, const c10::optional<torch::Tensor>& row_index) {
+  CheckQuantized(x, "x");
+  if (row_index.has_value()) {
+    TORCH_CHECK(x.dim() == 2, "grouped_gemm: with row_index, x must be 2-d");
+    TORCH_CHECK(row_index->dim() == 1 && row_index->scalar_type() == torch::kInt32 && row_index->is_contiguous() && row_index->device() == x.device(),
+                "grouped_gemm: row_index must be a contiguous 1-d int32 tensor on x's GPU");
+  }
+  RefuseGradients({&x}, "quantize_rows", "round to 8 bits what is served, not what is trained");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  const int64_t cols = x.size(-1), x_rows = x.numel() / cols, rows = row_index.has_value() ? row_index->size(0) : x_rows;
+  std::vector<int64_t> shape = x.sizes().vec(), of_scales(shape.begin(), shape.end() - 1);
+  if (row_index.has_value()) shape = {rows, cols}, of_scales = {rows};
+  const auto options = x.options().requires_grad(false);
+  torch::Tensor q = torch::empty(shape, options.dtype(torch::kInt8)), scales = torch::empty(of_scales, options.dtype(torch::kFloat32));
+  const int rc = gg_quantize_rows(x.data_ptr(), LogitsType(x.scalar_type()), rows, cols, RowStride(x),
+                                  row_index.has_value() ? row_index->data_ptr<int32_t>() : nullptr, x_rows, q.data_ptr<int8_t>(),
+                                  scales.data_ptr<float>(), CurrentStream(x.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return {q, scales};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> SwigluQuantize(const torch::Tensor& gate_up) {
+  CheckQuantized(gate_up, "gate_up");
+  TORCH_CHECK(gate_up.size(-1) % 2 == 0, "grouped_gemm: gate_up must hold gate | up, an even number of columns");
+  RefuseGradients({&gate_up}, "swiglu_quantize", "round to 8 bits what is served, not what is trained");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(gate_up.device());
+  const int64_t cols = gate_up.size(-1) / 2, rows = gate_up.numel() / (2 * cols);
+  std::vector<int64_t> shape = gate_up.sizes().vec(), of_scales(shape.begin(), shape.end() - 1);
+  shape.back() = cols;
+  const auto options = gate_up.options().requires_grad(false);
+  torch::Tensor q = torch::empty(shape, options.dtype(torch::kInt8)), scales = torch::empty(of_scales, options.dtype(torch::kFloat32));
+  const int rc = gg_swiglu_quantize(gate_up.data_ptr(), LogitsType(gate_up.scalar_type()), rows, cols, RowStride(gate_up), q.data_ptr<int8_t>(),
+                                    scales.data_ptr<float>(), CurrentStream(gate_up.device()));
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  return {q, scales};
+}
+
+torch::Tensor GmmInt8(const torch::Tensor& a, const torch::Tensor& a_scales, const torch::Tensor& b, const torch::Tensor& b_scales,
+                      const torch::Tensor& batch_sizes, bool to_f16, const c10::optional<torch::Tensor>& c) {
+  TORCH_CHECK(a.dim() == 2 && a.scalar_type() == torch::kInt8, "grouped_gemm: a must be int8 (tokens, hidden_in)");
+  TORCH_CHECK(b.dim() == 3 && b.scalar_type() == torch::kInt8, "grouped_gemm: b must be int8 (experts, hidden_out, hidden_in)");
+  const int64_t tokens = a.size(0), hidden_in = a.size(1), experts = b.size(0), hidden_out = b.size(1);
+  TORCH_CHECK(b.size(2) == hidden_in, "grouped_gemm: contraction dimensions of a and b differ");
+  TORCH_CHECK(a_scales.dim() == 1 && a_scales.size(0) == tokens && a_scales.scalar_type() == torch::kFloat32,
+              "grouped_gemm: a_scales must be float32, one per row of a");
+  TORCH_CHECK(b_scales.dim() == 2 && b_scales.size(0) == experts && b_scales.size(1) == hidden_out && b_scales.scalar_type() == torch::kFloat32,
+              "grouped_gemm: b_scales must be float32 (experts, hidden_out)");
+  TORCH_CHECK(batch_sizes.dim() == 1 && batch_sizes.size(0) == experts && batch_sizes.scalar_type() == torch::kInt64,
+              "grouped_gemm: batch_sizes must be int64, one per expert");
+  TORCH_CHECK(batch_sizes.is_cpu() || batch_sizes.is_contiguous(), "grouped_gemm: batch_sizes must be contiguous");
+  const torch::Tensor none, &to = c.has_value() ? *c : none;
+  const auto type = to_f16 ? torch::kFloat16 : torch::kBFloat16;
+  if (to.defined())
+    TORCH_CHECK(to.dim() == 2 && to.size(0) == tokens && to.size(1) == hidden_out && to.scalar_type() == type,
+                "grouped_gemm: c must be (tokens, hidden_out), of the type asked for");
+  for (const torch::Tensor* t : {&a, &a_scales, &b, &b_scales, &to})
+    TORCH_CHECK(!t->defined() || t->is_contiguous(), "grouped_gemm: a, a_scales, b, b_scales and c must be contiguous");
+  for (const torch::Tensor* t : {&a, &a_scales, &b, &b_scales, &to})
+    TORCH_CHECK(!t->defined() || (t->is_cuda() && t->device() == a.device()), "grouped_gemm: a, a_scales, b, b_scales and c must be on the same GPU");
+  TORCH_CHECK(batch_sizes.is_cpu() || batch_sizes.device() == a.device(), "grouped_gemm: batch_sizes must be on the host or on a's GPU");
+  RefuseGradients({&a_scales, &b_scales, &to}, "gmm_int8", "train through gmm");
+  if (to.defined())
+    for (const torch::Tensor* t : {&a, &a_scales, &b, &b_scales, &batch_sizes})
+      TORCH_CHECK(!Overlap(*t, to), "grouped_gemm: c must not overlap a, b, their scales or batch_sizes");
+  const torch::Tensor sizes = batch_sizes.is_cpu() ? batch_sizes.contiguous() : batch_sizes;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
+  torch::Tensor out = to.defined() ? to : torch::empty({tokens, hidden_out}, a.options().dtype(type));
+  TORCH_CHECK(gg_init() == GG_OK, "grouped_gemm: ", gg_last_error());
+  gg_gmm_args g = {};
+  g.struct_bytes = sizeof(g);
+  g.dtype = to_f16 ? GG_DTYPE_F16 : GG_DTYPE_BF16;
+  g.a = a.data_ptr();
+  g.b = b.data_ptr();
+  g.c = out.data_ptr();
+  g.batch_sizes = sizes.data_ptr<int64_t>();
+  g.batch_sizes_on_device = sizes.is_cuda() ? 1 : 0;
+  g.trans_b = 1;
+  g.num_groups = experts;
+  g.tokens = tokens;
+  g.hidden_in = hidden_in;
+  g.hidden_out = hidden_out;
+  g.stream = CurrentStream(a.device());
+  if (sizes.is_cuda()) g.size_status = CallSizeStatusWord();
+  const torch::Tensor workspace = AttachCallWorkspace(&g, gg_gmm_int8_workspace_bytes(&g), a.device(), g.stream);
+  const int rc = gg_gmm_int8(&g, a_scales.data_ptr<float>(), b_scales.data_ptr<float>());
+  TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  if (to.defined() && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();   // (as in Lora)
+  return out;
+}
+
 }  // namespace
 
 void RegisterOperators(pybind11::module_& m) {
   m.def("route", &Route, "weights, chosen experts, batch_sizes, row_index, order and mass of router logits.");
+  m.def("balance_loss", &BalanceLoss, "Balance loss and z-loss of router logits, and the experts' counts.");
+  m.def("quantize_rows", &QuantizeRows, "Rows as 8-bit integers, and their scales.");
+  m.def("swiglu_quantize", &SwigluQuantize, "silu(gate) * up as 8-bit integers, and their scales.");
+  m.def("gmm_int8", &GmmInt8, "Grouped GEMM of 8-bit integers with scales per row and column.");
   m.def("moe_few_tokens", &MoeFewTokens, "A gated expert layer for a few tokens.");
   m.attr("moe_few_tokens_max") = GG_FEW_TOKENS_MAX;
   m.def("lora", &Lora, "base + scale * (x @ a^T) @ b^T, with the adapter of each row.");

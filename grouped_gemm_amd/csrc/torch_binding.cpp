@@ -22,6 +22,10 @@ namespace grouped_gemm {
 
 void RegisterOperators(pybind11::module_& m);   // operators_binding.cpp
 
+// ... and what it takes from here: AttachWorkspace and SizeStatusWord below
+torch::Tensor AttachCallWorkspace(gg_gmm_args* g, uint64_t bytes, const torch::Device& device, void* stream);
+int32_t* CallSizeStatusWord();
+
 namespace {
 
 bool IsFloat8(torch::ScalarType t) { return t == torch::kFloat8_e4m3fn || t == torch::kFloat8_e5m2; }
@@ -637,6 +641,11 @@ torch::Tensor DebugSchedule(torch::Tensor batch_sizes, int64_t tokens, int64_t h
   TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
   return out;
 }
+
+torch::Tensor AttachCallWorkspace(gg_gmm_args* g, uint64_t bytes, const torch::Device& device, void* stream) {
+  return AttachWorkspace(g, bytes, device, static_cast<hipStream_t>(stream));
+}
+int32_t* CallSizeStatusWord() { return SizeStatusWord(); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gmm", &GroupedGemm, "Grouped GEMM.");

@@ -191,6 +191,75 @@ def route(logits, top_k, score="softmax", normalize=True, with_mass=False):
     return Routing(*backend.backend.route(logits, top_k, score, normalize, with_mass))
 
 
+class BalanceLoss(NamedTuple):
+    """What balance_loss returns."""
+    balance: torch.Tensor   # float32 (), differentiable
+    z: torch.Tensor         # float32 (), differentiable
+    counts: torch.Tensor    # int32 (sequences, experts): how often each sequence's tokens chose each expert
+
+
+def balance_loss(logits, experts, offsets=None, mask=None, score="softmax"):
+    """The losses that keep a router's experts evenly used and its logits small, over packed sequences:
+
+        balance = 1/T * sum over sequences s of T_s * sum over e of f[s, e] * P[s, e]
+        f[s, e] = num_experts / (top_k * T_s) * counts[s, e],  P[s, e] = mean over the tokens of s of p[t, e]
+        z       = mean over the tokens of log(sum over e of exp(logits[t, e])) ** 2
+
+    with p = softmax(logits), or with score="sigmoid" sigmoid(logits) divided by its sum over the experts; T_s tokens in
+    sequence s, T in all.  Evenly used experts give a balance of 1.  logits (tokens, experts) and experts int32 (tokens, top_k) as
+    route takes and returns them.  offsets int32 (sequences + 1): sequence s is the tokens offsets[s] .. offsets[s + 1] - 1,
+    ascending; tokens before the first and behind the last count nowhere.  None: all tokens are one sequence.  mask bool
+    (tokens): tokens that count, None: all.  Without tokens that count both losses are 0.
+
+    Everything is computed in float32.  Gradients flow from balance and z to the logits, those of tokens that do not count are 0; counts are
+    constants.  Second derivatives and forward mode are refused.  Nothing waits for the device.  Not part of the
+    reference's surface, which has no router."""
+    return BalanceLoss(*backend.backend.balance_loss(logits, experts, offsets, mask, score))
+
+
+# ------------------------------------------------------------------ 8-bit integers
+
+class Quantized(NamedTuple):
+    """Rows as 8-bit integers: row r stands for values[r] * scales[r]."""
+    values: torch.Tensor   # int8
+    scales: torch.Tensor   # float32, one per row
+
+
+def quantize_rows(x, row_index=None):
+    """Each row of x (its last dimension) as 8-bit integers and a scale, as gmm_int8 takes them:
+
+        scales[r] = max|x[r]| / 127,  values[r] = the integers nearest to 127 * x[r] / max|x[r]|, ties to even
+
+    exactly as that is defined.  x: float32, bfloat16 or float16, of any number of dimensions; weights (experts, hidden_out,
+    hidden_in) become b and b_scales of gmm_int8.  2-d rows may lie further apart than they are long.  With row_index int32
+    (rows), row r is x[row_index[r]] (as route returns it: tokens in the order of their experts); a number that names no row
+    gives zeros.  A row of zeros has a scale of 0; one with an infinity a scale of infinity, one with a NaN of NaN.  No gradient.
+    Not part of the reference's surface (csrc/grouped_gemm.h:5-9)."""
+    return Quantized(*backend.backend.quantize_rows(x, row_index))
+
+
+def swiglu_quantize(gate_up):
+    """quantize_rows(silu(gate) * up) for rows gate | up, as the first product of a gated layer gives them: computed in float32
+    and not rounded in between.  gate_up: float32, bfloat16 or float16 (..., 2 * ffn).  No gradient."""
+    return Quantized(*backend.backend.swiglu_quantize(gate_up))
+
+
+def gmm_int8(a, a_scales, b, b_scales, batch_sizes, dtype=torch.bfloat16, c=None):
+    """gmm of 8-bit integers with a scale for each row of a and each column of each expert's b:
+
+        out[r, n] = a_scales[r] * b_scales[e, n] * sum over k of a[r, k] * b[e, n, k],   e the expert of row r
+
+    a int8 (tokens, hidden_in), b int8 (experts, hidden_out, hidden_in), along the depth as quantize_rows leaves weights stored
+    (out, in), hidden_in at most 131071, a_scales float32 (tokens), b_scales float32 (experts, hidden_out); batch_sizes int64
+    (experts) on the host or on the device, as for gmm.  The sums are exact, scaled in float32 and rounded once, to dtype
+    (bfloat16 or float16).  c receives the result, and keeps its rows behind the last expert's.
+
+    No gradient.  Not part of the reference's surface, whose operands are bfloat16 (csrc/grouped_gemm.cu:490-506)."""
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("grouped_gemm: dtype must be torch.bfloat16 or torch.float16")
+    return backend.backend.gmm_int8(a, a_scales, b, b_scales, batch_sizes, dtype == torch.float16, c)
+
+
 # ------------------------------------------------------------------ expert layer of a decode step
 
 def moe_few_tokens(x, w13, w2, experts, weights, trans_b=False):

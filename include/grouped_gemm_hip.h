@@ -379,6 +379,32 @@ int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t exp
                       const int32_t* chosen, const float* weights_grad, const float* mass_grad, void* logits_grad, void* stream);
 
 /*
+ * The balance loss of a router, its z-loss, and their gradient, over packed sequences: sequence s is the tokens offsets[s] .. offsets[s + 1] - 1
+ * (ascending; tokens before the first and behind the last are not counted), with offsets NULL all tokens are one.  Of logits (tokens,
+ * experts) as for gg_route and chosen int32 (tokens, top_k) as gg_route writes it, with p = softmax(logits) (GG_SCORE_SOFTMAX) or sigmoid(logits)
+ * divided by its sum over the experts (GG_SCORE_SIGMOID), T_s and T the counted tokens of a sequence and of all:
+ *   counts   int32 (sequences, experts): how often the sequence's tokens chose the expert
+ *   balance  1 / T * sum over s, t in s, e of share[s, e] * p[t, e]
+ *   z        1 / T * sum over t of the square of log(sum over e of exp(logits[t, e]))
+ *   share    (sequences, experts): counts * experts / (top_k * T_s), and inverse: 1 / T, for the gradient
+ * A token whose mask is 0 (uint8 (tokens), NULL: all count) is not counted at all.  A number in chosen that names no expert is no choice.  A token
+ * all of whose logits are -inf has p and z of 0; NaN in a counted token makes both losses NaN, +inf z and, of the softmax, balance.  Without counted tokens all is 0.  Sums are in
+ * fp32, in a fixed order: the same bits on every call.  Limits as for gg_route, and sequences below 2^31.  `scratch`: gg_balance_scratch_bytes of
+ * device memory (0 for sizes that the call refuses), 4-byte aligned, of any contents; calls that share it must not overlap in time.
+ *
+ * gg_balance_backward: the gradient of the logits, of their element type, from those of balance and z (fp32, one number each in device memory,
+ * either may be NULL); rows that are not counted get zeros.  counts, and so share, are taken as constants.
+ * No counterpart in the reference, which has no router.
+ */
+uint64_t gg_balance_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t sequences);
+int gg_balance(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t top_k, int score, const int32_t* chosen,
+               const int32_t* offsets, int64_t sequences, const uint8_t* mask, float* balance, float* z, int32_t* counts, float* share,
+               float* inverse, void* scratch, void* stream);
+int gg_balance_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int score, const int32_t* offsets,
+                        int64_t sequences, const uint8_t* mask, const float* share, const float* inverse, const float* balance_grad,
+                        const float* z_grad, void* logits_grad, void* stream);
+
+/*
  * A gated expert layer for the few tokens of a decode step, in two launches: out[t] = sum over j of
  * weights[t, j] * (silu(x[t] @ gate_e) * (x[t] @ up_e)) @ down_e with e = chosen[t, j] and silu(x) = x / (1 + exp(-x)).
  *   x (tokens, hidden), out (tokens, hidden), element type dtype (GG_DTYPE_BF16 or GG_DTYPE_F16)
@@ -419,6 +445,34 @@ int gg_moe_few_tokens(const void* x, const void* w13, const void* w2, const int3
 uint64_t gg_lora_scratch_bytes(int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out);
 int gg_lora(const void* x, const void* a, const void* b, const int32_t* adapters, const float* scales, const void* base, void* out,
             int dtype, int64_t rows, int64_t num, int64_t rank, int64_t hidden_in, int64_t hidden_out, void* scratch, void* stream);
+
+/*
+ * Rows as 8-bit integers with a scale each, as gg_gmm_int8 takes them: with most = max |x| of a row, its scale is most / 127 (rounded to
+ * fp32) and q the integers nearest to 127 x / most, ties to even, exactly as that is defined.  A row of zeros has a scale of 0.  A row with
+ * an infinity has an infinite scale (its infinities +-127, all else 0), one with a NaN a scale of NaN.
+ *   x          rows of cols elements, x_stride elements apart, dtype GG_DTYPE_BF16, GG_DTYPE_F16 or GG_DTYPE_F32
+ *   row_index  int32 (rows) or NULL: row r is row row_index[r] of x, which has x_rows; a number that names no row gives zeros
+ *   q          int8 (rows, cols), scales fp32 (rows)
+ * gg_swiglu_quantize: the same of silu(gate) * up = gate / (1 + exp(-gate)) * up for rows gate | up of 2 * cols elements, computed in fp32 and
+ * not rounded in between.  All aligned to their elements; q and scales overlap nothing else.  cols below 2^22.
+ * No counterpart in the reference, whose operands are bf16 (csrc/grouped_gemm.cu:490-506).
+ */
+int gg_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, const int32_t* row_index, int64_t x_rows,
+                     int8_t* q, float* scales, void* stream);
+int gg_swiglu_quantize(const void* gate_up, int dtype, int64_t rows, int64_t cols, int64_t stride, int8_t* q, float* scales, void* stream);
+
+/*
+ * gg_gmm of 8-bit integers with a scale for each row of a and for each column of each group's b:
+ *   c[r, n] = a_scales[r] * b_scales[e, n] * sum over k of a[r, k] * b[e, n, k],   e the group of row r
+ * a int8 (tokens, hidden_in), b int8 (num_groups, hidden_out, hidden_in): trans_b set, trans_a not; dtype is c's, GG_DTYPE_BF16 or
+ * GG_DTYPE_F16.  a_scales fp32 (tokens), b_scales fp32 (num_groups, hidden_out).  All other fields as for gg_gmm, without row indices,
+ * epilogues and accumulation; sizes and alignment are any.  Sums are exact, for any of the 256 values, up to a hidden_in of 131071;
+ * they are scaled in fp32, by the row's first, and rounded once: the same bits on every call.  Rows behind the last group's are left as they are.
+ * gg_gmm_int8_workspace_bytes: 0, or GG_WORKSPACE_BYTES where the call can make use of a workspace (fields as for gg_workspace_bytes_for).
+ * No counterpart in the reference, whose operands are bf16 (csrc/grouped_gemm.cu:490-506).
+ */
+uint64_t gg_gmm_int8_workspace_bytes(const gg_gmm_args* args);
+int gg_gmm_int8(const gg_gmm_args* args, const float* a_scales, const float* b_scales);
 
 /*
  * Runs only the on-device scheduler of gg_gmm_bf16 (same device code, same

@@ -1,0 +1,259 @@
+"""Rows as 8-bit integers and their grouped products, against their definitions in 64 bits.
+
+quantize_rows is defined exactly: 127 x / max|x| to the nearest integer, ties to even, and the fp32 quotient max|x| / 127.  In 64 bits the quotient of
+a 32-bit number times 127 by another is exact where it is a tie, and otherwise further from one than its rounding, so that
+integers and scales are equal.
+
+swiglu_quantize's silu(gate) * up is computed in fp32: the exponential is off by two units in the last place, the sum, the quotient and the
+product by one each at most, together below 2^-21 of the value.  So scales are off by that and a rounding, below 2^-20, and a value
+that 127 / max takes to at most 127 moves by less than 127 * 2^-19 = 2^-12 steps: integers are within a half and 2^-12 of what they round.
+
+gmm_int8's sums are exact; they are rounded to fp32, multiplied twice and rounded to the type: off by 3 * 2^-24 and half a step of the
+type (bf16 2^-8, fp16 2^-11 of the value; below fp16's normal range half of 2^-24)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+ROUNDING = {torch.bfloat16: (2.0 ** -8, 0.0), torch.float16: (2.0 ** -11, 2.0 ** -25)}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    from grouped_gemm import ops as _ops
+    return _ops
+
+
+def _announce(*what):
+    print("[case]", *what, flush=True)
+
+
+def _quantized(x):
+    """By the definition, of finite rows."""
+    x = x.double()
+    most = x.abs().amax(-1, keepdim=True)
+    q = torch.round(127.0 * x / torch.where(most > 0, most, torch.ones_like(most)))
+    return q.to(torch.int8), (most / 127.0).float().squeeze(-1)
+
+
+def _check_rows(ops, x, what, row_index=None):
+    """x: on the CPU."""
+    got = ops.quantize_rows(x.cuda(), None if row_index is None else row_index.cuda())
+    rows = x if row_index is None else x[row_index.long()]
+    values, scales = _quantized(rows)
+    assert got.values.dtype == torch.int8 and got.scales.dtype == torch.float32
+    assert got.values.shape == rows.shape and got.scales.shape == rows.shape[:-1], what
+    assert torch.equal(got.scales.cpu(), scales), what
+    assert torch.equal(got.values.cpu(), values), (what, int((got.values.cpu() != values).sum()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7), (3, 8), (5, 63), (130, 65), (9, 512), (7, 513), (6, 1024), (5, 1025), (3, 2047), (66, 2048),
+                                       (3, 2049), (70, 4096), (2, 4099), (3, 8192), (2, 8193), (2, 16384), (2, 16391), (1, 70001)])
+def test_rows_are_the_nearest_integers(ops, dtype, rows, cols):
+    _announce("rows", dtype, rows, cols)
+    g = torch.Generator().manual_seed(rows * 100003 + cols)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(3 * torch.randn(rows, 1, generator=g))
+    _check_rows(ops, x.to(dtype), (dtype, rows, cols))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ties_go_to_the_even_integer(ops, dtype):
+    _announce("ties", dtype)
+    halves = torch.arange(-126.5, 127.0, 0.5)
+    rows = torch.stack([torch.cat([halves, torch.tensor([127.0])]) * scale for scale in (1.0, 2.0, 2.0 ** -9, 8.0)])
+    rows = torch.cat([rows, rows.flip(1)])
+    assert torch.equal(rows.to(dtype).float(), rows) or dtype == torch.bfloat16
+    _check_rows(ops, rows.to(dtype), ("ties", dtype))
+    # ... and next to them
+    if dtype == torch.float32:
+        near = torch.cat([torch.nextafter(rows, torch.tensor(INF)), torch.nextafter(rows, torch.tensor(-INF))])
+        near[:, 0] = 127.0 * 8
+        _check_rows(ops, near, "next to ties")
+        most = torch.tensor([[3.7], [1.1], [97.3], [5e-3]])   # ties that no float is: the two floats around each
+        t = (halves * most / 127.0).float()
+        near = torch.cat([t, torch.nextafter(t, torch.tensor(INF)), torch.nextafter(t, torch.tensor(-INF)), most], 1)
+        _check_rows(ops, near, "around ties")
+    # small integers and few bits: many quotients are ties
+    g = torch.Generator().manual_seed(1)
+    few = torch.randint(-254, 255, (200, 300), generator=g).float()
+    few[:, 0] = 254.0
+    _check_rows(ops, few.to(dtype), ("few bits", dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_any_size(ops, dtype):
+    _announce("sizes", dtype)
+    g = torch.Generator().manual_seed(2)
+    info = torch.finfo(dtype)
+    x = torch.randn(8, 600, generator=g).clamp(-3, 3)
+    x = x / x.abs().amax(1, keepdim=True)
+    factors = torch.tensor([info.max, info.tiny, info.tiny * 2 ** -4, info.tiny * info.eps * 3, info.tiny * info.eps, 1e-20, 1.0, 0.0], dtype=torch.float64)
+    _check_rows(ops, (x.double() * factors.unsqueeze(1)).to(dtype), ("sizes", dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [5, 700, 5000])
+def test_rows_with_infinities_and_nan(ops, dtype, cols):
+    _announce("odd values", dtype, cols)
+    x = torch.randn(6, cols)
+    x[1, 3], x[1, 1] = INF, -INF
+    x[2, 2] = NAN
+    x[3, 0], x[3, 4] = NAN, INF
+    x[4, cols - 1] = -NAN
+    got = ops.quantize_rows(x.to(dtype).cuda())
+    q, s = got.values.cpu(), got.scales.cpu()
+    want, scales = _quantized(x[[0, 5]].to(dtype))
+    assert torch.equal(q[[0, 5]], want) and torch.equal(s[[0, 5]], scales)
+    assert s[1] == INF and all(math.isnan(s[i]) for i in (2, 3, 4))
+    infinite = torch.zeros(cols, dtype=torch.int8)
+    infinite[3], infinite[1] = 127, -127
+    assert torch.equal(q[1], infinite)
+    # products of such rows are not finite, of the others not touched
+    b = ops.quantize_rows(torch.randn(1, 16, cols, device="cuda"))
+    out = ops.gmm_int8(got.values, got.scales, b.values, b.scales, torch.tensor([6])).cpu()
+    assert torch.isfinite(out[[0, 5]]).all() and not torch.isfinite(out[1:5]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [33, 1000, 4096])
+def test_rows_through_an_index(ops, dtype, cols):
+    _announce("index", dtype, cols)
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(50, cols, generator=g).to(dtype)
+    _check_rows(ops, x, "index", torch.randint(50, (173,), generator=g, dtype=torch.int32))
+    _check_rows(ops, x, "all the same", torch.full((20,), 7, dtype=torch.int32))
+    _check_rows(ops, x, "no rows", torch.empty(0, dtype=torch.int32))
+    # numbers that name no row: zeros
+    index = torch.tensor([3, -1, 50, 2 ** 31 - 1, -2 ** 31, 49], dtype=torch.int32)
+    got = ops.quantize_rows(x.cuda(), index.cuda())
+    want, scales = _quantized(x[[3, 49]])
+    assert torch.equal(got.values[[0, 5]].cpu(), want) and torch.equal(got.scales[[0, 5]].cpu(), scales)
+    assert not got.values[1:5].any() and not got.scales[1:5].any()
+    none = ops.quantize_rows(x[:0].cuda(), index.cuda())
+    assert none.values.shape == (6, cols) and not none.values.any() and not none.scales.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_weights_and_of_views(ops, dtype):
+    _announce("views", dtype)
+    g = torch.Generator().manual_seed(3)
+    _check_rows(ops, torch.randn(3, 20, 77, generator=g).to(dtype), "three dimensions")
+    _check_rows(ops, torch.randn(77, generator=g).to(dtype), "one dimension")
+    _check_rows(ops, torch.randn(0, 77, generator=g).to(dtype), "no rows")
+    wide = torch.randn(40, 900, generator=g).to(dtype)
+    for first, last in ((0, 500), (1, 900), (3, 40), (8, 136)):
+        got = ops.quantize_rows(wide.cuda()[:, first:last])
+        want, scales = _quantized(wide[:, first:last])
+        assert torch.equal(got.values.cpu(), want) and torch.equal(got.scales.cpu(), scales), (first, last)
+        got = ops.quantize_rows(wide.cuda()[::3, first:last], torch.tensor([2, 0], dtype=torch.int32, device="cuda"))
+        assert torch.equal(got.values.cpu(), want[[6, 0]]), (first, last)
+
+
+def _check_swiglu(ops, gate_up, what):
+    """Of finite results; gate_up on the CPU."""
+    got = ops.swiglu_quantize(gate_up.cuda())
+    gate, up = gate_up.double().chunk(2, -1)
+    h = gate / (1.0 + torch.exp(-gate)) * up
+    most = h.abs().amax(-1)
+    scales = got.scales.double().cpu()
+    assert ((scales - most / 127.0).abs() <= 2.0 ** -20 * most / 127.0 + 2.0 ** -149).all(), what
+    off = (got.values.double().cpu() * scales.unsqueeze(-1) - h).abs()
+    assert (off <= (0.5 + 2.0 ** -12) * (most / 127.0).unsqueeze(-1) + 2.0 ** -142).all(), what
+    assert got.values.shape == h.shape and got.scales.shape == h.shape[:-1]
+    largest = torch.where(most > 2.0 ** -120, got.values.abs().amax(-1).cpu().double(), torch.full_like(most, 127.0))
+    assert (largest == 127).all(), what
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,ffn", [(1, 1), (3, 9), (1, 1408), (5, 511), (4, 2047), (3, 2048), (2, 14336), (2, 20001), (300, 96)])
+def test_gated_rows(ops, dtype, rows, ffn):
+    _announce("gated", dtype, rows, ffn)
+    g = torch.Generator().manual_seed(ffn)
+    _check_swiglu(ops, (2 * torch.randn(rows, 2 * ffn, generator=g)).to(dtype), (dtype, rows, ffn))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_rows_of_any_size(ops, dtype):
+    _announce("gated sizes", dtype)
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(6, 400, generator=g)
+    x[0] *= 60      # (exponentials past a float's range)
+    x[1] *= 1e-4
+    x[2, 200:] = 0.0
+    x[3, :200] = -80.0
+    x[4, :200] = -30.0
+    _check_swiglu(ops, x.to(dtype)[[0, 1, 4, 5]], "sizes")
+    got = ops.swiglu_quantize(x.to(dtype).cuda())
+    assert not got.values[2].any() and got.scales[2] == 0
+    view = torch.randn(7, 700, generator=g).to(dtype)
+    got = ops.swiglu_quantize(view.cuda()[:, 5:305])
+    whole = ops.swiglu_quantize(view[:, 5:305].contiguous().cuda())
+    assert torch.equal(got.values, whole.values) and torch.equal(got.scales, whole.scales)
+    x[1, 7] = NAN
+    got = ops.swiglu_quantize(x.to(dtype).cuda())
+    assert math.isnan(got.scales[1]) and torch.isfinite(got.scales[[0, 3, 4, 5]]).all()
+
+
+# ------------------------------------------------------------------ grouped products
+
+def _operands(rows, experts, hidden_in, hidden_out, seed):
+    g = torch.Generator().manual_seed(seed)
+    a = torch.randint(-128, 128, (rows, hidden_in), generator=g, dtype=torch.int8)
+    b = torch.randint(-128, 128, (experts, hidden_out, hidden_in), generator=g, dtype=torch.int8)
+    return a, torch.rand(rows, generator=g) / 64 + 1e-3, b, torch.rand(experts, hidden_out, generator=g) / 64 + 1e-3
+
+
+def _product(a, a_scales, b, b_scales, sizes):
+    """In 64 bits; rows behind the last expert's are NaN."""
+    out = torch.full((a.shape[0], b.shape[1]), NAN, dtype=torch.float64)
+    start = 0
+    for e, n in enumerate(sizes):
+        if n > 0:
+            out[start:start + n] = (a[start:start + n].double() @ b[e].double().t()) * a_scales[start:start + n].double().unsqueeze(1) * b_scales[e].double()
+        start += n
+    return out
+
+
+def _check_close(got, want, dtype, what):
+    half, least = ROUNDING[dtype]
+    got = got.double().cpu()
+    held = ~torch.isnan(want)
+    off = (got - want).abs()[held] - ((half + 3 * 2.0 ** -24) * want.abs()[held] + least)
+    assert off.numel() == 0 or float(off.max()) <= 0, (what, float(off.max()))
+
+
+def _run(ops, a, a_scales, b, b_scales, sizes, dtype, on_device, c=None):
+    batch_sizes = torch.tensor(sizes, dtype=torch.int64)
+    return ops.gmm_int8(a.cuda(), a_scales.cuda(), b.cuda(), b_scales.cuda(), batch_sizes.cuda() if on_device else batch_sizes, dtype=dtype, c=c)
+
+
+SIZES = [
+    # few rows to a group, one to four windows of each kind; every alignment of the depth
+    ([1], 64, 64), ([1], 1, 1), ([2, 0, 1], 15, 3), ([5], 16, 65), ([3, 1], 17, 64), ([16], 127, 63), ([17, 16, 0, 1], 128, 129), ([33], 130, 31),
+    ([8, 9, 7], 1021, 100), ([20, 30, 10], 514, 70), ([64, 65, 63], 259, 130), ([200, 1], 1023, 17), ([0, 0, 3, 0], 640, 64), ([4], 4096, 512),
+    ([1, 1], 8192, 256), ([2], 14336, 128), ([40, 3], 6000, 64),
+    # tiles: short, small and full ones, ragged rows
+    ([100, 60, 0, 130], 256, 264), ([300, 700, 5], 512, 1024), ([129, 40, 257], 1040, 520), ([2000, 48, 1000], 2048, 2048), ([513], 4096, 8),
+    ([40] * 24, 112, 136), ([1500, 1700], 16, 256), ([700], 16384, 128), ([1024, 1024, 1024, 1024], 1408, 2816),
+    # ... that the streaming kernel does not take
+    ([300, 150], 250, 130), ([500], 513, 1001), ([333, 0, 400], 2047, 263),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,hidden_in,hidden_out", SIZES, ids=lambda v: str(v)[:24])
+def test_products_are_exact_sums_rounded_once(ops, dtype, sizes, hidden_in, hidden_out):
+    _announce("product", dtype, sizes, hidden_in, hidden_out)
+    rows = sum(sizes)
+    a, sa, b, sb = _operands(rows, len(sizes), hidden_in, hidden_out, hidden_in + rows)
+    want = _product(a, sa, b, sb, sizes)
+    got = [_run(ops, a, sa, b, sb, sizes, dtype, on_device) for on_device in (True, False)]
+    assert got[0].dtype == dtype and got[0].shape == (rows, hidden_out)
+    _check_close(got[0], want, dtype, (sizes, hidden_in, hidden_out))
+    assert torch.equal(got[0], got[1])
