@@ -787,7 +787,11 @@ int run_pair(const gg_gmm_args* first, const Strides* strides1, const gg_gmm_arg
 // ---- products of 8-bit integers (gg_gmm_int8)
 
 constexpr int64_t kInt8MostDepth = 131071;   // 128 * 128 * depth below 2^31: no sum overflows
-constexpr int64_t kInt8FewRows = 32;         // average rows to a group up to which they go to the kernel for few rows
+// Average rows to a group up to which a call goes to the kernel for few rows, which reads weights faster (it needs no tiles in LDS) but again
+// for every 16 to 64 rows.  us, streaming tiles / few rows, by rows to a group: 8 groups, 4096 -> 14336: 4 110 / 88, 16 111 / 93, 24 111 / 105, 32 111 / 122;
+// 8, 1024 -> 1024: 4 8.4 / 6.1, 24 8.4 / 8.2, 32 8.6 / 9.6; 32, 4096 -> 4096: 4 113 / 98, 16 118 / 105, 32 119 / 126; 64, 7168 -> 2048: 4 158 / 155,
+// 8 159 / 158, 16 160 / 164, 32 162 / 197; 64, 2048 -> 7168: 8 162 / 167, 16 166 / 192; 128, 2048 -> 1408: 4 67 / 63, 8 69 / 67, 16 70 / 78.
+int64_t int8_few_rows(int64_t num_groups) { return num_groups <= 8 ? 24 : (num_groups <= 32 ? 16 : 8); }
 
 int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_scales) {
   if (args == nullptr) return fail(GG_EINVAL, "args is null");
@@ -812,7 +816,7 @@ int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_sc
 }
 
 bool int8_streams(const gg_gmm_args& g) {
-  return g.tokens > kInt8FewRows * g.num_groups && g.hidden_in > 0 && g.hidden_in % 16 == 0 && g.hidden_out % 8 == 0 &&
+  return g.tokens > int8_few_rows(g.num_groups) * g.num_groups && g.hidden_in > 0 && g.hidden_in % 16 == 0 && g.hidden_out % 8 == 0 &&
          ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | reinterpret_cast<uintptr_t>(g.c)) & 15) == 0;
 }
 

@@ -400,6 +400,11 @@ __device__ __forceinline__ void load_to_lds_16(const rsrc_words& rsrc, uint32_t 
   }
 }
 
+// ... one dword per lane, right behind aim_lds
+__device__ __forceinline__ void load_to_lds_4(const rsrc_words& rsrc, uint32_t voffset) {
+  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(voffset), "s"(rsrc) : "memory");
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)reinterpret_cast<uintptr_t>(GG_LDS_PTR(p));
 }
@@ -454,10 +459,9 @@ __device__ __forceinline__ f32x16 mfma_32x32x64_f8(bf16x8 x_lo, bf16x8 x_hi, bf1
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc, FORMAT, FORMAT, 0, 0, 0, 0);
 }
 
-// The same depth of 8-bit integers, in two instructions: sums are exact, so that it does not matter which depth values meet in which.
-__device__ __forceinline__ i32x16 mfma_32x32x64_i8(bf16x8 x_lo, bf16x8 x_hi, bf16x8 y_lo, bf16x8 y_hi, i32x16 acc) {
-  acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, x_lo), __builtin_bit_cast(i32x4, y_lo), acc, 0, 0, 0);
-  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, x_hi), __builtin_bit_cast(i32x4, y_hi), acc, 0, 0, 0);
+// One 32x32x32 matrix instruction on fragments of 16 8-bit integers per lane.
+__device__ __forceinline__ i32x16 mfma_32x32x32_i8(bf16x8 x, bf16x8 y, i32x16 acc) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, y), acc, 0, 0, 0);
 }
 
 // Four fp32 values rounded (to nearest even) to the element type, as 8 bytes.
@@ -1399,6 +1403,13 @@ struct GmmConfig {
   static_assert(BK % 16 == 0 && STAGES >= 2, "");
 };
 
+// ... and of the kernels of 8-bit integers: the scales of each wave's columns behind that.
+template <typename Cfg>
+constexpr int int8_lds_bytes() {
+  static_assert((Cfg::LDS_BYTES + Cfg::NT / 64 * Cfg::WTN * 4) * Cfg::WORKGROUPS_PER_CU <= 160 * 1024, "");
+  return Cfg::LDS_BYTES + Cfg::NT / 64 * Cfg::WTN * 4;
+}
+
 // One output tile (or one piece of a tile of the last round) as the scheduler hands it out.
 struct TileInfo {
   GroupGeom g;
@@ -1691,7 +1702,8 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   constexpr bool ACC_F32 = EPI == kEpiAccF32 || EPI == kEpiAccF32Atomic, KEEP = EPI == kEpiSwiGLUKeep, GATE_UP = EPI == kEpiSwiGLU || KEEP;
   // One-byte elements (NT layout only: both operands depth-contiguous).  The tile movers see them
   // as two-byte elements, two to one: same bytes per row and slice, BK_ELEMS depth values a slice.
-  // I8: 8-bit integers, which move as fp8 does; only what multiplies and sums them differs.
+  // I8: 8-bit integers, which move and are held as fp8 is; the 64-deep step of an instruction there takes two here.  (In 16 x 16 x 64
+  // instructions, which alone sustain 5 % more of such operands, the compiler moves accumulators in and out of the loop.)
   constexpr bool I8 = is_i8(DT), F8 = is_f8(DT) || I8;
   constexpr int ES = F8 ? 1 : 2, BK_ELEMS = BK * 2 / ES, OUT_DT = DT == kF16 || DT == kI8ToF16 ? kF16 : kBF16;
   static_assert(!I8 || (LAYOUT == kNT && EPI == kEpiStore && !INDEXED), "8-bit integers: NT layout, plain rows and epilogue");
@@ -2015,29 +2027,29 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   auto partial_at = [&](int i, int j, int q) -> uint32_t { return (((i * NB + j) * 4 + q) * NT + threadIdx.x) * 16; };
   bool fix_pending = false;   // this workgroup's depth piece was the last of its tile to arrive
 
-  // 8-bit integers: the scales of a tile's BM rows, then of its BN columns, in LDS behind everything else.
-  float* const tile_scales = reinterpret_cast<float*>(smem + Cfg::LDS_BYTES);
-  // The waves load them in turns, 64 at a time, in the first slice of a tile once all waves have left the tile before; the wait for the next
-  // slice, whose loads come later, is one for them.
+  // 8-bit integers: while a tile is multiplied, the scales of the wave's rows wait in its strip for the epilogue, those of its columns in LDS
+  // behind everything else (int8_lds_bytes), where they are read as they are used: few registers are free then.  They are asked for as it begins, when the wave has left the tile before, and the first slice's wait is one for them: loads
+  // that come later are waited for.  (Asked for inside the depth loop, where all waves could share them, the condition makes the
+  // compiler move accumulators in every slice: 32768 rows, 4096 -> 14336, in 16 x 16 blocks: 2337 us.)
+  constexpr int ROW_UNITS = (MB + 1) / 2, COL_UNITS = Cfg::WTN / 64;   // of 64 scales
+  static_assert(!I8 || ROW_UNITS * 256 <= Cfg::EPILOGUE_WAVE_BYTES, "");
+  char* const column_scales = smem + Cfg::LDS_BYTES + wave * (COL_UNITS * 256);
   auto load_scales = [&](const TileInfo& tile) {
     if constexpr (I8) {
       const int group = uniform(tile_ring[(tile_n % Cfg::TILE_RING_SLOTS) * kTileInfoDwords + 23]);
-      const rsrc_words of_rows = make_rsrc_words(p.a_scales + tile.g.row0 + tile.m0, (uint32_t)tile.rows_valid * 4u);
-      const rsrc_words of_columns =
-          make_rsrc_words(p.b_scales + (int64_t)group * p.hidden_out + tile.n0, tile.valid ? (uint32_t)min(BN, tile.g.n - tile.n0) * 4u : 0u);
-#pragma unroll
-      for (int first = 0; first < (BM + BN) / 64; first += WAVES_M * WAVES_N) {
-        const int unit = first + wave;
-        if ((BM + BN) / 64 % (WAVES_M * WAVES_N) != 0 && unit >= (BM + BN) / 64) break;
-        const bool rows = unit < BM / 64;
-        rsrc_words rsrc;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) rsrc[w] = uniform(rows ? of_rows[w] : of_columns[w]);
-        settle<5>(rsrc);
-        const uint32_t offset = (uint32_t)(unit - (rows ? 0 : BM / 64)) * 256u + (uint32_t)lane * 4u;
-        const uint32_t to = uniform(lds_address(tile_scales) + (uint32_t)unit * 256u);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(to), "v"(offset), "s"(rsrc) : "memory", "m0");
-      }
+      rsrc_words of_rows = make_rsrc_words(p.a_scales + tile.g.row0 + tile.m0, (uint32_t)tile.rows_valid * 4u);
+      rsrc_words of_columns = make_rsrc_words(p.b_scales + (int64_t)group * p.hidden_out + tile.n0, (uint32_t)max(tile.g.n - tile.n0, 0) * 4u);
+      settle(of_rows);
+      settle<5>(of_columns);
+      const uint32_t strip = uniform(lds_address(smem) + Cfg::EPILOGUE_OFFSET + wave * Cfg::EPILOGUE_WAVE_BYTES);
+      const uint32_t columns = uniform(lds_address(column_scales));
+      static_for<ROW_UNITS + COL_UNITS>([&](auto u_tag) {
+        constexpr int U = decltype(u_tag)::value;
+        // (rows of the wave's 32-row blocks 2 U and 2 U + 1)
+        const uint32_t at = U < ROW_UNITS ? (wm + (2 * U + (lane >> 5)) * WAVES_M) * 32 + (lane & 31) : wn * Cfg::WTN + (U - ROW_UNITS) * 64 + lane;
+        aim_lds<(U < ROW_UNITS ? U : U - ROW_UNITS) * 256>(U < ROW_UNITS ? strip : columns);
+        load_to_lds_4(U < ROW_UNITS ? of_rows : of_columns, at * 4u);
+      });
     }
   };
 
@@ -2076,11 +2088,11 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   // copy of them costs a pass more than the product's own): whole chunks at once, which global memory takes on
   // any boundary, the last ones of a row by elements.  8 x 1024 rows, 2047 -> 5461, forward and gradients: 834 us with
   // padded results copied back (120 of them the copies), 760 so.
-  constexpr bool ANY_ROWS = EPI == kEpiStore && !INDEXED && !RAGGED_DEPTH && !F8;
+  constexpr bool ANY_ROWS = EPI == kEpiStore && !INDEXED && !RAGGED_DEPTH && !F8 && !I8;
   // ... or that are no whole groups of 4 columns, which the fix-up of depth pieces stores (whole tiles / pieces, us: weight
   // gradients of 21 Zipf (1.2) groups, 51204 rows, 128 x 558: 125 / 38; 64, 49152 rows, 2046 x 1406: 492 / 364; 16 groups, 600 rows,
   // 6144 -> 518: 46.8 / 33.8).
-  constexpr bool FIX_ANY_ROWS = EPI == kEpiStore && !INDEXED && !F8;
+  constexpr bool FIX_ANY_ROWS = EPI == kEpiStore && !INDEXED && !F8 && !I8;
   auto store_any = [&](const TileInfo& tile, uint32_t row_off, int col, int most, u32x4 v) {
     struct Chunk {
       u32x4 v;
@@ -2146,6 +2158,16 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       for (int j = 0; j < MFMA_N; ++j)
 #pragma unroll
         for (int r = 0; r < (F8 ? 16 : 4); ++r) acc[i][j][r] = 0;
+    float row_scale[I8 ? ML : 1][2];   // 8-bit integers: of this lane's groups, taken out of the strip before it is written
+    auto read_row_scales = [&]() {
+      if constexpr (I8) {
+        const float* strip = reinterpret_cast<const float*>(smem + Cfg::EPILOGUE_OFFSET + wave * Cfg::EPILOGUE_WAVE_BYTES);
+#pragma unroll
+        for (int i = 0; i < ML; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) row_scale[i][h] = strip[i * 32 + group_row(2 * h)];
+      }
+    };
     // Group q (see group_row) of the 32 x 32 block (i, j), moved out of the accumulation registers here and no earlier:
     // all of them at once would not fit beside the next tile's fragments.  (How that is said decides what the compiler
     // makes of it: read in assembly, the plain epilogues of full tiles get by without moves and spills; tied
@@ -2154,13 +2176,15 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       auto& from = F8 ? acc[i][j] : acc[2 * i + q / 2][2 * j + q % 2];
       constexpr bool TIED = !F8 && (GATE_UP || ((INDEXED || RAGGED_DEPTH) && BM > 128));
       if constexpr (TIED) asm volatile("" : "+a"(from));
+      f32x4 column_scale;
+      if constexpr (I8) column_scale = *reinterpret_cast<const f32x4*>(column_scales + (j * 32 + group_col(q)) * 4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         auto x = from[F8 ? 4 * q + r : r];
         if constexpr (I8) {
           int sum;
           asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(sum) : "a"(x));
-          v[r] = (float)sum * tile_scales[(wm + i * WAVES_M) * 32 + group_row(q)] * tile_scales[BM + wn * Cfg::WTN + j * 32 + group_col(q) + r];
+          v[r] = (float)sum * row_scale[i][q / 2] * column_scale[r];
         } else if constexpr (F8 || (MB * NB > 4 && !TIED)) {
           asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[r]) : "a"(x));
         } else {
@@ -2170,7 +2194,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       }
     };
 
-    constexpr int S = 2 * MFMA_M * MFMA_N;
+    constexpr int S = (I8 ? 4 : 2) * MFMA_M * MFMA_N;
     constexpr int READ_END = S * AT_READ_END / 32, RELEASE = S * AT_RELEASE / 32, READY = S * AT_READY / 32, LOAD_END = S * AT_LOAD_END / 32;
     static_assert(READ_END <= RELEASE && RELEASE <= READY && 2 * READY >= S && READ_END > 0 && READY < S && LOAD_END - S <= READ_END, "");
     using Loads = LoadSlots<LOADS_PER_STAGE, RELEASE, READY, LOAD_END, S>;
@@ -2183,13 +2207,14 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
         constexpr int m = FIRST + decltype(m_tag)::value, n = m % (S / 2), set = m < S / 2 ? 0 : 2;
         // serpentine over the 32 x 32 blocks and over the 16 x 16 ones in them: consecutive MFMAs share one operand, and the
         // fragments are wanted no faster than they come (columns of 16 x 16 blocks want all of A's at once)
-        constexpr int quarter = F8 ? 0 : n % 4, block = F8 ? n : n / 4;
+        // (8-bit integers: all blocks with the first half of their fragments, then all with the second, since a sum right behind itself waits)
+        constexpr int quarter = F8 ? 0 : n % 4, block = I8 ? n % (ML * NB) : (F8 ? n : n / 4);
         constexpr int j = block / ML, i = (j % 2 == 0) ? block % ML : ML - 1 - block % ML;
         constexpr int hi = quarter / 2, hj = quarter == 1 || quarter == 2 ? 1 : 0;   // halves of A's and of B's block
         // operands swapped: the result block is held transposed, so a lane owns four
         // consecutive columns of one output row
         if constexpr (I8) {
-          acc[i][j] = mfma_32x32x64_i8(fb[set][j], fb[set + 1][j], fa[set][i], fa[set + 1][i], acc[i][j]);
+          acc[i][j] = mfma_32x32x32_i8(fb[set + n / (ML * NB)][j], fa[set + n / (ML * NB)][i], acc[i][j]);
         } else if constexpr (F8) {   // (takes both halves of both fragments)
           acc[i][j] = mfma_32x32x64_f8<DT>(fb[set][j], fb[set + 1][j], fa[set][i], fa[set + 1][i], acc[i][j]);
         } else {
@@ -2227,6 +2252,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
     using IReady = std::integral_constant<int, READY>;
     using IAll = std::integral_constant<int, S>;
 
+    load_scales(ti);
     for (int kt = 0; kt < ti.nk; ++kt) {
       const int y = uniform(x ^ 1);   // (the same in every lane: keeps the LDS addresses scalar)
       if constexpr (LATE_LOADS) {
@@ -2243,7 +2269,6 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
       // every wave has all fragments of this slice in registers
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       block_barrier();
-      if (I8 && kt == 0) load_scales(ti);
       slots(IRelease{}, IReady{}, y);
       // the next slice has landed for every wave (only the loads just issued may be pending and, in the first
       // slice after a tile that was stored, its stores)
@@ -2488,6 +2513,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
         char* strip = smem + Cfg::EPILOGUE_OFFSET + wave * Cfg::EPILOGUE_WAVE_BYTES;
         constexpr int PITCH = Cfg::EPILOGUE_PITCH;
         const int out_row = lane >> 3, out_chunk = lane & 7;
+        read_row_scales();
         // an even width that is not a multiple of 8: rows of c then start on 4-byte boundaries
         // only, and the last 16-byte chunk of a row holds 2, 4 or 6 columns
         const bool ragged_width = uniform(ti.g.n & 7) != 0;

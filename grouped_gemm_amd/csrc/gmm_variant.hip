@@ -26,9 +26,10 @@ using V = VariantDef<GG_VARIANT_INDEX>;
 using S = V::Shape;
 using Cfg = GmmConfig<V::LAYOUT, S::BM, S::BN, BK, STAGES, S::WAVES_M, S::WAVES_N>;
 
-// (8-bit integers: the scales of a tile's rows and columns behind the rest)
-constexpr int LDS_BYTES = Cfg::LDS_BYTES + (is_i8(V::DT) ? (S::BM + S::BN) * 4 : 0);
-static_assert(LDS_BYTES * Cfg::WORKGROUPS_PER_CU <= 160 * 1024, "");
+constexpr int lds_bytes() {
+  if constexpr (is_i8(V::DT)) return int8_lds_bytes<Cfg>();
+  else return Cfg::LDS_BYTES;
+}
 
 const void* kernel_address() {
   return reinterpret_cast<const void*>(
@@ -37,7 +38,7 @@ const void* kernel_address() {
 }
 
 hipError_t prepare() {
-  return hipFuncSetAttribute(kernel_address(), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
+  return hipFuncSetAttribute(kernel_address(), hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes());
 }
 
 hipError_t launch(const GmmParams& p, const HostSizes& hs, int grid, hipStream_t stream) {
@@ -45,10 +46,10 @@ hipError_t launch(const GmmParams& p, const HostSizes& hs, int grid, hipStream_t
   HostSizes sizes = hs;
   void* args[2] = {&params, &sizes};
   return hipLaunchKernel(kernel_address(), dim3(grid), dim3(S::WAVES_M * S::WAVES_N * 64), args,
-                         LDS_BYTES, stream);
+                         lds_bytes(), stream);
 }
 
-const VariantOps kOps = {V::DT, V::LAYOUT, S::kId, V::EPI, V::INDEXED ? 1 : 0, LDS_BYTES, Cfg::WORKGROUPS_PER_CU, &prepare, &launch};
+const VariantOps kOps = {V::DT, V::LAYOUT, S::kId, V::EPI, V::INDEXED ? 1 : 0, lds_bytes(), Cfg::WORKGROUPS_PER_CU, &prepare, &launch};
 
 }  // namespace
 
