@@ -3,10 +3,18 @@
 //   most = max |x| of the row;  scale = most / 127;  q = the integer nearest to 127 x / most, ties to even.
 //
 // x is a row as it is, or (with a row index) one that the index names, or silu(gate) * up of a row gate | up, computed in
-// fp32 and not rounded in between.  q is what exact arithmetic gives: 127 x / most is computed in fp32, off by less than
-// 2^-15 at its largest, and where that leaves open which integer is the nearest, 127 x - q most is looked at in 64
-// bits, which hold it exactly.  scale is the fp32 quotient.  A row of zeros has a scale of 0.  An infinity in a row makes its scale
-// infinite (infinities are +-127, all else 0), a NaN makes it NaN: products of such rows are not finite.
+// fp32 and not rounded in between.  scale is the fp32 quotient.  A row of zeros has a scale of 0.  An infinity in a row makes its scale infinite
+// (infinities are +-127, all else 0), a NaN makes it NaN: products of such rows are not finite.
+//
+// q is what exact arithmetic gives, at one fused multiply-add for most elements (bound by reading and writing, the kernel has few instructions
+// for each):
+//   Two-byte x.  A tie is 254 x = (2 r + 1) most in whole numbers, so 127 divides most's significand, or it divides 2 r + 1 < 254, and then r is 63
+//   and the tie goes to 64, away from zero.  Where 127 does not divide the significand, x times a number just above 127 / most, off by at
+//   most 1.5 * 2^-23 of itself, rounds as it should: a value that is no tie is no nearer to one than 2^-20 of itself (x is a multiple of 2^-11 of its power
+//   of two, most of its own, and |x| <= most), and the ties at 63.5 are pushed away from zero.
+//   Otherwise 127 x / most comes out off by less than 2^-15, and where that leaves open which integer is the nearest, the sign of 127 x - (q +- 1/2) most
+//   decides, which sums of floats whose errors are kept have exactly.
+//   silu(gate) * up is off by more than any of that, and is rounded as it comes.
 #include "operators.hpp"
 
 #include <math.h>
@@ -27,170 +35,288 @@ struct QuantizeParams {
 struct Eight {
   float v[8];
 };
+struct __attribute__((packed, aligned(4))) Floats8 {
+  float v[8];
+};
 
-// 8 elements from p on, in fp32.
-template <int DT>
-__device__ __forceinline__ Eight widen8(const void* row, int64_t at) {
-  Eight e;
-  if constexpr (DT == kF32) {
-    struct __attribute__((packed, aligned(4))) Floats {
-      float v[8];
-    };
-    const Floats f = *reinterpret_cast<const Floats*>(static_cast<const float*>(row) + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = f.v[i];
-  } else {
-    const u32x4 raw = load8(static_cast<const uint16_t*>(row) + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = widen_bits<DT>((uint16_t)(raw[i / 2] >> (16 * (i % 2))));
-  }
-  return e;
-}
-template <int DT>
-__device__ __forceinline__ float widen1(const void* row, int64_t at) {
-  if constexpr (DT == kF32) return static_cast<const float*>(row)[at];
-  else return widen_bits<DT>(static_cast<const uint16_t*>(row)[at]);
-}
-// Chunk c of a row of `cols`: zeros past its end.
-template <int DT>
-__device__ __forceinline__ Eight chunk_of(const void* row, int c, int cols) {
-  if (c * 8 + 8 <= cols) return widen8<DT>(row, c * 8);
-  Eight e;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e.v[i] = c * 8 + i < cols ? widen1<DT>(row, c * 8 + i) : 0.0f;
-  return e;
-}
-
+// What a thread holds of a row between the two passes: 8 elements, as they are or (gated) as they came out.
 template <int DT, bool GATED>
-__device__ __forceinline__ Eight values_of(const void* row, int c, int cols) {
-  Eight x = chunk_of<DT>(row, c, cols);
-  if constexpr (GATED) {
-    constexpr int BYTES = DT == kF32 ? 4 : 2;
-    const Eight up = chunk_of<DT>(static_cast<const char*>(row) + (int64_t)cols * BYTES, c, cols);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x.v[i] = x.v[i] / (1.0f + expf(-x.v[i])) * up.v[i];
+struct Held {
+  static constexpr bool FLOATS = DT == kF32 || GATED;
+  std::conditional_t<FLOATS, Eight, u32x4> raw;
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (FLOATS) {
+      return raw.v[i];
+    } else if constexpr (DT == kBF16) {
+      return __builtin_bit_cast(float, i % 2 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
+    } else {
+      return widen_bits<DT>((uint16_t)(raw[i / 2] >> (16 * (i % 2))));
+    }
   }
-  return x;
+};
+
+// `count` elements of a row from `at` on, and zeros.
+template <int DT>
+__device__ __forceinline__ Held<DT, false> load_chunk(const void* row, int64_t at, int count = 8) {
+  Held<DT, false> h;
+  if constexpr (DT == kF32) {
+    const float* from = static_cast<const float*>(row) + at;
+    const Floats8 f = count == 8 ? *reinterpret_cast<const Floats8*>(from) : Floats8{};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h.raw.v[i] = count == 8 ? f.v[i] : (i < count ? from[i] : 0.0f);
+  } else {
+    const uint16_t* from = static_cast<const uint16_t*>(row) + at;
+    if (count == 8) {
+      h.raw = load8(from);
+    } else {
+      uint16_t e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = i < count ? from[i] : uint16_t(0);
+      h.raw = __builtin_bit_cast(u32x4, e);
+    }
+  }
+  return h;
 }
+
+// gate / (1 + exp(-gate)) * up.  The exponential by the hardware's power of two, with what rounding its argument lost put back: within two units in the
+// last place.  The quotient as in the streaming kernel's epilogue: the hardware's reciprocal (of a quarter of the divisor, whose reciprocal is
+// normal) and one correction by the remainder.
+__device__ __forceinline__ float gated(float gate, float up) {
+  constexpr float LOG2E = 0x1.715476p+0f, LOG2E_REST = 0x1.4ae0bep-26f, LN2 = 0x1.62e430p-1f;
+  const float t = -gate * LOG2E, rest = __builtin_fmaf(-gate, LOG2E_REST, __builtin_fmaf(-gate, LOG2E, -t));
+  const float power = __builtin_amdgcn_exp2f(t);
+  const float e = fabsf(t) < 128.0f ? __builtin_fmaf(power, rest * LN2, power) : power;   // (past a float's range: 0 or infinity)
+  const float d = 1.0f + e, inverse = 0.25f * __builtin_amdgcn_rcpf(0.25f * d);
+  const float quotient = gate * inverse, remainder = __builtin_fmaf(-d, quotient, gate);
+  return __builtin_fmaf(__builtin_fmaxf(remainder, -__FLT_MAX__), inverse, quotient) * up;
+}
+
+// What is loaded of a chunk, and what it is made into.
+template <int DT, bool GATED>
+struct Loaded {
+  Held<DT, false> x, up;
+  __device__ __forceinline__ void load(const void* row, int at, int cols, int count = 8) {
+    x = load_chunk<DT>(row, at, count);
+    if constexpr (GATED) up = load_chunk<DT>(row, (int64_t)cols + at, count);
+  }
+  __device__ __forceinline__ Held<DT, GATED> value() const {
+    if constexpr (!GATED) {
+      return x;
+    } else {
+      Held<DT, GATED> h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h.raw.v[i] = gated(x.value(i), up.value(i));
+      return h;
+    }
+  }
+};
 
 // The bits of |x| are ordered as the numbers are, NaN above all.
 __device__ __forceinline__ uint32_t size_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t most_of(const Eight& x, uint32_t most) {
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// The largest of the elements' bits without their signs so far: two halves of two-byte types, one word of fp32.
+template <int DT, bool GATED>
+__device__ __forceinline__ uint32_t most_of(const Held<DT, GATED>& h, uint32_t most) {
+  if constexpr (Held<DT, GATED>::FLOATS) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t s = size_bits(x.v[i]);
-    most = s > most ? s : most;
+    for (int i = 0; i < 8; ++i) most = max(most, size_bits(h.raw.v[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, h.raw[i] & 0x7fff7fffu)));
   }
   return most;
 }
 
+enum : int { kQuick, kExact, kOdd };   // one multiply-add; ties are looked at; an infinity or a NaN
 struct RowScale {
-  float most, unit, inverse;   // unit: a power of two that x and most are multiplied with, so that 127 / most is a float
-  bool finite;
+  float most, inverse;
+  float unit;   // kExact: a power of two that x and most are multiplied with, so that neither 127 / most nor 127 x leaves a float's range
+  int way;      // the same in all threads of a row
 };
+
+// most_bits: as most_of gives them
+template <int DT, bool GATED>
 __device__ __forceinline__ RowScale row_scale(uint32_t most_bits) {
   RowScale s;
-  s.most = __builtin_bit_cast(float, most_bits);
-  s.finite = most_bits < 0x7f800000u;
-  s.unit = s.most < 0x1p-64f ? 0x1p64f : 1.0f;
+  bool divides = !GATED;   // 127 may divide the significand
+  if constexpr (Held<DT, GATED>::FLOATS) {
+    s.most = __builtin_bit_cast(float, most_bits);
+  } else {
+    s.most = widen_bits<DT>((uint16_t)most_bits);
+    constexpr uint32_t IMPLICIT = DT == kBF16 ? 0x80u : 0x400u;
+    divides = ((most_bits & (IMPLICIT - 1)) | (most_bits >= IMPLICIT ? IMPLICIT : 0u)) % 127u == 0;
+  }
+  const bool small = s.most < 0x1p-64f;
+  s.way = !(s.most < INFINITY) ? kOdd : (divides || small ? kExact : kQuick);
+  s.unit = s.way != kExact ? 1.0f : (small ? 0x1p64f : (s.most > 0x1p64f ? 0x1p-64f : 1.0f));
   s.inverse = s.most > 0.0f ? 127.0f / (s.most * s.unit) : 0.0f;
+  if (s.way == kQuick && !GATED) s.inverse = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, s.inverse) + 1);
   return s;
 }
 
-// Eight integers, a byte each.
-__device__ __forceinline__ u32x2 round8(const Eight& x, const RowScale& s) {
-  constexpr float MAGIC = 0x1.8p23f;   // beside it a float has no places behind the point, and its lowest byte is the integer's
-  constexpr float OPEN = 0.5f - 0x1p-15f;
-  uint32_t bits[8];
-  if (!s.finite) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bits[i] = size_bits(x.v[i]) == 0x7f800000u ? (x.v[i] > 0.0f ? 127u : 129u) : 0u;
-  } else {
-    float furthest = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float t = x.v[i] * s.unit * s.inverse, m = t + MAGIC;
-      bits[i] = __builtin_bit_cast(uint32_t, m);
-      furthest = fmaxf(furthest, fabsf(t - (m - MAGIC)));
-    }
-    if (furthest > OPEN) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int q = (int)(bits[i] << 24) >> 24;
-        const double rest = fma(-(double)q, (double)s.most, 127.0 * (double)x.v[i]), half = 0.5 * (double)s.most;
-        const int odd = q & 1;
-        if (rest > half || (rest == half && odd)) bits[i] = (uint32_t)(q + 1);
-        if (rest < -half || (rest == -half && odd)) bits[i] = (uint32_t)(q - 1);
-      }
-    }
-  }
+constexpr float kMagic = 0x1.8p23f;   // beside it a float has no places behind the point, and its lowest byte is the integer's
+
+__device__ __forceinline__ u32x2 pack8(const uint32_t (&bits)[8]) {
   u32x2 packed;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t low = __builtin_amdgcn_perm(bits[4 * h + 1], bits[4 * h], 0x0c0c0400u);
-    const uint32_t high = __builtin_amdgcn_perm(bits[4 * h + 3], bits[4 * h + 2], 0x04000c0cu);
-    packed[h] = low | high;
+  for (int p = 0; p < 2; ++p) {
+    const uint32_t low = __builtin_amdgcn_perm(bits[4 * p + 1], bits[4 * p], 0x0c0c0400u);
+    const uint32_t high = __builtin_amdgcn_perm(bits[4 * p + 3], bits[4 * p + 2], 0x04000c0cu);
+    packed[p] = low | high;
   }
   return packed;
 }
+// Eight integers, a byte each.
+template <int DT, bool GATED>
+__device__ __forceinline__ u32x2 round_quick(const Held<DT, GATED>& h, const RowScale& s) {
+  uint32_t bits[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bits[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(h.value(i), s.inverse, kMagic));
+  return pack8(bits);
+}
+template <int DT, bool GATED>
+__device__ __forceinline__ u32x2 round_exact(const Held<DT, GATED>& h, const RowScale& s) {
+  uint32_t bits[8];
+  float furthest = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = h.value(i) * s.unit, m = __builtin_fmaf(x, s.inverse, kMagic);
+    bits[i] = __builtin_bit_cast(uint32_t, m);
+    furthest = fmaxf(furthest, fabsf(__builtin_fmaf(x, s.inverse, kMagic - m)));
+  }
+  if (furthest > 0.5f - 0x1p-15f) {
+    const float most = s.most * s.unit, half = 0.5f * most;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // 127 x = times + lost; times - q most is within half and 2^-15 of most, and a float; so is its difference from half
+      const float x = h.value(i) * s.unit, q = __builtin_bit_cast(float, bits[i]) - kMagic;
+      const float times = 127.0f * x, lost = __builtin_fmaf(127.0f, x, -times), rest = __builtin_fmaf(-q, most, times);
+      const float above = (rest - half) + lost, below = (rest + half) + lost;
+      const bool odd = (bits[i] & 1) != 0;
+      if (above > 0.0f || (above == 0.0f && odd)) bits[i] += 1;
+      if (below < 0.0f || (below == 0.0f && odd)) bits[i] -= 1;
+    }
+  }
+  return pack8(bits);
+}
+template <int DT, bool GATED>
+__device__ __forceinline__ u32x2 round_odd(const Held<DT, GATED>& h) {
+  uint32_t bits[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bits[i] = size_bits(h.value(i)) == 0x7f800000u ? (h.value(i) > 0.0f ? 127u : 129u) : 0u;
+  return pack8(bits);
+}
 
-__device__ __forceinline__ void store_chunk(int8_t* row, int c, int cols, u32x2 v) {
+template <int DT, bool GATED>
+__device__ __forceinline__ u32x2 round_any(const Held<DT, GATED>& h, const RowScale& s) {
+  return s.way == kOdd ? round_odd(h) : (s.way == kExact ? round_exact(h, s) : round_quick(h, s));
+}
+
+__device__ __forceinline__ void store8(int8_t* to, u32x2 v) {
   struct __attribute__((packed, aligned(1))) Bytes8 {
     u32x2 v;
   };
-  if (c * 8 + 8 <= cols) {
-    reinterpret_cast<Bytes8*>(row + c * 8)->v = v;
-  } else {
-    for (int i = 0; c * 8 + i < cols; ++i) row[c * 8 + i] = (int8_t)(v[i / 4] >> (8 * (i % 4)));
-  }
+  reinterpret_cast<Bytes8*>(to)->v = v;
 }
 
-// THREADS threads to a row, which hold HELD chunks of it each between the two passes; rows with more are read twice.
+struct SourceRow {
+  const void* x;
+  bool there;   // the index names a row
+};
+template <int DT>
+__device__ __forceinline__ SourceRow source_row(const QuantizeArgs& a, int64_t row) {
+  int64_t source = row;
+  if (a.row_index != nullptr) source = a.row_index[row];
+  const bool there = (uint64_t)source < (uint64_t)a.x_rows;
+  return {static_cast<const char*>(a.x) + (there ? source : 0) * a.x_stride * (DT == kF32 ? 4 : 2), there};
+}
+
+// THREADS threads to a row of at least 8, which hold HELD chunks of it each between the two passes; rows with more are read twice, and so are
+// those that are not rounded in the way that most of their type are.  A row's last chunk is its last 8 elements: where it overlaps the one
+// before, both write the same.  Threads without a chunk take the last one, and store nothing.
 template <int DT, bool GATED, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void quantize_kernel(QuantizeParams p) {
   constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, WAVES = THREADS / 64;
-  constexpr int BYTES = DT == kF32 ? 4 : 2;
   __shared__ uint32_t of_wave[WAVES];
   const QuantizeArgs& a = p.a;
-  const int t = threadIdx.x % THREADS;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
-    int64_t source = row;
-    if (a.row_index != nullptr) source = a.row_index[row];
-    const bool there = (uint64_t)source < (uint64_t)a.x_rows;
-    const void* x = static_cast<const char*>(a.x) + (there ? source : 0) * a.x_stride * BYTES;
-    const int cols = (int)a.cols, chunks = there ? p.chunks : 0;
-    Eight held[HELD];
+  const int t = threadIdx.x % THREADS, cols = (int)a.cols;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + uniform((int)(threadIdx.x / THREADS)); row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+    const SourceRow source = source_row<DT>(a, row);
+    int8_t* q = a.q + row * a.cols;
+    if (!source.there) {
+      if (t == 0) a.scales[row] = 0.0f;
+      for (int c = t; c < p.chunks; c += THREADS) store8(q + min(c * 8, cols - 8), u32x2{0u, 0u});
+      continue;
+    }
+    Held<DT, GATED> held[HELD];
     uint32_t most = 0;
+    {
+      Loaded<DT, GATED> loaded[HELD];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      const int c = t + h * THREADS;
-      if (c < chunks) {
-        held[h] = values_of<DT, GATED>(x, c, cols);
+      for (int h = 0; h < HELD; ++h) loaded[h].load(source.x, min((t + h * THREADS) * 8, cols - 8), cols);
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) {
+        held[h] = loaded[h].value();
         most = most_of(held[h], most);
       }
     }
-    for (int c = t + HELD * THREADS; c < chunks; c += THREADS) most = most_of(values_of<DT, GATED>(x, c, cols), most);
+    for (int c = t + HELD * THREADS; c < p.chunks; c += THREADS) {
+      Loaded<DT, GATED> more;
+      more.load(source.x, min(c * 8, cols - 8), cols);
+      most = most_of(more.value(), most);
+    }
+    if constexpr (!Held<DT, GATED>::FLOATS) most = max(most & 0xffffu, most >> 16);
     most = group_max<64>(most);
     if constexpr (WAVES > 1) {
       if ((threadIdx.x & 63) == 0) of_wave[t / 64] = most;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) most = of_wave[w] > most ? of_wave[w] : most;
+      for (int w = 0; w < WAVES; ++w) most = max(most, of_wave[w]);
       __syncthreads();   // (read before the next row's are written)
     }
-    const RowScale s = row_scale(most);
-    int8_t* q = a.q + row * a.cols;
+    const RowScale s = row_scale<DT, GATED>((uint32_t)uniform((int)most));
     if (t == 0) a.scales[row] = s.most / 127.0f;
-    if (!there) {
-      for (int c = t; c < p.chunks; c += THREADS) store_chunk(q, c, cols, u32x2{0u, 0u});
-      continue;
-    }
+    constexpr int WAY = DT == kF32 && !GATED ? kExact : kQuick;
+    if (s.way == WAY) {
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      const int c = t + h * THREADS;
-      if (c < chunks) store_chunk(q, c, cols, round8(held[h], s));
+      for (int h = 0; h < HELD; ++h) {
+        const int c = t + h * THREADS;
+        const u32x2 v = WAY == kExact ? round_exact(held[h], s) : round_quick(held[h], s);
+        if (c < p.chunks) store8(q + min(c * 8, cols - 8), v);
+      }
     }
-    for (int c = t + HELD * THREADS; c < chunks; c += THREADS) store_chunk(q, c, cols, round8(values_of<DT, GATED>(x, c, cols), s));
+#pragma unroll 1
+    for (int c = t + (s.way == WAY ? HELD * THREADS : 0); c < p.chunks; c += THREADS) {
+      Loaded<DT, GATED> more;
+      more.load(source.x, min(c * 8, cols - 8), cols);
+      store8(q + min(c * 8, cols - 8), round_any(more.value(), s));
+    }
+  }
+}
+
+// Rows of fewer than 8, a thread to each.
+template <int DT, bool GATED>
+__global__ __launch_bounds__(256) void quantize_short_kernel(QuantizeParams p) {
+  const QuantizeArgs& a = p.a;
+  const int cols = (int)a.cols;
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
+    const SourceRow source = source_row<DT>(a, row);
+    u32x2 v = {0u, 0u};
+    float scale = 0.0f;
+    if (source.there) {
+      Loaded<DT, GATED> loaded;
+      loaded.load(source.x, 0, cols, cols);
+      const Held<DT, GATED> h = loaded.value();
+      uint32_t most = most_of(h, 0u);
+      if constexpr (!Held<DT, GATED>::FLOATS) most = max(most & 0xffffu, most >> 16);
+      const RowScale s = row_scale<DT, GATED>(most);
+      v = round_any(h, s);
+      scale = s.most / 127.0f;
+    }
+    a.scales[row] = scale;
+    for (int i = 0; i < cols; ++i) a.q[row * cols + i] = (int8_t)(v[i / 4] >> (8 * (i % 4)));
   }
 }
 
@@ -207,6 +333,12 @@ hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
   QuantizeParams p;
   p.a = a;
   p.chunks = (int32_t)((a.cols + 7) / 8);
+  if (a.cols < 8) {
+    hipLaunchKernelGGL((quantize_short_kernel<DT, GATED>), dim3((uint32_t)std::min<int64_t>((a.rows + 255) / 256, 1 << 16)), dim3(256), 0, stream, p);
+    return hipGetLastError();
+  }
+  if (a.rows <= 512 && p.chunks > 256) return p.chunks <= 1024 ? launch_rows<DT, GATED, 1024, 1>(p, stream) : launch_rows<DT, GATED, 1024, 2>(p, stream);
+  if (a.rows <= 2048 && p.chunks > 64 && p.chunks <= 256) return launch_rows<DT, GATED, 256, 1>(p, stream);
   if (p.chunks <= 64) return launch_rows<DT, GATED, 64, 1>(p, stream);
   if (p.chunks <= 128) return launch_rows<DT, GATED, 64, 2>(p, stream);
   if (p.chunks <= 256) return launch_rows<DT, GATED, 64, 4>(p, stream);
