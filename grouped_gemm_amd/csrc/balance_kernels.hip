@@ -69,54 +69,89 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences
   return uniform(low) - 1;
 }
 
-// A token's exponentials, in the lanes of its group: softmax and the score, as multiples of what is common to all.
-template <int DT, int G, int VPL>
-struct Scores {
-  float x[VPL], softmax[VPL], score[VPL];
-  float lse;
+// A token's scores, in the lanes of its group, by one exponential (and, of sigmoids, one reciprocal) to a logit: with E = exp(x - top), softmax is E
+// over its sum, and sigmoid(x) = E / (E + exp(-top)), 1 - sigmoid(x) = exp(-top) / (E + exp(-top)).  Where top is negative both divisors are
+// taken times exp(top), which leaves sigmoids that are all too small for a float their proportions, and the division by their sum takes out
+// again.  Above kFarTop exp(-top) comes near the end of a float's range, and sigmoids are computed by themselves.
+constexpr float kFarTop = 60.0f;
 
-  __device__ __forceinline__ void compute(const Row<typename Logit<DT>::T, VPL>& raw, bool sigmoids) {
+template <int DT, bool SIGMOID, int G, int VPL>
+struct Scores {
+  float e[VPL];                   // exponentials: softmax / of_softmax
+  float s[SIGMOID ? VPL : 1];     // p / of_score (softmax: e),
+  float slope[SIGMOID ? VPL : 1];   // ... and (1 - sigmoid) / of_slope
+  float of_softmax, of_score, of_slope, lse;
+
+  __device__ __forceinline__ float score(int v) const { return SIGMOID ? s[v] : e[v]; }
+
+  __device__ __forceinline__ void compute(const Row<typename Logit<DT>::T, VPL>& raw) {
+    constexpr float LOG2E = 1.44269504f;
     float top = -INFINITY;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      x[v] = Logit<DT>::widen(raw.v[v]);
-      top = fmaxf(top, x[v]);
+      e[v] = Logit<DT>::widen(raw.v[v]);
+      top = fmaxf(top, e[v]);
     }
     top = group_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); });
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    const float base = top == -INFINITY ? 0.0f : top, base2 = base * LOG2E;   // (its rounding is a factor that all share)
+    auto power = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, -base2)); };
+    float sum = 0.0f, all = 0.0f;
+    if constexpr (SIGMOID) {
+      if (__builtin_expect(__any(base > kFarTop), 0)) {
+        of_slope = 1.0f;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      softmax[v] = quick_exp(x[v] - base);
-      sum += softmax[v];
+        for (int v = 0; v < VPL; ++v) {
+          const float x = e[v], least = fminf(base, 0.0f);
+          s[v] = (x >= 0.0f ? 1.0f : quick_exp(x - least)) * __builtin_amdgcn_rcpf(1.0f + quick_exp(-fabsf(x)));
+          slope[v] = quick_sigmoid(-x);
+          e[v] = power(x);
+        }
+      } else {
+        const float less = __builtin_amdgcn_exp2f(-fabsf(base2)), of_e = base < 0.0f ? less : 1.0f;
+        of_slope = base < 0.0f ? 1.0f : less;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+          e[v] = power(e[v]);
+          slope[v] = __builtin_amdgcn_rcpf(__builtin_fmaf(e[v], of_e, of_slope));
+          s[v] = e[v] * slope[v];
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) all += s[v];
+      all = group_sum<G>(all);
+    } else {
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) e[v] = power(e[v]);
     }
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) sum += e[v];
     sum = group_sum<G>(sum);
-    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-    lse = sum == 0.0f ? 0.0f : base + logf(sum);   // (no expert is open to the token: it adds nothing)
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) softmax[v] *= scale;
-    if (!sigmoids) {
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) score[v] = softmax[v];
-      return;
-    }
-    // (of sigmoids that are all too small for a float, what is left of them relative to the largest)
-    const float least = fminf(base, 0.0f);
-    float all = 0.0f;
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      score[v] = (x[v] >= 0.0f ? 1.0f : quick_exp(x[v] - least)) * __builtin_amdgcn_rcpf(1.0f + quick_exp(-fabsf(x[v])));
-      all += score[v];
-    }
-    all = group_sum<G>(all);
-    const float over = all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) score[v] *= over;
+    // (no expert is open to the token: it adds nothing)
+    of_softmax = sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum);
+    lse = sum == 0.0f ? 0.0f : base + logf(sum);
+    of_score = !SIGMOID ? of_softmax : (all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all));
   }
 };
 
+// A token's logits, asked for one turn ahead.
 template <int DT, int G, int VPL>
-__global__ __launch_bounds__(kBalanceThreads) void balance_units_kernel(BalanceParams p) {
+struct NextToken {
+  const void* logits;
+  const uint8_t* mask;
+  int experts, column;
+  Row<typename Logit<DT>::T, VPL> raw;
+  bool counted;
+  __device__ __forceinline__ NextToken(const void* logits_, const uint8_t* mask_, int experts_, int column_)
+      : logits(logits_), mask(mask_), experts(experts_), column(column_) {}
+  __device__ __forceinline__ void ask(int64_t t, int64_t end) {
+    if (t >= end) return;
+    raw = load_logits<DT, VPL>(logits, t, experts, column);
+    counted = mask == nullptr || mask[t] != 0;
+  }
+};
+
+template <int DT, bool SIGMOID, int G, int VPL>
+__global__ __launch_bounds__(kBalanceThreads, 4) void balance_units_kernel(BalanceParams p) {
   constexpr int GROUPS = kBalanceThreads / G, COLUMNS = G * VPL;
   __shared__ float rows[GROUPS * COLUMNS];
   __shared__ int32_t chosen[COLUMNS];
@@ -126,6 +161,9 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_units_kernel(BalanceP
   const int group = threadIdx.x / G, l = threadIdx.x % G, column = l * VPL;
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0;
   const int64_t first = (int64_t)blockIdx.x * p.chunk, last = min(first + p.chunk, a.tokens);
+  // (the first token's logits come while its sequence is looked for; they are asked for again where it begins later)
+  NextToken<DT, G, VPL> next(a.logits, a.mask, a.experts, column);
+  next.ask(first + group, last);
   int64_t at = first;
   for (int s = max(sequence_of(a.offsets, a.sequences, at), 0); s < a.sequences && at < last; ++s) {
     const int64_t begin = max(offset_of(a.offsets, a.tokens, s), at), end = min(offset_of(a.offsets, a.tokens, s + 1), last);
@@ -143,12 +181,16 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_units_kernel(BalanceP
     int32_t tokens = 0;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) mass[v] = 0.0f;
+    if (begin != first) next.ask(begin + group, end);
     for (int64_t t = begin + group; t < end; t += GROUPS) {
-      if (a.mask != nullptr && a.mask[t] == 0) continue;
-      Scores<DT, G, VPL> scores;
-      scores.compute(load_logits<DT, VPL>(a.logits, t, a.experts, column), a.sigmoid);
+      const auto raw = next.raw;
+      const bool counted = next.counted;
+      next.ask(t + GROUPS, end);
+      if (!counted) continue;
+      Scores<DT, SIGMOID, G, VPL> scores;
+      scores.compute(raw);
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) mass[v] += scores.score[v];
+      for (int v = 0; v < VPL; ++v) mass[v] = __builtin_fmaf(scores.score(v), scores.of_score, mass[v]);
       z += scores.lse * scores.lse;
       ++tokens;
     }
@@ -213,8 +255,20 @@ __global__ __launch_bounds__(THREADS) void balance_sums_kernel(BalanceParams p) 
     const int64_t from = begin / p.chunk + s, to = begin < end ? (end - 1) / p.chunk + s + 1 : from;   // units
     float mass = 0.0f, z = 0.0f;
     int32_t count = 0, tokens = 0;
-    if (e < a.experts) {
-      for (int64_t u = from + wave; u < to; u += WAVES) mass += p.mass[u * a.experts + e], count += p.counts[u * a.experts + e];
+    if (e < a.experts && from < to) {
+      constexpr int IN_FLIGHT = 8;
+      for (int64_t u = from + wave; u < to; u += IN_FLIGHT * WAVES) {
+        float m[IN_FLIGHT];
+        int32_t n[IN_FLIGHT];
+#pragma unroll
+        for (int f = 0; f < IN_FLIGHT; ++f) {
+          const int64_t at = min(u + f * WAVES, to - 1) * a.experts + e;
+          m[f] = p.mass[at], n[f] = p.counts[at];
+        }
+#pragma unroll
+        for (int f = 0; f < IN_FLIGHT; ++f)
+          if (u + f * WAVES < to) mass += m[f], count += n[f];
+      }
     }
     for (int64_t u = from + threadIdx.x; u < to; u += THREADS) z += p.z[u], tokens += p.tokens[u];
     mass_of[wave][lane] = mass, count_of[wave][lane] = count;
@@ -260,13 +314,51 @@ __global__ __launch_bounds__(THREADS) void balance_sums_kernel(BalanceParams p) 
   }
 }
 
-// The gradient, one pass: workgroups take neighbouring tokens, a sequence's shares stay in registers.
-template <int DT, int G, int VPL>
-__global__ __launch_bounds__(kBalanceThreads) void balance_backward_kernel(BalanceBackwardArgs a, int chunk) {
+// VPL neighbouring results to any element of a row, the last lane's only as far as the row goes.  (In words: element by element each would be a
+// store of its own, 16 in place of 2 for 256 experts, bf16: 27 us instead of 25 for 65536 tokens.)
+template <int DT, int VPL>
+__device__ __forceinline__ void store_logits(void* logits, int64_t token, int experts, int column, const float (&value)[VPL]) {
   using T = typename Logit<DT>::T;
+  constexpr int WORDS = VPL * (int)sizeof(T) / 4;
+  T* to = static_cast<T*>(logits) + token * experts + column;
+  if (column + VPL <= experts) {
+    using Words = __attribute__((ext_vector_type(WORDS < 4 ? WORDS : 4))) uint32_t;
+    struct __attribute__((packed, aligned(sizeof(T)))) Packed {
+      Words v;
+    };
+    uint32_t word[WORDS];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) word[w] = Logit<DT>::narrow(value[w]);
+    } else {
+#pragma unroll
+      for (int w = 0; w < WORDS; w += 2) {
+        const u32x2 four = round4<DT>(value[2 * w], value[2 * w + 1], value[2 * w + 2], value[2 * w + 3]);
+        word[w] = four[0], word[w + 1] = four[1];
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < WORDS; w += 4) {
+      Words v;
+#pragma unroll
+      for (int i = 0; i < (WORDS < 4 ? WORDS : 4); ++i) v[i] = word[w + i];
+      reinterpret_cast<Packed*>(reinterpret_cast<uint32_t*>(to) + w)->v = v;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (column + v < experts) to[v] = Logit<DT>::narrow(value[v]);
+  }
+}
+
+// The gradient, one pass: workgroups take neighbouring tokens, a sequence's shares stay in registers.
+template <int DT, bool SIGMOID, int G, int VPL>
+__global__ __launch_bounds__(kBalanceThreads, 4) void balance_backward_kernel(BalanceBackwardArgs a, int chunk) {
   constexpr int GROUPS = kBalanceThreads / G;
   const int group = threadIdx.x / G, l = threadIdx.x % G, column = l * VPL;
   const int64_t first = (int64_t)blockIdx.x * chunk, last = min(first + chunk, a.tokens);
+  NextToken<DT, G, VPL> next(a.logits, a.mask, a.experts, column);
+  next.ask(first + group, last);
   const float inverse = *a.inverse;
   const float of_balance = a.balance_grad != nullptr ? *a.balance_grad * inverse : 0.0f, of_z = a.z_grad != nullptr ? *a.z_grad * 2.0f * inverse : 0.0f;
   int s = sequence_of(a.offsets, a.sequences, first), held = -1;   // `held`: whose shares are here
@@ -275,41 +367,41 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_backward_kernel(Balan
   if (s >= a.sequences) begin = end = a.tokens;
   float share[VPL];
   for (int64_t t = first + group; t < last; t += GROUPS) {
+    const auto raw = next.raw;
+    const bool counted = next.counted;
+    next.ask(t + GROUPS, last);
     while (t >= end && s + 1 < a.sequences) {
       ++s;
       begin = offset_of(a.offsets, a.tokens, s), end = offset_of(a.offsets, a.tokens, s + 1);
     }
-    Row<T, VPL> out;
-    if (t < begin || t >= end || (a.mask != nullptr && a.mask[t] == 0)) {   // (not counted)
+    float grad[VPL];
+    if (t < begin || t >= end || !counted) {
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) out.v[v] = Logit<DT>::narrow(0.0f);
+      for (int v = 0; v < VPL; ++v) grad[v] = 0.0f;
     } else {
       if (held != s) {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) share[v] = column + v < a.experts ? a.share[(int64_t)s * a.experts + column + v] : 0.0f;
         held = s;
       }
-      Scores<DT, G, VPL> scores;
-      scores.compute(load_logits<DT, VPL>(a.logits, t, a.experts, column), a.sigmoid);
+      Scores<DT, SIGMOID, G, VPL> scores;
+      scores.compute(raw);
       float dot = 0.0f;
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) dot += scores.score[v] * share[v];
-      dot = group_sum<G>(dot);
-      const float of_softmax = of_z * scores.lse;
+      for (int v = 0; v < VPL; ++v) dot = __builtin_fmaf(scores.score(v), share[v], dot);
+      dot = group_sum<G>(dot) * scores.of_score;
+      const float of_score = of_balance * scores.of_score, of_softmax = of_z * scores.lse * scores.of_softmax;
+      if constexpr (SIGMOID) {
+        const float factor = of_score * scores.of_slope, rest = -dot * factor;
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const float slope = a.sigmoid ? quick_sigmoid(-scores.x[v]) : 1.0f;
-        out.v[v] = Logit<DT>::narrow(of_balance * scores.score[v] * slope * (share[v] - dot) + of_softmax * scores.softmax[v]);
+        for (int v = 0; v < VPL; ++v)
+          grad[v] = __builtin_fmaf(scores.s[v] * scores.slope[v], __builtin_fmaf(share[v], factor, rest), of_softmax * scores.e[v]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) grad[v] = scores.e[v] * __builtin_fmaf(share[v] - dot, of_score, of_softmax);
       }
     }
-    T* to = static_cast<T*>(a.logits_grad) + t * a.experts + column;
-    if (column + VPL <= a.experts) {
-      *reinterpret_cast<Row<T, VPL>*>(to) = out;
-    } else {
-#pragma unroll
-      for (int v = 0; v < VPL; ++v)
-        if (column + v < a.experts) to[v] = out.v[v];
-    }
+    store_logits<DT, VPL>(a.logits_grad, t, a.experts, column, grad);
   }
 }
 
@@ -343,7 +435,7 @@ BalanceScratch scratch_of(int64_t tokens, int64_t experts, int64_t sequences) {
   return b;
 }
 
-template <int DT, int G, int VPL>
+template <int DT, bool SIGMOID, int G, int VPL>
 hipError_t launch_balance(const BalanceArgs& a, hipStream_t stream) {
   const BalanceScratch b = scratch_of(a.tokens, a.experts, a.sequences);
   char* at = static_cast<char*>(a.scratch);
@@ -358,11 +450,11 @@ hipError_t launch_balance(const BalanceArgs& a, hipStream_t stream) {
   p.sequence_tokens = reinterpret_cast<int32_t*>(at + b.sequence_tokens);
   // (without tokens the first kernel still clears the counter)
   const int64_t chunks = std::max<int64_t>(1, (a.tokens + p.chunk - 1) / p.chunk);
-  hipLaunchKernelGGL((balance_units_kernel<DT, G, VPL>), dim3((uint32_t)chunks), dim3(kBalanceThreads), 0, stream, p);
+  hipLaunchKernelGGL((balance_units_kernel<DT, SIGMOID, G, VPL>), dim3((uint32_t)chunks), dim3(kBalanceThreads), 0, stream, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const uint32_t blocks = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(a.sequences * b.tiles, 2048));
-  if (chunks > 8 * a.sequences) {
+  if (chunks > 64 * a.sequences) {
     hipLaunchKernelGGL(balance_sums_kernel<1024>, dim3(blocks), dim3(1024), 0, stream, p);
   } else {
     hipLaunchKernelGGL(balance_sums_kernel<256>, dim3(blocks), dim3(256), 0, stream, p);
@@ -370,10 +462,10 @@ hipError_t launch_balance(const BalanceArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int DT, int G, int VPL>
+template <int DT, bool SIGMOID, int G, int VPL>
 hipError_t launch_balance_backward(const BalanceBackwardArgs& a, hipStream_t stream) {
   const int64_t chunk = chunk_of(a.tokens, a.experts);
-  hipLaunchKernelGGL((balance_backward_kernel<DT, G, VPL>), dim3((uint32_t)((a.tokens + chunk - 1) / chunk)), dim3(kBalanceThreads), 0, stream, a, (int)chunk);
+  hipLaunchKernelGGL((balance_backward_kernel<DT, SIGMOID, G, VPL>), dim3((uint32_t)((a.tokens + chunk - 1) / chunk)), dim3(kBalanceThreads), 0, stream, a, (int)chunk);
   return hipGetLastError();
 }
 
@@ -381,25 +473,29 @@ hipError_t launch_balance_backward(const BalanceBackwardArgs& a, hipStream_t str
 
 uint64_t balance_scratch_bytes(int64_t tokens, int64_t experts, int64_t sequences) { return scratch_of(tokens, experts, sequences).bytes; }
 
-#define GG_BY_EXPERTS(DT, launch, a, stream)                          \
-  do {                                                                \
-    if ((a).experts <= 64) return launch<DT, 16, 4>(a, stream);       \
-    if ((a).experts <= 128) return launch<DT, 16, 8>(a, stream);      \
-    if ((a).experts <= 256) return launch<DT, 16, 16>(a, stream);     \
-    if ((a).experts <= 512) return launch<DT, 64, 8>(a, stream);      \
-    return launch<DT, 64, 16>(a, stream);                             \
+#define GG_BY_EXPERTS(DT, SIGMOID, launch, a, stream)                   \
+  do {                                                                  \
+    if ((a).experts <= 64) return launch<DT, SIGMOID, 16, 4>(a, stream);     \
+    if ((a).experts <= 128) return launch<DT, SIGMOID, 16, 8>(a, stream);    \
+    if ((a).experts <= 256) return launch<DT, SIGMOID, 16, 16>(a, stream);   \
+    if ((a).experts <= 512) return launch<DT, SIGMOID, 64, 8>(a, stream);    \
+    return launch<DT, SIGMOID, 64, 16>(a, stream);                           \
+  } while (0)
+#define GG_BY_TYPE(SIGMOID, launch, a, stream)                              \
+  do {                                                                      \
+    if ((a).dt == kF32) GG_BY_EXPERTS(kF32, SIGMOID, launch, a, stream);    \
+    if ((a).dt == kBF16) GG_BY_EXPERTS(kBF16, SIGMOID, launch, a, stream);  \
+    GG_BY_EXPERTS(kF16, SIGMOID, launch, a, stream);                        \
   } while (0)
 
 hipError_t balance(const BalanceArgs& a, hipStream_t stream) {
-  if (a.dt == kF32) GG_BY_EXPERTS(kF32, launch_balance, a, stream);
-  if (a.dt == kBF16) GG_BY_EXPERTS(kBF16, launch_balance, a, stream);
-  GG_BY_EXPERTS(kF16, launch_balance, a, stream);
+  if (a.sigmoid) GG_BY_TYPE(true, launch_balance, a, stream);
+  GG_BY_TYPE(false, launch_balance, a, stream);
 }
 
 hipError_t balance_backward(const BalanceBackwardArgs& a, hipStream_t stream) {
-  if (a.dt == kF32) GG_BY_EXPERTS(kF32, launch_balance_backward, a, stream);
-  if (a.dt == kBF16) GG_BY_EXPERTS(kBF16, launch_balance_backward, a, stream);
-  GG_BY_EXPERTS(kF16, launch_balance_backward, a, stream);
+  if (a.sigmoid) GG_BY_TYPE(true, launch_balance_backward, a, stream);
+  GG_BY_TYPE(false, launch_balance_backward, a, stream);
 }
 
 }  // namespace gg
