@@ -323,6 +323,16 @@ Route strided_route(const gg_gmm_args& g) {
   return r;
 }
 
+// gg_gmm_int8 on the streaming kernels: as fp8 (whose tiles, schedule and workspace are the same), whatever c's width and address.
+Route int8_route(const gg_gmm_args& g) {
+  gg_gmm_args aligned = g;
+  aligned.hidden_out = (g.hidden_out + 7) / 8 * 8;
+  aligned.c = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(g.c) + 15) / 16 * 16);
+  Route r = classify(aligned);
+  r.address_bits = (r.address_bits & ~(uintptr_t)15) | (reinterpret_cast<uintptr_t>(g.c) & 15);
+  return r;
+}
+
 // Rows of a, b and c in memory, the bounds a row index is held against: an index that names no
 // row is a missing row (zeros on the way in, nothing stored on the way out) on every kernel.
 struct IndexedRows {
@@ -468,8 +478,9 @@ struct Plan {
 // gate_up: where gate | up are kept beside c (SwiGLU epilogue), or nullptr.
 // strides: where rows of a and b are further apart than they are long (gg_gmm_strided).
 // assumed: a device to plan for instead of the current one.
+// int8: a call of gg_gmm_int8, described as one on fp8.
 int plan_call(const gg_gmm_args& g, bool static_scratch, Plan* out, void* gate_up = nullptr, const Strides* strides = nullptr,
-              const DeviceInfo* assumed = nullptr) {
+              const DeviceInfo* assumed = nullptr, bool int8 = false) {
   const int64_t num_groups = g.num_groups, tokens = g.tokens;
   const int64_t hidden_in = g.hidden_in, hidden_out = g.hidden_out;
   const int trans_a = g.trans_a != 0, trans_b = g.trans_b != 0;
@@ -501,7 +512,7 @@ int plan_call(const gg_gmm_args& g, bool static_scratch, Plan* out, void* gate_u
   if (g.c == nullptr) return fail(GG_EINVAL, "c is null");
   if (tokens > 0 && (g.a == nullptr || g.b == nullptr)) return fail(GG_EINVAL, "a or b is null");
   if (strides != nullptr && !strides_fit(g, *strides)) return fail(GG_EINVAL, "row strides do not fit the call (gg_gmm_strided)");
-  const Route route = strides != nullptr ? strided_route(g) : classify(g);
+  const Route route = int8 ? int8_route(g) : (strides != nullptr ? strided_route(g) : classify(g));
   const uintptr_t address_bits = route.address_bits;
   if (address_bits & (uintptr_t)(elem_bytes - 1) || reinterpret_cast<uintptr_t>(g.c) & (out_f32 ? 3 : 1))
     return fail(GG_ELIMIT, "a, b and c must be aligned to their element size");
@@ -573,7 +584,7 @@ int plan_call(const gg_gmm_args& g, bool static_scratch, Plan* out, void* gate_u
   p.flags = g.flags & (GG_FLAG_WHOLE_TILES | GG_FLAG_ONE_CLASS | GG_FLAG_ROW_PIECES | GG_FLAG_GROUP_ORDER);
   if (merge_stores(g)) p.flags |= gg::kFlagMergeStores;
   if (trans_a && (g.flags & GG_FLAG_FEW_TILES)) p.flags |= gg::kFlagPiecesByLength;
-  if (strides != nullptr && (hidden_out % 8 != 0 || (reinterpret_cast<uintptr_t>(g.c) & 15))) p.flags |= gg::kFlagAnyRows;
+  if ((strides != nullptr || int8) && (hidden_out % 8 != 0 || (reinterpret_cast<uintptr_t>(g.c) & 15))) p.flags |= gg::kFlagAnyRows;
   const bool depth_pieces = !generic && may_cut_depth(g, route, shape);
   p.sched_out = nullptr;
   if (static_scratch) {
@@ -786,7 +797,7 @@ int run_pair(const gg_gmm_args* first, const Strides* strides1, const gg_gmm_arg
 
 // ---- products of 8-bit integers (gg_gmm_int8)
 
-constexpr int64_t kInt8MostDepth = 131071;   // 128 * 128 * depth below 2^31: no sum overflows
+static_assert(int64_t(128) * 128 * GG_INT8_MAX_DEPTH < (int64_t(1) << 31), "no sum overflows");
 // Average rows to a group up to which a call goes to the kernel for few rows, which reads weights faster (it needs no tiles in LDS) but again
 // for every 16 to 64 rows.  us, streaming tiles / few rows, by rows to a group: 8 groups, 4096 -> 14336: 4 110 / 88, 16 111 / 93, 24 111 / 105, 32 111 / 122;
 // 8, 1024 -> 1024: 4 8.4 / 6.1, 24 8.4 / 8.2, 32 8.6 / 9.6; 32, 4096 -> 4096: 4 113 / 98, 16 118 / 105, 32 119 / 126; 64, 7168 -> 2048: 4 158 / 155,
@@ -804,7 +815,7 @@ int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_sc
   if (g.trans_a || !g.trans_b) return fail(GG_EINVAL, "8-bit integers come with b stored transposed (trans_b, not trans_a)");
   if (g.epilogue != GG_EPILOGUE_NONE || g.accumulate_f32 || g.a_row_index || g.b_row_index || g.c_row_index)
     return fail(GG_EINVAL, "8-bit integers have neither an epilogue, an fp32 c nor row indices");
-  if (g.hidden_in > kInt8MostDepth) return fail(GG_ELIMIT, "hidden_in of 8-bit integers must be at most %lld", (long long)kInt8MostDepth);
+  if (g.hidden_in > GG_INT8_MAX_DEPTH) return fail(GG_ELIMIT, "hidden_in of 8-bit integers must be at most %d", GG_INT8_MAX_DEPTH);
   if (g.num_groups == 0 || g.tokens == 0 || g.hidden_out == 0) return GG_OK;
   if (g.c == nullptr || a_scales == nullptr || b_scales == nullptr) return fail(GG_EINVAL, "c, a_scales or b_scales is null");
   if (g.hidden_in > 0 && (g.a == nullptr || g.b == nullptr)) return fail(GG_EINVAL, "a or b is null");
@@ -816,11 +827,10 @@ int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_sc
 }
 
 bool int8_streams(const gg_gmm_args& g) {
-  return g.tokens > int8_few_rows(g.num_groups) * g.num_groups && g.hidden_in > 0 && g.hidden_in % 16 == 0 && g.hidden_out % 8 == 0 &&
-         ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | reinterpret_cast<uintptr_t>(g.c)) & 15) == 0;
+  return g.tokens > int8_few_rows(g.num_groups) * g.num_groups && g.hidden_in > 0 && g.hidden_in % 16 == 0 &&
+         ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b)) & 15) == 0;
 }
 
-// The same call on fp8 operands, whose tiles, schedule and workspace those of 8-bit integers are.
 gg_gmm_args int8_as_fp8(const gg_gmm_args& g) {
   gg_gmm_args f = g;
   f.dtype = GG_DTYPE_F8E4M3;
@@ -861,7 +871,7 @@ int int8_by_rows(const gg_gmm_args& g, const float* a_scales, const float* b_sca
 int int8_by_tiles(const gg_gmm_args& g, const float* a_scales, const float* b_scales) {
   const gg_gmm_args f = int8_as_fp8(g);
   Plan plan;
-  const int rc = plan_call(f, false, &plan);
+  const int rc = plan_call(f, false, &plan, nullptr, nullptr, nullptr, /*int8=*/true);
   if (rc != GG_OK || plan.empty) return rc;
   plan.variant = find_variant(g.dtype == GG_DTYPE_F16 ? gg::kI8ToF16 : gg::kI8, plan.layout, plan.shape.id, gg::kEpiStore, 0);
   if (plan.variant == nullptr) return fail(GG_EINVAL, "no kernel for this combination of arguments");
@@ -914,7 +924,8 @@ uint64_t gg_gmm_int8_workspace_bytes(const gg_gmm_args* args) {
     return 0;
   if (int8_streams(*args)) {
     const gg_gmm_args f = int8_as_fp8(*args);
-    return gg_workspace_bytes_for(&f);
+    const Route r = int8_route(f);
+    return may_cut_depth(f, r, pick_shape(f, r)) ? GG_WORKSPACE_BYTES : 0;
   }
   const int64_t groups = std::min<int64_t>(args->num_groups, GG_MAX_GROUPS_PER_LAUNCH);
   return gg::int8_rows_in_pieces(args->tokens, groups, args->hidden_in, args->hidden_out) ? GG_WORKSPACE_BYTES : 0;

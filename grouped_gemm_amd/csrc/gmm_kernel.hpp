@@ -2088,11 +2088,11 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   // copy of them costs a pass more than the product's own): whole chunks at once, which global memory takes on
   // any boundary, the last ones of a row by elements.  8 x 1024 rows, 2047 -> 5461, forward and gradients: 834 us with
   // padded results copied back (120 of them the copies), 760 so.
-  constexpr bool ANY_ROWS = EPI == kEpiStore && !INDEXED && !RAGGED_DEPTH && !F8 && !I8;
+  constexpr bool ANY_ROWS = EPI == kEpiStore && !INDEXED && !RAGGED_DEPTH && (!F8 || I8);
   // ... or that are no whole groups of 4 columns, which the fix-up of depth pieces stores (whole tiles / pieces, us: weight
   // gradients of 21 Zipf (1.2) groups, 51204 rows, 128 x 558: 125 / 38; 64, 49152 rows, 2046 x 1406: 492 / 364; 16 groups, 600 rows,
   // 6144 -> 518: 46.8 / 33.8).
-  constexpr bool FIX_ANY_ROWS = EPI == kEpiStore && !INDEXED && !F8 && !I8;
+  constexpr bool FIX_ANY_ROWS = EPI == kEpiStore && !INDEXED && (!F8 || I8);
   auto store_any = [&](const TileInfo& tile, uint32_t row_off, int col, int most, u32x4 v) {
     struct Chunk {
       u32x4 v;
@@ -2184,7 +2184,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
         if constexpr (I8) {
           int sum;
           asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(sum) : "a"(x));
-          v[r] = (float)sum * row_scale[i][q / 2] * column_scale[r];
+          v[r] = (float)sum * column_scale[r] * row_scale[i][q / 2];
         } else if constexpr (F8 || (MB * NB > 4 && !TIED)) {
           asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[r]) : "a"(x));
         } else {
@@ -2682,8 +2682,13 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
               const float* of_columns = p.b_scales + (int64_t)uniform(words[23]) * p.hidden_out + col;
               float v[4];
 #pragma unroll
-              for (int r = 0; r < 4; ++r) v[r] = (float)sum[j][q][r] * of_row * (col < ft.g.n ? of_columns[r] : 0.0f);
-              __builtin_amdgcn_raw_buffer_store_b64(round4<OUT_DT>(v[0], v[1], v[2], v[3]), rc, off, 0, kStoreMerging);
+              for (int r = 0; r < 4; ++r) v[r] = (float)sum[j][q][r] * (col + r < ft.g.n ? of_columns[r] : 0.0f) * of_row;
+              const u32x2 rounded = round4<OUT_DT>(v[0], v[1], v[2], v[3]);
+              if ((p.flags & kFlagAnyRows) != 0) {
+                store_any(ft, row_off, col, 4, u32x4{rounded[0], rounded[1], 0u, 0u});
+              } else {
+                __builtin_amdgcn_raw_buffer_store_b64(rounded, rc, off, 0, kStoreMerging);
+              }
             } else if (FIX_ANY_ROWS && ((p.flags & kFlagAnyRows) != 0 || uniform(ft.g.n & 3) != 0)) {
               const u32x2 v = round4<OUT_DT>(sum[j][q][0], sum[j][q][1], sum[j][q][2], sum[j][q][3]);
               store_any(ft, row_off, col, 4, u32x4{v[0], v[1], 0u, 0u});

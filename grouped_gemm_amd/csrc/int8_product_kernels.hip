@@ -2,7 +2,8 @@
 //
 //   c[r, n] = a_scales[r] * b_scales[e, n] * sum over k of a[r, k] * b[e, n, k],   e the group of row r
 //
-// The sums are exact (in 32 bits, up to a depth of 131071), so that neither the order nor the pieces they are made in matter.
+// The sums are exact (in 32 bits, up to a depth of 131071), so that neither the order nor the pieces they are made in matter.  They are scaled by
+// the column's first: weights have scales of ordinary size, and where a row's is very large or small nothing in between leaves a float's range.
 //
 // Few rows are bound by reading b once.  A workgroup has a strip of 64 columns of a group's b, over the whole depth or a piece of it, and a
 // window of up to 16, 32 or 64 of its rows; its four waves take the depth in turns, 128 deep at a time, each with its own loads from HBM
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void int8_rows_kernel
   s.run(wave, (int)((int64_t)steps * piece / p.pieces), (int)((int64_t)steps * (piece + 1) / p.pieces));
   const float* of_columns = a.b_scales + (int64_t)at.group * a.hidden_out + column0;
   auto store = [&](int row, int column, int sum) {
-    const float v = (float)sum * a.a_scales[row0 + row] * of_columns[column];
+    const float v = (float)sum * of_columns[column] * a.a_scales[row0 + row];
     static_cast<uint16_t*>(a.c)[(int64_t)(row0 + row) * a.hidden_out + column0 + column] =
         a.to_f16 ? round_bits<kF16>(v) : round_bits<kBF16>(v);
   };
@@ -388,11 +389,15 @@ constexpr int64_t kInt8Units = 256;   // compute units
 Int8Plan int8_plan(int64_t tokens, int64_t num_groups, int64_t hidden_in, int64_t hidden_out, uint64_t workspace_bytes) {
   Int8Plan f;
   const int64_t named = std::max<int64_t>(1, std::min(tokens, num_groups));
-  f.rows_of_window = tokens <= 8 * named ? 1 : (tokens <= 24 * named ? 2 : 4);
-  const int64_t window = 16 * f.rows_of_window;
-  f.windows = tokens / window + named;
-  if (tokens <= named) f.windows = tokens;
   f.strips = (hidden_out + kStrip - 1) / kStrip;
+  // Rows of a window by how many a group has on average (those that do not fit read the strip again), and fewer where such windows leave compute units.
+  // us with 16, 32 and 64: 8 rows to a group (8 groups, 4096 -> 4096) 23, 24, 25; 16 31, 25, 27; 31 (64, 1023 -> 1407) 55, 46, 45; 375 (8, 2047 -> 1023)
+  // 80, 60, 54; 67 (5, 2047 -> 1023: 368, 240 and 160 workgroups) 17, 14, 19; 13 (8, 1021 -> 513: 129, 99) 7.4, 8.0, 8.4.
+  f.rows_of_window = tokens <= 8 * named ? 1 : (tokens <= 24 * named ? 2 : 4);
+  auto windows = [&] { return tokens <= named ? tokens : tokens / (16 * f.rows_of_window) + named; };
+  while (f.rows_of_window > 1 && windows() * f.strips < kInt8Units * 3 / 4) f.rows_of_window /= 2;
+  const int64_t window = 16 * f.rows_of_window;
+  f.windows = windows();
   const int64_t steps = (hidden_in + kStep - 1) / kStep, fit = 2 * kInt8Units / (f.windows * f.strips), deep = steps / (4 * kFewWaves);
   f.pieces = std::max<int64_t>(1, std::min({fit, deep, int64_t(16)}));
   const uint64_t need = kWsCounterBytes + (uint64_t)f.windows * f.strips * f.pieces * window * kStrip * 4;

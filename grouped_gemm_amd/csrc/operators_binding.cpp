@@ -416,6 +416,8 @@ std::tuple<torch::Tensor, torch::Tensor> SwigluQuantize(const torch::Tensor& gat
   return {q, scales};
 }
 
+constexpr int64_t kInt8PadRows = 128;   // average rows to a group
+
 torch::Tensor GmmInt8(const torch::Tensor& a, const torch::Tensor& a_scales, const torch::Tensor& b, const torch::Tensor& b_scales,
                       const torch::Tensor& batch_sizes, bool to_f16, const c10::optional<torch::Tensor>& c) {
   TORCH_CHECK(a.dim() == 2 && a.scalar_type() == torch::kInt8, "grouped_gemm: a must be int8 (tokens, hidden_in)");
@@ -447,18 +449,34 @@ torch::Tensor GmmInt8(const torch::Tensor& a, const torch::Tensor& a_scales, con
   c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
   torch::Tensor out = to.defined() ? to : torch::empty({tokens, hidden_out}, a.options().dtype(type));
   TORCH_CHECK(gg_init() == GG_OK, "grouped_gemm: ", gg_last_error());
+  torch::Tensor lhs = a, rhs = b;
+  int64_t depth = hidden_in;
+  // Rows that do not begin on boundaries of 16 bytes are read by the kernel for few rows, at a third of the streaming kernel's rate; with this many
+  // of them it pays to lay them out again, with zeros behind.  us, padded / as they are, by rows to a group: 8 groups,
+  // 2047 -> 1023: 64 27 / 19, 128 27 / 29, 256 31 / 48, 1024 53 / 117; 8, 4095 -> 4097: 96 95 / 97, 128 93 / 123, 1024 223 / 686; 64, 2047 -> 1407: 64 127 /
+  // 117, 128 143 / 179; 32, 4095 -> 2047: 96 209 / 181, 128 214 / 241; 8, 1021 -> 1021: 128 23 / 19, 256 24 / 30.
+  const bool aligned = hidden_in % 16 == 0 && ((reinterpret_cast<uintptr_t>(a.data_ptr()) | reinterpret_cast<uintptr_t>(b.data_ptr())) & 15) == 0;
+  const int64_t padded = (hidden_in + 15) / 16 * 16;
+  if (!aligned && tokens >= kInt8PadRows * experts && hidden_in > 0 && hidden_out > 0 && padded <= GG_INT8_MAX_DEPTH) {
+    depth = padded;
+    lhs = torch::empty({tokens, depth}, a.options());
+    rhs = torch::empty({experts, hidden_out, depth}, a.options());
+    int rc = gg_pad_rows(a.data_ptr(), lhs.data_ptr(), 1, tokens, hidden_in, tokens, depth, 1, CurrentStream(a.device()));
+    if (rc == GG_OK) rc = gg_pad_rows(b.data_ptr(), rhs.data_ptr(), 1, experts * hidden_out, hidden_in, experts * hidden_out, depth, 1, CurrentStream(a.device()));
+    TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
+  }
   gg_gmm_args g = {};
   g.struct_bytes = sizeof(g);
   g.dtype = to_f16 ? GG_DTYPE_F16 : GG_DTYPE_BF16;
-  g.a = a.data_ptr();
-  g.b = b.data_ptr();
+  g.a = lhs.data_ptr();
+  g.b = rhs.data_ptr();
   g.c = out.data_ptr();
   g.batch_sizes = sizes.data_ptr<int64_t>();
   g.batch_sizes_on_device = sizes.is_cuda() ? 1 : 0;
   g.trans_b = 1;
   g.num_groups = experts;
   g.tokens = tokens;
-  g.hidden_in = hidden_in;
+  g.hidden_in = depth;
   g.hidden_out = hidden_out;
   g.stream = CurrentStream(a.device());
   if (sizes.is_cuda()) g.size_status = CallSizeStatusWord();

@@ -223,7 +223,9 @@ def _product(a, a_scales, b, b_scales, sizes):
 def _check_close(got, want, dtype, what):
     half, least = ROUNDING[dtype]
     got = got.double().cpu()
-    held = ~torch.isnan(want)
+    beyond = want.abs() > (1 + half) * torch.finfo(dtype).max   # (more than the type holds: an infinity of its sign)
+    assert torch.equal(got[beyond], torch.sign(want[beyond]) * INF), what
+    held = ~torch.isnan(want) & ~beyond
     off = (got - want).abs()[held] - ((half + 3 * 2.0 ** -24) * want.abs()[held] + least)
     assert off.numel() == 0 or float(off.max()) <= 0, (what, float(off.max()))
 
@@ -243,6 +245,9 @@ SIZES = [
     ([40] * 24, 112, 136), ([1500, 1700], 16, 256), ([700], 16384, 128), ([1024, 1024, 1024, 1024], 1408, 2816),
     # ... that the streaming kernel does not take
     ([300, 150], 250, 130), ([500], 513, 1001), ([333, 0, 400], 2047, 263),
+    # ... and of any width, whole tiles and pieces of the depth
+    ([300, 700, 5], 512, 1021), ([100, 60, 0, 130], 256, 263), ([700], 16384, 121), ([513], 4096, 9), ([2000, 48, 1000], 2048, 2047), ([40] * 24, 112, 129),
+    ([257, 300], 4112, 1), ([600], 8192, 514),
 ]
 
 
@@ -257,3 +262,217 @@ def test_products_are_exact_sums_rounded_once(ops, dtype, sizes, hidden_in, hidd
     assert got[0].dtype == dtype and got[0].shape == (rows, hidden_out)
     _check_close(got[0], want, dtype, (sizes, hidden_in, hidden_out))
     assert torch.equal(got[0], got[1])
+
+
+def _misaligned(t, elements):
+    """A contiguous copy that begins `elements` behind a boundary."""
+    buffer = torch.empty(t.numel() + 64, dtype=t.dtype, device="cuda")
+    view = buffer[elements:elements + t.numel()].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("sizes,hidden_in,hidden_out", [([5, 1], 256, 70), ([3, 20], 1024, 64), ([300, 200], 512, 264), ([700], 1040, 128), ([90, 40], 30, 33)])
+def test_operands_on_any_boundary(ops, sizes, hidden_in, hidden_out):
+    _announce("boundaries", sizes, hidden_in, hidden_out)
+    rows = sum(sizes)
+    a, sa, b, sb = _operands(rows, len(sizes), hidden_in, hidden_out, 7)
+    want = _product(a, sa, b, sb, sizes)
+    batch_sizes = torch.tensor(sizes).cuda()
+    for off_a, off_b, off_c in ((1, 0, 0), (0, 3, 1), (2, 2, 2), (5, 15, 3), (8, 4, 4), (0, 0, 1)):
+        buffer = torch.full((rows * hidden_out + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+        c = buffer[off_c:off_c + rows * hidden_out].view(rows, hidden_out)
+        out = ops.gmm_int8(_misaligned(a, off_a), _misaligned(sa, 1), _misaligned(b, off_b), _misaligned(sb, 3), batch_sizes, c=c)
+        assert out.data_ptr() == c.data_ptr()
+        _check_close(out, want, torch.bfloat16, (off_a, off_b, off_c))
+        assert (buffer[:off_c] == 7).all() and (buffer[off_c + rows * hidden_out:] == 7).all()
+
+
+@pytest.mark.parametrize("hidden_in,hidden_out", [(64, 64), (256, 1024), (63, 65), (4096, 128)])
+@pytest.mark.parametrize("sizes", [[3, 0, 2], [40, 30, 0, 7], [300, 200, 100], [2000]])
+def test_rows_behind_the_last_group_keep_what_they_hold(ops, sizes, hidden_in, hidden_out):
+    _announce("behind", sizes, hidden_in, hidden_out)
+    rows = sum(sizes) + 37
+    a, sa, b, sb = _operands(rows, len(sizes), hidden_in, hidden_out, 9)
+    want = _product(a, sa, b, sb, sizes)
+    for on_device in (True, False):
+        c = torch.full((rows, hidden_out), 3.0, dtype=torch.float16, device="cuda")
+        out = _run(ops, a, sa, b, sb, sizes, torch.float16, on_device, c=c)
+        _check_close(out, want, torch.float16, sizes)
+        assert (c[sum(sizes):] == 3).all()
+
+
+def test_largest_sums(ops):
+    """-128 * -128 over the largest depth, and just below zero; and the scales' own range."""
+    depth = 131071
+    a = torch.full((3, depth), -128, dtype=torch.int8)
+    a[1] = 127
+    b = torch.full((2, 9, depth), -128, dtype=torch.int8)
+    sa, sb = torch.tensor([1.0, 2.0 ** -100, 2.0 ** 100]), torch.full((2, 9), 1.0)
+    sb[1] = 2.0 ** -30
+    for sizes in ([2, 1], [0, 3], [3, 0]):
+        _check_close(_run(ops, a, sa, b, sb, sizes, torch.bfloat16, True), _product(a, sa, b, sb, sizes), torch.bfloat16, sizes)
+    a, b = a[:, :131056].repeat(30, 1).contiguous(), b[:, :, :131056].contiguous()   # (the streaming kernel)
+    sa = torch.ones(90)
+    _check_close(_run(ops, a, sa, b, sb, [50, 40], torch.bfloat16, True), _product(a, sa, b, sb, [50, 40]), torch.bfloat16, "stream")
+
+
+def test_no_depth_no_rows_no_columns(ops):
+    sizes = torch.tensor([2, 0, 1])
+    out = ops.gmm_int8(torch.empty(3, 0, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"), torch.empty(3, 5, 0, dtype=torch.int8, device="cuda"),
+                       torch.ones(3, 5, device="cuda"), sizes)
+    assert out.shape == (3, 5) and not out.any()
+    for on_device in (True, False):
+        a, sa, b, sb = _operands(0, 3, 64, 40, 1)
+        assert _run(ops, a, sa, b, sb, [0, 0, 0], torch.bfloat16, on_device).shape == (0, 40)
+        a, sa, b, sb = _operands(4, 3, 64, 0, 1)
+        assert _run(ops, a, sa, b, sb, [1, 2, 1], torch.bfloat16, on_device).shape == (4, 0)
+        a, sa, b, sb = _operands(4, 0, 64, 8, 1)
+        c = torch.full((4, 8), 2.0, dtype=torch.bfloat16, device="cuda")
+        assert (_run(ops, a, sa, b, sb, [], torch.bfloat16, on_device, c=c) == 2).all()
+        a, sa, b, sb = _operands(5, 2, 64, 8, 1)   # (sizes of zero, rows behind)
+        c = torch.full((5, 8), 2.0, dtype=torch.bfloat16, device="cuda")
+        assert (_run(ops, a, sa, b, sb, [0, 0], torch.bfloat16, on_device, c=c) == 2).all()
+
+
+@pytest.mark.parametrize("experts,rows", [(513, 700), (700, 40000), (1500, 1500), (600, 20)])
+def test_more_groups_than_a_launch_takes(ops, experts, rows):
+    _announce("groups", experts, rows)
+    g = torch.Generator().manual_seed(experts)
+    sizes = torch.bincount(torch.randint(experts, (rows,), generator=g), minlength=experts)
+    a, sa, b, sb = _operands(rows, experts, 48, 24, 4)
+    want = torch.empty(rows, 24, dtype=torch.float64)
+    of_row = torch.repeat_interleave(torch.arange(experts), sizes)
+    want = torch.matmul(b[of_row].double(), a.double().unsqueeze(2)).squeeze(2) * sa.double().unsqueeze(1) * sb[of_row].double()
+    for on_device in (True, False):
+        _check_close(_run(ops, a, sa, b, sb, sizes.tolist(), torch.bfloat16, on_device), want, torch.bfloat16, (experts, rows))
+
+
+@pytest.mark.parametrize("hidden_in,hidden_out,rows", [(64, 40, 30), (256, 512, 900), (63, 40, 300)])
+def test_wild_device_sizes_are_clamped_and_reported(ops, hidden_in, hidden_out, rows):
+    from grouped_gemm_amd import backend
+    _announce("wild sizes", hidden_in, hidden_out, rows)
+    a, sa, b, sb = _operands(rows, 4, hidden_in, hidden_out, 3)
+    backend.backend.size_status(torch.device("cuda", 0))
+    for sizes, taken, status in (([5, 2, rows, 9], [5, 2, rows - 7, 0], True), ([-3, 4, 2, 0], [0, 4, 2, 0], True), ([2 ** 62, 2 ** 62, 1, 1], [rows, 0, 0, 0], True),
+                                 ([1, 2, 3, 4], [1, 2, 3, 4], False), ([-2 ** 63, 1, 2 ** 63 - 1, -1], [0, 1, rows - 1, 0], True)):
+        c = torch.full((rows, hidden_out), 9.0, dtype=torch.bfloat16, device="cuda")
+        out = _run(ops, a, sa, b, sb, sizes, torch.bfloat16, True, c=c)
+        _check_close(out, _product(a, sa, b, sb, taken), torch.bfloat16, sizes)
+        assert (out[sum(taken):] == 9).all()
+        assert bool(backend.backend.size_status(torch.device("cuda", 0))) == status, sizes
+        if status:
+            with pytest.raises(RuntimeError):
+                _run(ops, a, sa, b, sb, sizes, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("sizes,hidden_in,hidden_out", [([2, 1], 14336, 128), ([40, 9, 30], 2048, 192), ([700], 8192, 128), ([600, 300], 513, 64)])
+def test_the_same_bits_on_every_call_and_stream(ops, sizes, hidden_in, hidden_out):
+    _announce("repeats", sizes, hidden_in, hidden_out)
+    a, sa, b, sb = (v.cuda() for v in _operands(sum(sizes), len(sizes), hidden_in, hidden_out, 11))
+    batch_sizes = torch.tensor(sizes).cuda()
+    first = ops.gmm_int8(a, sa, b, sb, batch_sizes)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ops.gmm_int8(a, sa, b, sb, batch_sizes))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.parametrize("sizes,hidden_in,hidden_out", [([2, 1, 0], 4096, 128), ([30, 9, 1], 1024, 64), ([300, 700, 200], 512, 256), ([300, 0, 233], 511, 63)])
+def test_captured_and_replayed(ops, sizes, hidden_in, hidden_out):
+    """A chain from rows to rows, replayed with other rows and other sizes, with eager work between."""
+    _announce("graph", sizes, hidden_in, hidden_out)
+    rows, experts = sum(sizes), len(sizes)
+    x = torch.randn(rows, hidden_in, device="cuda", dtype=torch.bfloat16)
+    b = ops.quantize_rows(torch.randn(experts, 2 * hidden_out, hidden_in, device="cuda"))
+    batch_sizes = torch.tensor(sizes).cuda()
+
+    def chain():
+        q = ops.quantize_rows(x)
+        return ops.swiglu_quantize(ops.gmm_int8(q.values, q.scales, b.values, b.scales, batch_sizes, dtype=torch.float16))
+
+    chain()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain()
+    for n in range(4):
+        x.copy_(torch.randn_like(x) * (n + 1))
+        batch_sizes.copy_(torch.tensor(sizes[n % experts:] + sizes[:n % experts]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.values.clone(), out.scales.clone()
+        eager = chain()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], eager.values) and torch.equal(got[1], eager.scales), n
+
+
+def test_offsets_past_32_bits(ops):
+    """More than 4 GiB of weights, and more than 4 GiB of rows."""
+    _announce("large")
+    experts, hidden_out, hidden_in = 3, 28672, 65536   # 5.6e9 bytes
+    b = torch.empty(experts, hidden_out, hidden_in, dtype=torch.int8, device="cuda").random_(-128, 128)
+    sb = torch.rand(experts, hidden_out, device="cuda") / 64 + 1e-3
+    for rows, sizes in ((4, [1, 1, 2]), (120, [40, 50, 30])):
+        a = torch.empty(rows, hidden_in, dtype=torch.int8, device="cuda").random_(-128, 128)
+        sa = torch.rand(rows, device="cuda") / 64 + 1e-3
+        got = ops.gmm_int8(a, sa, b, sb, torch.tensor(sizes).cuda())
+        for e, first in ((0, 0), (2, rows - 1)):
+            at = slice(hidden_out - 300, hidden_out)
+            want = (a[first].double() @ b[e, at].double().t() * sa[first].double() * sb[e, at].double()).cpu()
+            _check_close(got[first, at], want, torch.bfloat16, (rows, e))
+    del b, a, got
+    rows, hidden_in = 1 << 18, 17408   # 4.6e9 bytes
+    x = torch.randn(512, hidden_in, device="cuda", dtype=torch.bfloat16)
+    index = (torch.arange(rows, device="cuda") % 512).to(torch.int32)
+    q = ops.quantize_rows(x, index)
+    want, scales = _quantized(x.cpu())
+    for r in (0, 511, rows - 513, rows - 1):
+        assert torch.equal(q.values[r].cpu(), want[r % 512]) and q.scales[r].cpu() == scales[r % 512], r
+    b = torch.randint(-128, 128, (2, 24, hidden_in), dtype=torch.int8, device="cuda")
+    sb = torch.rand(2, 24, device="cuda") + 0.5
+    got = ops.gmm_int8(q.values, q.scales, b, sb, torch.tensor([rows - 1000, 1000]))
+    for r in (0, rows - 1001, rows - 1000, rows - 1):
+        e = 0 if r < rows - 1000 else 1
+        want_r = (want[r % 512].double() @ b[e].double().cpu().t()) * scales[r % 512].double() * sb[e].double().cpu()
+        _check_close(got[r], want_r, torch.bfloat16, r)
+
+
+def test_an_expert_layer_in_8_bits(ops):
+    """A run of the operators together, routed, against the same layer in 64 bits on the values that the 8-bit numbers stand for; quantising the rows
+    in between moves each by half a step, 1/254 of its row's largest, which the next product averages over its depth."""
+    _announce("layer")
+    tokens, experts, k, hidden, ffn = 200, 8, 2, 256, 320
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(tokens, hidden, generator=g).to(torch.bfloat16).cuda()
+    w13 = ops.quantize_rows((torch.randn(experts, 2 * ffn, hidden, generator=g) * hidden ** -0.5).cuda())
+    w2 = ops.quantize_rows((torch.randn(experts, hidden, ffn, generator=g) * ffn ** -0.5).cuda())
+    r = ops.route(torch.randn(tokens, experts, generator=g).cuda(), k)
+    q = ops.quantize_rows(x, r.row_index)
+    gate_up = ops.gmm_int8(q.values, q.scales, w13.values, w13.scales, r.batch_sizes)
+    h = ops.swiglu_quantize(gate_up)
+    # (the router's weights go into the scales of the second product's rows)
+    rows = ops.gmm_int8(h.values, h.scales * r.weights.view(-1)[r.order.long()], w2.values, w2.scales, r.batch_sizes)
+    out = torch.zeros(tokens, hidden, dtype=torch.float64, device="cuda").index_add_(0, r.row_index.long(), rows.double())
+    of_row = torch.repeat_interleave(torch.arange(experts, device="cuda"), r.batch_sizes)
+    real = lambda v: v.values.double() * v.scales.double().unsqueeze(-1)  # noqa: E731
+
+    def product(w, q, scales):   # (whole numbers first, so that what cancels does)
+        return torch.matmul(w.values[of_row].double(), q.values.double().unsqueeze(2)).squeeze(2) * w.scales[of_row].double() * scales.unsqueeze(1)
+
+    both = product(w13, q, q.scales.double())
+    _check_close(gate_up, both.cpu(), torch.bfloat16, "first product")
+    gate, up = gate_up.double().chunk(2, 1)
+    exact_h = torch.nn.functional.silu(gate) * up
+    assert ((real(h) - exact_h).abs() <= 0.501 * h.scales.double().unsqueeze(1)).all()
+    want = product(w2, h, h.scales.double() * r.weights.double().view(-1)[r.order.long()])
+    # (a weight times a scale is rounded once more: 2^-24)
+    assert ((rows.double() - want).abs() <= (2.0 ** -8 + 5 * 2.0 ** -24) * want.abs()).all()
+    dense = torch.matmul(real(w2)[of_row], exact_h.unsqueeze(2)).squeeze(2) * r.weights.double().view(-1)[r.order.long()].unsqueeze(1)
+    dense = torch.zeros_like(out).index_add_(0, r.row_index.long(), dense)
+    assert float((out - dense).norm() / dense.norm()) < 0.02
