@@ -327,35 +327,45 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void int8_rows_kernel
   const int strip = (int)(place / (uint32_t)at.windows), window = (int)place - strip * at.windows;
   const int column0 = strip * kStrip, columns = min(kStrip, a.hidden_out - column0);
   const int row0 = at.row0 + window * WINDOW, rows = min(WINDOW, at.rows - window * WINDOW);
+  // A thread's results: column `mine` of rows first_row, first_row + kFewWaves, ...  Their scales come while the weights do (of 64 rows, which leave
+  // no registers for them, when they are wanted).
+  const int mine = threadIdx.x % kStrip, first_row = threadIdx.x / kStrip;
+  static_assert(kFewThreads == kFewWaves * kStrip, "");
+  const float of_column = a.b_scales[(int64_t)at.group * a.hidden_out + column0 + min(mine, columns - 1)];
+  auto scale_of_row = [&](int i) { return a.a_scales[row0 + min(first_row + kFewWaves * i, rows - 1)]; };
+  float of_row[MT < 4 ? 4 * MT : 1];
+  if constexpr (MT < 4) {
+#pragma unroll
+    for (int i = 0; i < 4 * MT; ++i) of_row[i] = scale_of_row(i);
+  }
   Int8Stream<MT, ODD> s;
   s.setup(a.b + ((int64_t)at.group * a.hidden_out + column0) * depth, columns, a.a + (int64_t)row0 * depth, rows, depth);
   s.run(wave, (int)((int64_t)steps * piece / p.pieces), (int)((int64_t)steps * (piece + 1) / p.pieces));
-  const float* of_columns = a.b_scales + (int64_t)at.group * a.hidden_out + column0;
-  auto store = [&](int row, int column, int sum) {
-    const float v = (float)sum * of_columns[column] * a.a_scales[row0 + row];
-    static_cast<uint16_t*>(a.c)[(int64_t)(row0 + row) * a.hidden_out + column0 + column] =
+  auto store = [&](int i, int sum) {
+    const float v = (float)sum * of_column * (MT < 4 ? of_row[MT < 4 ? i : 0] : scale_of_row(i));
+    static_cast<uint16_t*>(a.c)[(int64_t)(row0 + first_row + kFewWaves * i) * a.hidden_out + column0 + mine] =
         a.to_f16 ? round_bits<kF16>(v) : round_bits<kBF16>(v);
   };
   int32_t* parts = a.parts + (int64_t)task / p.pieces * p.pieces * (WINDOW * kStrip);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
+    if (16 * m >= rows) break;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kStrip / 16; ++i) lds[wave * 256 + i * 64 + (threadIdx.x & 63)] = s.acc[i][m];
     __syncthreads();
-    if (16 * m >= rows) continue;
 #pragma unroll
-    for (int item = threadIdx.x; item < 16 * kStrip; item += kFewThreads) {
-      const int row = 16 * m + item / kStrip, column = item % kStrip;
-      const int* from = reinterpret_cast<const int*>(lds) + ((column >> 4) * 64 + ((column >> 2) & 3) * 16 + item / kStrip) * 4 + (column & 3);
+    for (int i = 0; i < 4; ++i) {
+      const int row = first_row + kFewWaves * i;   // of the 16
+      const int* from = reinterpret_cast<const int*>(lds) + ((mine >> 4) * 64 + ((mine >> 2) & 3) * 16 + row) * 4 + (mine & 3);
       int sum = 0;
 #pragma unroll
       for (int w = 0; w < kFewWaves; ++w) sum += from[w * 1024];
-      if (row >= rows || column >= columns) continue;
+      if (16 * m + row >= rows || mine >= columns) continue;
       if (p.pieces == 1) {
-        store(row, column, sum);
+        store(4 * m + i, sum);
       } else {
-        __hip_atomic_store(parts + piece * (WINDOW * kStrip) + row * kStrip + column, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(parts + piece * (WINDOW * kStrip) + (16 * m + row) * kStrip + mine, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
@@ -367,13 +377,14 @@ __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void int8_rows_kernel
     __syncthreads();
     if (arrived == p.pieces - 1) {
       if (threadIdx.x == 0) __hip_atomic_store(a.arrivals + task / p.pieces, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (as it was found)
-      for (int item = threadIdx.x; item < rows * kStrip; item += kFewThreads) {
-        const int row = item / kStrip, column = item % kStrip;
-        if (column >= columns) continue;
+#pragma unroll
+      for (int i = 0; i < 4 * MT; ++i) {
+        const int row = first_row + kFewWaves * i;
+        if (row >= rows || mine >= columns) continue;
         int sum = 0;
         for (int q = 0; q < p.pieces; ++q)
-          sum += __hip_atomic_load(parts + q * (WINDOW * kStrip) + item, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        store(row, column, sum);
+          sum += __hip_atomic_load(parts + q * (WINDOW * kStrip) + row * kStrip + mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        store(i, sum);
       }
     }
   }
