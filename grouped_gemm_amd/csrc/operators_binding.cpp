@@ -244,9 +244,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> BalanceLoss(const torch:
                                                                     const c10::optional<torch::Tensor>& mask, const std::string& score) {
   const int which = Score(score);
   TORCH_CHECK(experts.dim() == 2 && experts.scalar_type() == torch::kInt32, "grouped_gemm: experts must be int32 (tokens, top_k)");
-  CheckLogits(logits, experts.size(1));
-  TORCH_CHECK(experts.size(0) == logits.size(0), "grouped_gemm: experts must be int32 (tokens, top_k)");
+  TORCH_CHECK(logits.dim() != 2 || experts.size(0) == logits.size(0), "grouped_gemm: experts must be int32 (tokens, top_k), a row to each of logits");
   TORCH_CHECK(experts.is_contiguous(), "grouped_gemm: experts must be contiguous");
+  CheckLogits(logits, experts.size(1));
   TORCH_CHECK(experts.device() == logits.device(), "grouped_gemm: logits and experts must be on the same GPU");
   if (offsets.has_value())
     TORCH_CHECK(offsets->dim() == 1 && offsets->size(0) >= 1 && offsets->scalar_type() == torch::kInt32 && offsets->is_contiguous() &&

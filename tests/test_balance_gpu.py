@@ -79,7 +79,7 @@ def _check(ops, logits, experts, offsets=None, mask=None, score="softmax", what=
     want = _reference(logits, experts, offsets, mask, score, grads)
     assert got.counts.dtype == torch.int32 and got.balance.dtype == got.z.dtype == torch.float32 and got.balance.shape == got.z.shape == ()
     assert torch.equal(got.counts.cpu().long(), want["counts"]), what
-    balance, z = float(got.balance), float(got.z)
+    balance, z = float(got.balance.detach()), float(got.z.detach())
     assert abs(balance - float(want["balance"])) <= 2e-5 * float(want["balance"]), (what, balance, float(want["balance"]))
     assert abs(z - float(want["z"])) <= 2e-5 * float(want["z"]) + 2e-6 * float(want["z_scale"]), (what, z, float(want["z"]))
     grad, = torch.autograd.grad((got.balance, got.z), leaf, tuple(torch.tensor(v, device="cuda") for v in grads))
@@ -130,11 +130,11 @@ def test_sequences_of_every_kind(ops, score):
     mask[100:220] = False
     _check(ops, logits, chosen, torch.tensor([0, 100, 220, 500], dtype=torch.int32), mask, score, "a masked sequence")
     got, grad = _check(ops, logits, chosen, torch.tensor([0, 100, 500], dtype=torch.int32), torch.zeros(500, dtype=torch.bool), score, "nothing")
-    assert float(got.balance) == 0 and float(got.z) == 0 and not grad.any()
+    assert float(got.balance.detach()) == 0 and float(got.z.detach()) == 0 and not grad.any()
     # no tokens
     for offsets in (None, torch.tensor([0], dtype=torch.int32), torch.tensor([0, 0, 0], dtype=torch.int32)):
         got, grad = _check(ops, logits[:0], chosen[:0], offsets, None, score, "no tokens")
-        assert float(got.balance) == 0 and grad.shape == (0, 40)
+        assert float(got.balance.detach()) == 0 and grad.shape == (0, 40)
 
 
 def test_evenly_used_experts_give_one(ops):
@@ -209,3 +209,154 @@ def test_one_gradient_alone_and_differences(ops):
     (loss.balance * 0.01 + loss.z * 0.001).backward()
     want = _reference(logits, chosen, None, None, "softmax", (0.01, 0.001))
     assert ((leaf.grad.double().cpu() - want["grad"]).abs() <= 2e-5 * want["grad_scale"] + 2.0 ** -23 * want["grad"].abs()).all()
+
+
+def test_second_derivatives_and_forward_mode_are_refused(ops):
+    logits, chosen, g = _inputs(20, 8, 2, torch.float32, 10)
+    leaf = logits.cuda().requires_grad_(True)
+    loss = ops.balance_loss(leaf, chosen.cuda())
+    grad, = torch.autograd.grad(loss.balance, leaf, create_graph=True)
+    want = _reference(logits, chosen, None, None, "softmax", (1.0, 0.0))
+    assert ((grad.detach().double().cpu() - want["grad"]).abs() <= 2e-5 * want["grad_scale"] + 1e-37).all()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        grad.sum().backward()
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        ops.balance_loss(fwd.make_dual(logits.cuda(), torch.ones_like(logits).cuda()), chosen.cuda())
+    q = torch.randn(3, 16, device="cuda", requires_grad=True)
+    for call in (lambda: ops.quantize_rows(q), lambda: ops.swiglu_quantize(q)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    with torch.no_grad():
+        v = ops.quantize_rows(q)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.gmm_int8(v.values, v.scales.clone().requires_grad_(True), v.values.view(1, 3, 16), v.scales.view(1, 3), torch.tensor([3]))
+
+
+def test_wrong_arguments_on_the_device(ops):
+    logits, chosen, g = _inputs(20, 8, 2, torch.float32, 10)
+    x, e = logits.cuda(), chosen.cuda()
+    offsets, mask = torch.tensor([0, 20], dtype=torch.int32, device="cuda"), torch.ones(20, dtype=torch.bool, device="cuda")
+    for kw, text in ((dict(offsets=offsets.long()), "offsets"), (dict(offsets=offsets.cpu()), "offsets"), (dict(offsets=offsets[:0]), "offsets"),
+                     (dict(offsets=offsets.view(1, 2)), "offsets"), (dict(mask=mask.int()), "mask"), (dict(mask=mask[:5]), "mask"), (dict(mask=mask.cpu()), "mask")):
+        with pytest.raises(RuntimeError, match=text):
+            ops.balance_loss(x, e, **kw)
+    with pytest.raises(RuntimeError, match="same GPU"):
+        ops.balance_loss(x, chosen)
+    with pytest.raises(RuntimeError, match="row_index"):
+        ops.quantize_rows(x, torch.zeros(3, dtype=torch.int64, device="cuda"))
+    with pytest.raises(RuntimeError, match="row_index"):
+        ops.quantize_rows(x, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="2-d"):
+        ops.quantize_rows(x.view(2, 10, 8), torch.zeros(3, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="even"):
+        ops.swiglu_quantize(x[:, :7].contiguous())
+    a, b = torch.zeros(2, 16, dtype=torch.int8, device="cuda"), torch.zeros(1, 8, 16, dtype=torch.int8, device="cuda")
+    s, t = torch.ones(2, device="cuda"), torch.ones(1, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="same GPU"):
+        ops.gmm_int8(a, s.cpu(), b, t, torch.tensor([2]))
+    with pytest.raises(RuntimeError, match="negative"):
+        ops.gmm_int8(a, s, b, t, torch.tensor([-1]))
+    with pytest.raises(RuntimeError, match="sum past"):
+        ops.gmm_int8(a, s, b, t, torch.tensor([3]))
+    with pytest.raises(RuntimeError, match="overlap"):   # c within the rows of a
+        ops.gmm_int8(a, s, b, t, torch.tensor([2]), c=a.view(-1).view(torch.bfloat16).view(2, 8))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_captured_with_its_gradient_and_replayed(ops, score):
+    """Forward and backward in one graph, replayed with other logits, choices, sequences and masks, with eager work between."""
+    logits, chosen, g = _inputs(700, 40, 4, torch.bfloat16, 12)
+    x = logits.cuda().requires_grad_(True)
+    experts, offsets, mask = chosen.cuda(), _offsets(700, 9, g).cuda(), torch.ones(700, dtype=torch.bool, device="cuda")
+    grads = torch.tensor(0.3, device="cuda"), torch.tensor(0.2, device="cuda")
+
+    def step():
+        loss = ops.balance_loss(x, experts, offsets, mask, score)
+        return loss, torch.autograd.grad((loss.balance, loss.z), x, grads)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = step()
+    for n in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, device="cuda") * (n + 1))
+            experts.random_(0, 40)
+            offsets.copy_(_offsets(700, 9, g))
+            mask.copy_(torch.rand(700, device="cuda") < 0.8)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.detach().clone() for v in (loss.balance, loss.z, loss.counts, grad)]
+        eager, eager_grad = step()
+        torch.cuda.synchronize()
+        for a, b in zip(got, (eager.balance, eager.z, eager.counts, eager_grad)):
+            assert torch.equal(a, b.detach()), n
+
+
+def test_two_calls_at_once(ops):
+    logits, chosen, g = _inputs(3000, 64, 6, torch.float32, 13)
+    x, e, offsets = logits.cuda().requires_grad_(True), chosen.cuda(), _offsets(3000, 11, g).cuda()
+    first = ops.balance_loss(x, e, offsets)
+    want, = torch.autograd.grad((first.balance, first.z), x, (torch.ones((), device="cuda"), torch.ones((), device="cuda")))
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                loss = ops.balance_loss(x, e, offsets)
+                outs.append((loss, torch.autograd.grad(loss.balance + loss.z, x)[0]))
+    torch.cuda.synchronize()
+    for loss, grad in outs:
+        assert torch.equal(loss.balance, first.balance) and torch.equal(loss.z, first.z) and torch.equal(grad, want)
+
+
+def test_a_router_learns_to_spread_its_tokens(ops):
+    """route and balance_loss in a step, whose gradients are those of the same step by the formulas."""
+    g = torch.Generator().manual_seed(14)
+    tokens, hidden, experts, k = 256, 32, 16, 2
+    x, w = torch.randn(tokens, hidden, generator=g), torch.randn(hidden, experts, generator=g)
+    offsets = torch.tensor([0, 100, 256], dtype=torch.int32)
+    weight = w.cuda().requires_grad_(True)
+    logits = x.cuda() @ weight
+    r = ops.route(logits, k)
+    loss = ops.balance_loss(logits, r.experts, offsets.cuda())
+    assert torch.equal(loss.counts.sum(0).long(), r.batch_sizes)
+    (r.weights.square().sum() * 0.1 + loss.balance + 0.01 * loss.z).backward()
+    # the same in 64 bits, from the logits and choices of the step
+    l64 = logits.detach().double().cpu().requires_grad_(True)
+    chosen = r.experts.cpu().long()
+    picked = torch.softmax(l64, 1).gather(1, chosen)
+    (0.1 * (picked / picked.sum(1, keepdim=True)).square().sum()).backward()
+    want = l64.grad + _reference(logits.detach().cpu(), r.experts.cpu(), offsets, None, "softmax", (1.0, 0.01))["grad"]
+    weight_grad = x.double().t() @ want
+    # (a product of 256 terms in fp32, of gradients that are off by 2e-5 of terms below one)
+    scale = (x.double().abs().t() @ (want.abs() + 0.2)).max()
+    assert ((weight.grad.double().cpu() - weight_grad).abs() <= 1e-4 * scale).all()
+
+
+def test_many_tokens_and_sequences(ops):
+    """Offsets past 32 bits of bytes, and as many sequences as tokens."""
+    _announce("large")
+    tokens, experts = 1 << 22, 512   # 4.3e9 bytes of bf16
+    x = torch.randn(1 << 16, experts, device="cuda", dtype=torch.bfloat16).repeat(tokens >> 16, 1).requires_grad_(True)
+    e = torch.randint(experts, (1 << 16, 2), dtype=torch.int32, device="cuda").repeat(tokens >> 16, 1)
+    loss = ops.balance_loss(x, e)
+    grad, = torch.autograd.grad((loss.balance, loss.z), x, (torch.tensor(float(tokens), device="cuda"), torch.tensor(float(tokens), device="cuda")))
+    part = x[:1 << 16].detach().requires_grad_(True)
+    want = ops.balance_loss(part, e[:1 << 16])
+    part_grad, = torch.autograd.grad((want.balance, want.z), part, (torch.tensor(65536.0, device="cuda"), torch.tensor(65536.0, device="cuda")))
+    # the same tokens over and over: the same means, by other sums
+    assert abs(float(loss.balance.detach() - want.balance)) <= 4e-5 * float(want.balance.detach()) and abs(float(loss.z.detach() - want.z)) <= 4e-5 * float(want.z.detach())
+    assert torch.equal(loss.counts, want.counts * (tokens >> 16))
+    last = grad[-(1 << 16):].float()
+    assert ((last - part_grad.float()).abs() <= 2.0 ** -7 * part_grad.float().abs() + 1e-4).all()
+    del x, e, grad, last
+    tokens = 20000
+    logits, chosen, g = _inputs(tokens, 24, 3, torch.float32, 15)
+    _check(ops, logits, chosen, torch.arange(tokens + 1, dtype=torch.int32), None, "softmax", "a sequence to a token")
