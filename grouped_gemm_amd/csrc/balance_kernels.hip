@@ -74,6 +74,7 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences
 // taken times exp(top), which leaves sigmoids that are all too small for a float their proportions, and the division by their sum takes out
 // again.  Above kFarTop exp(-top) comes near the end of a float's range, and sigmoids are computed by themselves.
 constexpr float kFarTop = 60.0f;
+constexpr float kNoPower = 1e38f;
 
 template <int DT, bool SIGMOID, int G, int VPL>
 struct Scores {
@@ -93,7 +94,16 @@ struct Scores {
       top = fmaxf(top, e[v]);
     }
     top = group_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); });
-    const float base = top == -INFINITY ? 0.0f : top, base2 = base * LOG2E;   // (its rounding is a factor that all share)
+    const float base = top == -INFINITY ? 0.0f : top;
+    float base2 = base * LOG2E;   // (its rounding is a factor that all share)
+    // logits near the lowest or the largest of a float (a mask by the type's lowest, in all of a row): base2 would be infinite
+    auto bring_near = [&]() {
+      if (__builtin_expect(__any(fabsf(base) > kNoPower), 0)) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) e[v] -= base;
+        base2 = 0.0f;
+      }
+    };
     auto power = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, -base2)); };
     float sum = 0.0f, all = 0.0f;
     if constexpr (SIGMOID) {
@@ -104,11 +114,14 @@ struct Scores {
           const float x = e[v], least = fminf(base, 0.0f);
           s[v] = (x >= 0.0f ? 1.0f : quick_exp(x - least)) * __builtin_amdgcn_rcpf(1.0f + quick_exp(-fabsf(x)));
           slope[v] = quick_sigmoid(-x);
-          e[v] = power(x);
         }
+        bring_near();
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) e[v] = power(e[v]);
       } else {
         const float less = __builtin_amdgcn_exp2f(-fabsf(base2)), of_e = base < 0.0f ? less : 1.0f;
         of_slope = base < 0.0f ? 1.0f : less;
+        bring_near();
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
           e[v] = power(e[v]);
@@ -120,6 +133,7 @@ struct Scores {
       for (int v = 0; v < VPL; ++v) all += s[v];
       all = group_sum<G>(all);
     } else {
+      bring_near();
 #pragma unroll
       for (int v = 0; v < VPL; ++v) e[v] = power(e[v]);
     }

@@ -177,6 +177,41 @@ def test_closed_experts_and_extreme_logits(ops, dtype, score):
     assert math.isnan(got.balance) and math.isnan(got.z)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_masks_by_the_lowest_value_of_the_type(ops, dtype, score):
+    """All of a row, or all but one: the balance and its gradient, and of fp16, whose lowest has a square in fp32, also z."""
+    _announce("lowest", dtype, score)
+    for experts in (8, 30, 256, 700):
+        logits, chosen, g = _inputs(64, experts, 3, dtype, 7 + experts)
+        low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+        logits[3] = low
+        logits[4, 1:] = low
+        logits[5, ::2] = low
+        logits[6, :-1] = high     # (one expert closed, the others at the largest)
+        logits[7] = low
+        logits[7, 2] = -INF
+        logits[8] = low / 2
+        if score == "softmax":
+            logits[9, :-1] = low  # (sigmoid(x) of the last is 1 whatever the others)
+            logits[9, -1] = high
+        for mask in (None, torch.rand(64, generator=g) < 0.7):
+            if dtype == torch.float16:
+                _check(ops, logits, chosen, torch.tensor([0, 20, 64], dtype=torch.int32), mask, score, (experts, "all"))
+                continue
+            offsets = torch.tensor([0, 20, 64], dtype=torch.int32)
+            want = _reference(logits, chosen, offsets, mask, score, (0.7, 0.0))
+            leaf = logits.cuda().requires_grad_(True)
+            got = ops.balance_loss(leaf, chosen.cuda(), offsets=offsets.cuda(), mask=None if mask is None else mask.cuda(), score=score)
+            assert torch.equal(got.counts.cpu().long(), want["counts"])
+            assert abs(float(got.balance.detach()) - float(want["balance"])) <= 2e-5 * float(want["balance"]), (experts, float(got.balance.detach()))
+            assert float(want["z"]) < 1e38 or float(got.z.detach()) == INF
+            grad, = torch.autograd.grad(got.balance, leaf, torch.tensor(0.7, device="cuda"))
+            half, least = ROUNDING[dtype]
+            off = (grad.double().cpu() - want["grad"]).abs() - (2e-5 * want["grad_scale"] + half * want["grad"].abs() + least + 1e-37)
+            assert float(off.max()) <= 0, (experts, float(off.max()))
+
+
 def test_numbers_that_name_no_expert_are_no_choice(ops):
     logits, chosen, g = _inputs(300, 20, 4, torch.float32, 8)
     chosen[torch.rand(300, 4, generator=g) < 0.3] = -1
