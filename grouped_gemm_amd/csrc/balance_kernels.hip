@@ -26,13 +26,15 @@ namespace gg {
 namespace {
 
 constexpr int kBalanceThreads = 256;
+// Workgroups that the tokens are cut into, at most: four to a compute unit, all there at once.  Units / sums / backward of 65536 tokens, 256
+// experts in us with 512: 20.4 / 6.8 / 32.2, with 1024: 18.8 / 7.5 / 30.0, with 2048: 19.8 / 10.6 / 34.8.
 constexpr int64_t kBalanceBlocks = 1024;
-constexpr int kSumColumns = 64;   // of the second kernel's workgroups
+
 
 struct BalanceParams {
   BalanceArgs a;
   int32_t chunk;     // tokens of a workgroup
-  int32_t tiles;     // of kSumColumns experts
+  int32_t tiles;     // of the second kernel's columns of experts
   float* mass;       // [units][experts]
   int32_t* counts;   // [units][experts]
   float* z;          // [units]
@@ -252,55 +254,56 @@ __device__ __forceinline__ T block_sum(T v, T* lds) {
 }
 
 // A sequence's sums over its units, kSumColumns experts to a workgroup, whose waves take the units in turns.
-template <int THREADS>
+template <int THREADS, int COLUMNS>
 __global__ __launch_bounds__(THREADS) void balance_sums_kernel(BalanceParams p) {
-  constexpr int WAVES = THREADS / 64;
-  __shared__ float mass_of[WAVES][64];
-  __shared__ int32_t count_of[WAVES][64];
+  constexpr int WAVES = THREADS / 64, TURNS = THREADS / COLUMNS;
+  __shared__ float mass_of[TURNS][COLUMNS];
+  __shared__ int32_t count_of[TURNS][COLUMNS];
   __shared__ float sums[WAVES];
   __shared__ int32_t whole[WAVES];
   __shared__ int32_t arrived;
   const BalanceArgs& a = p.a;
-  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x / 64));
+  const int column = threadIdx.x % COLUMNS, turn = threadIdx.x / COLUMNS;
   const int64_t tasks = (int64_t)a.sequences * p.tiles;
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int s = (int)(task / p.tiles), tile = (int)(task - (int64_t)s * p.tiles), e = tile * kSumColumns + lane;
+    const int s = (int)(task / p.tiles), tile = (int)(task - (int64_t)s * p.tiles), e = tile * COLUMNS + column;
     const int64_t begin = offset_of(a.offsets, a.tokens, s), end = offset_of(a.offsets, a.tokens, s + 1);
     const int64_t from = begin / p.chunk + s, to = begin < end ? (end - 1) / p.chunk + s + 1 : from;   // units
     float mass = 0.0f, z = 0.0f;
     int32_t count = 0, tokens = 0;
     if (e < a.experts && from < to) {
       constexpr int IN_FLIGHT = 8;
-      for (int64_t u = from + wave; u < to; u += IN_FLIGHT * WAVES) {
+      for (int64_t u = from + turn; u < to; u += IN_FLIGHT * TURNS) {
         float m[IN_FLIGHT];
         int32_t n[IN_FLIGHT];
 #pragma unroll
         for (int f = 0; f < IN_FLIGHT; ++f) {
-          const int64_t at = min(u + f * WAVES, to - 1) * a.experts + e;
+          const int64_t at = min(u + f * TURNS, to - 1) * a.experts + e;
           m[f] = p.mass[at], n[f] = p.counts[at];
         }
 #pragma unroll
         for (int f = 0; f < IN_FLIGHT; ++f)
-          if (u + f * WAVES < to) mass += m[f], count += n[f];
+          if (u + f * TURNS < to) mass += m[f], count += n[f];
       }
     }
     for (int64_t u = from + threadIdx.x; u < to; u += THREADS) z += p.z[u], tokens += p.tokens[u];
-    mass_of[wave][lane] = mass, count_of[wave][lane] = count;
+    mass_of[turn][column] = mass, count_of[turn][column] = count;
     z = block_sum<THREADS>(z, sums);   // (barriers inside)
     tokens = block_sum<THREADS>(tokens, whole);
     float loss = 0.0f;
-    if (wave == 0) {
+    if (threadIdx.x < 64) {
       mass = 0.0f, count = 0;
+      if (turn == 0)
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) mass += mass_of[w][lane], count += count_of[w][lane];
+        for (int w = 0; w < TURNS; ++w) mass += mass_of[w][column], count += count_of[w][column];
       const float share = tokens > 0 ? (float)count * (float)a.experts / ((float)a.top_k * (float)tokens) : 0.0f;
-      if (e < a.experts) {
+      if (turn == 0 && e < a.experts) {
         a.counts[(int64_t)s * a.experts + e] = count;
         a.share[(int64_t)s * a.experts + e] = share;
         loss = share * mass;
       }
       loss = group_sum<64>(loss);
-      if (lane == 0) {
+      if (threadIdx.x == 0) {
         store_shared(p.loss + task, loss);
         if (tile == 0) store_shared(p.sequence_z + s, z), store_shared(p.sequence_tokens + s, tokens);
       }
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(kBalanceThreads, 4) void balance_backward_kernel(Ba
 
 // Tokens of a workgroup: at least a round, and no more than kBalanceBlocks workgroups.
 int64_t chunk_of(int64_t tokens, int64_t experts) {
-  const int64_t round = kBalanceThreads / (experts <= 256 ? 16 : 64), each = (tokens + kBalanceBlocks - 1) / kBalanceBlocks;
+  const int64_t round = kBalanceThreads / (experts <= 16 ? 4 : (experts <= 256 ? 16 : 64)), each = (tokens + kBalanceBlocks - 1) / kBalanceBlocks;
   return std::max(round, (each + round - 1) / round * round);
 }
 int64_t units_of(int64_t tokens, int64_t experts, int64_t sequences) {
@@ -431,12 +434,20 @@ int64_t units_of(int64_t tokens, int64_t experts, int64_t sequences) {
 
 struct BalanceScratch {
   int64_t units, tiles;
+  int columns;          // of the second kernel's workgroups
+  bool few_sequences;   // a sequence has many units: their sums by larger workgroups
   uint64_t mass, counts, z, tokens, loss, sequence_z, sequence_tokens, bytes;   // where they are, behind the counter
 };
 BalanceScratch scratch_of(int64_t tokens, int64_t experts, int64_t sequences) {
   BalanceScratch b;
   b.units = units_of(tokens, experts, sequences);
-  b.tiles = (experts + kSumColumns - 1) / kSumColumns;
+  b.few_sequences = b.units > 65 * sequences;
+  // Where a sequence has more than 64 units, 1024 threads take them, so that each has few to wait for, and 32 columns, so that more workgroups do
+  // (all three kernels of 65536 x 256, one sequence: 50.6 us with 64 columns, 48.0 with 32, 49.0 with 16, 49.7 with 8).  Otherwise whole rows of
+  // 64 columns are better, as one workgroup takes each sequence's tile (64 sequences: 53.2, with 16 columns 62.8).  Few experts leave
+  // wider tiles idle lanes (65536 x 8, 16 sequences: 28.6 with 64 columns, 24.5 with 16, the units' kernel being what it was).
+  b.columns = experts <= 16 ? 16 : (b.few_sequences ? 32 : 64);
+  b.tiles = (experts + b.columns - 1) / b.columns;
   uint64_t at = 16;
   auto take = [&](int64_t words) {
     const uint64_t here = at;
@@ -468,10 +479,12 @@ hipError_t launch_balance(const BalanceArgs& a, hipStream_t stream) {
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const uint32_t blocks = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(a.sequences * b.tiles, 2048));
-  if (chunks > 64 * a.sequences) {
-    hipLaunchKernelGGL(balance_sums_kernel<1024>, dim3(blocks), dim3(1024), 0, stream, p);
+  if (b.few_sequences) {
+    if (b.columns == 16) hipLaunchKernelGGL((balance_sums_kernel<1024, 16>), dim3(blocks), dim3(1024), 0, stream, p);
+    else hipLaunchKernelGGL((balance_sums_kernel<1024, 32>), dim3(blocks), dim3(1024), 0, stream, p);
   } else {
-    hipLaunchKernelGGL(balance_sums_kernel<256>, dim3(blocks), dim3(256), 0, stream, p);
+    if (b.columns == 16) hipLaunchKernelGGL((balance_sums_kernel<256, 16>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((balance_sums_kernel<256, 64>), dim3(blocks), dim3(256), 0, stream, p);
   }
   return hipGetLastError();
 }
@@ -487,8 +500,11 @@ hipError_t launch_balance_backward(const BalanceBackwardArgs& a, hipStream_t str
 
 uint64_t balance_scratch_bytes(int64_t tokens, int64_t experts, int64_t sequences) { return scratch_of(tokens, experts, sequences).bytes; }
 
+// The fewest lanes that hold a token's logits, 16 each at most: more of them leave lanes idle, and each reduction takes more steps.  (16 lanes
+// for up to 16 experts, as up to 64: 65536 x 8, 16 sequences, 28.6 us in place of 20.9; 8192 x 8, 20.0 in place of 18.4.)
 #define GG_BY_EXPERTS(DT, SIGMOID, launch, a, stream)                   \
   do {                                                                  \
+    if ((a).experts <= 16) return launch<DT, SIGMOID, 4, 4>(a, stream);      \
     if ((a).experts <= 64) return launch<DT, SIGMOID, 16, 4>(a, stream);     \
     if ((a).experts <= 128) return launch<DT, SIGMOID, 16, 8>(a, stream);    \
     if ((a).experts <= 256) return launch<DT, SIGMOID, 16, 16>(a, stream);   \

@@ -15,6 +15,10 @@
 //   Otherwise 127 x / most comes out off by less than 2^-15, and where that leaves open which integer is the nearest, the sign of 127 x - (q +- 1/2) most
 //   decides, which sums of floats whose errors are kept have exactly.
 //   silu(gate) * up is off by more than any of that, and is rounded as it comes.
+//
+// Read once, written once: 16384 rows of 4096 bf16 in 30 us, 6.7 TB/s (where x is in the last level of cache in part; a copy from and to
+// memory reaches 5.2), 8192 x 4096 in fp32 in 26 us, 6.5 TB/s; 24576 rows of 2048 that an index takes from 4096 in 23 us; silu(gate) * up, 8192 rows of
+// 4096, in 29 us, 5.8 TB/s, by its arithmetic as much as by memory; one token in 2.8 us, next to an empty launch.
 #include "operators.hpp"
 
 #include <math.h>
@@ -235,13 +239,15 @@ __device__ __forceinline__ SourceRow source_row(const QuantizeArgs& a, int64_t r
 
 // THREADS threads to a row of at least 8, which hold HELD chunks of it each between the two passes; rows with more are read twice, and so are
 // those that are not rounded in the way that most of their type are.  A row's last chunk is its last 8 elements: where it overlaps the one
-// before, both write the same.  Threads without a chunk take the last one, and store nothing.
+// before, both write the same.  Threads without a chunk take the last one, and store nothing; waves without one leave out silu(gate) * up, which
+// costs as much as its traffic (8192 rows of 5632, fp16: 41 us in place of 49.5; rows as they are lose 1 to 3 % by the branch, and go without).
 template <int DT, bool GATED, int THREADS, int HELD>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void quantize_kernel(QuantizeParams p) {
-  constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, WAVES = THREADS / 64;
+__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void quantize_kernel(QuantizeParams p) {
+  constexpr int BLOCK = THREADS == 64 ? 256 : THREADS, ROWS = BLOCK / THREADS, WAVES = THREADS / 64;
+  static_assert(ROWS == 1 || WAVES == 1, "rows of one workgroup meet at no barrier");
   __shared__ uint32_t of_wave[WAVES];
   const QuantizeArgs& a = p.a;
-  const int t = threadIdx.x % THREADS, cols = (int)a.cols;
+  const int t = threadIdx.x % THREADS, first = uniform(t / 64 * 64), cols = (int)a.cols;   // `first` of the wave
   for (int64_t row = (int64_t)blockIdx.x * ROWS + uniform((int)(threadIdx.x / THREADS)); row < a.rows; row += (int64_t)gridDim.x * ROWS) {
     const SourceRow source = source_row<DT>(a, row);
     int8_t* q = a.q + row * a.cols;
@@ -258,6 +264,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void quantize_kernel
       for (int h = 0; h < HELD; ++h) loaded[h].load(source.x, min((t + h * THREADS) * 8, cols - 8), cols);
 #pragma unroll
       for (int h = 0; h < HELD; ++h) {
+        if (GATED && first + h * THREADS >= p.chunks) break;
         held[h] = loaded[h].value();
         most = most_of(held[h], most);
       }
@@ -282,6 +289,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void quantize_kernel
     if (s.way == WAY) {
 #pragma unroll
       for (int h = 0; h < HELD; ++h) {
+        if (GATED && first + h * THREADS >= p.chunks) break;
         const int c = t + h * THREADS;
         const u32x2 v = WAY == kExact ? round_exact(held[h], s) : round_quick(held[h], s);
         if (c < p.chunks) store8(q + min(c * 8, cols - 8), v);
@@ -322,7 +330,7 @@ __global__ __launch_bounds__(256) void quantize_short_kernel(QuantizeParams p) {
 
 template <int DT, bool GATED, int THREADS, int HELD>
 hipError_t launch_rows(const QuantizeParams& p, hipStream_t stream) {
-  constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS;
+  constexpr int BLOCK = THREADS == 64 ? 256 : THREADS, ROWS = BLOCK / THREADS;
   const int64_t blocks = std::min<int64_t>((p.a.rows + ROWS - 1) / ROWS, 1 << 16);
   hipLaunchKernelGGL((quantize_kernel<DT, GATED, THREADS, HELD>), dim3((uint32_t)blocks), dim3(BLOCK), 0, stream, p);
   return hipGetLastError();
@@ -337,14 +345,21 @@ hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((quantize_short_kernel<DT, GATED>), dim3((uint32_t)std::min<int64_t>((a.rows + 255) / 256, 1 << 16)), dim3(256), 0, stream, p);
     return hipGetLastError();
   }
-  if (a.rows <= 512 && p.chunks > 256) return p.chunks <= 1024 ? launch_rows<DT, GATED, 1024, 1>(p, stream) : launch_rows<DT, GATED, 1024, 2>(p, stream);
-  if (a.rows <= 2048 && p.chunks > 64 && p.chunks <= 256) return launch_rows<DT, GATED, 256, 1>(p, stream);
+  // Threads to a row and chunks to a thread: more threads where there are few rows to fill the device with or a row is long, fewer, which meet at no
+  // barrier or a small one, elsewhere.  In us, one call after the other, x partly in the last level of cache:
+  //   up to 256 chunks, 256 x 1 / the lines below: 512 x 2048 bf16 2.9 / 3.8, 2048 x 2048 4.1 / 4.3, 8192 x 2048 11.0 / 10.5, 8192 x 1024 8.1 / 5.6;
+  //   128 x 2 / 64 x 4: 4096 x 2048 6.0 / 6.9, 16384 x 2048 17.3 / 18.3; silu(gate) * up 8192 x 2048 17.2 / 15.7, 24576 x 1408 40.5 / 37.6;
+  //   up to 512, 512 x 1 / 256 x 2: 512 x 4096 3.2 / 4.0, 1024 x 4096 4.2 / 4.5, 8192 x 4096 18.3 / 16.8;
+  //   up to 1024, 512 x 2 / 256 x 4: 8192 x 8192 30.3 / 31.8, 1024 x 8192 5.8 / 6.9; 1024 x 1: 36.3 and 6.9;
+  //   more, 1024 x 2 / 512 x 4 / 256 x 8: 8192 x 14336 62.6 / 62.4 / 64.9, in fp32 100 / 107 / 111, 512 x 14336 6.1 / 6.6 / 8.7; silu(gate) * up,
+  //   whose waves without a chunk do less, 4096 x 9000 48 / 35.7 / 34.9, 4096 x 14336 56 / 54 / 56, 64 x 14336 5.1 / 5.0 / 5.9.
   if (p.chunks <= 64) return launch_rows<DT, GATED, 64, 1>(p, stream);
+  if (p.chunks <= 256 && a.rows <= 2048) return launch_rows<DT, GATED, 256, 1>(p, stream);
   if (p.chunks <= 128) return launch_rows<DT, GATED, 64, 2>(p, stream);
-  if (p.chunks <= 256) return launch_rows<DT, GATED, 64, 4>(p, stream);
-  if (p.chunks <= 512) return launch_rows<DT, GATED, 256, 2>(p, stream);
-  if (p.chunks <= 1024) return launch_rows<DT, GATED, 256, 4>(p, stream);
-  return launch_rows<DT, GATED, 256, 8>(p, stream);
+  if (p.chunks <= 256) return launch_rows<DT, GATED, GATED ? 64 : 128, GATED ? 4 : 2>(p, stream);
+  if (p.chunks <= 512) return a.rows <= 1024 ? launch_rows<DT, GATED, 512, 1>(p, stream) : launch_rows<DT, GATED, 256, 2>(p, stream);
+  if (p.chunks <= 1024) return launch_rows<DT, GATED, 512, 2>(p, stream);
+  return launch_rows<DT, GATED, GATED ? 512 : 1024, GATED ? 4 : 2>(p, stream);
 }
 
 }  // namespace

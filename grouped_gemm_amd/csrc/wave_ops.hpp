@@ -16,15 +16,15 @@ __device__ __forceinline__ uint32_t dpp(uint32_t v) {
 }
 enum : int { kDppXor1 = 0xb1, kDppXor2 = 0x4e, kDppHalfMirror = 0x141, kDppMirror = 0x140 };
 
-// All lanes of a group of G (16, 32 or 64) get op over the group.
+// All lanes of a group of G (4, 8, 16, 32 or 64) get op over the group.
 template <int G, typename T, typename Op>
 __device__ __forceinline__ T group_reduce(T v, Op op) {
-  static_assert(sizeof(T) == 4 && (G == 16 || G == 32 || G == 64), "");
+  static_assert(sizeof(T) == 4 && (G == 4 || G == 8 || G == 16 || G == 32 || G == 64), "");
   auto step = [&](auto other) { v = op(v, __builtin_bit_cast(T, other)); };
   step(dpp<kDppXor1>(__builtin_bit_cast(uint32_t, v)));
   step(dpp<kDppXor2>(__builtin_bit_cast(uint32_t, v)));
-  step(dpp<kDppHalfMirror>(__builtin_bit_cast(uint32_t, v)));
-  step(dpp<kDppMirror>(__builtin_bit_cast(uint32_t, v)));
+  if constexpr (G >= 8) step(dpp<kDppHalfMirror>(__builtin_bit_cast(uint32_t, v)));
+  if constexpr (G >= 16) step(dpp<kDppMirror>(__builtin_bit_cast(uint32_t, v)));
   if constexpr (G >= 32) v = op(v, __shfl_xor(v, 16));
   if constexpr (G == 64) v = op(v, __shfl_xor(v, 32));
   return v;

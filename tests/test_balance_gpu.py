@@ -119,6 +119,15 @@ def test_losses_counts_and_gradient(ops, tokens, experts, k, sequences, dtype, s
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens,experts,sequences", [(5003, 8, 1), (9001, 16, 2), (70001, 3, 1), (20011, 17, 3), (17000, 100, 1), (6000, 513, 2)])
+def test_long_sequences(ops, tokens, experts, sequences, score):
+    """More units to a sequence than one turn of the second kernel takes."""
+    _announce("long", tokens, experts, sequences, score)
+    logits, chosen, g = _inputs(tokens, experts, 2, torch.bfloat16, tokens)
+    _check(ops, logits, chosen, _offsets(tokens, sequences, g), torch.rand(tokens, generator=g) < 0.8, score, "long")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_sequences_of_every_kind(ops, score):
     _announce("sequences", score)
     logits, chosen, g = _inputs(500, 40, 4, torch.float32, 3)
