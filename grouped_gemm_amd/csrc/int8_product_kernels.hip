@@ -11,6 +11,9 @@
 // loop; the waves' sums are added up through LDS at its end.
 //
 // Workgroups of one strip and neighbouring windows are neighbours, so that groups of many rows find the strip in L2.
+//
+// 512 rows over 128 groups, 7168 -> 4096 (3.7 GB): 0.59 ms, 6.2 TB/s, faster than a copy, which writes too; 2 rows of 2 groups, 4096 -> 28672
+// (235 MB): 46 us, of which a launch, the sizes and the first loads' way from memory take 6.6.
 #include "operators.hpp"
 
 #include <algorithm>
@@ -310,6 +313,7 @@ __device__ __forceinline__ Window find_window(const Int8Args& a, const Groups& g
   return w;
 }
 
+// (Two, three or four workgroups to a compute unit make no difference, 14336 -> 4096 for 2 rows: 23.7, 23.0, 23.8 us; 64 rows' sums take two.)
 template <int MT, bool ODD>
 __global__ __launch_bounds__(kFewThreads, MT == 1 ? 3 : 2) void int8_rows_kernel(Int8Params p, HostSizes hs) {
   constexpr int WINDOW = 16 * MT;
@@ -409,7 +413,12 @@ Int8Plan int8_plan(int64_t tokens, int64_t num_groups, int64_t hidden_in, int64_
   while (f.rows_of_window > 1 && windows() * f.strips < kInt8Units * 3 / 4) f.rows_of_window /= 2;
   const int64_t window = 16 * f.rows_of_window;
   f.windows = windows();
-  const int64_t steps = (hidden_in + kStep - 1) / kStep, fit = 2 * kInt8Units / (f.windows * f.strips), deep = steps / (4 * kFewWaves);
+  // Pieces of the depth while they are no more than the compute units, of at least four steps to a wave: b is read no faster by more workgroups,
+  // and a piece is a sum to write and join.  us with whole depths, with up to 256, 512 and 1024 pieces: 1 row, 14336 -> 512 29.6, 11.9, 11.8, 11.9;
+  // 2 rows of 2 groups, 8192 -> 1024 18.9, 11.6, 11.6, 11.6; 14336 -> 4096 29.9, 23.3, 23.0, 25.2; 4096 -> 8192 13.8, 13.7, 16.3, 16.3; 4 of 64 groups,
+  // 7168 -> 2048 17.2, 15.4, 17.1, 17.0.  With two steps to a wave: 8 rows of 8 groups, 2048 -> 512 9.1 in place of 7.9, 2 of 8, 4096 -> 1024 9.7 in
+  // place of 10.9; with eight 1, 14336 -> 512 15.8.
+  const int64_t steps = (hidden_in + kStep - 1) / kStep, fit = kInt8Units / (f.windows * f.strips), deep = steps / (4 * kFewWaves);
   f.pieces = std::max<int64_t>(1, std::min({fit, deep, int64_t(16)}));
   const uint64_t need = kWsCounterBytes + (uint64_t)f.windows * f.strips * f.pieces * window * kStrip * 4;
   if (f.pieces > 1 && (need > workspace_bytes || f.windows * f.strips > kWsCounterBytes / 4)) f.pieces = 1;
