@@ -209,9 +209,10 @@ def balance_loss(logits, experts, offsets=None, mask=None, score="softmax"):
     sequence s, T in all.  Evenly used experts give a balance of 1.  logits (tokens, experts) and experts int32 (tokens, top_k) as
     route takes and returns them.  offsets int32 (sequences + 1): sequence s is the tokens offsets[s] .. offsets[s + 1] - 1,
     ascending; tokens before the first and behind the last count nowhere.  None: all tokens are one sequence.  mask bool
-    (tokens): tokens that count, None: all.  Without tokens that count both losses are 0.
+    (tokens): tokens that count, None: all.  Without tokens that count both losses are 0.  An expert whose logit is -inf is closed to the
+    token, a token that none is open to adds nothing; a NaN or +inf of a token that counts makes both losses NaN.
 
-    Everything is computed in float32.  Gradients flow from balance and z to the logits, those of tokens that do not count are 0; counts are
+    Everything is computed in float32 (where a token's largest logit is beyond 1.8e19, of either sign, z is infinite).  Gradients flow from balance and z to the logits, those of tokens that do not count are 0; counts are
     constants.  Second derivatives and forward mode are refused.  Nothing waits for the device.  Not part of the
     reference's surface, which has no router."""
     return BalanceLoss(*backend.backend.balance_loss(logits, experts, offsets, mask, score))
@@ -252,7 +253,8 @@ def gmm_int8(a, a_scales, b, b_scales, batch_sizes, dtype=torch.bfloat16, c=None
     a int8 (tokens, hidden_in), b int8 (experts, hidden_out, hidden_in), along the depth as quantize_rows leaves weights stored
     (out, in), hidden_in at most 131071, a_scales float32 (tokens), b_scales float32 (experts, hidden_out); batch_sizes int64
     (experts) on the host or on the device, as for gmm.  The sums are exact, scaled in float32 and rounded once, to dtype
-    (bfloat16 or float16).  c receives the result, and keeps its rows behind the last expert's.
+    (bfloat16 or float16).  c receives the result, and keeps its rows behind the last expert's
+    (without c they hold anything).
 
     No gradient.  Not part of the reference's surface, whose operands are bfloat16 (csrc/grouped_gemm.cu:490-506)."""
     if dtype not in (torch.bfloat16, torch.float16):
