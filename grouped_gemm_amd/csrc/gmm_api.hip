@@ -801,8 +801,9 @@ static_assert(int64_t(128) * 128 * GG_INT8_MAX_DEPTH < (int64_t(1) << 31), "no s
 // Average rows to a group up to which a call goes to the kernel for few rows, which reads weights faster (it needs no tiles in LDS) but again
 // for every 16 to 64 rows.  us, streaming tiles / few rows, by rows to a group: 8 groups, 4096 -> 14336: 4 110 / 88, 16 111 / 93, 24 111 / 105, 32 111 / 122;
 // 8, 1024 -> 1024: 4 8.4 / 6.1, 24 8.4 / 8.2, 32 8.6 / 9.6; 32, 4096 -> 4096: 4 113 / 98, 16 118 / 105, 32 119 / 126; 64, 7168 -> 2048: 4 158 / 155,
-// 8 159 / 158, 16 160 / 164, 32 162 / 197; 64, 2048 -> 7168: 8 162 / 167, 16 166 / 192; 128, 2048 -> 1408: 4 67 / 63, 8 69 / 67, 16 70 / 78.
-int64_t int8_few_rows(int64_t num_groups) { return num_groups <= 8 ? 24 : (num_groups <= 32 ? 16 : 8); }
+// 8 159 / 158, 16 160 / 164, 32 162 / 197; 64, 2048 -> 7168: 8 162 / 167, 16 166 / 192; 128, 2048 -> 1408: 4 67 / 63, 8 69 / 67, 16 70 / 78; 1 group,
+// 4096 -> 4096: 32 16 / 14, 64 18 / 13; 4096 -> 14336: 32 23 / 19, 64 22 / 23; 9072 -> 5632: 32 24 / 20, 48 23 / 33; 2048 -> 8192: 32 10.9 / 9.0.
+int64_t int8_few_rows(int64_t num_groups) { return num_groups == 1 ? 32 : (num_groups <= 8 ? 24 : (num_groups <= 32 ? 16 : 8)); }
 
 int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_scales) {
   if (args == nullptr) return fail(GG_EINVAL, "args is null");

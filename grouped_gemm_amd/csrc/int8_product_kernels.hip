@@ -407,9 +407,11 @@ Int8Plan int8_plan(int64_t tokens, int64_t num_groups, int64_t hidden_in, int64_
   f.strips = (hidden_out + kStrip - 1) / kStrip;
   // Rows of a window by how many a group has on average (those that do not fit read the strip again), and fewer where such windows leave compute units.
   // us with 16, 32 and 64: 8 rows to a group (8 groups, 4096 -> 4096) 23, 24, 25; 16 31, 25, 27; 31 (64, 1023 -> 1407) 55, 46, 45; 375 (8, 2047 -> 1023)
-  // 80, 60, 54; 67 (5, 2047 -> 1023: 368, 240 and 160 workgroups) 17, 14, 19; 13 (8, 1021 -> 513: 129, 99) 7.4, 8.0, 8.4.
+  // 80, 60, 54; 67 (5, 2047 -> 1023: 368, 240 and 160 workgroups) 17, 14, 19; 13 (8, 1021 -> 513: 129, 99) 7.4, 8.0, 8.4.  (Pieces of the depth instead of fewer rows, where it is deep
+  // enough: 1 group of 48, 4096 -> 4096 17.7 in place of 13.2, 9072 -> 5632 27.8 in place of 32.6; 8 of 12, 8192 -> 1024 25.3 and 22.4, 14336 -> 512 21.9 and 24.9.)
   f.rows_of_window = tokens <= 8 * named ? 1 : (tokens <= 24 * named ? 2 : 4);
-  auto windows = [&] { return tokens <= named ? tokens : tokens / (16 * f.rows_of_window) + named; };
+  // (of n rows in a group, (n - 1) / window and one more)
+  auto windows = [&] { return std::max<int64_t>(tokens - named, 0) / (16 * f.rows_of_window) + std::min(tokens, named); };
   while (f.rows_of_window > 1 && windows() * f.strips < kInt8Units * 3 / 4) f.rows_of_window /= 2;
   const int64_t window = 16 * f.rows_of_window;
   f.windows = windows();
