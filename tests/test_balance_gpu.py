@@ -119,6 +119,20 @@ def test_losses_counts_and_gradient(ops, tokens, experts, k, sequences, dtype, s
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens,experts,sequences", [(50, 9, 50), (13, 111, 69), (280, 74, 109), (2, 300, 114), (700, 40, 3000), (3000, 6, 2500), (2500, 20, 900)])
+def test_short_and_empty_sequences(ops, tokens, experts, sequences, score):
+    """Sequences shorter than what a workgroup takes at once, with runs of empty ones before, between and behind them."""
+    _announce("short", tokens, experts, sequences, score)
+    logits, chosen, g = _inputs(tokens, experts, 2, torch.float32, tokens + sequences)
+    at = torch.sort(torch.randint(tokens + 1, (sequences + 1,), generator=g)).values
+    few = torch.sort(torch.randint(0, tokens // 3 + 1, (sequences + 1,), generator=g) * 3).values   # (runs of alike)
+    one = torch.arange(sequences + 1).clamp(max=tokens)
+    ends = torch.cat([torch.full((sequences - sequences // 2,), tokens // 2), torch.full((sequences // 2 + 1,), tokens)])
+    for what, offsets in (("at random", at), ("runs", few), ("of one", one), ("two places", ends)):
+        _check(ops, logits, chosen, offsets.clamp(max=tokens).to(torch.int32), torch.rand(tokens, generator=g) < 0.9, score, what)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("tokens,experts,sequences", [(5003, 8, 1), (9001, 16, 2), (70001, 3, 1), (20011, 17, 3), (17000, 100, 1), (6000, 513, 2)])
 def test_long_sequences(ops, tokens, experts, sequences, score):
     """More units to a sequence than one turn of the second kernel takes."""
