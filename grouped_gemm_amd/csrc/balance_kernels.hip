@@ -29,6 +29,9 @@ constexpr int kBalanceThreads = 256;
 // Workgroups that the tokens are cut into, at most: four to a compute unit, all there at once.  Units / sums / backward of 65536 tokens, 256
 // experts in us with 512: 20.4 / 6.8 / 32.2, with 1024: 18.8 / 7.5 / 30.0, with 2048: 19.8 / 10.6 / 34.8.
 constexpr int64_t kBalanceBlocks = 1024;
+// Units of a sequence, on average, up to which a wave adds them up, and needs no barrier for it.  All three kernels, wave / workgroup: 65536 x 64, 8192 sequences
+// (1.1 units) 85 / 102 us; 4096 x 64, 512 25.7 / 29.7; 65536 x 256, 64 sequences (17) 57.5 / 52.
+constexpr int64_t kWaveUnits = 8;
 
 
 struct BalanceParams {
@@ -259,26 +262,26 @@ __device__ __forceinline__ T block_sum(T v, T* lds) {
   return sum;
 }
 
-// A sequence's sums over its units, kSumColumns experts to a workgroup, whose waves take the units in turns.
-template <int THREADS, int COLUMNS>
+// A sequence's sums over its units, COLUMNS experts at a time, by TEAM threads (a wave, or all), which take the units in turns.
+template <int THREADS, int TEAM, int COLUMNS>
 __global__ __launch_bounds__(THREADS) void balance_sums_kernel(BalanceParams p) {
-  constexpr int WAVES = THREADS / 64, TURNS = THREADS / COLUMNS;
-  __shared__ float mass_of[TURNS][COLUMNS];
-  __shared__ int32_t count_of[TURNS][COLUMNS];
+  constexpr int WAVES = THREADS / 64, TURNS = TEAM / COLUMNS, IN_FLIGHT = 8;
+  static_assert(TEAM == 64 || TEAM == THREADS, "");
+  __shared__ float mass_of[TEAM == 64 ? 1 : TURNS][COLUMNS];
+  __shared__ int32_t count_of[TEAM == 64 ? 1 : TURNS][COLUMNS];
   __shared__ float sums[WAVES];
   __shared__ int32_t whole[WAVES];
   __shared__ int32_t arrived;
   const BalanceArgs& a = p.a;
-  const int column = threadIdx.x % COLUMNS, turn = threadIdx.x / COLUMNS;
+  const int member = threadIdx.x % TEAM, column = member % COLUMNS, turn = member / COLUMNS;
   const int64_t tasks = (int64_t)a.sequences * p.tiles;
-  for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+  for (int64_t task = (int64_t)blockIdx.x * (THREADS / TEAM) + uniform((int)(threadIdx.x / TEAM)); task < tasks; task += (int64_t)gridDim.x * (THREADS / TEAM)) {
     const int s = (int)(task / p.tiles), tile = (int)(task - (int64_t)s * p.tiles), e = tile * COLUMNS + column;
     const int64_t begin = offset_of(a.offsets, a.tokens, s), end = offset_of(a.offsets, a.tokens, s + 1);
     const int64_t from = begin / p.chunk + s, to = begin < end ? (end - 1) / p.chunk + s + 1 : from;   // units
     float mass = 0.0f, z = 0.0f;
     int32_t count = 0, tokens = 0;
     if (e < a.experts && from < to) {
-      constexpr int IN_FLIGHT = 8;
       for (int64_t u = from + turn; u < to; u += IN_FLIGHT * TURNS) {
         float m[IN_FLIGHT];
         int32_t n[IN_FLIGHT];
@@ -292,29 +295,36 @@ __global__ __launch_bounds__(THREADS) void balance_sums_kernel(BalanceParams p) 
           if (u + f * TURNS < to) mass += m[f], count += n[f];
       }
     }
-    for (int64_t u = from + threadIdx.x; u < to; u += THREADS) z += p.z[u], tokens += p.tokens[u];
-    mass_of[turn][column] = mass, count_of[turn][column] = count;
-    z = block_sum<THREADS>(z, sums);   // (barriers inside)
-    tokens = block_sum<THREADS>(tokens, whole);
-    float loss = 0.0f;
-    if (threadIdx.x < 64) {
+    for (int64_t u = from + member; u < to; u += TEAM) z += p.z[u], tokens += p.tokens[u];
+    if constexpr (TEAM == 64) {
+      z = group_sum<64>(z);
+      tokens = group_reduce<64>(tokens, [](int p, int q) { return p + q; });
+#pragma unroll
+      for (int d = COLUMNS; d < 64; d <<= 1) mass += __shfl_xor(mass, d), count += __shfl_xor(count, d);
+    } else {
+      mass_of[turn][column] = mass, count_of[turn][column] = count;
+      z = block_sum<THREADS>(z, sums);   // (barriers inside)
+      tokens = block_sum<THREADS>(tokens, whole);
       mass = 0.0f, count = 0;
       if (turn == 0)
 #pragma unroll
         for (int w = 0; w < TURNS; ++w) mass += mass_of[w][column], count += count_of[w][column];
+    }
+    if (member < 64) {
       const float share = tokens > 0 ? (float)count * (float)a.experts / ((float)a.top_k * (float)tokens) : 0.0f;
+      float loss = 0.0f;
       if (turn == 0 && e < a.experts) {
         a.counts[(int64_t)s * a.experts + e] = count;
         a.share[(int64_t)s * a.experts + e] = share;
         loss = share * mass;
       }
       loss = group_sum<64>(loss);
-      if (threadIdx.x == 0) {
+      if (member == 0) {
         store_shared(p.loss + task, loss);
         if (tile == 0) store_shared(p.sequence_z + s, z), store_shared(p.sequence_tokens + s, tokens);
       }
     }
-    __syncthreads();   // (LDS is read before the next task's sums)
+    if constexpr (TEAM != 64) __syncthreads();   // (LDS is read before the next task's sums)
   }
   // the last workgroup to arrive adds up the sequences
   wait_vmcnt<0>();
@@ -324,8 +334,21 @@ __global__ __launch_bounds__(THREADS) void balance_sums_kernel(BalanceParams p) 
   if (arrived != (int)gridDim.x - 1) return;
   float loss = 0.0f, z = 0.0f;
   int32_t tokens = 0;
-  for (int64_t i = threadIdx.x; i < tasks; i += THREADS) loss += load_shared(p.loss + i);
-  for (int i = threadIdx.x; i < a.sequences; i += THREADS) z += load_shared(p.sequence_z + i), tokens += load_shared(p.sequence_tokens + i);
+  for (int64_t first = threadIdx.x; first < tasks; first += IN_FLIGHT * THREADS) {
+    float of_loss[IN_FLIGHT], of_z[IN_FLIGHT];
+    int32_t of_tokens[IN_FLIGHT];
+#pragma unroll
+    for (int f = 0; f < IN_FLIGHT; ++f) {
+      of_loss[f] = load_shared(p.loss + min(first + f * THREADS, tasks - 1));
+      const int64_t s = min(first + f * THREADS, (int64_t)a.sequences - 1);
+      of_z[f] = load_shared(p.sequence_z + s), of_tokens[f] = load_shared(p.sequence_tokens + s);
+    }
+#pragma unroll
+    for (int f = 0; f < IN_FLIGHT; ++f) {
+      if (first + f * THREADS < tasks) loss += of_loss[f];
+      if (first + f * THREADS < a.sequences) z += of_z[f], tokens += of_tokens[f];
+    }
+  }
   loss = block_sum<THREADS>(loss, sums);
   z = block_sum<THREADS>(z, sums);
   tokens = block_sum<THREADS>(tokens, whole);
@@ -397,17 +420,15 @@ __global__ __launch_bounds__(kBalanceThreads, 4) void balance_backward_kernel(Ba
     const auto raw = next.raw;
     const bool counted = next.counted;
     next.ask(t + GROUPS, last);
-    if (t >= end && s + 1 < a.sequences) {   // the next one; if that ends before t too, they are halved
-      enter(s + 1);
-      if (t >= end && s + 1 < a.sequences) {
-        int low = s + 1, high = a.sequences - 1;
-        while (low < high) {
-          const int middle = (low + high + 1) / 2;
-          if (offset_of(a.offsets, a.tokens, middle) <= t) low = middle;
-          else high = middle - 1;
-        }
-        enter(low);
+    for (int further = 0; t >= end && s + 1 < a.sequences && further < 4; ++further) enter(s + 1);
+    if (t >= end && s + 1 < a.sequences) {   // far from here: those that are left are halved
+      int low = s + 1, high = a.sequences - 1;
+      while (low < high) {
+        const int middle = (low + high + 1) / 2;
+        if (offset_of(a.offsets, a.tokens, middle) <= t) low = middle;
+        else high = middle - 1;
       }
+      enter(low);
     }
     float grad[VPL];
     if (t < begin || t >= end || !counted) {
@@ -457,18 +478,19 @@ int64_t units_of(int64_t tokens, int64_t experts, int64_t sequences) {
 struct BalanceScratch {
   int64_t units, tiles;
   int columns;          // of the second kernel's workgroups
-  bool few_sequences;   // a sequence has many units: their sums by larger workgroups
+  int threads, team;    // ... of these workgroups, and of those that take a sequence's tile
   uint64_t mass, counts, z, tokens, loss, sequence_z, sequence_tokens, bytes;   // where they are, behind the counter
 };
 BalanceScratch scratch_of(int64_t tokens, int64_t experts, int64_t sequences) {
   BalanceScratch b;
   b.units = units_of(tokens, experts, sequences);
-  b.few_sequences = b.units > 65 * sequences;
+  b.threads = b.units > 65 * sequences ? 1024 : 256;
+  b.team = b.units <= kWaveUnits * sequences ? 64 : b.threads;
   // Where a sequence has more than 64 units, 1024 threads take them, so that each has few to wait for, and 32 columns, so that more workgroups do
   // (all three kernels of 65536 x 256, one sequence: 50.6 us with 64 columns, 48.0 with 32, 49.0 with 16, 49.7 with 8).  Otherwise whole rows of
   // 64 columns are better, as one workgroup takes each sequence's tile (64 sequences: 53.2, with 16 columns 62.8).  Few experts leave
   // wider tiles idle lanes (65536 x 8, 16 sequences: 28.6 with 64 columns, 24.5 with 16, the units' kernel being what it was).
-  b.columns = experts <= 16 ? 16 : (b.few_sequences ? 32 : 64);
+  b.columns = experts <= 16 ? 16 : (b.threads == 1024 ? 32 : 64);
   b.tiles = (experts + b.columns - 1) / b.columns;
   uint64_t at = 16;
   auto take = [&](int64_t words) {
@@ -500,13 +522,18 @@ hipError_t launch_balance(const BalanceArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((balance_units_kernel<DT, SIGMOID, G, VPL>), dim3((uint32_t)chunks), dim3(kBalanceThreads), 0, stream, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const uint32_t blocks = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(a.sequences * b.tiles, 2048));
-  if (b.few_sequences) {
-    if (b.columns == 16) hipLaunchKernelGGL((balance_sums_kernel<1024, 16>), dim3(blocks), dim3(1024), 0, stream, p);
-    else hipLaunchKernelGGL((balance_sums_kernel<1024, 32>), dim3(blocks), dim3(1024), 0, stream, p);
+  const int64_t teams = b.threads / b.team, tasks = a.sequences * b.tiles;
+  const dim3 blocks((uint32_t)std::max<int64_t>(1, std::min<int64_t>((tasks + teams - 1) / teams, 2048))), threads(b.threads);
+  const bool few = b.columns == 16;
+  if (b.threads == 1024) {
+    if (few) hipLaunchKernelGGL((balance_sums_kernel<1024, 1024, 16>), blocks, threads, 0, stream, p);
+    else hipLaunchKernelGGL((balance_sums_kernel<1024, 1024, 32>), blocks, threads, 0, stream, p);
+  } else if (b.team == 64) {
+    if (few) hipLaunchKernelGGL((balance_sums_kernel<256, 64, 16>), blocks, threads, 0, stream, p);
+    else hipLaunchKernelGGL((balance_sums_kernel<256, 64, 64>), blocks, threads, 0, stream, p);
   } else {
-    if (b.columns == 16) hipLaunchKernelGGL((balance_sums_kernel<256, 16>), dim3(blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((balance_sums_kernel<256, 64>), dim3(blocks), dim3(256), 0, stream, p);
+    if (few) hipLaunchKernelGGL((balance_sums_kernel<256, 256, 16>), blocks, threads, 0, stream, p);
+    else hipLaunchKernelGGL((balance_sums_kernel<256, 256, 64>), blocks, threads, 0, stream, p);
   }
   return hipGetLastError();
 }
