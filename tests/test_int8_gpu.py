@@ -179,6 +179,23 @@ def test_gated_rows(ops, dtype, rows, ffn):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(2048, 515), (2049, 515), (2049, 1030), (2048, 2040), (2051, 2040), (1024, 2056), (1025, 2056), (1025, 4095), (700, 5000), (300, 9001)])
+def test_many_rows(ops, dtype, rows, cols):
+    """Either side of the numbers of rows at which other kernels take them, of rows and of rows that an index names or not."""
+    _announce("many rows", dtype, rows, cols)
+    g = torch.Generator().manual_seed(rows + cols)
+    x = (torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))).to(dtype)
+    _check_rows(ops, x, (dtype, rows, cols))
+    index = torch.randint(-20, rows + 20, (rows,), generator=g).to(torch.int32)
+    got = ops.quantize_rows(x.cuda(), index.cuda())
+    named = (index >= 0) & (index < rows)
+    values, scales = _quantized(x[index.clamp(0, rows - 1).long()])
+    assert torch.equal(got.values.cpu(), torch.where(named.unsqueeze(1), values, 0)) and torch.equal(got.scales.cpu(), torch.where(named, scales, 0.0))
+    half = cols // 2
+    _check_swiglu(ops, (1.5 * torch.randn(rows, 2 * half, generator=g)).to(dtype), (dtype, rows, half))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_gated_rows_of_any_size(ops, dtype):
     _announce("gated sizes", dtype)
     g = torch.Generator().manual_seed(5)
