@@ -71,8 +71,11 @@ __device__ __forceinline__ u32x4 without_before(u32x4 v, int k, int depth) {
 
 // One wave's stream: its share of the depth of a strip against up to 16 * MT rows.  A lane loads 32 neighbouring elements of a row of each
 // operand, in two halves; which depth meets in which instruction is free as long as it is the same in both.
-// ODD: rows may begin on any element.  Loads of 16 bytes that are not on a boundary of 4 are slow, so a lane loads from the boundary before
-// its 32 elements on, one dword more, and shifts; each of those dwords holds an element of its own, so that nothing is read that could not be.
+// ODD: rows may begin on any element.  Loads of 16 bytes that are not on a boundary of 4 are slow, so a lane takes what is from the boundary before
+// its 32 elements on, and one dword more, and shifts; each dword that is loaded holds an element of the lane's own, so that nothing is read that could not be.
+// The one more is the first of the lane that has the next 32 of the row, so that only the lanes with a step's last 32 load it, where there are registers
+// for that (up to 32 rows; the other lanes' loads are out of range and reach no memory).  A load by all lanes costs as much as one of 16 bytes
+// each: 8 rows of 8 groups, 4095 -> 14336 85 us, so 71 (4092: 57); 512 of 128, 2047 -> 1408 107 and 92.5 (2044: 78).  64 rows spill: 600 of 8, 1061 -> 2898 38 in place of 27.
 template <int MT, bool ODD>
 struct Int8Stream {
   static constexpr int TILES = kStrip / 16;
@@ -84,6 +87,9 @@ struct Int8Stream {
   const int8_t *w, *x;              // the strip and the window, the same in all lanes; ODD: the boundary before
   uint32_t w_at[TILES], x_at[MT];   // where in them this lane's elements of step 0 begin; ODD: ... of the boundary before
   uint32_t w_turn[ODD ? TILES : 1], x_turn[ODD ? MT : 1];   // ODD: elements from there
+  static constexpr bool FROM_NEIGHBOUR = ODD && MT < 4;
+  __amdgpu_buffer_rsrc_t w_ends, x_ends;                    // FROM_NEIGHBOUR: what the dwords behind are loaded by
+  static constexpr uint32_t kNowhere = 0x80000000u;         // out of their range
   int depth;
   i32x4 acc[TILES][MT];
 
@@ -95,6 +101,7 @@ struct Int8Stream {
     const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
     depth = depth_;
     w = boundary(strip), x = boundary(window);
+    if constexpr (FROM_NEIGHBOUR) w_ends = make_rsrc(w, kNowhere - 1), x_ends = make_rsrc(x, kNowhere - 1);
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       w_at[i] = (uint32_t)min(16 * i + c, columns - 1) * (uint32_t)depth + q * 32;
@@ -121,7 +128,14 @@ struct Int8Stream {
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) s.x[m][h] = load16_at(x + k, x_at[m], 16 * h);
-    if constexpr (ODD) {   // (where nothing is to be shifted: the last dword again, not one past it)
+    // (not where nothing is to be shifted: there may be nothing)
+    if constexpr (FROM_NEIGHBOUR) {
+      const bool last = (threadIdx.x & 63) >= 48;
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) s.w_end[i] = __builtin_amdgcn_raw_buffer_load_b32(w_ends, last && w_turn[i] != 0 ? w_at[i] + 32 : kNowhere, k, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s.x_end[m] = __builtin_amdgcn_raw_buffer_load_b32(x_ends, last && x_turn[m] != 0 ? x_at[m] + 32 : kNowhere, k, 0);
+    } else if constexpr (ODD) {
 #pragma unroll
       for (int i = 0; i < TILES; ++i) s.w_end[i] = load_dword_at(w + k, w_at[i] + (w_turn[i] != 0 ? 32 : 28));
 #pragma unroll
@@ -150,6 +164,11 @@ struct Int8Stream {
 
   // ODD, of what load brought: from the boundary on -> from the lane's first element on
   static __device__ __forceinline__ void shift(u32x4 (&v)[2], uint32_t end, uint32_t elements) {
+    if constexpr (FROM_NEIGHBOUR) {
+      const int lane = threadIdx.x & 63;
+      const uint32_t next = (uint32_t)__builtin_amdgcn_ds_bpermute((lane + 16) * 4, (int)v[0][0]);
+      if (lane < 48) end = next;
+    }
     const uint32_t d[9] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3], end};
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j / 4][j % 4] = __builtin_amdgcn_alignbyte(d[j + 1], d[j], elements);
