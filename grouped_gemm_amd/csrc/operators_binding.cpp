@@ -161,30 +161,30 @@ struct BalanceInputs {
   const uint8_t* mask_data() const { return static_cast<const uint8_t*>(Pointer(mask)); }
 };
 
-// balance, z, counts, and for the gradient share and inverse
+// balance, z, counts, and what the gradient takes besides the inputs: (sequences, experts) shares, and behind them the inverse of the tokens' number
 torch::autograd::variable_list RunBalance(const BalanceInputs& in, const torch::Tensor& chosen) {
   const torch::Tensor& logits = in.logits;
   c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   const auto f32 = logits.options().dtype(torch::kFloat32).requires_grad(false);
-  torch::Tensor balance = torch::empty({}, f32), z = torch::empty({}, f32), inverse = torch::empty({}, f32);
-  torch::Tensor counts = torch::empty({in.sequences(), experts}, f32.dtype(torch::kInt32)), share = torch::empty({in.sequences(), experts}, f32);
+  const int64_t shares = in.sequences() * experts;
+  torch::Tensor balance = torch::empty({}, f32), z = torch::empty({}, f32), kept = torch::empty({shares + 1}, f32);
+  torch::Tensor counts = torch::empty({in.sequences(), experts}, f32.dtype(torch::kInt32));
   const torch::Tensor scratch = Scratch(gg_balance_scratch_bytes(tokens, experts, chosen.size(1), in.sequences()), balance);
   const int rc = gg_balance(logits.data_ptr(), LogitsType(logits.scalar_type()), tokens, experts, chosen.size(1), in.score,
                             chosen.data_ptr<int32_t>(), in.offsets_data(), in.sequences(), in.mask_data(), balance.data_ptr<float>(),
-                            z.data_ptr<float>(), counts.data_ptr<int32_t>(), share.data_ptr<float>(), inverse.data_ptr<float>(), Pointer(scratch),
+                            z.data_ptr<float>(), counts.data_ptr<int32_t>(), kept.data_ptr<float>(), kept.data_ptr<float>() + shares, Pointer(scratch),
                             CurrentStream(logits.device()));
   TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
-  return {balance, z, counts, share, inverse};
+  return {balance, z, counts, kept};
 }
 
-torch::Tensor RunBalanceBackward(const BalanceInputs& in, const torch::Tensor& share, const torch::Tensor& inverse, torch::Tensor balance_grad,
-                                 torch::Tensor z_grad) {
+torch::Tensor RunBalanceBackward(const BalanceInputs& in, const torch::Tensor& kept, torch::Tensor balance_grad, torch::Tensor z_grad) {
   const torch::Tensor& logits = in.logits;
   c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
   torch::Tensor out = torch::empty(logits.sizes(), logits.options().requires_grad(false));
   const int rc = gg_balance_backward(logits.data_ptr(), LogitsType(logits.scalar_type()), logits.size(0), logits.size(1), in.score, in.offsets_data(),
-                                     in.sequences(), in.mask_data(), share.data_ptr<float>(), inverse.data_ptr<float>(),
+                                     in.sequences(), in.mask_data(), kept.data_ptr<float>(), kept.data_ptr<float>() + in.sequences() * logits.size(1),
                                      static_cast<const float*>(Pointer(balance_grad)), static_cast<const float*>(Pointer(z_grad)), out.data_ptr(),
                                      CurrentStream(logits.device()));
   TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
@@ -196,11 +196,11 @@ c10::optional<torch::Tensor> Given(const torch::Tensor& t) { return t.defined() 
 // (as RouteGradientNode)
 class BalanceGradientNode : public torch::autograd::Function<BalanceGradientNode> {
  public:
-  static torch::Tensor forward(torch::autograd::AutogradContext*, const torch::Tensor& logits, const torch::Tensor& share, const torch::Tensor& inverse,
+  static torch::Tensor forward(torch::autograd::AutogradContext*, const torch::Tensor& logits, const torch::Tensor& kept,
                                const c10::optional<torch::Tensor>& offsets, const c10::optional<torch::Tensor>& mask,
                                const c10::optional<torch::Tensor>& balance_grad, const c10::optional<torch::Tensor>& z_grad, int64_t score) {
     const torch::Tensor none;
-    return RunBalanceBackward({logits, offsets.value_or(none), mask.value_or(none), (int)score}, share, inverse, balance_grad.value_or(none),
+    return RunBalanceBackward({logits, offsets.value_or(none), mask.value_or(none), (int)score}, kept, balance_grad.value_or(none),
                               z_grad.value_or(none));
   }
 
@@ -215,7 +215,7 @@ class BalanceNode : public torch::autograd::Function<BalanceNode> {
                                                 const c10::optional<torch::Tensor>& offsets, const c10::optional<torch::Tensor>& mask, int64_t score) {
     const BalanceInputs in = {logits, offsets.value_or(torch::Tensor()), mask.value_or(torch::Tensor()), (int)score};
     auto out = RunBalance(in, chosen);
-    ctx->save_for_backward({logits, in.offsets, in.mask, out[3], out[4]});
+    ctx->save_for_backward({logits, in.offsets, in.mask, out[3]});
     ctx->saved_data["score"] = score;
     ctx->mark_non_differentiable({out[2]});
     ctx->set_materialize_grads(false);
@@ -231,9 +231,9 @@ class BalanceNode : public torch::autograd::Function<BalanceNode> {
     const BalanceInputs in = {saved[0], saved[1], saved[2], (int)ctx->saved_data["score"].toInt()};
     torch::Tensor out;
     if (torch::GradMode::is_enabled()) {
-      out = BalanceGradientNode::apply(in.logits, saved[3], saved[4], Given(in.offsets), Given(in.mask), Given(balance_grad), Given(z_grad), (int64_t)in.score);
+      out = BalanceGradientNode::apply(in.logits, saved[3], Given(in.offsets), Given(in.mask), Given(balance_grad), Given(z_grad), (int64_t)in.score);
     } else {
-      out = RunBalanceBackward(in, saved[3], saved[4], balance_grad, z_grad);
+      out = RunBalanceBackward(in, saved[3], balance_grad, z_grad);
     }
     return {out, none, none, none, none};
   }
