@@ -305,6 +305,20 @@ def test_operands_on_any_boundary(ops, sizes, hidden_in, hidden_out):
         assert (buffer[:off_c] == 7).all() and (buffer[off_c + rows * hidden_out:] == 7).all()
 
 
+@pytest.mark.parametrize("sizes,hidden_in,hidden_out", [([1, 2], 4095, 130), ([16], 4097, 65), ([17, 9, 20], 4098, 600), ([40, 33], 2047, 1023), ([64, 50], 6001, 200), ([3] * 9, 2303, 64),
+                                                        ([1], 14335, 63)] + [([n], 2049, 700) for n in (24, 25, 32, 33, 64, 65)] + [([n], 1040, 700) for n in (24, 25, 32, 33, 64, 65)])
+def test_deep_products_of_few_rows_on_any_boundary(ops, sizes, hidden_in, hidden_out):
+    """Steps of the depth in the kernel's loop, of windows of 16, 32 and 64 rows; one group either side of the rows at which tiles take it."""
+    _announce("deep", sizes, hidden_in, hidden_out)
+    rows = sum(sizes)
+    a, sa, b, sb = _operands(rows, len(sizes), hidden_in, hidden_out, rows + hidden_in)
+    want = _product(a, sa, b, sb, sizes)
+    batch_sizes = torch.tensor(sizes).cuda()
+    for off_a, off_b in ((0, 0), (1, 2), (3, 0), (4, 8)):
+        out = ops.gmm_int8(_misaligned(a, off_a), sa.cuda(), _misaligned(b, off_b), sb.cuda(), batch_sizes, dtype=torch.float16)
+        _check_close(out, want, torch.float16, (off_a, off_b))
+
+
 @pytest.mark.parametrize("hidden_in,hidden_out", [(64, 64), (256, 1024), (63, 65), (4096, 128)])
 @pytest.mark.parametrize("sizes", [[3, 0, 2], [40, 30, 0, 7], [300, 200, 100], [2000]])
 def test_rows_behind_the_last_group_keep_what_they_hold(ops, sizes, hidden_in, hidden_out):
