@@ -191,6 +191,23 @@ torch::Tensor RunBalanceBackward(const BalanceInputs& in, const torch::Tensor& k
   return out;
 }
 
+// torch hands a leaf's gradient over on the stream where a graph of the leaf was first made, as long as one lives.  From a captured backward pass to the
+// default stream, which a capture cannot wait for, that ends the process: an error here, before torch gets there.
+void RefuseLivingGraph(const torch::Tensor& leaf, const char* name) {
+  if (!leaf.is_leaf()) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (accumulator == nullptr) return;
+  const auto made_on = accumulator->stream();
+  if (!made_on.has_value() || made_on->id() != 0) return;   // (0: the default one)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(CurrentStream(leaf.device())), &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return;
+  }
+  TORCH_CHECK(status == hipStreamCaptureStatusNone, "grouped_gemm: a captured backward pass of ", name,
+              " cannot reach a leaf of which a graph made outside the capture still lives: free what that graph returned first");
+}
+
 c10::optional<torch::Tensor> Given(const torch::Tensor& t) { return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt; }
 
 // (as RouteGradientNode)
@@ -228,6 +245,7 @@ class BalanceNode : public torch::autograd::Function<BalanceNode> {
     const torch::Tensor &balance_grad = grads[0], &z_grad = grads[1], none;
     if (!balance_grad.defined() && !z_grad.defined()) return {none, none, none, none, none};
     RefuseTangents({&balance_grad, &z_grad}, "the gradient of balance_loss");
+    RefuseLivingGraph(saved[0], "balance_loss");
     const BalanceInputs in = {saved[0], saved[1], saved[2], (int)ctx->saved_data["score"].toInt()};
     torch::Tensor out;
     if (torch::GradMode::is_enabled()) {

@@ -213,7 +213,8 @@ def balance_loss(logits, experts, offsets=None, mask=None, score="softmax"):
     token, a token that none is open to adds nothing; a NaN or +inf of a token that counts makes both losses NaN.
 
     Everything is computed in float32 (where a token's largest logit is beyond 1.8e19, of either sign, z is infinite).  Gradients flow from balance and z to the logits, those of tokens that do not count are 0; counts are
-    constants.  Second derivatives and forward mode are refused.  Nothing waits for the device.  Not part of the
+    constants.  Second derivatives and forward mode are refused, and a backward pass that is captured into a graph while another graph of the same leaf,
+    made outside the capture on the default stream, still lives.  Nothing waits for the device.  Not part of the
     reference's surface, which has no router."""
     return BalanceLoss(*backend.backend.balance_loss(logits, experts, offsets, mask, score))
 

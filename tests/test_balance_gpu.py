@@ -357,6 +357,35 @@ def test_captured_with_its_gradient_and_replayed(ops, score):
             assert torch.equal(a, b.detach()), n
 
 
+def test_a_captured_gradient_beside_a_living_graph_is_refused(ops):
+    """While a graph of the same logits lives that was made outside the capture, on the default stream; then, without it, captured and replayed."""
+    logits, chosen, g = _inputs(60, 20, 2, torch.float32, 31)
+    x, experts = logits.cuda().requires_grad_(True), chosen.cuda()
+
+    def step():
+        loss = ops.balance_loss(x, experts)
+        return torch.autograd.grad((loss.balance, loss.z), x, (torch.ones((), device="cuda"), torch.ones((), device="cuda")))[0]
+
+    want = step()
+    living = ops.balance_loss(x, experts)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured backward pass of balance_loss"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    grad, = torch.autograd.grad(living.balance, x)     # (the graph outside is as it was)
+    assert torch.isfinite(grad).all()
+    del living, grad
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_two_calls_at_once(ops):
     logits, chosen, g = _inputs(3000, 64, 6, torch.float32, 13)
     x, e, offsets = logits.cuda().requires_grad_(True), chosen.cuda(), _offsets(3000, 11, g).cuda()
