@@ -78,8 +78,12 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences
 // over its sum, and sigmoid(x) = E / (E + exp(-top)), 1 - sigmoid(x) = exp(-top) / (E + exp(-top)).  Where top is negative both divisors are
 // taken times exp(top), which leaves sigmoids that are all too small for a float their proportions, and the division by their sum takes out
 // again.  Above kFarTop exp(-top) comes near the end of a float's range, and sigmoids are computed by themselves.
+//
+// top * log2 e is rounded, by at most half a unit in its last place, and each power of two comes out times two to that: a factor that all of a token's share, and
+// that p and lse lose again, as long as it is near one.  Past kNoPower, where it is 2^(1/16) at most (at 3e9 it would be 2^72 or 2^-72, at
+// 1e10 past a float's range), differences from top are taken first, which floats of that size have nearly exactly.
 constexpr float kFarTop = 60.0f;
-constexpr float kNoPower = 1e38f;
+constexpr float kNoPower = 0x1p20f;
 
 template <int DT, bool SIGMOID, int G, int VPL>
 struct Scores {
@@ -100,8 +104,7 @@ struct Scores {
     }
     top = group_reduce<G>(top, [](float p, float q) { return fmaxf(p, q); });
     const float base = top == -INFINITY ? 0.0f : top;
-    float base2 = base * LOG2E;   // (its rounding is a factor that all share)
-    // logits near the lowest or the largest of a float (a mask by the type's lowest, in all of a row): base2 would be infinite
+    float base2 = base * LOG2E;
     auto bring_near = [&]() {
       if (__builtin_expect(__any(fabsf(base) > kNoPower), 0)) {
 #pragma unroll

@@ -235,6 +235,41 @@ def test_masks_by_the_lowest_value_of_the_type(ops, dtype, score):
             assert float(off.max()) <= 0, (experts, float(off.max()))
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_any_size(ops, dtype, score):
+    """Rows whose largest logit is anywhere between ordinary numbers and the largest of the type: all alike, all but one, around a size, and among
+    ordinary rows.  z and its gradient too where a float holds the sum of its squares: 17 of 3e18 do, one of 1e20 does not."""
+    _announce("sizes", dtype, score)
+    sizes = [1e3, 1e5, 2.0 ** 20 * 0.999, 2.0 ** 20 * 1.01, 1e7, 1e8, 1e9, 1.5e9, 3e9, 1e10, 1e12, 1e15, 1e18, 3e18, 1e20, 1e25, 1e30, 1e37, 2e38]
+    offsets = torch.tensor([0, 20, 32], dtype=torch.int32)
+    for experts in (8, 30, 256, 700):
+        for size in sizes:
+            for sign in (1.0, -1.0):
+                logits, chosen, g = _inputs(32, experts, 3, dtype, 11 + experts)
+                at = sign * size
+                logits[3] = at
+                logits[4, 1:] = at
+                logits[5, ::2] = at
+                logits[6] = (at + 3.0 * torch.randn(experts, generator=g).double()).to(dtype)
+                logits[7, :-1] = at
+                logits[7, -1] = -INF
+                logits[8:12] = (at * (1.0 + torch.randint(3, (4, experts), generator=g) * 2.0 ** -7)).to(dtype)   # steps of bf16
+                logits[25:28] = at
+                if size < 1e19:
+                    _check(ops, logits, chosen, offsets, None, score, (experts, at))
+                    continue
+                want = _reference(logits, chosen, offsets, None, score, (0.7, 0.0))
+                leaf = logits.cuda().requires_grad_(True)
+                got = ops.balance_loss(leaf, chosen.cuda(), offsets=offsets.cuda(), score=score)
+                assert abs(float(got.balance.detach()) - float(want["balance"])) <= 2e-5 * float(want["balance"]), (experts, at, float(got.balance.detach()))
+                assert float(got.z.detach()) == INF, (experts, at)
+                grad, = torch.autograd.grad(got.balance, leaf, torch.tensor(0.7, device="cuda"))
+                half, least = ROUNDING[dtype]
+                off = (grad.double().cpu() - want["grad"]).abs() - (2e-5 * want["grad_scale"] + half * want["grad"].abs() + least + 1e-37)
+                assert float(off.max()) <= 0, (experts, at, float(off.max()))
+
+
 def test_numbers_that_name_no_expert_are_no_choice(ops):
     logits, chosen, g = _inputs(300, 20, 4, torch.float32, 8)
     chosen[torch.rand(300, 4, generator=g) < 0.3] = -1
