@@ -453,8 +453,12 @@ __global__ __launch_bounds__(kBalanceThreads, 4) void balance_backward_kernel(Ba
       if constexpr (SIGMOID) {
         const float factor = of_score * scores.of_slope, rest = -dot * factor;
 #pragma unroll
-        for (int v = 0; v < VPL; ++v)
-          grad[v] = __builtin_fmaf(scores.s[v] * scores.slope[v], __builtin_fmaf(share[v], factor, rest), of_softmax * scores.e[v]);
+        for (int v = 0; v < VPL; ++v) grad[v] = scores.s[v] * scores.slope[v] * __builtin_fmaf(share[v], factor, rest);
+        // (without a gradient of z its softmax stays out: that of a row with +inf is NaN, the balance of its sigmoids is not)
+        if (a.z_grad != nullptr) {
+#pragma unroll
+          for (int v = 0; v < VPL; ++v) grad[v] = __builtin_fmaf(of_softmax, scores.e[v], grad[v]);
+        }
       } else {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) grad[v] = scores.e[v] * __builtin_fmaf(share[v] - dot, of_score, of_softmax);

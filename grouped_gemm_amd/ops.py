@@ -210,9 +210,11 @@ def balance_loss(logits, experts, offsets=None, mask=None, score="softmax"):
     route takes and returns them.  offsets int32 (sequences + 1): sequence s is the tokens offsets[s] .. offsets[s + 1] - 1,
     ascending; tokens before the first and behind the last count nowhere.  None: all tokens are one sequence.  mask bool
     (tokens): tokens that count, None: all.  Without tokens that count both losses are 0.  An expert whose logit is -inf is closed to the
-    token, a token that none is open to adds nothing; a NaN or +inf of a token that counts makes both losses NaN.
+    token, a token that none is open to adds nothing; a NaN of a token that counts makes both losses NaN, a +inf z and, of the softmax,
+    balance (sigmoid(+inf) is 1, and balance and its gradient are what that gives).
 
-    Everything is computed in float32 (where a token's largest logit is beyond 1.8e19, of either sign, z is infinite).  Gradients flow from balance and z to the logits, those of tokens that do not count are 0; counts are
+    Everything is computed in float32 (where a token's largest logit is beyond 1.8e19, of either sign, or the sum of such squares leaves a
+    float's range, z is infinite).  Gradients flow from balance and z to the logits, those of tokens that do not count are 0; counts are
     constants.  Second derivatives and forward mode are refused, and a backward pass that is captured into a graph while another graph of the same leaf,
     made outside the capture on the default stream, still lives.  Nothing waits for the device.  Not part of the
     reference's surface, which has no router."""

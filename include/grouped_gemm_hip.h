@@ -393,7 +393,8 @@ int gg_route_backward(const void* logits, int dtype, int64_t tokens, int64_t exp
  * device memory (0 for sizes that the call refuses), 4-byte aligned, of any contents; calls that share it must not overlap in time.
  *
  * gg_balance_backward: the gradient of the logits, of their element type, from those of balance and z (fp32, one number each in device memory,
- * either may be NULL); rows that are not counted get zeros.  counts, and so share, are taken as constants.
+ * either may be NULL: without a gradient of z, +inf leaves that of sigmoids' balance finite); rows that are not counted get zeros.  counts, and
+ * so share, are taken as constants.
  * No counterpart in the reference, which has no router.
  */
 uint64_t gg_balance_scratch_bytes(int64_t tokens, int64_t experts, int64_t top_k, int64_t sequences);

@@ -270,6 +270,43 @@ def test_rows_of_any_size(ops, dtype, score):
                 assert float(off.max()) <= 0, (experts, at, float(off.max()))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_infinite_logits_that_count(ops, dtype):
+    """+inf in a counted token: z is none, and softmax's balance; sigmoid(+inf) is 1, so the balance of sigmoids and its gradient are what the
+    definition gives (as at 1e4, where a sigmoid is 1 and its slope 0 in 64 bits), and other tokens' gradients are what they were."""
+    _announce("infinite", dtype)
+    for experts in (8, 30, 256, 700):
+        logits, chosen, g = _inputs(64, experts, 3, dtype, 21 + experts)
+        at = torch.zeros(64, experts, dtype=torch.bool)
+        at[5, 2] = at[40, ::3] = at[41] = True
+        logits[42, 1:] = -INF
+        at[42, 0] = True
+        offsets, near = torch.tensor([0, 20, 64], dtype=torch.int32), logits.double().masked_fill(at, 1e4)
+        logits = logits.masked_fill(at, INF)
+        rest = ~at.any(1)
+        half, least = ROUNDING[dtype]
+        for score in ("softmax", "sigmoid"):
+            def grads(which, of):
+                leaf = logits.cuda().requires_grad_(True)
+                loss = ops.balance_loss(leaf, chosen.cuda(), offsets=offsets.cuda(), score=score)
+                return loss, torch.autograd.grad(loss[which], leaf, torch.tensor(of, device="cuda"))[0].double().cpu()
+
+            (balance, z, counts), grad = grads(0, 0.7)
+            want = _reference(near, chosen, offsets, None, score, (0.7, 0.0))
+            assert math.isnan(z.detach())
+            off = (grad - want["grad"]).abs() - (2e-5 * want["grad_scale"] + half * want["grad"].abs() + least + 1e-37)
+            if score == "sigmoid":
+                assert abs(float(balance.detach()) - float(want["balance"])) <= 2e-5 * float(want["balance"]), (experts, float(balance.detach()))
+                assert float(off.max()) <= 0, (experts, float(off.max()))
+            else:
+                assert math.isnan(balance.detach())
+                assert float(off[rest].max()) <= 0, experts
+            want = _reference(near, chosen, offsets, None, score, (0.0, 1.3))
+            grad = grads(1, 1.3)[1]
+            off = (grad - want["grad"]).abs() - (2e-5 * want["grad_scale"] + half * want["grad"].abs() + least + 1e-37)
+            assert float(off[rest].max()) <= 0 and torch.isnan(grad[~rest]).any(1).all(), experts
+
+
 def test_numbers_that_name_no_expert_are_no_choice(ops):
     logits, chosen, g = _inputs(300, 20, 4, torch.float32, 8)
     chosen[torch.rand(300, 4, generator=g) < 0.3] = -1
