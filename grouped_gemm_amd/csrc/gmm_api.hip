@@ -822,8 +822,6 @@ int check_int8(const gg_gmm_args* args, const float* a_scales, const float* b_sc
   if (g.hidden_in > 0 && (g.a == nullptr || g.b == nullptr)) return fail(GG_EINVAL, "a or b is null");
   if ((reinterpret_cast<uintptr_t>(g.c) & 1) || ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3))
     return fail(GG_ELIMIT, "c and the scales must be aligned to their element size");
-  if (!gg::int8_rows_fit(g.tokens, std::min<int64_t>(g.num_groups, GG_MAX_GROUPS_PER_LAUNCH), g.hidden_in, g.hidden_out))
-    return fail(GG_ELIMIT, "tokens times hidden_out are too large for one launch");
   return GG_OK;
 }
 
@@ -839,9 +837,9 @@ gg_gmm_args int8_as_fp8(const gg_gmm_args& g) {
 }
 
 int int8_by_rows(const gg_gmm_args& g, const float* a_scales, const float* b_scales) {
-  DeviceInfo info;
-  int rc = device_info(&info);
-  if (rc != GG_OK) return rc;
+  // (a workgroup to each window of rows and strip of columns: not a limit of the streaming kernels)
+  if (!gg::int8_rows_fit(g.tokens, std::min<int64_t>(g.num_groups, GG_MAX_GROUPS_PER_LAUNCH), g.hidden_in, g.hidden_out))
+    return fail(GG_ELIMIT, "tokens times hidden_out are too large for one launch");
   if (reinterpret_cast<uintptr_t>(g.workspace) & 255) return fail(GG_ELIMIT, "the workspace must be 256-byte aligned");
   if (!g.batch_sizes_on_device) {
     int64_t row = 0;
@@ -852,6 +850,9 @@ int int8_by_rows(const gg_gmm_args& g, const float* a_scales, const float* b_sca
       row += g.batch_sizes[e];
     }
   }
+  DeviceInfo info;
+  const int rc = device_info(&info);
+  if (rc != GG_OK) return rc;
   int64_t row = 0;
   for (int64_t first = 0; first < g.num_groups; first += GG_MAX_GROUPS_PER_LAUNCH) {
     const int64_t count = std::min<int64_t>(g.num_groups - first, GG_MAX_GROUPS_PER_LAUNCH);

@@ -467,7 +467,8 @@ int gg_swiglu_quantize(const void* gate_up, int dtype, int64_t rows, int64_t col
  *   c[r, n] = a_scales[r] * b_scales[e, n] * sum over k of a[r, k] * b[e, n, k],   e the group of row r
  * a int8 (tokens, hidden_in), b int8 (num_groups, hidden_out, hidden_in): trans_b set, trans_a not; dtype is c's, GG_DTYPE_BF16 or
  * GG_DTYPE_F16.  a_scales fp32 (tokens), b_scales fp32 (num_groups, hidden_out).  All other fields as for gg_gmm, without row indices,
- * epilogues and accumulation; sizes and alignment are any.  Sums are exact, for any of the 256 values, up to a hidden_in of 131071;
+ * epilogues and accumulation; sizes and alignment are any (GG_ELIMIT past 2^24 workgroups where groups have few rows or a row of a or b does not begin on 16
+ * bytes: one to each 64 columns of 16 to 64 rows of a group).  Sums are exact, for any of the 256 values, up to a hidden_in of 131071;
  * they are scaled in fp32, by the column's first, and rounded once: the same bits on every call.  Rows behind the last group's are left as they are.
  * gg_gmm_int8_workspace_bytes: 0, or GG_WORKSPACE_BYTES where the call can make use of a workspace (fields as for gg_workspace_bytes_for).
  * No counterpart in the reference, whose operands are bf16 (csrc/grouped_gemm.cu:490-506).

@@ -84,6 +84,25 @@ def test_gmm_int8_argument_errors_need_no_device(lib):
     assert call(hidden_out=0, c=None) == 0 and call(num_groups=0, batch_sizes=None) == 0
 
 
+def test_gmm_int8_limits_are_those_of_the_kernel_that_runs(lib):
+    """More windows of rows and strips of columns than one launch of the kernel for few rows takes: refused where that kernel would run, not where the
+    streaming one does (which then gets as far as the sizes, wrong here on purpose)."""
+    def call(**kw):
+        args, host = _args(sizes=(-1,) * kw.pop("groups"), **kw)
+        return lib.gg_gmm_int8(ctypes.byref(args), 4096, 4096), lib.gg_last_error()
+
+    for kw in (dict(groups=8, tokens=1 << 20, hidden_in=16, hidden_out=65536), dict(groups=512, tokens=4097, hidden_in=16, hidden_out=1 << 21)):
+        rc, text = call(**kw)
+        assert rc == -1 and b"negative" in text, (kw, rc, text)
+        for odd in (dict(hidden_in=15), dict(a=4097), dict(b=8200)):
+            rc, text = call(**{**kw, **odd})
+            assert rc == -2 and b"too large" in text, (kw, odd, rc, text)
+    rc, text = call(groups=512, tokens=4096, hidden_in=16, hidden_out=1 << 21)   # (few rows to a group)
+    assert rc == -2 and b"too large" in text
+    rc, text = call(groups=8, tokens=1 << 10, hidden_in=15, hidden_out=65536)
+    assert rc == -1 and b"negative" in text
+
+
 def test_gmm_int8_workspace_goes_by_the_sizes(lib):
     def wanted(sizes, hidden_in, hidden_out, tokens=None):
         args, host = _args(sizes=sizes, tokens=sum(sizes) if tokens is None else tokens, hidden_in=hidden_in, hidden_out=hidden_out)

@@ -443,6 +443,26 @@ def test_captured_and_replayed(ops, sizes, hidden_in, hidden_out):
         assert torch.equal(got[0], eager.values) and torch.equal(got[1], eager.scales), n
 
 
+def test_more_columns_than_a_launch_for_few_rows_takes(ops):
+    """Windows of rows times strips of columns past 2^24, a limit of the kernel for few rows, on the streaming one."""
+    _announce("wide")
+    experts, hidden_in, hidden_out = 512, 16, 1_725_440
+    sizes = torch.full((experts,), 8)
+    sizes[::100] += 1
+    rows = int(sizes.sum())   # (8 to an expert and a few more)
+    b = torch.empty(experts, hidden_out, hidden_in, dtype=torch.int8, device="cuda").random_(-128, 128)   # 14 GB, and as much of results
+    sb = torch.rand(experts, hidden_out, device="cuda") / 64 + 1e-3
+    a = torch.empty(rows, hidden_in, dtype=torch.int8, device="cuda").random_(-128, 128)
+    sa = torch.rand(rows, device="cuda") / 64 + 1e-3
+    got = ops.gmm_int8(a, sa, b, sb, sizes.cuda())
+    ends = sizes.cumsum(0)
+    for e in (0, 1, 255, 300, 511):
+        for r in (int(ends[e] - sizes[e]), int(ends[e]) - 1):
+            for at in (slice(0, 300), slice(hidden_out // 2, hidden_out // 2 + 300), slice(hidden_out - 300, hidden_out)):
+                want = ((b[e, at].double() * a[r].double()).sum(1) * sa[r].double() * sb[e, at].double()).cpu()
+                _check_close(got[r, at], want, torch.bfloat16, (e, r))
+
+
 def test_offsets_past_32_bits(ops):
     """More than 4 GiB of weights, and more than 4 GiB of rows."""
     _announce("large")
