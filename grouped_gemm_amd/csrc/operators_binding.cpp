@@ -33,6 +33,23 @@ void RefuseTangents(std::initializer_list<const torch::Tensor*> tensors, const c
     TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "grouped_gemm: ", name, " has no forward-mode derivative");
 }
 
+// torch hands a leaf's gradient over on the stream where a graph of the leaf was first made, as long as one lives.  From a captured backward pass to the
+// default stream, which a capture cannot wait for, that ends the process: an error here, before torch gets there.
+void RefuseLivingGraph(const torch::Tensor& leaf, const char* name) {
+  if (!leaf.is_leaf()) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (accumulator == nullptr) return;
+  const auto made_on = accumulator->stream();
+  if (!made_on.has_value() || made_on->id() != 0) return;   // (0: the default one)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(CurrentStream(leaf.device())), &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return;
+  }
+  TORCH_CHECK(status == hipStreamCaptureStatusNone, "grouped_gemm: a captured backward pass of ", name,
+              " cannot reach a leaf of which a graph made outside the capture still lives: free what that graph returned first");
+}
+
 // ------------------------------------------------------------------ router
 
 int LogitsType(torch::ScalarType t) {
@@ -122,6 +139,7 @@ class RouteNode : public torch::autograd::Function<RouteNode> {
     const torch::Tensor weights_grad = grads[0], mass_grad = grads.size() > 5 ? grads[5] : torch::Tensor(), none;
     if (!weights_grad.defined() && !mass_grad.defined()) return {none, none, none, none, none};
     RefuseTangents({&weights_grad, &mass_grad}, "the gradient of route");
+    RefuseLivingGraph(logits, "route");
     const int64_t score = ctx->saved_data["score"].toInt();
     const bool normalize = ctx->saved_data["normalize"].toBool();
     torch::Tensor out;
@@ -189,23 +207,6 @@ torch::Tensor RunBalanceBackward(const BalanceInputs& in, const torch::Tensor& k
                                      CurrentStream(logits.device()));
   TORCH_CHECK(rc == GG_OK, "grouped_gemm: ", gg_last_error());
   return out;
-}
-
-// torch hands a leaf's gradient over on the stream where a graph of the leaf was first made, as long as one lives.  From a captured backward pass to the
-// default stream, which a capture cannot wait for, that ends the process: an error here, before torch gets there.
-void RefuseLivingGraph(const torch::Tensor& leaf, const char* name) {
-  if (!leaf.is_leaf()) return;
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
-  if (accumulator == nullptr) return;
-  const auto made_on = accumulator->stream();
-  if (!made_on.has_value() || made_on->id() != 0) return;   // (0: the default one)
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(static_cast<hipStream_t>(CurrentStream(leaf.device())), &status) != hipSuccess) {
-    (void)hipGetLastError();
-    return;
-  }
-  TORCH_CHECK(status == hipStreamCaptureStatusNone, "grouped_gemm: a captured backward pass of ", name,
-              " cannot reach a leaf of which a graph made outside the capture still lives: free what that graph returned first");
 }
 
 c10::optional<torch::Tensor> Given(const torch::Tensor& t) { return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt; }

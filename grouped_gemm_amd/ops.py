@@ -186,8 +186,9 @@ def route(logits, top_k, score="softmax", normalize=True, with_mass=False):
     weights of 0.  logits: float32, bfloat16 or float16; everything is computed in float32.
 
     `mass`, with with_mass, is what balancing losses need beside batch_sizes.  Gradients flow from weights and mass
-    to the logits; second derivatives and forward mode are refused.  Nothing waits for the device: batch_sizes stays there, as gmm takes it.  Not part of the reference's surface, which
-    takes rows already sorted (grouped_gemm/ops.py:8)."""
+    to the logits; second derivatives and forward mode are refused, and a backward pass that is captured into a graph while another graph of the
+    same leaf, made outside the capture on the default stream, still lives.  Nothing waits for the device: batch_sizes stays there, as gmm takes it.
+    Not part of the reference's surface, which takes rows already sorted (grouped_gemm/ops.py:8)."""
     return Routing(*backend.backend.route(logits, top_k, score, normalize, with_mass))
 
 

@@ -275,6 +275,35 @@ def test_route_refuses_a_second_derivative(ops, normalize, parts):
     assert torch.equal(second, 6 * w.detach())
 
 
+def test_route_captured_gradient_beside_a_living_graph_is_refused(ops):
+    """While a graph of the same logits lives that was made outside the capture, on the default stream; then, without it, captured and replayed."""
+    x = torch.randn(60, 20, device="cuda").requires_grad_(True)
+    grads = torch.randn(60, 3, device="cuda"), torch.randn(20, device="cuda")
+
+    def step():
+        r = ops.route(x, 3, with_mass=True)
+        return torch.autograd.grad((r.weights, r.mass), x, grads)[0]
+
+    want = step()
+    living = ops.route(x, 3)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured backward pass of route"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    grad, = torch.autograd.grad(living.weights, x, grads[0])     # (the graph outside is as it was)
+    assert torch.isfinite(grad).all()
+    del living, grad
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_route_on_other_streams_and_in_a_graph(ops):
     """The same bits on another stream, on every call and in every replay of a captured one, with eager work in between."""
     logits = torch.randn(5000, 96, device="cuda").bfloat16()
