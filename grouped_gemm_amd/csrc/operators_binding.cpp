@@ -476,7 +476,7 @@ torch::Tensor GmmInt8(const torch::Tensor& a, const torch::Tensor& a_scales, con
   // 117, 128 143 / 179; 32, 4095 -> 2047: 96 209 / 181, 128 214 / 241; 8, 1021 -> 1021: 128 23 / 19, 256 24 / 30.
   const bool aligned = hidden_in % 16 == 0 && ((reinterpret_cast<uintptr_t>(a.data_ptr()) | reinterpret_cast<uintptr_t>(b.data_ptr())) & 15) == 0;
   const int64_t padded = (hidden_in + 15) / 16 * 16;
-  if (!aligned && tokens >= kInt8PadRows * experts && hidden_in > 0 && hidden_out > 0 && padded <= GG_INT8_MAX_DEPTH) {
+  if (!aligned && experts > 0 && tokens >= kInt8PadRows * experts && hidden_in > 0 && hidden_out > 0 && padded <= GG_INT8_MAX_DEPTH) {
     depth = padded;
     lhs = torch::empty({tokens, depth}, a.options());
     rhs = torch::empty({experts, hidden_out, depth}, a.options());

@@ -366,6 +366,17 @@ def test_no_depth_no_rows_no_columns(ops):
         assert (_run(ops, a, sa, b, sb, [0, 0], torch.bfloat16, on_device, c=c) == 2).all()
 
 
+@pytest.mark.parametrize("on_device", [True, False])
+@pytest.mark.parametrize("rows", [0, 5, 700])
+def test_no_experts_on_any_boundary(ops, rows, on_device):
+    """Nothing is named, nothing is read: rows of c stay, whatever the depth."""
+    for hidden_in, hidden_out in ((63, 8), (64, 8), (15, 9)):
+        a, sa, b, sb = _operands(rows, 0, hidden_in, hidden_out, 1)
+        c = torch.full((rows, hidden_out), 2.0, dtype=torch.bfloat16, device="cuda")
+        assert (_run(ops, a, sa, b, sb, [], torch.bfloat16, on_device, c=c) == 2).all()
+        assert _run(ops, a, sa, b, sb, [], torch.float16, on_device).shape == (rows, hidden_out)
+
+
 @pytest.mark.parametrize("experts,rows", [(513, 700), (700, 40000), (1500, 1500), (600, 20)])
 def test_more_groups_than_a_launch_takes(ops, experts, rows):
     _announce("groups", experts, rows)
