@@ -307,6 +307,32 @@ def test_infinite_logits_that_count(ops, dtype):
             assert float(off[rest].max()) <= 0 and torch.isnan(grad[~rest]).any(1).all(), experts
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_small_sigmoids_beside_large_logits(ops, dtype):
+    """A sigmoid has its size whatever the token's largest logit, and its element of the balance's gradient too: each to 2e-5 of itself (one
+    exponential, off by 2^-24 of |x| <= 60, and some units in the last place), a rounding of the type, and 1e-37 where fp32 ends."""
+    _announce("small sigmoids", dtype)
+    for experts in (8, 30, 256, 700):
+        logits, chosen, g = _inputs(64, experts, 3, dtype, 51 + experts)
+        top = torch.linspace(0.0, 60.0, 64)
+        logits = (torch.rand(64, experts, generator=g) * 110.0 - 60.0).minimum(top.unsqueeze(1))
+        logits[:, 1] = top
+        logits = logits.to(dtype)
+        want = _reference(logits, chosen, None, None, "sigmoid", (64.0, 0.0))
+        leaf = logits.cuda().requires_grad_(True)
+        got = ops.balance_loss(leaf, chosen.cuda(), score="sigmoid")
+        assert abs(float(got.balance.detach()) - float(want["balance"])) <= 2e-5 * float(want["balance"])
+        grad, = torch.autograd.grad(got.balance, leaf, torch.tensor(64.0, device="cuda"))
+        half, least = ROUNDING[dtype]
+        # (the difference of share and its mean by p, each off by 2e-5 of itself, times the element's own p and slope)
+        x = logits.double()
+        p = torch.softmax(torch.nn.functional.logsigmoid(x), 1)
+        share = want["counts"][0].double() * experts / (3 * 64)
+        scale = p * torch.sigmoid(-x) * torch.maximum(share, (share * p).sum(1, keepdim=True))
+        off = (grad.double().cpu() - want["grad"]).abs() - (2e-5 * scale + half * want["grad"].abs() + least + 1e-37)
+        assert float(off.max()) <= 0, (experts, float(off.max()))
+
+
 def test_numbers_that_name_no_expert_are_no_choice(ops):
     logits, chosen, g = _inputs(300, 20, 4, torch.float32, 8)
     chosen[torch.rand(300, 4, generator=g) < 0.3] = -1
