@@ -26,13 +26,14 @@ namespace gg {
 namespace {
 
 constexpr int kBalanceThreads = 256;
-// Workgroups that the tokens are cut into, at most: four to a compute unit, all there at once.  Units / sums / backward of 65536 tokens, 256
-// experts in us with 512: 20.4 / 6.8 / 32.2, with 1024: 18.8 / 7.5 / 30.0, with 2048: 19.8 / 10.6 / 34.8.
+// Workgroups that the tokens are cut into, at most: four to a compute unit, all there at once.  Units / sums / backward in us with 512, 1024 and
+// 2048: 65536 x 256, bf16, sigmoid, 64 sequences 18.2 / 7.3 / 25.1, 16.3 / 8.1 / 24.7, 17.9 / 10.4 / 29.7; softmax 14.5 / 7.3 / 23.3, 13.4 / 8.1 /
+// 22.6, 14.9 / 10.4 / 28.0; 32768 x 128, 16 sequences 7.3 / 6.9 / 10.0, 6.7 / 9.0 / 9.8, 7.9 / 8.2 / 12.4; 65536 x 64, fp32, 8 9.2 / 7.2 / 10.0, 8.3 / 8.1 /
+// 9.0, 9.2 / 9.2 / 8.6.
 constexpr int64_t kBalanceBlocks = 1024;
 // Units of a sequence, on average, up to which a wave adds them up, and needs no barrier for it.  All three kernels, wave / workgroup: 65536 x 64, 8192 sequences
 // (1.1 units) 85 / 102 us; 4096 x 64, 512 25.7 / 29.7; 65536 x 256, 64 sequences (17) 57.5 / 52.
 constexpr int64_t kWaveUnits = 8;
-
 
 struct BalanceParams {
   BalanceArgs a;
@@ -173,6 +174,8 @@ struct NextToken {
   }
 };
 
+// (Four workgroups to a compute unit leave 128 registers.  Sigmoids of fp16, 16 to a lane, do not fit beside the next token's logits: 2 registers spill here with
+// more than 512 experts, 4 in the gradient with 129 to 256 and 8 with more than 512.  65536 x 256, fp16 55 us, bf16 52, all three kernels.)
 template <int DT, bool SIGMOID, int G, int VPL>
 __global__ __launch_bounds__(kBalanceThreads, 4) void balance_units_kernel(BalanceParams p) {
   constexpr int GROUPS = kBalanceThreads / G, COLUMNS = G * VPL;

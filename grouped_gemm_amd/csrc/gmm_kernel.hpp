@@ -1704,7 +1704,7 @@ __device__ __forceinline__ void gmm_tiles(const GmmParams& given, const HostSize
   // as two-byte elements, two to one: same bytes per row and slice, BK_ELEMS depth values a slice.
   // I8: 8-bit integers, which move and are held as fp8 is; the 64-deep step of an instruction there takes two here.  (In 16 x 16 x 64
   // instructions, which alone sustain 5 % more of such operands, the compiler moves accumulators in and out of the loop.)  32768 rows over 8
-  // uneven groups, 4096 -> 14336: 1.57 to 1.63 ms, 2360-2450 TOPS, where the instruction alone sustains 3520 on such operands (fp8's 4160) and
+  // uneven groups, 4096 -> 14336: 1.57 to 1.79 ms by card and minute, 2150-2450 TOPS, where the instruction alone sustains 3520 on such operands (fp8's 4160) and
   // 4950 on zeros, on which the whole product takes 1.18 ms, as many cycles: the matrix pipe is busy in two thirds of them, and power sets their length.  24576 rows over 64 groups, 2048 -> 2816: 167-182 us, half of which is
   // the tiles' traffic, begun and ended by all workgroups at about the same time.
   constexpr bool I8 = is_i8(DT), F8 = is_f8(DT) || I8;

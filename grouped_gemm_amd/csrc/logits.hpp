@@ -1,4 +1,4 @@
-// Router logits of three element types, a token's in 16 or 64 lanes, and the functions of them: what the router and its losses share.
+// Router logits of three element types, a token's in 4, 16 or 64 lanes, and the functions of them: what the router and its losses share.
 #pragma once
 
 #include <hip/hip_runtime.h>
