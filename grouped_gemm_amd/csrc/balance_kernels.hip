@@ -61,7 +61,7 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences
   const int lane = threadIdx.x & 63;
   int low = 0, n = sequences + 1;   // the first of the offsets not yet known to be at t or before, and how many are open
   while (n > 0) {
-    const int step = (n + 63) / 64, at = lane * step;
+    const int step = (n - 1) / 64 + 1, at = lane * step;   // (of up to 2^31 - 1)
     const int before = __popcll(__ballot(at < n && offsets[low + at] <= t));
     if (before == 0) break;
     if (step == 1) {
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(kBalanceThreads, 4) void balance_backward_kernel(Ba
     if (t >= end && s + 1 < a.sequences) {   // far from here: those that are left are halved
       int low = s + 1, high = a.sequences - 1;
       while (low < high) {
-        const int middle = (low + high + 1) / 2;
+        const int middle = low + (high - low + 1) / 2;   // (their sum may pass 31 bits)
         if (offset_of(a.offsets, a.tokens, middle) <= t) low = middle;
         else high = middle - 1;
       }

@@ -547,6 +547,28 @@ def test_many_tokens_and_sequences(ops):
     _check(ops, logits, chosen, torch.arange(tokens + 1, dtype=torch.int32), None, "softmax", "a sequence to a token")
 
 
+def test_more_sequences_than_30_bits_count(ops):
+    """Sequences past 2^30, nearly all of them empty: the numbers of two that a search is between do not fit 31 bits together."""
+    _announce("sequences past 2^30")
+    tokens, experts, sequences = 8192, 2, (1 << 30) + 1000
+    logits, chosen, g = _inputs(tokens, experts, 1, torch.float32, 61)
+    # (token 8 n + 4 and those behind it are in another sequence than the four before: far apart for the first ones, among the last for the rest)
+    places = torch.cat([torch.tensor([10, (1 << 30) + 100]), (1 << 30) + 101 + torch.sort(torch.randperm(890, generator=g)[:60]).values, torch.tensor([sequences - 2])])
+    ends = torch.cat([torch.tensor([4, 8]), 12 + 8 * torch.sort(torch.randperm(1000, generator=g)[:60]).values, torch.tensor([tokens])])
+    offsets = torch.zeros(sequences + 1, dtype=torch.int32, device="cuda")
+    for place, end, behind in zip(places.tolist(), ends.tolist(), places.tolist()[1:] + [sequences]):
+        offsets[place + 1:behind + 1] = end
+    few = torch.cat([torch.tensor([0]), ends]).to(torch.int32)
+    want = _reference(logits, chosen, few, None, "softmax", (0.7, 1.3))
+    leaf = logits.cuda().requires_grad_(True)
+    got = ops.balance_loss(leaf, chosen.cuda(), offsets)
+    grad, = torch.autograd.grad((got.balance, got.z), leaf, (torch.tensor(0.7, device="cuda"), torch.tensor(1.3, device="cuda")))
+    assert abs(float(got.balance.detach()) - float(want["balance"])) <= 2e-5 * float(want["balance"])
+    assert abs(float(got.z.detach()) - float(want["z"])) <= 2e-5 * float(want["z"]) + 2e-6 * float(want["z_scale"])
+    assert torch.equal(got.counts[places.cuda()].cpu().long(), want["counts"])
+    assert ((grad.double().cpu() - want["grad"]).abs() <= 2e-5 * want["grad_scale"] + 2.0 ** -24 * want["grad"].abs() + 1e-37).all()
+
+
 def test_the_example_runs(ops):
     """examples/int8_expert_layer.py: that it runs, that every parameter gets a gradient, and that the layer in 8 bits is the layer that
     was trained.  Quantising moves each element of a row by up to half a step, 1/254 of the row's largest: uniformly distributed, by 1/880 of it
